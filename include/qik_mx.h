@@ -1,0 +1,170 @@
+/*
+ * qik_mx.h -- C ABI of the microscaled (MX) operators beside the fp8 linear:
+ *
+ *   qik_mx_quantize        rows -> MXFP4 or MXFP8 codes and block scales
+ *   qik_mx_quantize_host   the same for rows in host memory, on the CPU
+ *   qik_mx_dequantize      codes and block scales -> the values they stand for
+ *   qik_residual_rms_norm  h = x + residual, RMSNorm of h; the output in the
+ *                          element type or microscaled
+ *   qik_mx_gemm            out = A . W^T + bias, A in MXFP4 or MXFP8, W in MXFP4
+ *   qik_mx_linear          the same with A quantised from bf16 / fp16 / fp32 rows
+ *
+ * Same conventions as qik_attn.h: plain C, no allocation, device pointers of
+ * the current HIP device, `stream` a hipStream_t as void*, asynchronous and
+ * stream-ordered launches, return QIK_OK or a negative qik_status.
+ *
+ * Microscaled rows (OCP MX v1.0): a row of K elements, K a multiple of 32, is
+ * cut into blocks of 32.  A block has one scale byte e (E8M0: 2^(e - 127), 255
+ * is NaN) and 32 elements, E2M1 in MXFP4 (two to a byte, the first in the low
+ * half) or E4M3 in MXFP8.  With E the fp32 exponent field of the block's
+ * largest magnitude, e = 255 if E is 255 (an infinity or NaN poisons its
+ * block: codes 0), else max(E - emax, 0) with emax 2 (E2M1) or 8 (E4M3); the
+ * elements are x * 2^(127 - e) rounded to nearest even, saturated at 6 or 448.
+ *
+ * Layout of the scales: the byte of row m, block b is at
+ *   ((m / 32) * C + b / 8) * 256 + (m % 32) * 8 + b % 8,   C = ceil(K / 256),
+ * so 32 rows x 256 k are 256 contiguous bytes, what one lane group of the
+ * product reads at once.  Rows M .. 32 * ceil(M / 32) and blocks K / 32 .. 8 C
+ * are padding: the writers set it to 0, and a reader needs it not to be 255.
+ * qik_mx_scales_size gives the bytes.
+ */
+#ifndef QIK_MX_H
+#define QIK_MX_H
+
+#include <stdint.h>
+
+#include "qik_fp8.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+enum qik_mx_format {
+  QIK_MX_NONE = 0, /* qik_residual_rms_norm only: output in the element type */
+  QIK_MXFP4 = 1,   /* E2M1, K / 2 bytes a row                                */
+  QIK_MXFP8 = 2    /* E4M3, K bytes a row                                    */
+};
+
+/* Bytes of the scales of M rows of K elements (M >= 0, K a multiple of 32). */
+int qik_mx_scales_size(int64_t M, int64_t K, int64_t* bytes);
+
+/* x: rows of `dtype` with row stride ldx (elements, >= K), unit element stride,
+ * any alignment of at least the element's.  codes: row stride K / 2 or K bytes,
+ * 16-byte aligned; scales: 4-byte aligned.  M >= 0 (0: nothing is launched), 32
+ * <= K <= 262144, M < 2^31. */
+typedef struct qik_mx_quant_args {
+  int32_t abi_version;        /* QIK_ABI_VERSION                                     */
+  int32_t dtype;              /* QIK_DTYPE_BF16, QIK_DTYPE_FP16 or QIK_DTYPE_FP32      */
+  int32_t format;             /* QIK_MXFP4 or QIK_MXFP8                              */
+  int32_t reserved0;          /* must be 0                                           */
+  const void* x;              /* [M, K]                                              */
+  void* codes;                /* written                                             */
+  void* scales;               /* written, padding included                           */
+  int64_t M, K;
+  int64_t ldx;                /* row stride of x, elements                           */
+} qik_mx_quant_args;
+
+int qik_mx_quantize(const qik_mx_quant_args* args, void* stream);
+
+/* qik_mx_quantize for x, codes and scales in HOST memory, on the CPU: the same
+ * bytes.  `threads` host threads at most (< 1 means 1). Blocking. */
+int qik_mx_quantize_host(const qik_mx_quant_args* args, int32_t threads);
+
+/* out[m, k] = element * 2^(e - 127), rounded once to nearest even into dtype
+ * (exact in bf16 and fp32); NaN where e is 255.  out: row stride K, 16-byte
+ * aligned; codes and scales as qik_mx_quantize writes them. */
+typedef struct qik_mx_dequant_args {
+  int32_t abi_version;        /* QIK_ABI_VERSION                                     */
+  int32_t dtype;              /* of out: QIK_DTYPE_BF16, _FP16 or _FP32                */
+  int32_t format;             /* QIK_MXFP4 or QIK_MXFP8                              */
+  int32_t reserved0;          /* must be 0                                           */
+  const void* codes;
+  const void* scales;
+  void* out;                  /* [M, K], written                                     */
+  int64_t M, K;
+} qik_mx_dequant_args;
+
+int qik_mx_dequantize(const qik_mx_dequant_args* args, void* stream);
+
+/* Per row of D elements:
+ *   h = round(x + residual)            (h = x without a residual)
+ *   r = fp32(1 / sqrt(mean(h^2) + eps))  the mean, the sum and the root in fp64
+ *   y = (h * r) * weight               fp32, each product rounded
+ *   out = round(y), or y microscaled; sum = h
+ * x, residual: row strides ldx, ldr (elements, >= D), unit element stride, any
+ * alignment of at least the element's; sum and out (QIK_MX_NONE) have row
+ * stride D.  A microscaled out needs D a multiple of 32, rows of x, residual
+ * and sum and the weight at multiples of 16 bytes (QIK_ERR_ALIGN), 16-byte
+ * aligned codes and 4-byte aligned scales.  1 <= D <= 32768, M < 2^31 (0:
+ * nothing is launched).  residual and sum are both given or both NULL.  sum, out and
+ * scales overlap no input. */
+typedef struct qik_residual_rms_norm_args {
+  int32_t abi_version;        /* QIK_ABI_VERSION                                     */
+  int32_t dtype;              /* of x, residual, sum: QIK_DTYPE_BF16, _FP16 or _FP32   */
+  int32_t format;             /* enum qik_mx_format of out                           */
+  int32_t weight_dtype;       /* QIK_DTYPE_FP32 or dtype                             */
+  const void* x;              /* [M, D]                                              */
+  const void* residual;       /* [M, D] or NULL                                      */
+  const void* weight;         /* [D]                                                 */
+  void* sum;                  /* [M, D], written, or NULL                            */
+  void* out;                  /* [M, D] in dtype, or the codes                       */
+  void* scales;               /* of a microscaled out, else NULL                     */
+  int64_t M, D;
+  int64_t ldx, ldr;           /* row strides, elements                               */
+  double eps;
+} qik_residual_rms_norm_args;
+
+int qik_residual_rms_norm(const qik_residual_rms_norm_args* args, void* stream);
+
+/* out[m, n] = round(sum_k A[m, k] * W[n, k] + bias[n]): the values the codes
+ * stand for, multiplied exactly and summed in fp32, the bias added in fp32, one
+ * rounding to nearest even into out_dtype.  A block whose scale is 255 makes
+ * its row's outputs NaN.  a: rows of a_format (row stride lda bytes), w: rows
+ * of MXFP4 (ldw bytes); both row strides multiples of 16 and at least a row,
+ * 16-byte aligned; scales in the layout above, 16-byte aligned.  bias [N] and
+ * out (row stride ldc elements, >= N) in out_dtype, aligned to an element.
+ * 0 <= M < 2^31 (0: nothing is launched), 1 <= N < 2^31, K a multiple of 32,
+ * 32 <= K <= 262144. */
+typedef struct qik_mx_gemm_args {
+  int32_t abi_version;        /* QIK_ABI_VERSION                                     */
+  int32_t out_dtype;          /* QIK_DTYPE_BF16 or QIK_DTYPE_FP16 (bias has it too)   */
+  int32_t a_format;           /* QIK_MXFP4 or QIK_MXFP8                              */
+  int32_t reserved0;          /* must be 0                                           */
+  const void* a;              /* codes of [M, K]                                     */
+  const void* a_scales;
+  const void* w;              /* MXFP4 codes of [N, K]                               */
+  const void* w_scales;
+  const void* bias;           /* [N] or NULL                                         */
+  void* out;                  /* [M, N]                                              */
+  int64_t M, N, K;
+  int64_t lda, ldw;           /* row strides of a and w, bytes                       */
+  int64_t ldc;                /* row stride of out, elements                         */
+} qik_mx_gemm_args;
+
+/* The workspace holds the fp32 sums of a K split: qik_mx_gemm_workspace_size
+ * gives the bytes a call needs, 0 (and the pointer may be NULL) where it does
+ * not split.  256-byte aligned, its contents irrelevant; calls that overlap
+ * must not share one.  QIK_ERR_WORKSPACE if it is missing, misaligned or short. */
+int qik_mx_gemm_workspace_size(const qik_mx_gemm_args* args, int64_t* bytes);
+int qik_mx_gemm(const qik_mx_gemm_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* qik_mx_gemm of x quantised to g.a_format: x is [M, K] of x_dtype with row
+ * stride ldx as in qik_mx_quantize; g.a, g.a_scales and g.lda are not read.
+ * The workspace holds the codes and scales of x too; where the launch
+ * quantises x as it loads it (few rows) no memory is needed for them. */
+typedef struct qik_mx_linear_args {
+  qik_mx_gemm_args g;
+  const void* x;
+  int64_t ldx;                /* elements                                            */
+  int32_t x_dtype;            /* QIK_DTYPE_BF16, QIK_DTYPE_FP16 or QIK_DTYPE_FP32      */
+  int32_t reserved0;          /* must be 0                                           */
+} qik_mx_linear_args;
+
+int qik_mx_linear_workspace_size(const qik_mx_linear_args* args, int64_t* bytes);
+int qik_mx_linear(const qik_mx_linear_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* QIK_MX_H */

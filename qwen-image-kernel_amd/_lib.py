@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI declared in include/qik_attn.h and include/qik_ops.h.
+"""ctypes binding of the C ABI declared in include/qik_attn.h, qik_ops.h, qik_fp8.h and qik_mx.h.
 
 The shared library is built in-tree (``lib/libqik_attn.so`` next to this file)
 by ``build.py``.  There is no fallback: if the library is missing or fails to
@@ -29,6 +29,11 @@ DTYPE_FP32 = 2  # quantiser input only (include/qik_fp8.h)
 
 FP8_ACTIVATION = 0
 FP8_WEIGHT = 1
+
+# enum qik_mx_format (include/qik_mx.h)
+MX_NONE = 0
+MXFP4 = 1
+MXFP8 = 2
 
 # leading bytes of a qik_attn_fwd_ws workspace that hold its control words
 WS_CTL_BYTES = 32768
@@ -182,7 +187,97 @@ class QikFp8GemmArgs(ctypes.Structure):
     ]
 
 
-# (name, restype, argtypes) of every exported entry point
+class QikMxQuantArgs(ctypes.Structure):
+    """Mirror of ``struct qik_mx_quant_args`` (include/qik_mx.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("format", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("M", ctypes.c_int64),
+        ("K", ctypes.c_int64),
+        ("ldx", ctypes.c_int64),
+    ]
+
+
+class QikMxDequantArgs(ctypes.Structure):
+    """Mirror of ``struct qik_mx_dequant_args`` (include/qik_mx.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("format", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("M", ctypes.c_int64),
+        ("K", ctypes.c_int64),
+    ]
+
+
+class QikResidualRmsNormArgs(ctypes.Structure):
+    """Mirror of ``struct qik_residual_rms_norm_args`` (include/qik_mx.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("format", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("sum", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("M", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("ldx", ctypes.c_int64),
+        ("ldr", ctypes.c_int64),
+        ("eps", ctypes.c_double),
+    ]
+
+
+class QikMxGemmArgs(ctypes.Structure):
+    """Mirror of ``struct qik_mx_gemm_args`` (include/qik_mx.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("a_format", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+        ("a", ctypes.c_void_p),
+        ("a_scales", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("w_scales", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("M", ctypes.c_int64),
+        ("N", ctypes.c_int64),
+        ("K", ctypes.c_int64),
+        ("lda", ctypes.c_int64),
+        ("ldw", ctypes.c_int64),
+        ("ldc", ctypes.c_int64),
+    ]
+
+
+class QikMxLinearArgs(ctypes.Structure):
+    """Mirror of ``struct qik_mx_linear_args`` (include/qik_mx.h)."""
+
+    _fields_ = [
+        ("g", QikMxGemmArgs),
+        ("x", ctypes.c_void_p),
+        ("ldx", ctypes.c_int64),
+        ("x_dtype", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
+# (name, restype, argtypes) of every entry point of qik_attn.h, qik_ops.h and qik_fp8.h
 EXPORTS = (
     ("qik_abi_version", ctypes.c_int, ()),
     ("qik_strerror", ctypes.c_char_p, (ctypes.c_int,)),
@@ -246,6 +341,23 @@ EXPORTS = (
      (ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32)),
 )
 
+# and of qik_mx.h
+MX_EXPORTS = (
+    ("qik_mx_scales_size", ctypes.c_int, (ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_int64))),
+    ("qik_mx_quantize", ctypes.c_int, (ctypes.POINTER(QikMxQuantArgs), ctypes.c_void_p)),
+    ("qik_mx_quantize_host", ctypes.c_int, (ctypes.POINTER(QikMxQuantArgs), ctypes.c_int32)),
+    ("qik_mx_dequantize", ctypes.c_int, (ctypes.POINTER(QikMxDequantArgs), ctypes.c_void_p)),
+    ("qik_residual_rms_norm", ctypes.c_int, (ctypes.POINTER(QikResidualRmsNormArgs), ctypes.c_void_p)),
+    ("qik_mx_gemm_workspace_size", ctypes.c_int,
+     (ctypes.POINTER(QikMxGemmArgs), ctypes.POINTER(ctypes.c_int64))),
+    ("qik_mx_gemm", ctypes.c_int,
+     (ctypes.POINTER(QikMxGemmArgs), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p)),
+    ("qik_mx_linear_workspace_size", ctypes.c_int,
+     (ctypes.POINTER(QikMxLinearArgs), ctypes.POINTER(ctypes.c_int64))),
+    ("qik_mx_linear", ctypes.c_int,
+     (ctypes.POINTER(QikMxLinearArgs), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p)),
+)
+
 _lock = threading.Lock()
 _lib = None
 
@@ -264,7 +376,7 @@ def load() -> ctypes.CDLL:
                 "run __graft_entry__.build() or python -m qwen_image_kernel_amd.build"
             )
         lib = ctypes.CDLL(LIB_PATH)
-        for name, restype, argtypes in EXPORTS:
+        for name, restype, argtypes in EXPORTS + MX_EXPORTS:
             fn = getattr(lib, name)
             fn.restype = restype
             fn.argtypes = list(argtypes)

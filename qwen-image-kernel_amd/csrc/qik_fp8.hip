@@ -40,8 +40,12 @@
 #include <vector>
 
 #include "qik_fp8.h"
+#include "qik_host.h"
 
 namespace qik_fp8 {
+
+using qik_host::host_e4m3fn;
+using qik_host::host_elem;
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
@@ -1339,54 +1343,6 @@ int launch_split(GemmParams& p, const qik_fp8_gemm_args* a, bool fp16, hipStream
 // multiplies by the fp32 reciprocal of 448 instead, which is what the device
 // quantiser reproduces).  Elementwise, so any thread split gives the same
 // bytes.
-
-// exact fp32 value of element i of a bf16 / fp16 / fp32 host array
-inline float host_elem(const void* w, int32_t dtype, int64_t i) {
-  if (dtype == QIK_DTYPE_FP32) return static_cast<const float*>(w)[i];
-  const uint16_t h = static_cast<const uint16_t*>(w)[i];
-  uint32_t bits;
-  if (dtype == QIK_DTYPE_BF16) {
-    bits = (uint32_t)h << 16;
-  } else {
-    // binary16: 1 sign, 5 exponent bits (bias 15), 10 mantissa bits
-    const uint32_t sign = (uint32_t)(h & 0x8000u) << 16;
-    const uint32_t e = (h >> 10) & 0x1fu, m = h & 0x3ffu;
-    if (e == 0x1f) {
-      bits = sign | 0x7f800000u | (m << 13);
-    } else if (e != 0) {
-      bits = sign | ((e + 112u) << 23) | (m << 13);
-    } else {
-      // zero or subnormal: m * 2^-24, exact in fp32
-      const float f = (float)m * 5.9604644775390625e-8f;
-      memcpy(&bits, &f, 4);
-      bits |= sign;
-    }
-  }
-  float f;
-  memcpy(&f, &bits, 4);
-  return f;
-}
-
-// e4m3fn code of q (|q| <= 448 or NaN), round to nearest even; NaN keeps its
-// sign bit (0x7f / 0xff), and a magnitude that rounds past 448 is NaN (the
-// format has no infinity)
-inline unsigned char host_e4m3fn(float q) {
-  uint32_t u;
-  memcpy(&u, &q, 4);
-  const unsigned char sign = (unsigned char)((u >> 24) & 0x80u);
-  const uint32_t a = u & 0x7fffffffu;
-  if (a >= 0x43e80000u) return sign | 0x7f;  // NaN, or |q| >= 464 (= 448 + half a step)
-  if (a < 0x3c800000u) {
-    // below 2^-6: subnormal codes m * 2^-9, m = round_even(|q| * 512) (exact scaling)
-    float fa;
-    memcpy(&fa, &a, 4);
-    return sign | (unsigned char)std::nearbyint(fa * 512.0f);
-  }
-  // normal: keep 3 mantissa bits with round-to-nearest-even at bit 20, then
-  // move the exponent from bias 127 to bias 7
-  const uint32_t r = a + 0x7ffffu + ((a >> 20) & 1u);
-  return sign | (unsigned char)((r >> 20) - (120u << 3));
-}
 
 int host_quantize_weight(const void* w, int32_t dtype, int64_t n, unsigned char* out, float* scale_out,
                          int32_t threads) {

@@ -14,6 +14,10 @@ the input dtype.  Differences from the reference, both on the safe side:
   instead of being copied to a contiguous tensor first (triton_fused.py:84-85);
 * ``1 / sqrt`` is taken in fp64 and rounded once to fp32 (the reference uses the
   approximate fp32 ``rsqrt``), and every fp32 operation rounds on its own.
+
+``fused_residual_rms_norm`` is the norm between a layer's linears: the residual
+added, RMSNorm over the last dimension, the result in the element type or
+microscaled for ``MXFP4Linear`` (qik_residual_rms_norm, include/qik_mx.h).
 """
 
 from __future__ import annotations
@@ -23,8 +27,11 @@ import ctypes
 import torch
 
 from . import _lib
+from .mx import _DTYPES as _NORM_DTYPES
+from .mx import MX_FORMATS, MXTensor, _as_rows, _check_format, _check_width, _CODE_DTYPE, _code_shape, _on_device, \
+    _row_stride, _scales_shape
 
-__all__ = ["fused_rms_norm_rope"]
+__all__ = ["fused_rms_norm_rope", "fused_residual_rms_norm"]
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 
@@ -177,3 +184,72 @@ def rms_rope_args(x, weight, cos, sin, out, eps) -> _lib.QikRmsRopeArgs:
     a.stride_out = _lib._i64x3(out.stride(0), out.stride(1), out.stride(2))
     a.eps = float(eps)
     return a
+
+
+_MAX_NORM_WIDTH = 32768
+
+
+def fused_residual_rms_norm(
+    x: torch.Tensor,                   # [..., D] bf16, fp16 or fp32
+    residual: torch.Tensor | None,     # x's shape and dtype, or None
+    weight: torch.Tensor,              # [D] fp32, or x's dtype
+    eps: float,
+    out_format: str | None = None,     # None, "mxfp8" or "mxfp4"
+):
+    """RMSNorm over the last dimension of ``h = x + residual``.
+
+    Returns ``(out, h)``, or ``out`` alone where residual is None (h is x).  h
+    is rounded to x's dtype, and the norm is of the rounded h: ``y = (h * r) *
+    weight`` in fp32 with ``r = 1 / sqrt(mean(h^2) + eps)`` taken in fp64 and
+    rounded to fp32.  ``out`` is y rounded to x's dtype, or with ``out_format`` y
+    in that microscaled format (an MXTensor, D a multiple of 32), with no
+    rounding in between.  Asynchronous on the current stream; records no
+    gradients."""
+    fmt = _lib.MX_NONE if out_format is None else MX_FORMATS[_check_format(out_format)]
+    if x.dtype not in _NORM_DTYPES:
+        raise ValueError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    if not x.is_cuda:
+        raise ValueError("x must be a device tensor (the kernel runs on the GPU)")
+    D = x.shape[-1]
+    if not 1 <= D <= _MAX_NORM_WIDTH:
+        raise ValueError(f"the last dimension must be 1 to {_MAX_NORM_WIDTH}, got {D}")
+    if fmt:
+        _check_width(D)
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError(f"residual must be {tuple(x.shape)} {x.dtype} on {x.device}, "
+                         f"got {tuple(residual.shape)} {residual.dtype} on {residual.device}")
+    if weight.shape != (D,) or weight.device != x.device:
+        raise ValueError(f"weight must be [{D}] on {x.device}, got {tuple(weight.shape)} on {weight.device}")
+    if weight.dtype != torch.float32 and weight.dtype != x.dtype:
+        raise ValueError(f"weight must be fp32 or {x.dtype}, got {weight.dtype}")
+    x2 = _norm_rows(x, fmt)
+    r2 = None if residual is None else _norm_rows(residual, fmt)
+    if not weight.is_contiguous() or (fmt and weight.data_ptr() % 16 != 0):
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    M = x2.shape[0]
+    h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    scales = None
+    if fmt:
+        out = torch.empty(_code_shape(x.shape, out_format), dtype=_CODE_DTYPE[out_format], device=x.device)
+        scales = torch.empty(_scales_shape(M, D), dtype=torch.uint8, device=x.device)
+    else:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    a = _lib.QikResidualRmsNormArgs(
+        _lib.ABI_VERSION, _NORM_DTYPES[x.dtype], fmt, _NORM_DTYPES[weight.dtype], x2.data_ptr(),
+        None if r2 is None else r2.data_ptr(), weight.data_ptr(), None if h is None else h.data_ptr(), out.data_ptr(),
+        None if scales is None else scales.data_ptr(), M, D, _row_stride(x2), D if r2 is None else _row_stride(r2),
+        float(eps))
+    _on_device(x.device, _lib.load().qik_residual_rms_norm, "qik_residual_rms_norm", ctypes.byref(a))
+    if fmt:
+        out = MXTensor._make(out, scales, out_format, x.shape)
+    return out if residual is None else (out, h)
+
+
+def _norm_rows(t: torch.Tensor, fmt: int) -> torch.Tensor:
+    """t as rows; a microscaled output reads them in 16-byte vectors, so rows at other addresses are copied."""
+    t2 = _as_rows(t)
+    if fmt and (t2.data_ptr() % 16 != 0 or (t2.shape[0] > 1 and t2.stride(0) * t2.element_size() % 16 != 0)):
+        t2 = t2.clone(memory_format=torch.contiguous_format)
+    return t2

@@ -1,0 +1,457 @@
+"""Microscaled (MX) tensors and the 4-bit linear beside ``FP8Linear``.
+
+``quantize_mx`` turns rows into MXFP4 (E2M1 elements, two to a byte) or MXFP8
+(E4M3 elements) with one power-of-two scale byte (E8M0) per 32 elements, as an
+``MXTensor``; ``MXTensor.dequantize`` gives the values back.  ``mx_linear``
+multiplies microscaled rows by an MXFP4 weight on gfx950's scaled matrix
+instructions, and ``MXFP4Linear`` is the ``nn.Linear`` made of it: it quantises
+its input (or takes an ``MXTensor``, such as ``fused_residual_rms_norm`` writes)
+and multiplies.  The device work is behind include/qik_mx.h, asynchronously on
+the current stream.  None of it records gradients.
+
+A block's scale is ``2^(e - 127)`` with ``e = max(E - emax, 0)``, E the fp32
+exponent field of the block's largest magnitude and emax 2 (MXFP4) or 8
+(MXFP8); its elements are ``x / scale`` rounded to nearest even and saturated at
+6 or 448.  An infinity or NaN makes its block's scale 255, and the values NaN.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import weakref
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+
+__all__ = ["MXTensor", "quantize_mx", "mx_linear", "MXFP4Linear", "convert_linears_mxfp4"]
+
+MX_BLOCK = 32
+MX_FORMATS = {"mxfp4": _lib.MXFP4, "mxfp8": _lib.MXFP8}
+_CODE_DTYPE = {"mxfp4": torch.uint8, "mxfp8": torch.float8_e4m3fn}
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
+_OUT_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
+_MAX_K = 262144
+
+# scratch of the linears and K-split products, one per (device index, stream): see _workspace
+_WS: dict = {}
+
+
+def _check_format(fmt: str) -> str:
+    if fmt not in MX_FORMATS:
+        raise ValueError(f"format must be one of {sorted(MX_FORMATS)}, got {fmt!r}")
+    return fmt
+
+
+def _check_width(K: int) -> None:
+    if K < MX_BLOCK or K % MX_BLOCK != 0 or K > _MAX_K:
+        raise ValueError(f"the last dimension must be a multiple of {MX_BLOCK} up to {_MAX_K}, got {K}")
+
+
+def _scales_shape(M: int, K: int) -> tuple[int, int, int]:
+    return (M + 31) // 32, (K + 255) // 256, 256
+
+
+def _code_shape(shape, fmt: str) -> tuple[int, ...]:
+    return (*shape[:-1], shape[-1] // 2 if fmt == "mxfp4" else shape[-1])
+
+
+def _rows(shape) -> int:
+    n = 1
+    for s in shape[:-1]:
+        n *= s
+    return n
+
+
+class MXTensor:
+    """Rows in a microscaled format.
+
+    ``shape`` and ``fmt`` ("mxfp4" or "mxfp8") say what it stands for;
+    ``codes`` holds the elements (uint8 ``[..., K / 2]``, the even element in
+    the low half; or float8_e4m3fn ``[..., K]``) and ``scales`` the scale bytes
+    in the layout the product reads: uint8 ``[ceil(M / 32), ceil(K / 256),
+    256]`` over the M rows, byte ``(m % 32) * 8 + b % 8`` of ``[m // 32, b //
+    8]`` for block b of row m, padding 0.  ``block_scales`` gives them as
+    ``[..., K / 32]``; ``from_block_scales`` takes them so.
+    """
+
+    __slots__ = ("codes", "scales", "fmt", "shape")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str):
+        _check_format(fmt)
+        if codes.dim() < 1 or codes.dtype != _CODE_DTYPE[fmt]:
+            raise ValueError(f"{fmt} codes must be {_CODE_DTYPE[fmt]}, got {codes.dtype}")
+        K = codes.shape[-1] * (2 if fmt == "mxfp4" else 1)
+        _check_width(K)
+        self.shape = torch.Size((*codes.shape[:-1], K))
+        if not codes.is_contiguous() or codes.data_ptr() % 16 != 0:
+            codes = codes.clone(memory_format=torch.contiguous_format)
+        want = _scales_shape(_rows(self.shape), K)
+        if scales.dtype != torch.uint8 or tuple(scales.shape) != want:
+            raise ValueError(f"scales must be uint8 {want}, got {scales.dtype} {tuple(scales.shape)}")
+        if scales.device != codes.device:
+            raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
+        if not scales.is_contiguous() or scales.data_ptr() % 16 != 0:
+            scales = scales.clone(memory_format=torch.contiguous_format)
+        self.codes, self.scales, self.fmt = codes, scales, fmt
+
+    @staticmethod
+    def _make(codes, scales, fmt, shape) -> "MXTensor":
+        t = MXTensor.__new__(MXTensor)
+        t.codes, t.scales, t.fmt, t.shape = codes, scales, fmt, shape
+        return t
+
+    @staticmethod
+    def from_block_scales(codes: torch.Tensor, block_scales: torch.Tensor, fmt: str) -> "MXTensor":
+        """From codes and one scale byte per block, uint8 ``[..., K / 32]`` (a checkpoint's, say)."""
+        _check_format(fmt)
+        K = codes.shape[-1] * (2 if fmt == "mxfp4" else 1) if codes.dim() else 0
+        _check_width(K)
+        if block_scales.dtype != torch.uint8 or tuple(block_scales.shape) != (*codes.shape[:-1], K // MX_BLOCK):
+            raise ValueError(f"block scales must be uint8 {(*codes.shape[:-1], K // MX_BLOCK)}, "
+                             f"got {block_scales.dtype} {tuple(block_scales.shape)}")
+        M = _rows((*codes.shape[:-1], K))
+        R, C, _ = _scales_shape(M, K)
+        full = torch.zeros((R * 32, C * 8), dtype=torch.uint8, device=block_scales.device)
+        full[:M, :K // MX_BLOCK] = block_scales.reshape(M, K // MX_BLOCK)
+        scales = full.view(R, 32, C, 8).transpose(1, 2).contiguous().view(R, C, 256)
+        return MXTensor(codes, scales, fmt)
+
+    def block_scales(self) -> torch.Tensor:
+        """The scale byte of each block, uint8 ``[..., K / 32]``."""
+        K = self.shape[-1]
+        M = _rows(self.shape)
+        R, C, _ = self.scales.shape
+        full = self.scales.view(R, C, 32, 8).transpose(1, 2).reshape(R * 32, C * 8)
+        return full[:M, :K // MX_BLOCK].reshape(*self.shape[:-1], K // MX_BLOCK)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def to(self, device) -> "MXTensor":
+        return MXTensor._make(self.codes.to(device), self.scales.to(device), self.fmt, self.shape)
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The values, ``element * 2^(e - 127)`` rounded once to dtype (bf16, fp16 or fp32; exact in bf16 and fp32)."""
+        if dtype not in _DTYPES:
+            raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
+        if not self.codes.is_cuda:
+            raise ValueError("dequantize runs on a HIP device; move the tensor there first")
+        out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
+        a = _lib.QikMxDequantArgs(_lib.ABI_VERSION, _DTYPES[dtype], MX_FORMATS[self.fmt], 0, self.codes.data_ptr(),
+                                  self.scales.data_ptr(), out.data_ptr(), _rows(self.shape), self.shape[-1])
+        _on_device(out.device, _lib.load().qik_mx_dequantize, "qik_mx_dequantize", ctypes.byref(a))
+        return out
+
+    def __repr__(self) -> str:
+        return f"MXTensor({tuple(self.shape)}, fmt={self.fmt!r}, device={str(self.device)!r})"
+
+
+def _on_device(dev: torch.device, fn, name: str, *args) -> None:
+    """fn(*args, current stream of dev) with dev current."""
+    idx = dev.index
+    if idx != torch.cuda.current_device():
+        with torch.cuda.device(idx):
+            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(idx)), name)
+    else:
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(idx)), name)
+
+
+def _as_rows(x: torch.Tensor) -> torch.Tensor:
+    """x as [M, K] with unit element stride and rows that do not overlap (a copy where it has another layout)."""
+    K = x.shape[-1]
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    if (x2.stride(1) != 1 and K > 1) or (x2.shape[0] > 1 and x2.stride(0) < K):
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2
+
+
+def _row_stride(x2: torch.Tensor) -> int:
+    return max(x2.stride(0), x2.shape[1])  # a single row's stride says nothing
+
+
+def quantize_mx(x: torch.Tensor, fmt: str = "mxfp4") -> MXTensor:
+    """x ``[..., K]`` (bf16, fp16 or fp32; K a multiple of 32) in a microscaled format.
+
+    A CPU tensor is quantised on the CPU by the library's host routine, to the
+    same bytes, so that a model can be converted on a machine without a GPU."""
+    _check_format(fmt)
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    if not x.is_cuda and x.device.type != "cpu":
+        raise ValueError(f"quantize_mx takes a HIP or CPU tensor, got {x.device}")
+    K = x.shape[-1]
+    _check_width(K)
+    x2 = _as_rows(x)
+    M = x2.shape[0]
+    codes = torch.empty(_code_shape(x.shape, fmt), dtype=_CODE_DTYPE[fmt], device=x.device)
+    scales = torch.empty(_scales_shape(M, K), dtype=torch.uint8, device=x.device)
+    a = _lib.QikMxQuantArgs(_lib.ABI_VERSION, _DTYPES[x.dtype], MX_FORMATS[fmt], 0, x2.data_ptr(), codes.data_ptr(),
+                            scales.data_ptr(), M, K, _row_stride(x2))
+    if x.is_cuda:
+        _on_device(x.device, _lib.load().qik_mx_quantize, "qik_mx_quantize", ctypes.byref(a))
+    else:
+        _lib.check(_lib.load().qik_mx_quantize_host(ctypes.byref(a), torch.get_num_threads()), "qik_mx_quantize_host")
+    return MXTensor._make(codes, scales, fmt, x.shape)
+
+
+def _workspace(dev: torch.device, stream: int, nbytes: int):
+    """Scratch of at least nbytes on this stream (None for 0).  One per (device,
+    stream), grown as needed: calls on one stream run in order, so they share
+    it.  Under graph capture a fresh one from the graph's pool, so that two
+    graphs replayed on different streams never share memory."""
+    if nbytes <= 0:
+        return None
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    key = (dev.index, stream)
+    ws = _WS.get(key)
+    if ws is None or ws.numel() < nbytes:
+        if len(_WS) >= 64:
+            _WS.clear()
+        ws = _WS[key] = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return ws
+
+
+def _gemm_args(a_fmt: str, w_codes, w_scales, bias, out_dtype, M: int, N: int, K: int) -> _lib.QikMxGemmArgs:
+    return _lib.QikMxGemmArgs(_lib.ABI_VERSION, _OUT_DTYPES[out_dtype], MX_FORMATS[a_fmt], 0, None, None,
+                              w_codes.data_ptr(), w_scales.data_ptr(), None if bias is None else bias.data_ptr(), None,
+                              M, N, K, K // 2 if a_fmt == "mxfp4" else K, K // 2, N)
+
+
+def mx_linear(
+    a: MXTensor,                        # [..., K]
+    w: MXTensor,                        # [N, K], mxfp4
+    bias: torch.Tensor | None = None,   # [N]
+    out_dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """``round(a . w^T + bias)``, ``[..., N]``: the values multiplied exactly, summed in fp32, rounded once."""
+    if not isinstance(a, MXTensor) or not isinstance(w, MXTensor):
+        raise ValueError("mx_linear takes MXTensor operands (quantize_mx makes them)")
+    if w.fmt != "mxfp4" or len(w.shape) != 2:
+        raise ValueError(f"the weight must be mxfp4 [N, K], got {w.fmt} {tuple(w.shape)}")
+    if a.shape[-1] != w.shape[1]:
+        raise ValueError(f"shapes {tuple(a.shape)} and {tuple(w.shape)} do not multiply as A . W^T")
+    if out_dtype not in _OUT_DTYPES:
+        raise ValueError(f"out_dtype must be bf16 or fp16, got {out_dtype}")
+    dev = a.codes.device
+    if not a.codes.is_cuda:
+        raise ValueError("mx_linear runs on a HIP device; move the operands there first")
+    N, K = w.shape
+    for name, t in (("w", w.codes), ("bias", bias)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} must be on {dev}")
+    if bias is not None:
+        if bias.numel() != N:
+            raise ValueError(f"bias must have {N} elements, got {bias.numel()}")
+        bias = bias.reshape(-1).to(out_dtype).contiguous()
+    M = _rows(a.shape)
+    out = torch.empty((*a.shape[:-1], N), dtype=out_dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    g = _gemm_args(a.fmt, w.codes, w.scales, bias, out_dtype, M, N, K)
+    g.a, g.a_scales, g.out = a.codes.data_ptr(), a.scales.data_ptr(), out.data_ptr()
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        need = ctypes.c_int64(0)
+        _lib.check(lib.qik_mx_gemm_workspace_size(ctypes.byref(g), ctypes.byref(need)), "qik_mx_gemm")
+        stream = torch._C._cuda_getCurrentRawStream(dev.index)
+        ws = _workspace(dev, stream, need.value)
+        _lib.check(lib.qik_mx_gemm(ctypes.byref(g), None if ws is None else ws.data_ptr(), need.value, stream),
+                   "qik_mx_gemm")
+    return out
+
+
+class _LinearCall:
+    """What one MXFP4Linear input geometry needs at call time: the argument
+    struct without the addresses of x and the output, and weak references to
+    the buffers it was made for (with their addresses), so that it is used only
+    while the module still holds exactly them and never keeps them alive."""
+
+    __slots__ = ("args", "index", "shape", "ws_bytes", "refs", "addresses", "copy", "cast_bias")
+
+    def matches(self, weight, scales, bias) -> bool:
+        r = self.refs
+        if r[0]() is not weight or r[1]() is not scales:
+            return False
+        if (r[2] is None) != (bias is None) or (bias is not None and r[2]() is not bias):
+            return False
+        return self.addresses == (weight.data_ptr(), scales.data_ptr(), None if bias is None else bias.data_ptr())
+
+
+class MXFP4Linear(nn.Module):
+    """``nn.Linear`` with an MXFP4 weight and microscaled activations.
+
+    ``forward`` takes a tensor (bf16, fp16 or fp32 ``[..., in_features]``), which
+    it quantises to ``activations`` ("mxfp4": both operands in 4 bits, the
+    matrix cores' fastest form; "mxfp8": 8-bit activations, closer to the
+    input), or an ``MXTensor`` of either format.  The result has the input's
+    dtype, bf16 for an ``MXTensor``; it is summed in fp32 and rounded to bf16
+    once.  Buffers: ``weight`` uint8 ``[out, in / 2]``, ``weight_scale`` uint8
+    ``[ceil(out / 32), ceil(in / 256), 256]`` (the layout of
+    ``MXTensor.scales``), ``bias`` bf16 ``[out]`` or None.  ``in_features`` is a
+    multiple of 32."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = False, activations: str = "mxfp4"):
+        super().__init__()
+        _check_width(in_features)
+        if out_features < 1:
+            raise ValueError(f"out_features must be at least 1, got {out_features}")
+        self.in_features = in_features
+        self.out_features = out_features
+        self.activations = _check_format(activations)
+        self.register_buffer("weight", torch.zeros(out_features, in_features // 2, dtype=torch.uint8))
+        self.register_buffer("weight_scale", torch.zeros(_scales_shape(out_features, in_features), dtype=torch.uint8))
+        if bias:
+            self.register_buffer("bias", torch.zeros(out_features, dtype=torch.bfloat16))
+        else:
+            self.bias = None
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, "
+                f"activations={self.activations}")
+
+    def mx_weight(self) -> MXTensor:
+        """The weight as an MXTensor on the module's buffers."""
+        return MXTensor(self.weight, self.weight_scale, "mxfp4")
+
+    def forward(self, x) -> torch.Tensor:
+        if isinstance(x, MXTensor):
+            return mx_linear(x, self.mx_weight(), self.bias)
+        weight, scales, bias = self.weight, self.weight_scale, self.bias
+        key = (x.shape, x.stride(), x.dtype, x.device, self.activations)
+        calls = self.__dict__.get("_calls")
+        if calls is None:
+            calls = self.__dict__["_calls"] = {}
+        ent = calls.get(key)
+        if ent is None or not ent.matches(weight, scales, bias):
+            ent = self._prepare(x, weight, scales, bias)
+            if len(calls) >= 8:
+                calls.clear()
+            calls[key] = ent
+        out = torch.empty(ent.shape, dtype=torch.bfloat16, device=x.device)
+        if ent.args is not None:
+            idx = ent.index
+            if idx != torch.cuda.current_device():
+                with torch.cuda.device(idx):
+                    self._launch(ent, x, out, idx)
+            else:
+                self._launch(ent, x, out, idx)
+        return out if x.dtype == torch.bfloat16 else out.to(x.dtype)
+
+    def _launch(self, ent: _LinearCall, x, out, idx: int) -> None:
+        stream = torch._C._cuda_getCurrentRawStream(idx)
+        x2 = _as_rows(x) if ent.copy else x
+        a = _lib.QikMxLinearArgs.from_buffer_copy(ent.args)
+        a.x = x2.data_ptr()
+        a.g.out = out.data_ptr()
+        if ent.cast_bias:  # the module was moved to another dtype
+            bias = self.bias.to(torch.bfloat16).contiguous()
+            a.g.bias = bias.data_ptr()
+        ws = _workspace(x.device, stream, ent.ws_bytes)
+        _lib.check(_lib.load().qik_mx_linear(ctypes.byref(a), None if ws is None else ws.data_ptr(), ent.ws_bytes,
+                                             stream), "qik_mx_linear")
+
+    def _prepare(self, x, weight, scales, bias) -> _LinearCall:
+        """Checks and the argument struct of one input geometry."""
+        N, K = self.out_features, self.in_features
+        if x.dtype not in _DTYPES:
+            raise ValueError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
+        if x.dim() < 1 or x.shape[-1] != K:
+            raise ValueError(f"x must be [..., {K}], got {tuple(x.shape)}")
+        if not x.is_cuda:
+            raise ValueError("MXFP4Linear runs on a HIP device; move its input and the module there first")
+        for name, t, shape in (("weight", weight, (N, K // 2)), ("weight_scale", scales, _scales_shape(N, K)),
+                               ("bias", bias, (N,))):
+            if t is None:
+                continue
+            if t.device != x.device:
+                raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+            if tuple(t.shape) != shape or (name != "bias" and (t.dtype != torch.uint8 or not t.is_contiguous()
+                                                               or t.data_ptr() % 16 != 0)):
+                raise ValueError(f"{name} must be {shape}{'' if name == 'bias' else ' contiguous uint8, 16-byte aligned'}, "
+                                 f"got {t.dtype} {tuple(t.shape)}")
+        c = _LinearCall()
+        c.index = x.device.index
+        c.shape = (*x.shape[:-1], N)
+        c.refs = (weakref.ref(weight), weakref.ref(scales), None if bias is None else weakref.ref(bias))
+        c.addresses = (weight.data_ptr(), scales.data_ptr(), None if bias is None else bias.data_ptr())
+        c.args, c.ws_bytes = None, 0
+        c.cast_bias = bias is not None and (bias.dtype != torch.bfloat16 or not bias.is_contiguous())
+        x2 = _as_rows(x)
+        # a view of x with x's own address needs no work per call
+        c.copy = x2.data_ptr() != x.data_ptr()
+        M = x2.shape[0]
+        if M == 0:
+            return c
+        a = _lib.QikMxLinearArgs(_gemm_args(self.activations, weight, scales, bias, torch.bfloat16, M, N, K),
+                                 x2.data_ptr(), _row_stride(x2), _DTYPES[x.dtype], 0)
+        a.g.out = x2.data_ptr()  # any address: the size does not go by it
+        need = ctypes.c_int64(0)
+        with torch.cuda.device(x.device):
+            _lib.check(_lib.load().qik_mx_linear_workspace_size(ctypes.byref(a), ctypes.byref(need)), "qik_mx_linear")
+        c.args, c.ws_bytes = a, need.value
+        return c
+
+    def _apply(self, fn, recurse=True):
+        # .to() / .cuda() replace the buffers: drop the launch cache
+        self.__dict__.pop("_calls", None)
+        return super()._apply(fn, recurse)
+
+    def __getstate__(self):
+        # copies and pickles carry the buffers, not the launch cache (ctypes
+        # structs of device addresses)
+        state = super().__getstate__()
+        state.pop("_calls", None)
+        return state
+
+    @staticmethod
+    def from_quantized(weight: MXTensor, bias: torch.Tensor | None = None, activations: str = "mxfp4") -> "MXFP4Linear":
+        """From an MXFP4 weight ``[out, in]`` and a bias; the module takes the weight's buffers as they are."""
+        if not isinstance(weight, MXTensor) or weight.fmt != "mxfp4" or len(weight.shape) != 2:
+            raise ValueError("the weight must be an mxfp4 MXTensor [out, in]")
+        N, K = weight.shape
+        if bias is not None and tuple(bias.shape) != (N,):
+            raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
+        mod = MXFP4Linear.__new__(MXFP4Linear)
+        nn.Module.__init__(mod)
+        mod.in_features, mod.out_features, mod.activations = K, N, _check_format(activations)
+        mod.register_buffer("weight", weight.codes)
+        mod.register_buffer("weight_scale", weight.scales)
+        if bias is not None:
+            mod.register_buffer("bias", bias.detach().to(device=weight.device, dtype=torch.bfloat16).clone())
+        else:
+            mod.bias = None
+        return mod
+
+    @staticmethod
+    def from_linear(linear: nn.Linear, activations: str = "mxfp4") -> "MXFP4Linear":
+        """Convert a loaded nn.Linear (weights on the CPU or a HIP device)."""
+        w = linear.weight.data
+        w = w if w.dtype in _DTYPES else w.float()
+        bias = None if linear.bias is None else linear.bias.data
+        return MXFP4Linear.from_quantized(quantize_mx(w, "mxfp4"), bias, activations)
+
+
+def convert_linears_mxfp4(module: nn.Module, skip_patterns: tuple[str, ...] = (), prefix: str = "",
+                          activations: str = "mxfp4") -> list[str]:
+    """Replace every nn.Linear below `module` whose in_features is a multiple of
+    32 with MXFP4Linear in place; returns the converted names, skipping names
+    that contain a skip pattern (the counterpart of convert_linears_fp8)."""
+    _check_format(activations)
+    converted = []
+    for name, child in list(module.named_children()):
+        full = f"{prefix}.{name}" if prefix else name
+        if any(p in full for p in skip_patterns):
+            continue
+        if isinstance(child, nn.Linear):
+            if child.in_features % MX_BLOCK == 0 and MX_BLOCK <= child.in_features <= _MAX_K:
+                setattr(module, name, MXFP4Linear.from_linear(child, activations))
+                converted.append(full)
+        else:
+            converted.extend(convert_linears_mxfp4(child, skip_patterns, full, activations))
+    return converted
