@@ -2,6 +2,12 @@
 // MXFP4, on the scaled matrix instructions v_mfma_scale_f32_*_f8f6f4, which
 // multiply each block of 32 by its two power-of-two scales as they sum it.
 //
+// Many rows (`tile_kernel`): a workgroup computes a BM x BN tile of out^T = W .
+// A^T (first operand weight rows n, second activation rows m, so that a lane
+// ends with 4 consecutive n of one row m per register quad).  Codes and scales
+// reach LDS directly, two to four stages in flight, and the fragments of the
+// next k-step are read while the matrix cores run on the current ones.
+//
 // Few rows (`rows_kernel`): every wave takes 16 weight rows and a share of K,
 // loads the codes straight into registers and meets the others of its
 // workgroup in LDS.  It is bound by the weight's bytes.
@@ -11,15 +17,20 @@
 #include <string.h>
 #include <limits.h>
 #include <algorithm>
+#include <type_traits>
 
 #include "qik_mx.h"
+#include "qik_tile.h"
 
 namespace qik_mx {
+
+using namespace qik_tile;
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int FMT_E4M3 = 0, FMT_E2M1 = 4;  // the instruction's operand formats
 
@@ -32,6 +43,9 @@ struct MxGemmParams {
   char* out;
   int M, N, K, C;  // C = ceil(K / 256)
   int64_t lda, ldw, ldc;
+  // tiles only
+  int ntm, ntn, group_m;  // tiles along m and n; tile rows per group of the tile order
+  bool vec;               // out's rows are at multiples of 16 bytes
 };
 
 template <bool FP16>
@@ -48,6 +62,333 @@ __device__ __forceinline__ float widen16(unsigned short h) {
 
 __device__ __forceinline__ i32x8 operand(u32x4 lo, u32x4 hi) {
   return i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+}
+
+// ---------------------------------------------------------------------------
+// Tiles
+// ---------------------------------------------------------------------------
+
+// Tile shape BM x BN, WGM x WGN waves, NS stages.  A stage holds 128 bytes of
+// every A row (256 k of MXFP4, 128 of MXFP8), the W codes of the same k (128 or
+// 64 bytes a row), and of every 32 rows the 256 bytes of scales of the 256 k
+// around them.
+template <int BM_, int BN_, int WGM_, int WGN_, int NS_, bool A8_>
+struct Tile {
+  static constexpr bool A8 = A8_;
+  static constexpr int BM = BM_, BN = BN_, NS = NS_;
+  static constexpr int WGM = WGM_, WGN = WGN_;        // waves along m and n
+  static constexpr int NW = WGM * WGN, NT = 64 * NW;
+  static constexpr int WM = BM / WGM, WN = BN / WGN;  // wave tile
+  static constexpr int MI = WM / 32, NJ = WN / 32;
+  static constexpr int KV = A8 ? 128 : 256;           // k of a stage
+  static constexpr int KS = KV / 64;                  // MFMA k-steps of a stage
+  static constexpr int RA = 128, RW = A8 ? 64 : 128;  // bytes of a stage's row
+  static constexpr int W_AT = BM * RA;                // stage: A codes, W codes, A scales, W scales
+  static constexpr int S_AT = W_AT + BN * RW;
+  static constexpr int SBLK = (BM + BN) / 32;
+  static constexpr int STAGE = S_AT + SBLK * 256;
+  static constexpr int AI = BM * RA / (1024 * NW);    // 1 KiB copies per wave and stage
+  static constexpr int WI = BN * RW / (1024 * NW);
+  static constexpr int SI = (SBLK + NW - 1) / NW;     // 256-byte copies
+  static constexpr int COPIES = AI + WI + SI;
+  static_assert(NW == 4 || NW == 8, "one or two waves per SIMD");
+  static_assert(NS >= 2 && (NS - 1) * COPIES < 64, "the prologue's copies fit the vmcnt field");
+  static_assert(NS * STAGE <= 160 * 1024, "the stages fit LDS");
+  static_assert(AI * 1024 * NW == BM * RA && WI * 1024 * NW == BN * RW, "whole copies per wave");
+  static_assert(MI * 32 == WM && NJ * 32 == WN, "whole MFMA blocks per wave");
+  static_assert((BN & (BN - 1)) == 0, "the output staging's swizzle needs a power of two");
+  static_assert(BM * BN * 2 <= NS * STAGE, "the output tile fits the stages");
+};
+
+// Origin of the tile of workgroup bx (bx % 8 is its XCD): XCD x takes a
+// contiguous run of the tile order, which walks group_m tile rows at a time, so
+// that one XCD's L2 serves a compact block of tiles.  False for a padding
+// workgroup.
+template <class T>
+__device__ __forceinline__ bool tile_origin(const MxGemmParams& p, const int bx, int& m0, int& n0) {
+  const int tiles = p.ntm * p.ntn;
+  const int x = bx & 7, s = bx >> 3;
+  const int q = tiles >> 3, r = tiles & 7;
+  if (s >= q + (x < r ? 1 : 0)) return false;
+  const int t = x * q + min(x, r) + s;
+  const int full = p.group_m * p.ntn;
+  const int g = t / full;
+  const int first = g * p.group_m;
+  const int gm = min(p.group_m, p.ntm - first);
+  const int tr = t - g * full;
+  m0 = (first + tr % gm) * T::BM;
+  n0 = (tr / gm) * T::BN;
+  return true;
+}
+
+// The tile's outputs, staged through LDS (the stages, once every copy has
+// landed and every wave is done with them) so that a store writes whole rows:
+// staged row ml keeps its 16-byte chunk c at c ^ (ml % CPR), which spreads a
+// fragment's 32 rows over the banks.  Rows of out at other than multiples of 16
+// bytes, and the last columns of an N that is no multiple of 8, are stored an
+// element at a time.
+template <class T, bool FP16>
+__device__ __forceinline__ void store_tile(const MxGemmParams& p, const int m0, const int n0,
+                                           const f32x16 (&acc)[T::NJ][T::MI], unsigned char* lds, const int wave,
+                                           const int lane) {
+  const int wm = wave % T::WGM, wn = wave / T::WGM;
+  constexpr int RB = T::BN * 2;  // bytes of a staged row
+  constexpr int CPR = RB / 16;   // 16-byte chunks per row
+  constexpr int RPI = 64 / CPR;  // rows per store instruction
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < T::NJ; ++j) {
+#pragma unroll
+    for (int qd = 0; qd < 4; ++qd) {
+      const int nl = wn * T::WN + j * 32 + qd * 8 + (lane >> 5) * 4;
+      float bv[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        bv[e] = p.bias != nullptr && n0 + nl + e < p.N
+                    ? widen16<FP16>(reinterpret_cast<const unsigned short*>(p.bias)[n0 + nl + e])
+                    : 0.0f;
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i) {
+        const int ml = wm * T::WM + i * 32 + (lane & 31);
+        unsigned short y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = round16<FP16>(acc[j][i][qd * 4 + e] + bv[e]);
+        const u32x2 o = {(unsigned)y[0] | (unsigned)y[1] << 16, (unsigned)y[2] | (unsigned)y[3] << 16};
+        *reinterpret_cast<u32x2*>(lds + ml * RB + ((nl >> 3) ^ (ml & (CPR - 1))) * 16 + (lane >> 5) * 8) = o;
+      }
+    }
+  }
+  __syncthreads();
+  const int c = lane % CPR;
+  const int n = n0 + c * 8;
+#pragma unroll 4
+  for (int r0 = wave * RPI; r0 < T::BM; r0 += T::NW * RPI) {
+    const int ml = r0 + lane / CPR;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(lds + ml * RB + ((c ^ (ml & (CPR - 1))) * 16));
+    const int m = m0 + ml;
+    if (m >= p.M) continue;
+    char* o = p.out + (m * p.ldc + n) * 2;
+    if (p.vec && n + 8 <= p.N) {
+      *reinterpret_cast<u32x4*>(o) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (n + e < p.N) reinterpret_cast<unsigned short*>(o)[e] = (unsigned short)(v[e / 2] >> (16 * (e % 2)));
+    }
+  }
+}
+
+// One BM x BN tile.  In LDS the 16-byte chunk c of a 128-byte row r sits at
+// chunk c ^ (r / 2) % 8, of a 64-byte row at c ^ (r / 4) % 4: a fragment read
+// (16 lanes on 16 consecutive rows, one chunk each) then touches all 64 banks
+// once, and a 1 KiB copy writes one contiguous KiB.
+//
+// The matrix instruction is 32x32x64: lane l of a wave holds row l % 32.  Which
+// k of memory a lane's k of an instruction stand for is free as long as both
+// operands and the scales agree.  MXFP4: lane half h = l / 32 takes block 4 h +
+// s of the stage's 8 at k-step s, so its four scales are four consecutive bytes
+// and the instruction picks byte s.  With MXFP8 activations an E4M3 lane holds
+// two runs of 16 k, h and 2 + h of the step's four, its scale that of block h;
+// half h takes W's block 2 s + h and shifts its scale bytes down by h.
+template <class T, bool FP16>
+__global__ void __launch_bounds__(T::NT) __attribute__((amdgpu_waves_per_eu(T::NW / 4, T::NW / 4)))
+tile_kernel(const MxGemmParams p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[T::NS * T::STAGE];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform: copy targets go to SGPRs
+  const int wm = wave % T::WGM, wn = wave / T::WGM;
+  int m0, n0;
+  if (!tile_origin<T>(p, blockIdx.x, m0, n0)) return;
+  const int mrows = min(T::BM, p.M - m0), nrows = min(T::BN, p.N - n0);
+
+  // copies: one of A fills 8 rows (lane l: row l / 8, chunk l % 8), one of W 8
+  // rows of 128 bytes or 16 of 64, one of scales the 256 bytes of 32 rows.  The
+  // rows of a wave's copies are a multiple of 16 apart, so one chunk serves all.
+  const int arow = wave * 8 + (lane >> 3);
+  const int achunk = ((lane & 7) ^ ((arow >> 1) & 7)) * 16;
+  const int wrow = T::A8 ? wave * 16 + (lane >> 2) : arow;
+  const int wchunk = T::A8 ? ((lane & 3) ^ ((wrow >> 2) & 3)) * 16 : achunk;
+  constexpr int WROWS = 1024 / T::RW;  // rows of a copy of W
+  uint32_t aoff[T::AI], woff[T::WI];
+#pragma unroll
+  for (int i = 0; i < T::AI; ++i) aoff[i] = (uint32_t)((arow + 8 * T::NW * i) * (int)p.lda + achunk);
+#pragma unroll
+  for (int i = 0; i < T::WI; ++i) woff[i] = (uint32_t)((wrow + WROWS * T::NW * i) * (int)p.ldw + wchunk);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
+  const unsigned char* abase = p.a + (int64_t)m0 * p.lda;
+  const unsigned char* wbase = p.w + (int64_t)n0 * p.ldw;
+  const int group = p.C * 256;  // bytes of a row group's scales
+  const unsigned char* asbase = p.as + (int64_t)(m0 / 32) * group;
+  const unsigned char* wsbase = p.ws + (int64_t)(n0 / 32) * group;
+  const int agroups = (mrows + 31) / 32, wgroups = (nrows + 31) / 32;
+  const int nk = (p.K + T::KV - 1) / T::KV;
+
+  // The copies of one step: past the end of K a lane's chunk would read the
+  // next row, so its offset gets the top bit (out of range: zeros); a step at
+  // or past the end gets empty resources, so that every step issues the same
+  // copies and the waits stay uniform.
+  struct Step {
+    u32x4 ra, rw, sa, sw;
+    uint32_t st;
+    uint32_t adead, wdead;
+  };
+  auto prepare = [&](const int kt, const int stage) __attribute__((always_inline)) {
+    Step sc;
+    const int ka = kt * T::RA, kw = kt * T::RW, ks = (T::A8 ? kt >> 1 : kt) * 256;
+    const int la = (T::A8 ? p.K : p.K / 2) - ka, lw = p.K / 2 - kw;
+    const bool in = kt < nk;
+    sc.ra = rsrc_words(abase + ka, in ? (uint32_t)((mrows - 1) * (int)p.lda + min(T::RA, la)) : 0u);
+    sc.rw = rsrc_words(wbase + kw, in ? (uint32_t)((nrows - 1) * (int)p.ldw + min(T::RW, lw)) : 0u);
+    sc.sa = rsrc_words(asbase + ks, in ? (uint32_t)(agroups * group - ks) : 0u);
+    sc.sw = rsrc_words(wsbase + ks, in ? (uint32_t)(wgroups * group - ks) : 0u);
+    sc.st = lds0 + (uint32_t)(stage * T::STAGE);
+    sc.adead = (la < T::RA && achunk >= la) ? 0x80000000u : 0u;
+    sc.wdead = (lw < T::RW && wchunk >= lw) ? 0x80000000u : 0u;
+    return sc;
+  };
+  auto issue = [&](const Step& sc, const int i) __attribute__((always_inline)) {
+    if (i < T::AI) {
+      dma16(sc.ra, sc.st + (uint32_t)((wave + T::NW * i) * 1024), aoff[i] | sc.adead);
+    } else if (i < T::AI + T::WI) {
+      const int k = i - T::AI;
+      dma16(sc.rw, sc.st + (uint32_t)(T::W_AT + (wave + T::NW * k) * 1024), woff[k] | sc.wdead);
+    } else {
+      // the surplus waves of the last round copy the last group again
+      const int b = min(wave + T::NW * (i - T::AI - T::WI), T::SBLK - 1);
+      const bool of_a = b < T::BM / 32;
+      const uint32_t off = (uint32_t)((of_a ? b : b - T::BM / 32) * group + lane * 4);
+      dma4(of_a ? sc.sa : sc.sw, sc.st + (uint32_t)(T::S_AT + b * 256), off);
+    }
+  };
+
+  // fragment reads: lane l reads row l % 32 of a 32-row block
+  const int frow = lane & 31, half = lane >> 5;
+  constexpr int ACH = T::A8 ? 2 : 1;  // chunks of an A fragment
+  uint32_t fa_off[T::KS][ACH], fw_off[T::KS];
+#pragma unroll
+  for (int s = 0; s < T::KS; ++s) {
+    const int c0 = T::A8 ? 4 * s + half : 4 * half + s;
+    fa_off[s][0] = (uint32_t)(frow * 128 + ((c0 ^ ((frow >> 1) & 7)) * 16));
+    if constexpr (T::A8) fa_off[s][ACH - 1] = (uint32_t)(frow * 128 + (((c0 + 2) ^ ((frow >> 1) & 7)) * 16));
+    fw_off[s] = T::A8 ? (uint32_t)(frow * 64 + (((2 * s + half) ^ ((frow >> 2) & 3)) * 16)) : fa_off[s][0];
+  }
+  const uint32_t sc_off = (uint32_t)(T::S_AT + frow * 8 + (T::A8 ? 0 : half * 4));
+
+  u32x4 fa[2][T::MI][ACH], fw[2][T::NJ];
+  int sa[T::MI], sw[T::NJ], nsa[T::MI], nsw[T::NJ];
+  constexpr int NRD = T::MI * ACH + T::NJ;  // reads of a k-step's fragments
+  constexpr int NSR = T::MI + T::NJ;        // reads of a stage's scales
+  auto read_frag = [&](const int stage, const int s, const int r, const int buf) __attribute__((always_inline)) {
+    const unsigned char* st = lds + stage * T::STAGE;
+    if (r < T::MI * ACH) {
+      const int f = r / ACH;
+      fa[buf][f][r % ACH] = *reinterpret_cast<const u32x4*>(st + (wm * T::WM + f * 32) * T::RA + fa_off[s][r % ACH]);
+    } else {
+      const int f = r - T::MI * ACH;
+      fw[buf][f] = *reinterpret_cast<const u32x4*>(st + T::W_AT + (wn * T::WN + f * 32) * T::RW + fw_off[s]);
+    }
+  };
+  auto read_scale = [&](const int stage, const int odd, const int r) __attribute__((always_inline)) {
+    const int b = r < T::MI ? wm * T::MI + r : T::BM / 32 + wn * T::NJ + r - T::MI;
+    const unsigned char* at = lds + stage * T::STAGE + b * 256 + sc_off;
+    const int v = *reinterpret_cast<const int*>(at + (T::A8 ? odd * 4 : 0));
+    if (r < T::MI) nsa[r] = v;
+    else nsw[r - T::MI] = v;
+  };
+  auto take_scales = [&]() __attribute__((always_inline)) {
+    const int sh = T::A8 ? 8 * half : 0;
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i) sa[i] = T::A8 ? (int)((unsigned)nsa[i] >> sh) : nsa[i];
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) sw[j] = T::A8 ? (int)((unsigned)nsw[j] >> sh) : nsw[j];
+  };
+
+  f32x16 acc[T::NJ][T::MI];
+#pragma unroll
+  for (int j = 0; j < T::NJ; ++j)
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i) acc[j][i] = f32x16{};
+
+  // prologue: every stage in flight, stage 0 published, its first fragments read
+#pragma unroll
+  for (int s0 = 0; s0 < T::NS; ++s0) {
+    const Step sc = prepare(s0, s0);
+#pragma unroll
+    for (int c = 0; c < T::COPIES; ++c) issue(sc, c);
+  }
+  wait_vmcnt<(T::NS - 1) * T::COPIES>();
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < NRD; ++r) read_frag(0, 0, r, 0);
+#pragma unroll
+  for (int r = 0; r < NSR; ++r) read_scale(0, 0, r);
+
+  // k-step S of a stage on fragments S % 2, with the reads of the next k-step
+  // into the others between its MFMAs.  The last one (COPY) issues its first
+  // PRE MFMAs before the wait for the next stage's copies and the barrier,
+  // which publishes that stage and releases this one (every wave has read all
+  // of it; the barrier's LDS fence waits for those reads), then the reads of
+  // the next stage and the copies of the stage after next into this one's
+  // memory.
+  constexpr int NMF = T::NJ * T::MI;
+  constexpr int PRE = 2 < NMF ? 2 : 1;
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  auto kstep = [&](auto s_tag, const int stage, const int next, const int next_odd, const Step& sc)
+      __attribute__((always_inline)) {
+    constexpr int S = decltype(s_tag)::value;
+    constexpr bool COPY = S == T::KS - 1;
+    constexpr int cur = S % 2;
+    constexpr int OP = T::A8 ? 2 * S : S;  // the scale's byte
+    // reads (and copies) after MFMAs [R0, R0 + H)
+    constexpr int R0 = COPY ? (NMF > PRE ? PRE : PRE - 1) : 0;
+    constexpr int H = COPY ? NMF - R0 : (NMF >= 2 ? NMF / 2 : 1);
+    constexpr int RD = NRD + (COPY ? NSR : 0);
+#pragma unroll
+    for (int idx = 0; idx < NMF; ++idx) {
+      const int j = idx / T::MI, i = idx % T::MI;
+      acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+          operand(fw[cur][j], zero), operand(fa[cur][i][0], T::A8 ? fa[cur][i][ACH - 1] : zero), acc[j][i], FMT_E2M1,
+          T::A8 ? FMT_E4M3 : FMT_E2M1, OP, sw[j], OP, sa[i]);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (COPY) {
+        if (idx == PRE - 1) {
+          wait_vmcnt<(T::NS - 2) * T::COPIES>();  // the next stage's copies have landed
+          __syncthreads();
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (idx >= R0 && idx < R0 + H) {
+#pragma unroll
+        for (int r = (idx - R0) * RD / H; r < (idx - R0 + 1) * RD / H; ++r) {
+          if (r < NRD) read_frag(COPY ? next : stage, COPY ? 0 : S + 1, r, cur ^ 1);
+          else read_scale(next, next_odd, r - NRD);
+        }
+        if constexpr (COPY) {
+#pragma unroll
+          for (int c = (idx - R0) * T::COPIES / H; c < (idx - R0 + 1) * T::COPIES / H; ++c) issue(sc, c);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  int st = 0;  // stage of step kt
+  for (int kt = 0; kt < nk; ++kt) {
+    const Step none = {};
+    const int nst = st + 1 == T::NS ? 0 : st + 1;
+    take_scales();
+    kstep(std::integral_constant<int, 0>{}, st, nst, 0, none);
+    if constexpr (T::KS == 4) {
+      kstep(std::integral_constant<int, 1>{}, st, nst, 0, none);
+      kstep(std::integral_constant<int, 2>{}, st, nst, 0, none);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const Step sc = prepare(kt + T::NS, st);
+    kstep(std::integral_constant<int, T::KS - 1>{}, st, nst, (kt + 1) & 1, sc);
+    st = nst;
+  }
+  wait_vmcnt<0>();  // the copies of the steps past the end still land in their stages
+  store_tile<T, FP16>(p, m0, n0, acc, lds, wave, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -212,6 +553,7 @@ MxGemmParams gemm_params(const qik_mx_gemm_args* a) {
   p.lda = a->lda;
   p.ldw = a->ldw;
   p.ldc = a->ldc;
+  p.vec = aligned_to(a->out, 16) && a->ldc % 8 == 0;
   return p;
 }
 
@@ -226,11 +568,82 @@ int launch_rows(MxGemmParams& p, hipStream_t s) {
              : QIK_ERR_LAUNCH;
 }
 
+// tile rows per group of the tile order: the group size that minimises the
+// bytes one XCD's run of tiles reads (its distinct A row blocks + W row blocks)
+int choose_group_m(int ntm, int ntn, int abytes, int wbytes) {
+  const int64_t per_xcd = std::max<int64_t>(1, ((int64_t)ntm * ntn + 7) / 8);
+  int best = 1;
+  double best_bytes = 1e300;
+  for (int gm = 1; gm <= std::min(ntm, 16); ++gm) {
+    const int64_t rows = std::min<int64_t>(gm, per_xcd);
+    const int64_t cols = std::min<int64_t>(ntn, (per_xcd + gm - 1) / gm);
+    const double bytes = (double)rows * abytes + (double)cols * wbytes;
+    if (bytes < best_bytes) {
+      best_bytes = bytes;
+      best = gm;
+    }
+  }
+  return best;
+}
+
+template <class T, bool FP16>
+int launch_tiles(MxGemmParams& p, hipStream_t s) {
+  const int64_t ntm = cdiv(p.M, T::BM), ntn = cdiv(p.N, T::BN);
+  const int64_t grid = cdiv(ntm * ntn, 8) * 8;
+  if (grid > (int64_t)INT_MAX / 2) return QIK_ERR_SHAPE;
+  p.ntm = (int)ntm;
+  p.ntn = (int)ntn;
+  p.group_m = choose_group_m(p.ntm, p.ntn, T::BM * T::RA, T::BN * T::RW);
+  void* args[] = {&p};
+  return hipLaunchKernel((const void*)tile_kernel<T, FP16>, dim3((unsigned)grid), dim3(T::NT), args, 0, s) == hipSuccess
+             ? QIK_OK
+             : QIK_ERR_LAUNCH;
+}
+
+enum { T256x256, T256x128, T128x256, T128x128, T64x128, T64x64, NSHAPES };
+struct TileShape {
+  int bm, bn;
+  double t0, t1;  // us of a tile: t0 + t1 per stage
+};
+static const TileShape kShapes[NSHAPES] = {{256, 256, 6.0, 1.5},   {256, 128, 6.0, 0.775}, {128, 256, 6.0, 0.81},
+                                           {128, 128, 4.6, 0.485}, {64, 128, 3.8, 0.32},   {64, 64, 3.8, 0.215}};
+
+int choose_shape(int64_t M, int64_t N, int64_t steps) {
+  int best = 0;
+  double best_t = 1e300;
+  for (int i = 0; i < NSHAPES; ++i) {
+    const TileShape& t = kShapes[i];
+    const int64_t rounds = cdiv(cdiv(cdiv(M, t.bm) * cdiv(N, t.bn), 8), 32);
+    const double us = (double)rounds * (t.t0 + t.t1 * (double)steps);
+    if (us < best_t) {
+      best_t = us;
+      best = i;
+    }
+  }
+  return best;
+}
+
+template <bool A8, bool FP16>
+int launch_shape(MxGemmParams& p, hipStream_t s) {
+  switch (choose_shape(p.M, p.N, cdiv(p.K, A8 ? 128 : 256))) {
+    case T256x256: return launch_tiles<Tile<256, 256, 2, 4, A8 ? 3 : 2, A8>, FP16>(p, s);
+    case T256x128: return launch_tiles<Tile<256, 128, 2, 4, 3, A8>, FP16>(p, s);
+    case T128x256: return launch_tiles<Tile<128, 256, 2, 4, 3, A8>, FP16>(p, s);
+    case T128x128: return launch_tiles<Tile<128, 128, 2, 4, A8 ? 4 : 3, A8>, FP16>(p, s);
+    case T64x128: return launch_tiles<Tile<64, 128, 1, 4, 4, A8>, FP16>(p, s);
+    default: return launch_tiles<Tile<64, 64, 2, 2, 4, A8>, FP16>(p, s);
+  }
+}
+
 int launch_gemm(const qik_mx_gemm_args* a, hipStream_t s) {
   MxGemmParams p = gemm_params(a);
   const bool fp16 = a->out_dtype == QIK_DTYPE_FP16;
-  if (a->a_format == QIK_MXFP8) return fp16 ? launch_rows<true, true>(p, s) : launch_rows<true, false>(p, s);
-  return fp16 ? launch_rows<false, true>(p, s) : launch_rows<false, false>(p, s);
+  if (p.M <= 32) {
+    if (a->a_format == QIK_MXFP8) return fp16 ? launch_rows<true, true>(p, s) : launch_rows<true, false>(p, s);
+    return fp16 ? launch_rows<false, true>(p, s) : launch_rows<false, false>(p, s);
+  }
+  if (a->a_format == QIK_MXFP8) return fp16 ? launch_shape<true, true>(p, s) : launch_shape<true, false>(p, s);
+  return fp16 ? launch_shape<false, true>(p, s) : launch_shape<false, false>(p, s);
 }
 
 inline int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
