@@ -60,21 +60,6 @@ typedef _Float16 f16x2 __attribute__((__vector_size__(2 * sizeof(_Float16))));
 
 inline bool aligned_to(const void* ptr, uintptr_t a) { return (reinterpret_cast<uintptr_t>(ptr) % a) == 0; }
 
-// CUs of the current device (0 if the runtime cannot say), cached per device
-int device_cus() {
-  static int cache[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess) return 0;
-  if (dev >= 0 && dev < 64) {
-    const int c = __atomic_load_n(&cache[dev], __ATOMIC_RELAXED);
-    if (c > 0) return c;
-  }
-  int cus = 0;
-  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
-  if (dev >= 0 && dev < 64) __atomic_store_n(&cache[dev], cus, __ATOMIC_RELAXED);
-  return cus;
-}
-
 // ---------------------------------------------------------------------------
 // Quantiser
 // ---------------------------------------------------------------------------
@@ -522,13 +507,11 @@ __global__ void __launch_bounds__(QT) dequant_kernel(const unsigned char* w, con
 // ---------------------------------------------------------------------------
 
 // A range of output columns computed with one tile shape.
-struct GemmRegion {
+struct GemmRegion : TileRun {
   const unsigned char* w;  // weight row of the region's first column
   const char* bias;        // its first bias element, or null
   char* out;               // its first output column
   int N;                   // columns in the region
-  int ntm, ntn;            // tiles along m and n
-  int group_m;             // tile rows per group of the tile order
   int wgs;                 // workgroups: tiles rounded up to a multiple of 8
 };
 
@@ -582,27 +565,6 @@ struct CfgK128 {
   static_assert(MI * 32 == WM && NJ * 32 == WN, "whole MFMA blocks per wave");
   static_assert((BN & (BN - 1)) == 0, "the output staging's swizzle needs a power of two");
 };
-
-// Origin of the tile of workgroup bx of region rg (bx % 8 is the XCD: every
-// region starts at a multiple of 8): XCD x takes a contiguous run of the tile
-// order, which walks group_m tile rows at a time.  False for a padding
-// workgroup.
-template <class C>
-__device__ __forceinline__ bool tile_origin(const GemmRegion& rg, const int bx, int& m0, int& n0) {
-  const int T = rg.ntm * rg.ntn;
-  const int x = bx & 7, s = bx >> 3;
-  const int q = T >> 3, r = T & 7;
-  if (s >= q + (x < r ? 1 : 0)) return false;
-  const int t = x * q + min(x, r) + s;
-  const int gsz_full = rg.group_m * rg.ntn;
-  const int g = t / gsz_full;
-  const int first = g * rg.group_m;
-  const int gm = min(rg.group_m, rg.ntm - first);
-  const int tr = t - g * gsz_full;
-  m0 = (first + tr % gm) * C::BM;
-  n0 = (tr / gm) * C::BN;
-  return true;
-}
 
 template <class C, bool FP16>
 __device__ __forceinline__ void store_tile(const GemmParams& p, const GemmRegion& rg, const int m0, const int n0,
@@ -722,7 +684,7 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, const GemmRegion&
   const int wm = wave % C::WGM, wn = wave / C::WGM;
 
   int m0, n0;
-  if (!tile_origin<C>(rg, bx, m0, n0)) return;
+  if (!tile_origin(rg, C::BM, C::BN, bx, m0, n0)) return;
   const int mrows = min(C::BM, p.M - m0);
   const int nrows = min(C::BN, rg.N - n0);
 
@@ -1102,10 +1064,6 @@ typedef CfgK128<64, 64, 2, 2, 4> Cfg64x64;
 // to 4352 rows the plan they give is within 2% of the fastest of all tile shapes
 // and mixes measured there, on average 0.7% from it
 // (profiles/fp8_gemm_plan_candidates.md).
-struct TileShape {
-  int bm, bn;
-  double t0, t1;
-};
 enum { T256x256, T256x128, T128x128, T192x128, T192x256, T128x256, T64x128, T64x64, NSHAPES };
 static const TileShape kShapes[NSHAPES] = {{256, 256, 6.0, 1.5},   {256, 128, 6.0, 0.775}, {128, 128, 4.6, 0.485},
                                            {192, 128, 4.6, 0.67},  {192, 256, 4.5, 1.23},   {128, 256, 6.0, 0.81},
@@ -1116,50 +1074,11 @@ constexpr int NPAIRS = 6;
 static const int kPairs[NPAIRS][2] = {{T256x256, T256x128}, {T256x128, T128x128}, {T192x128, T128x128},
                                       {T192x256, T192x128}, {T128x256, T128x128}, {T64x128, T64x64}};
 
-inline double tile_time(int shape, int64_t steps) { return kShapes[shape].t0 + kShapes[shape].t1 * (double)steps; }
 
-inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t steps_of(int64_t K) { return cdiv(K, 128); }  // 128-k-byte steps
 
-// Finish time of one XCD whose P CUs run t1 tiles of time d1 and then t2
-// tiles of time d2, one workgroup per CU (a workgroup of these tiles holds
-// a CU's four SIMDs), each started on the CU that frees first.
-double xcd_makespan(int64_t t1, double d1, int64_t t2, double d2, int64_t P) {
-  const int64_t full = t1 / P, rem = t1 % P;
-  const double a = (double)full * d1, b = a + d1;  // CUs free after t1: P - rem at a, rem at b
-  const int64_t na = P - rem, nb = rem;
-  const double end1 = nb > 0 ? b : a;
-  if (t2 == 0) return end1;
-  // the j-th tile of t2 starts at the j-th smallest of {a + k d2} (na times
-  // each) and {b + k d2} (nb times each)
-  int64_t ka = 0, kb = 0, placed = 0;
-  double last = a;
-  while (placed < t2) {
-    const double ta = a + (double)ka * d2, tb = nb > 0 ? b + (double)kb * d2 : 1e300;
-    if (ta <= tb) {
-      last = ta;
-      placed += na;
-      ++ka;
-    } else {
-      last = tb;
-      placed += nb;
-      ++kb;
-    }
-  }
-  return std::max(end1, last + d2);
-}
-
-// Columns [0, n1) with the pair's first tile shape, [n1, N) with its second.
-struct GemmPlan {
-  int pair;  // index into kPairs
-  int64_t n1;
-  double t;  // makespan from the tile times, us
-  bool small_first;  // launch the small tiles' region first (fp8_gemm_kernel)
-};
-
-// Estimated time of a launch whose busiest XCD of P CUs has `work` of tile time
-// and ends after `t`.  From 24 steps (K = 3072) on the matrix cores run long
-// enough that the clock follows the load: the tile times hold with three quarters of the CUs
+// The clock under load (TileTable): from 24 steps (K = 3072) on the matrix cores run long
+// enough that the clock follows it: the tile times hold with three quarters of the CUs
 // busy, and with all of them busy a tile takes 14% longer.  (Quantiser + GEMM,
 // the weights of six layers in turn: time / makespan from the tile times, the
 // median over 1100 launches of 1000 to 4352 rows with each plan forced, 0.90 at
@@ -1168,57 +1087,11 @@ struct GemmPlan {
 // mixes of smaller tiles win against fewer large ones that are faster: 4096 x
 // 3072 x 12288 (M x N x K) 143.8 us with 512 tiles of 256 x 128 and 128 x 128,
 // 137.3 with 192 of 256 x 256; 3456 x 3072 x 12288 130.2 and 117.1 (192 x 256).
-constexpr int64_t LONG_STEPS = 24;
-inline double launch_time(double t, double work, int64_t P, int64_t steps) {
-  return steps < LONG_STEPS ? t : t * (1.0 + 0.55 * std::max(0.0, work / (t * (double)P) - 0.75));
-}
+static const TileTable kTable = {kShapes, kPairs, NPAIRS, 24, 0.55, 0.75};
 
-// The split with the shortest estimated time on `cus` CUs.  Workgroups go
-// to the XCDs in turn, so the XCD that finishes last holds ceil(tiles / 8) of
-// each region.  The split points are whole big-tile columns; n1 = N is one
-// region of the big shape, n1 = 0 one of the small shape.  A later candidate
-// replaces an earlier one only if it is estimated faster by what the estimate
-// is good to (1%; 3% below LONG_STEPS); the first candidate is 256 x 256 tiles.
-GemmPlan choose_plan(int64_t M, int64_t N, int64_t K, int cus) {
-  const int64_t P = std::max(1, (cus > 0 ? cus : 256) / 8);
-  GemmPlan best = {0, N, 0.0, false};
-  double best_t = 1e300;
-  const int64_t steps = steps_of(K);
-  const double ahead = steps < LONG_STEPS ? 0.97 : 0.99;
-  for (int pr = 0; pr < NPAIRS; ++pr) {
-    const TileShape& s1 = kShapes[kPairs[pr][0]];
-    const TileShape& s2 = kShapes[kPairs[pr][1]];
-    const double d1 = tile_time(kPairs[pr][0], steps), d2 = tile_time(kPairs[pr][1], steps);
-    const int64_t rows1 = cdiv(M, s1.bm), rows2 = cdiv(M, s2.bm);
-    for (int64_t k = cdiv(N, s1.bn); k >= 0; --k) {
-      // no launch with a big tile ends before that tile: on to the small ones
-      // alone (a few rows into 9216 columns: 4.4 us of host time a call -> 0.2)
-      if (d1 >= best_t * ahead) k = 0;
-      const int64_t n1 = std::min(k * s1.bn, N);
-      const int64_t t1 = rows1 * k;
-      const int64_t t2 = rows2 * ((uint32_t)(N - n1 + s2.bn - 1) / (uint32_t)s2.bn);
-      // no order of the tiles ends before their total time shared by the CUs
-      const double work = (double)cdiv(t1, 8) * d1 + (double)cdiv(t2, 8) * d2;
-      if (launch_time(work / (double)P, work, P, steps) >= best_t * ahead) continue;
-      const double t = xcd_makespan(cdiv(t1, 8), d1, cdiv(t2, 8), d2, P);
-      const double est = launch_time(t, work, P, steps);
-      if (est < best_t * ahead) {
-        best_t = est;
-        best = {pr, n1, t, false};
-      }
-    }
-  }
-  // the small tiles first when that is estimated no slower (measured: 1-2%
-  // faster at 4352 x 9216 x 3072 and 4352 x 12288 x 3072, whose makespans are
-  // equal either way; 12% slower at 1543 x 9232 x 1104, whose is not)
-  const TileShape& s1 = kShapes[kPairs[best.pair][0]];
-  const TileShape& s2 = kShapes[kPairs[best.pair][1]];
-  const int64_t t1 = cdiv(M, s1.bm) * cdiv(best.n1, s1.bn);
-  const int64_t t2 = cdiv(M, s2.bm) * cdiv(N - best.n1, s2.bn);
-  if (t1 > 0 && t2 > 0)
-    best.small_first = xcd_makespan(cdiv(t2, 8), tile_time(kPairs[best.pair][1], steps), cdiv(t1, 8),
-                                    tile_time(kPairs[best.pair][0], steps), P) <= best.t * 1.0001;
-  return best;
+inline double tile_time(int shape, int64_t steps) { return kShapes[shape].time(steps); }
+inline GemmPlan choose_plan(int64_t M, int64_t N, int64_t K, int cus) {
+  return qik_tile::choose_plan(kTable, M, N, steps_of(K), cus);
 }
 
 // K-split of a launch with few tiles and a long K: S slices, each summing its
@@ -1248,25 +1121,6 @@ KSplit choose_ksplit(int64_t M, int64_t N, int64_t K, int cus) {
   if (S < 2) return {1, shape};
   const double t_split = tile_time(shape, cdiv(steps, S)) + 2.5 + (double)(S * M * N) * 4.0 / 5e6;
   return {t_split < 0.95 * choose_plan(M, N, K, cus).t ? S : 1, shape};
-}
-
-// tile rows per group of the tile order: the group size that minimises the
-// bytes one XCD's run of tiles reads (its distinct A row blocks + W row blocks)
-int choose_group_m(int ntm, int ntn, int bm, int bn) {
-  const int64_t T = (int64_t)ntm * ntn;
-  const int64_t per_xcd = std::max<int64_t>(1, (T + 7) / 8);
-  int best = 1;
-  double best_bytes = 1e300;
-  for (int gm = 1; gm <= std::min(ntm, 16); ++gm) {
-    const int64_t rows = std::min<int64_t>(gm, per_xcd);
-    const int64_t cols = std::min<int64_t>(ntn, (per_xcd + gm - 1) / gm);
-    const double bytes = (double)rows * bm + (double)cols * bn;
-    if (bytes < best_bytes) {
-      best_bytes = bytes;
-      best = gm;
-    }
-  }
-  return best;
 }
 
 // Region of columns [c0, c1) of the call with tile shape C.

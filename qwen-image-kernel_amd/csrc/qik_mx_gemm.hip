@@ -34,30 +34,41 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int FMT_E4M3 = 0, FMT_E2M1 = 4;  // the instruction's operand formats
 
+// A range of output columns computed with one tile shape.
+struct MxRegion : TileRun {
+  const unsigned char* w;   // weight row of the region's first column
+  const unsigned char* ws;  // its group of scales
+  const char* bias;         // its first bias element, or null
+  char* out;                // its first output column
+  int N;                    // columns in the region
+  int wgs;                  // workgroups: tiles rounded up to a multiple of 8
+};
+
 struct MxGemmParams {
   const unsigned char* a;
   const unsigned char* as;
-  const unsigned char* w;
-  const unsigned char* ws;
-  const char* bias;
-  char* out;
-  int M, N, K, C;  // C = ceil(K / 256)
-  int64_t lda, ldw, ldc;
-  // tiles only
-  int ntm, ntn, group_m;  // tiles along m and n; tile rows per group of the tile order
-  bool vec;               // out's rows are at multiples of 16 bytes
+  int M, K, C;      // C = ceil(K / 256)
+  int64_t lda, ldw;  // bytes
+  int64_t ldc;       // elements
+  bool fp16;         // type of bias and out
+  bool vec;          // out's rows are at multiples of 16 bytes
+  MxRegion r[2];     // columns [0, n1) with the larger tile, then [n1, N)
+  int small_first;   // 1: region 1's workgroups come first in blockIdx order
+  int ksplit;        // split launches: k-slices per tile (region 0 only)
+  float* partial;    // split launches: [ksplit][M][ldp] fp32 sums of each slice
+  int64_t ldp;       // N rounded up to 4
 };
 
-template <bool FP16>
-__device__ __forceinline__ unsigned short round16(float f) {
+// round to nearest even into bf16 or fp16
+__device__ __forceinline__ unsigned short round16(float f, bool fp16) {
   asm volatile("" : "+v"(f));  // an fp32 value: no mixed-precision fma rounds it
-  if constexpr (FP16) return __builtin_bit_cast(unsigned short, (_Float16)f);
-  else return __builtin_bit_cast(unsigned short, (__bf16)f);
+  return fp16 ? __builtin_bit_cast(unsigned short, (_Float16)f) : __builtin_bit_cast(unsigned short, (__bf16)f);
 }
-template <bool FP16>
-__device__ __forceinline__ float widen16(unsigned short h) {
-  if constexpr (FP16) return (float)__builtin_bit_cast(_Float16, h);
-  else return __uint_as_float((unsigned)h << 16);
+__device__ __forceinline__ float widen16(unsigned short h, bool fp16) {
+  return fp16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((unsigned)h << 16);
+}
+__device__ __forceinline__ float bias_at(const MxGemmParams& p, const MxRegion& rg, int n) {
+  return rg.bias != nullptr && n < rg.N ? widen16(reinterpret_cast<const unsigned short*>(rg.bias)[n], p.fp16) : 0.0f;
 }
 
 __device__ __forceinline__ i32x8 operand(u32x4 lo, u32x4 hi) {
@@ -72,8 +83,9 @@ __device__ __forceinline__ i32x8 operand(u32x4 lo, u32x4 hi) {
 // every A row (256 k of MXFP4, 128 of MXFP8), the W codes of the same k (128 or
 // 64 bytes a row), and of every 32 rows the 256 bytes of scales of the 256 k
 // around them.
-template <int BM_, int BN_, int WGM_, int WGN_, int NS_, bool A8_>
+template <int BM_, int BN_, int WGM_, int WGN_, int NS_, bool A8_, bool WS_>
 struct Tile {
+  static constexpr bool WS = WS_;  // fragments are read a whole stage at a time (gemm_tile)
   static constexpr bool A8 = A8_;
   static constexpr int BM = BM_, BN = BN_, NS = NS_;
   static constexpr int WGM = WGM_, WGN = WGN_;        // waves along m and n
@@ -100,35 +112,14 @@ struct Tile {
   static_assert(BM * BN * 2 <= NS * STAGE, "the output tile fits the stages");
 };
 
-// Origin of the tile of workgroup bx (bx % 8 is its XCD): XCD x takes a
-// contiguous run of the tile order, which walks group_m tile rows at a time, so
-// that one XCD's L2 serves a compact block of tiles.  False for a padding
-// workgroup.
-template <class T>
-__device__ __forceinline__ bool tile_origin(const MxGemmParams& p, const int bx, int& m0, int& n0) {
-  const int tiles = p.ntm * p.ntn;
-  const int x = bx & 7, s = bx >> 3;
-  const int q = tiles >> 3, r = tiles & 7;
-  if (s >= q + (x < r ? 1 : 0)) return false;
-  const int t = x * q + min(x, r) + s;
-  const int full = p.group_m * p.ntn;
-  const int g = t / full;
-  const int first = g * p.group_m;
-  const int gm = min(p.group_m, p.ntm - first);
-  const int tr = t - g * full;
-  m0 = (first + tr % gm) * T::BM;
-  n0 = (tr / gm) * T::BN;
-  return true;
-}
-
 // The tile's outputs, staged through LDS (the stages, once every copy has
 // landed and every wave is done with them) so that a store writes whole rows:
 // staged row ml keeps its 16-byte chunk c at c ^ (ml % CPR), which spreads a
 // fragment's 32 rows over the banks.  Rows of out at other than multiples of 16
 // bytes, and the last columns of an N that is no multiple of 8, are stored an
 // element at a time.
-template <class T, bool FP16>
-__device__ __forceinline__ void store_tile(const MxGemmParams& p, const int m0, const int n0,
+template <class T>
+__device__ __forceinline__ void store_tile(const MxGemmParams& p, const MxRegion& rg, const int m0, const int n0,
                                            const f32x16 (&acc)[T::NJ][T::MI], unsigned char* lds, const int wave,
                                            const int lane) {
   const int wm = wave % T::WGM, wn = wave / T::WGM;
@@ -143,16 +134,13 @@ __device__ __forceinline__ void store_tile(const MxGemmParams& p, const int m0, 
       const int nl = wn * T::WN + j * 32 + qd * 8 + (lane >> 5) * 4;
       float bv[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        bv[e] = p.bias != nullptr && n0 + nl + e < p.N
-                    ? widen16<FP16>(reinterpret_cast<const unsigned short*>(p.bias)[n0 + nl + e])
-                    : 0.0f;
+      for (int e = 0; e < 4; ++e) bv[e] = bias_at(p, rg, n0 + nl + e);
 #pragma unroll
       for (int i = 0; i < T::MI; ++i) {
         const int ml = wm * T::WM + i * 32 + (lane & 31);
         unsigned short y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = round16<FP16>(acc[j][i][qd * 4 + e] + bv[e]);
+        for (int e = 0; e < 4; ++e) y[e] = round16(acc[j][i][qd * 4 + e] + bv[e], p.fp16);
         const u32x2 o = {(unsigned)y[0] | (unsigned)y[1] << 16, (unsigned)y[2] | (unsigned)y[3] << 16};
         *reinterpret_cast<u32x2*>(lds + ml * RB + ((nl >> 3) ^ (ml & (CPR - 1))) * 16 + (lane >> 5) * 8) = o;
       }
@@ -167,18 +155,43 @@ __device__ __forceinline__ void store_tile(const MxGemmParams& p, const int m0, 
     const u32x4 v = *reinterpret_cast<const u32x4*>(lds + ml * RB + ((c ^ (ml & (CPR - 1))) * 16));
     const int m = m0 + ml;
     if (m >= p.M) continue;
-    char* o = p.out + (m * p.ldc + n) * 2;
-    if (p.vec && n + 8 <= p.N) {
+    char* o = rg.out + (m * p.ldc + n) * 2;
+    if (p.vec && n + 8 <= rg.N) {
       *reinterpret_cast<u32x4*>(o) = v;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (n + e < p.N) reinterpret_cast<unsigned short*>(o)[e] = (unsigned short)(v[e / 2] >> (16 * (e % 2)));
+        if (n + e < rg.N) reinterpret_cast<unsigned short*>(o)[e] = (unsigned short)(v[e / 2] >> (16 * (e % 2)));
     }
   }
 }
 
-// One BM x BN tile.  In LDS the 16-byte chunk c of a 128-byte row r sits at
+// The fp32 sums of one k-slice of a tile into p.partial, 4 columns of one row
+// per lane and register quad.
+template <class T>
+__device__ __forceinline__ void store_partial(const MxGemmParams& p, const MxRegion& rg, const int m0, const int n0,
+                                              const f32x16 (&acc)[T::NJ][T::MI], const int slice, const int wave,
+                                              const int lane) {
+  const int wm = wave % T::WGM, wn = wave / T::WGM;
+  float* dst = p.partial + (int64_t)slice * p.M * p.ldp;
+#pragma unroll
+  for (int j = 0; j < T::NJ; ++j) {
+#pragma unroll
+    for (int qd = 0; qd < 4; ++qd) {
+      const int n = n0 + wn * T::WN + j * 32 + qd * 8 + (lane >> 5) * 4;
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i) {
+        const int m = m0 + wm * T::WM + i * 32 + (lane & 31);
+        if (m < p.M && n < rg.N)
+          *reinterpret_cast<f32x4*>(dst + m * p.ldp + n) =
+              f32x4{acc[j][i][qd * 4], acc[j][i][qd * 4 + 1], acc[j][i][qd * 4 + 2], acc[j][i][qd * 4 + 3]};
+      }
+    }
+  }
+}
+
+// One BM x BN tile of region rg; bx counts the region's workgroups.  SPLIT: the
+// sums of slice `slice` of the stages, into p.partial.  In LDS the 16-byte chunk c of a 128-byte row r sits at
 // chunk c ^ (r / 2) % 8, of a 64-byte row at c ^ (r / 4) % 4: a fragment read
 // (16 lanes on 16 consecutive rows, one chunk each) then touches all 64 banks
 // once, and a 1 KiB copy writes one contiguous KiB.
@@ -190,17 +203,16 @@ __device__ __forceinline__ void store_tile(const MxGemmParams& p, const int m0, 
 // and the instruction picks byte s.  With MXFP8 activations an E4M3 lane holds
 // two runs of 16 k, h and 2 + h of the step's four, its scale that of block h;
 // half h takes W's block 2 s + h and shifts its scale bytes down by h.
-template <class T, bool FP16>
-__global__ void __launch_bounds__(T::NT) __attribute__((amdgpu_waves_per_eu(T::NW / 4, T::NW / 4)))
-tile_kernel(const MxGemmParams p) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[T::NS * T::STAGE];
+template <class T, bool SPLIT>
+__device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion& rg, const int bx, unsigned char* lds,
+                                          const int slice) {
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform: copy targets go to SGPRs
   const int wm = wave % T::WGM, wn = wave / T::WGM;
   int m0, n0;
-  if (!tile_origin<T>(p, blockIdx.x, m0, n0)) return;
-  const int mrows = min(T::BM, p.M - m0), nrows = min(T::BN, p.N - n0);
+  if (!tile_origin(rg, T::BM, T::BN, bx, m0, n0)) return;
+  const int mrows = min(T::BM, p.M - m0), nrows = min(T::BN, rg.N - n0);
 
   // copies: one of A fills 8 rows (lane l: row l / 8, chunk l % 8), one of W 8
   // rows of 128 bytes or 16 of 64, one of scales the 256 bytes of 32 rows.  The
@@ -217,12 +229,14 @@ tile_kernel(const MxGemmParams p) {
   for (int i = 0; i < T::WI; ++i) woff[i] = (uint32_t)((wrow + WROWS * T::NW * i) * (int)p.ldw + wchunk);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
   const unsigned char* abase = p.a + (int64_t)m0 * p.lda;
-  const unsigned char* wbase = p.w + (int64_t)n0 * p.ldw;
+  const unsigned char* wbase = rg.w + (int64_t)n0 * p.ldw;
   const int group = p.C * 256;  // bytes of a row group's scales
   const unsigned char* asbase = p.as + (int64_t)(m0 / 32) * group;
-  const unsigned char* wsbase = p.ws + (int64_t)(n0 / 32) * group;
+  const unsigned char* wsbase = rg.ws + (int64_t)(n0 / 32) * group;
   const int agroups = (mrows + 31) / 32, wgroups = (nrows + 31) / 32;
-  const int nk = (p.K + T::KV - 1) / T::KV;
+  const int nkall = (p.K + T::KV - 1) / T::KV;
+  const int kb = SPLIT ? (int)((int64_t)nkall * slice / p.ksplit) : 0;
+  const int nk = SPLIT ? (int)((int64_t)nkall * (slice + 1) / p.ksplit) : nkall;  // end of the stages
 
   // The copies of one step: past the end of K a lane's chunk would read the
   // next row, so its offset gets the top bit (out of range: zeros); a step at
@@ -275,18 +289,21 @@ tile_kernel(const MxGemmParams p) {
   }
   const uint32_t sc_off = (uint32_t)(T::S_AT + frow * 8 + (T::A8 ? 0 : half * 4));
 
-  u32x4 fa[2][T::MI][ACH], fw[2][T::NJ];
+  // fragments in two buffers, of a k-step each, or of a whole stage (T::WS)
+  constexpr int SLOTS = T::WS ? T::KS : 1;
+  u32x4 fa[2][SLOTS][T::MI][ACH], fw[2][SLOTS][T::NJ];
   int sa[T::MI], sw[T::NJ], nsa[T::MI], nsw[T::NJ];
   constexpr int NRD = T::MI * ACH + T::NJ;  // reads of a k-step's fragments
   constexpr int NSR = T::MI + T::NJ;        // reads of a stage's scales
   auto read_frag = [&](const int stage, const int s, const int r, const int buf) __attribute__((always_inline)) {
     const unsigned char* st = lds + stage * T::STAGE;
+    const int slot = T::WS ? s : 0;
     if (r < T::MI * ACH) {
       const int f = r / ACH;
-      fa[buf][f][r % ACH] = *reinterpret_cast<const u32x4*>(st + (wm * T::WM + f * 32) * T::RA + fa_off[s][r % ACH]);
+      fa[buf][slot][f][r % ACH] = *reinterpret_cast<const u32x4*>(st + (wm * T::WM + f * 32) * T::RA + fa_off[s][r % ACH]);
     } else {
       const int f = r - T::MI * ACH;
-      fw[buf][f] = *reinterpret_cast<const u32x4*>(st + T::W_AT + (wn * T::WN + f * 32) * T::RW + fw_off[s]);
+      fw[buf][slot][f] = *reinterpret_cast<const u32x4*>(st + T::W_AT + (wn * T::WN + f * 32) * T::RW + fw_off[s]);
     }
   };
   auto read_scale = [&](const int stage, const int odd, const int r) __attribute__((always_inline)) {
@@ -313,82 +330,196 @@ tile_kernel(const MxGemmParams p) {
   // prologue: every stage in flight, stage 0 published, its first fragments read
 #pragma unroll
   for (int s0 = 0; s0 < T::NS; ++s0) {
-    const Step sc = prepare(s0, s0);
+    const Step sc = prepare(kb + s0, s0);
 #pragma unroll
     for (int c = 0; c < T::COPIES; ++c) issue(sc, c);
   }
   wait_vmcnt<(T::NS - 1) * T::COPIES>();
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < NRD; ++r) read_frag(0, 0, r, 0);
+  for (int r = 0; r < SLOTS * NRD; ++r) read_frag(0, r / NRD, r % NRD, 0);
 #pragma unroll
-  for (int r = 0; r < NSR; ++r) read_scale(0, 0, r);
+  for (int r = 0; r < NSR; ++r) read_scale(0, kb & 1, r);
 
-  // k-step S of a stage on fragments S % 2, with the reads of the next k-step
-  // into the others between its MFMAs.  The last one (COPY) issues its first
-  // PRE MFMAs before the wait for the next stage's copies and the barrier,
-  // which publishes that stage and releases this one (every wave has read all
-  // of it; the barrier's LDS fence waits for those reads), then the reads of
-  // the next stage and the copies of the stage after next into this one's
-  // memory.
-  constexpr int NMF = T::NJ * T::MI;
-  constexpr int PRE = 2 < NMF ? 2 : 1;
+  constexpr int NMF = T::NJ * T::MI;  // MFMAs of a k-step
   const u32x4 zero = {0u, 0u, 0u, 0u};
-  auto kstep = [&](auto s_tag, const int stage, const int next, const int next_odd, const Step& sc)
-      __attribute__((always_inline)) {
+  auto mfma = [&](auto s_tag, const int idx, const int buf) __attribute__((always_inline)) {
     constexpr int S = decltype(s_tag)::value;
-    constexpr bool COPY = S == T::KS - 1;
-    constexpr int cur = S % 2;
     constexpr int OP = T::A8 ? 2 * S : S;  // the scale's byte
-    // reads (and copies) after MFMAs [R0, R0 + H)
-    constexpr int R0 = COPY ? (NMF > PRE ? PRE : PRE - 1) : 0;
-    constexpr int H = COPY ? NMF - R0 : (NMF >= 2 ? NMF / 2 : 1);
-    constexpr int RD = NRD + (COPY ? NSR : 0);
+    const int j = idx / T::MI, i = idx % T::MI, slot = T::WS ? S : 0;
+    acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+        operand(fw[buf][slot][j], zero), operand(fa[buf][slot][i][0], T::A8 ? fa[buf][slot][i][ACH - 1] : zero), acc[j][i],
+        FMT_E2M1, T::A8 ? FMT_E4M3 : FMT_E2M1, OP, sw[j], OP, sa[i]);
+  };
+
+  int st = 0;  // LDS stage of step kt
+  if constexpr (!T::WS) {
+    // k-step S of a stage on fragments S % 2, with the reads of the next k-step
+    // into the others between its MFMAs.  The last one (COPY) issues its first
+    // PRE MFMAs before the wait for the next stage's copies and the barrier,
+    // which publishes that stage and releases this one (every wave has read all
+    // of it; the barrier's LDS fence waits for those reads), then the reads of
+    // the next stage and the copies of the stage after next into this one's
+    // memory.
+    constexpr int PRE = 2 < NMF ? 2 : 1;
+    auto kstep = [&](auto s_tag, const int stage, const int next, const int next_odd, const Step& sc)
+        __attribute__((always_inline)) {
+      constexpr int S = decltype(s_tag)::value;
+      constexpr bool COPY = S == T::KS - 1;
+      // reads (and copies) after MFMAs [R0, R0 + H)
+      constexpr int R0 = COPY ? (NMF > PRE ? PRE : PRE - 1) : 0;
+      constexpr int H = COPY ? NMF - R0 : (NMF >= 2 ? NMF / 2 : 1);
+      constexpr int RD = NRD + (COPY ? NSR : 0);
 #pragma unroll
-    for (int idx = 0; idx < NMF; ++idx) {
-      const int j = idx / T::MI, i = idx % T::MI;
-      acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-          operand(fw[cur][j], zero), operand(fa[cur][i][0], T::A8 ? fa[cur][i][ACH - 1] : zero), acc[j][i], FMT_E2M1,
-          T::A8 ? FMT_E4M3 : FMT_E2M1, OP, sw[j], OP, sa[i]);
+      for (int idx = 0; idx < NMF; ++idx) {
+        mfma(s_tag, idx, S % 2);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (COPY) {
+          if (idx == PRE - 1) {
+            wait_vmcnt<(T::NS - 2) * T::COPIES>();  // the next stage's copies have landed
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        if (idx >= R0 && idx < R0 + H) {
+#pragma unroll
+          for (int r = (idx - R0) * RD / H; r < (idx - R0 + 1) * RD / H; ++r) {
+            if (r < NRD) read_frag(COPY ? next : stage, COPY ? 0 : S + 1, r, (S + 1) % 2);
+            else read_scale(next, next_odd, r - NRD);
+          }
+          if constexpr (COPY) {
+#pragma unroll
+            for (int c = (idx - R0) * T::COPIES / H; c < (idx - R0 + 1) * T::COPIES / H; ++c) issue(sc, c);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    for (int kt = kb; kt < nk; ++kt) {
+      const Step none = {};
+      const int nst = st + 1 == T::NS ? 0 : st + 1;
+      take_scales();
+      kstep(std::integral_constant<int, 0>{}, st, nst, 0, none);
+      if constexpr (T::KS == 4) {
+        kstep(std::integral_constant<int, 1>{}, st, nst, 0, none);
+        kstep(std::integral_constant<int, 2>{}, st, nst, 0, none);
+      }
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (COPY) {
-        if (idx == PRE - 1) {
-          wait_vmcnt<(T::NS - 2) * T::COPIES>();  // the next stage's copies have landed
-          __syncthreads();
+      const Step sc = prepare(kt + T::NS, st);
+      kstep(std::integral_constant<int, T::KS - 1>{}, st, nst, (kt + 1) & 1, sc);
+      st = nst;
+    }
+  } else {
+    // A tile of few MFMAs per k-step is bound by the latency of its fragment
+    // reads (about 130 cycles a k-step at one MFMA of 32), so a whole stage of
+    // fragments is read at a time, one stage ahead: all MFMAs of a stage run on
+    // registers, and the stage's memory is free for the copies of the stage NS
+    // later as soon as the barrier says that every wave has its fragments.
+    auto stage_step = [&](auto buf_tag, const int kt) __attribute__((always_inline)) {
+      constexpr int BUF = decltype(buf_tag)::value;
+      constexpr int TOTAL = T::KS * NMF;
+      constexpr int PRE = TOTAL / 4 < 2 ? 1 : 2;
+      constexpr int H = TOTAL - PRE;  // MFMAs with reads and copies beside them
+      constexpr int RD = T::KS * NRD + NSR;
+      const int nst = st + 1 == T::NS ? 0 : st + 1;
+      take_scales();
+      const Step sc = prepare(kt + T::NS, st);
+      auto run = [&](auto s_tag) __attribute__((always_inline)) {
+        constexpr int S = decltype(s_tag)::value;
+#pragma unroll
+        for (int i = 0; i < NMF; ++i) {
+          const int idx = S * NMF + i;
+          mfma(s_tag, i, BUF);
+          __builtin_amdgcn_sched_barrier(0);
+          if (idx == PRE - 1) {
+            wait_vmcnt<(T::NS - 2) * T::COPIES>();  // the next stage's copies have landed
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (idx >= PRE - 1 && idx < PRE - 1 + H) {
+            const int q = idx - (PRE - 1);
+#pragma unroll
+            for (int r = q * RD / H; r < (q + 1) * RD / H; ++r) {
+              if (r < T::KS * NRD) read_frag(nst, r / NRD, r % NRD, BUF ^ 1);
+              else read_scale(nst, (kt + 1) & 1, r - T::KS * NRD);
+            }
+#pragma unroll
+            for (int c = q * T::COPIES / H; c < (q + 1) * T::COPIES / H; ++c) issue(sc, c);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
+      };
+      run(std::integral_constant<int, 0>{});
+      run(std::integral_constant<int, 1>{});
+      if constexpr (T::KS == 4) {
+        run(std::integral_constant<int, 2>{});
+        run(std::integral_constant<int, 3>{});
       }
-      if (idx >= R0 && idx < R0 + H) {
-#pragma unroll
-        for (int r = (idx - R0) * RD / H; r < (idx - R0 + 1) * RD / H; ++r) {
-          if (r < NRD) read_frag(COPY ? next : stage, COPY ? 0 : S + 1, r, cur ^ 1);
-          else read_scale(next, next_odd, r - NRD);
-        }
-        if constexpr (COPY) {
-#pragma unroll
-          for (int c = (idx - R0) * T::COPIES / H; c < (idx - R0 + 1) * T::COPIES / H; ++c) issue(sc, c);
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      st = nst;
+    };
+    for (int kt = kb; kt < nk; kt += 2) {
+      stage_step(std::integral_constant<int, 0>{}, kt);
+      if (kt + 1 < nk) stage_step(std::integral_constant<int, 1>{}, kt + 1);
     }
-  };
-  int st = 0;  // stage of step kt
-  for (int kt = 0; kt < nk; ++kt) {
-    const Step none = {};
-    const int nst = st + 1 == T::NS ? 0 : st + 1;
-    take_scales();
-    kstep(std::integral_constant<int, 0>{}, st, nst, 0, none);
-    if constexpr (T::KS == 4) {
-      kstep(std::integral_constant<int, 1>{}, st, nst, 0, none);
-      kstep(std::integral_constant<int, 2>{}, st, nst, 0, none);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    const Step sc = prepare(kt + T::NS, st);
-    kstep(std::integral_constant<int, T::KS - 1>{}, st, nst, (kt + 1) & 1, sc);
-    st = nst;
   }
   wait_vmcnt<0>();  // the copies of the steps past the end still land in their stages
-  store_tile<T, FP16>(p, m0, n0, acc, lds, wave, lane);
+  if constexpr (SPLIT) store_partial<T>(p, rg, m0, n0, acc, slice, wave, lane);
+  else store_tile<T>(p, rg, m0, n0, acc, lds, wave, lane);
+}
+
+// Region 0 (T1 tiles) and region 1 (T2 tiles), one after the other in blockIdx
+// order; the smaller tiles fill the CUs that the big ones' last round leaves
+// free (small_first: the other way round, when it is estimated no slower).
+template <class T1, class T2>
+__global__ void __launch_bounds__(T1::NT) __attribute__((amdgpu_waves_per_eu(T1::NW / 4, T1::NW / 4)))
+tile_kernel(const MxGemmParams p) {
+  static_assert(T1::NT == T2::NT, "one workgroup size per launch");
+  constexpr int L1 = T1::NS * T1::STAGE, L2 = T2::NS * T2::STAGE;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[L1 > L2 ? L1 : L2];
+  const int bx = blockIdx.x;
+  const int off0 = p.small_first ? p.r[1].wgs : 0;  // first workgroup of each region
+  const int off1 = p.small_first ? 0 : p.r[0].wgs;
+  if (bx >= off0 && bx < off0 + p.r[0].wgs) gemm_tile<T1, false>(p, p.r[0], bx - off0, lds, 0);
+  else gemm_tile<T2, false>(p, p.r[1], bx - off1, lds, 0);
+}
+
+// Split launch: workgroup b sums slice b / wgs of tile b % wgs (wgs is a
+// multiple of 8, so a tile's slices run on one XCD).
+template <class T>
+__global__ void __launch_bounds__(T::NT) __attribute__((amdgpu_waves_per_eu(T::NW / 4, T::NW / 4)))
+split_kernel(const MxGemmParams p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[T::NS * T::STAGE];
+  const int wgs = p.r[0].wgs;
+  gemm_tile<T, true>(p, p.r[0], blockIdx.x % wgs, lds, blockIdx.x / wgs);
+}
+
+// out = round(the slices' sums in slice order + bias), 4 outputs per thread.
+__global__ void __launch_bounds__(256) join_kernel(const MxGemmParams p) {
+  const MxRegion& rg = p.r[0];
+  const int per_row = (int)(p.ldp / 4);
+  const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (g >= (int64_t)p.M * per_row) return;
+  const int m = (int)(g / per_row);
+  const int n = (int)(g - (int64_t)m * per_row) * 4;
+  const int64_t slice = (int64_t)p.M * p.ldp;
+  const float* src = p.partial + m * p.ldp + n;
+  f32x4 y = *reinterpret_cast<const f32x4*>(src);
+  for (int k = 1; k < p.ksplit; ++k) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(src + k * slice);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] += v[e];
+  }
+  unsigned short o[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = round16(y[e] + bias_at(p, rg, n + e), p.fp16);
+  unsigned short* to = reinterpret_cast<unsigned short*>(rg.out) + m * p.ldc + n;
+  if (p.vec && n + 4 <= rg.N) {
+    *reinterpret_cast<u32x2*>(to) = u32x2{(unsigned)o[0] | (unsigned)o[1] << 16, (unsigned)o[2] | (unsigned)o[3] << 16};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < rg.N) to[e] = o[e];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -403,11 +534,12 @@ tile_kernel(const MxGemmParams p) {
 
 constexpr int RK = 4;  // waves of a workgroup, each with its share of the 256-k chunks
 
-template <bool A8, int MB, int NB, bool FP16>
+template <bool A8, int MB, int NB>
 __global__ void __launch_bounds__(64 * RK) rows_kernel(const MxGemmParams p) {
   __shared__ f32x4 red[RK][NB * MB][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, g = lane >> 4;
+  const MxRegion& rg = p.r[0];
   const int n0 = blockIdx.x * (16 * NB), m0 = blockIdx.y * (16 * MB);
 
   // rows past the end repeat the last one; their sums are not stored
@@ -415,9 +547,9 @@ __global__ void __launch_bounds__(64 * RK) rows_kernel(const MxGemmParams p) {
   const unsigned char* wsr[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
-    const int n = min(n0 + j * 16 + r, p.N - 1);
-    wr[j] = p.w + n * p.ldw;
-    wsr[j] = p.ws + (int64_t)(n >> 5) * p.C * 256 + (n & 31) * 8;
+    const int n = min(n0 + j * 16 + r, rg.N - 1);
+    wr[j] = rg.w + n * p.ldw;
+    wsr[j] = rg.ws + (int64_t)(n >> 5) * p.C * 256 + (n & 31) * 8;
   }
   const unsigned char* ar[MB];
   const unsigned char* asr[MB];
@@ -485,13 +617,12 @@ __global__ void __launch_bounds__(64 * RK) rows_kernel(const MxGemmParams p) {
   for (int e = threadIdx.x; e < NB * MB * 256; e += 64 * RK) {
     const int nl = e % (16 * NB), ml = e / (16 * NB);
     const int n = n0 + nl, m = m0 + ml;
-    if (n >= p.N || m >= p.M) continue;
+    if (n >= rg.N || m >= p.M) continue;
     const int tile = (nl / 16) * MB + ml / 16, ln = (nl % 16) / 4 * 16 + ml % 16;
     float y = 0.0f;
 #pragma unroll
     for (int k = 0; k < RK; ++k) y += red[k][tile][ln][nl % 4];  // the shares in order
-    if (p.bias != nullptr) y += widen16<FP16>(reinterpret_cast<const unsigned short*>(p.bias)[n]);
-    reinterpret_cast<unsigned short*>(p.out)[m * p.ldc + n] = round16<FP16>(y);
+    reinterpret_cast<unsigned short*>(rg.out)[m * p.ldc + n] = round16(y + bias_at(p, rg, n), p.fp16);
   }
 }
 
@@ -500,7 +631,6 @@ __global__ void __launch_bounds__(64 * RK) rows_kernel(const MxGemmParams p) {
 // ---------------------------------------------------------------------------
 
 inline bool aligned_to(const void* ptr, uintptr_t a) { return (reinterpret_cast<uintptr_t>(ptr) % a) == 0; }
-inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // with_a: a, a_scales and lda are checked too
 int validate_gemm(const qik_mx_gemm_args* a, bool with_a) {
@@ -542,108 +672,142 @@ MxGemmParams gemm_params(const qik_mx_gemm_args* a) {
   memset(&p, 0, sizeof(p));
   p.a = static_cast<const unsigned char*>(a->a);
   p.as = static_cast<const unsigned char*>(a->a_scales);
-  p.w = static_cast<const unsigned char*>(a->w);
-  p.ws = static_cast<const unsigned char*>(a->w_scales);
-  p.bias = static_cast<const char*>(a->bias);
-  p.out = static_cast<char*>(a->out);
   p.M = (int)a->M;
-  p.N = (int)a->N;
   p.K = (int)a->K;
   p.C = (int)cdiv(a->K, 256);
   p.lda = a->lda;
   p.ldw = a->ldw;
   p.ldc = a->ldc;
+  p.fp16 = a->out_dtype == QIK_DTYPE_FP16;
   p.vec = aligned_to(a->out, 16) && a->ldc % 8 == 0;
   return p;
 }
 
-template <bool A8, bool FP16>
-int launch_rows(MxGemmParams& p, hipStream_t s) {
-  const int64_t gy = cdiv(p.M, 16);
-  if (gy > 65535) return QIK_ERR_SHAPE;
+// Region of columns [c0, c1) with tiles of bm x bn (of `abytes` and `wbytes` a stage).
+int set_region(MxRegion& rg, const qik_mx_gemm_args* a, int64_t c0, int64_t c1, int bm, int bn, int abytes, int wbytes) {
+  rg.w = static_cast<const unsigned char*>(a->w) + c0 * a->ldw;
+  rg.ws = static_cast<const unsigned char*>(a->w_scales) + c0 / 32 * cdiv(a->K, 256) * 256;  // c0: whole tiles
+  rg.bias = a->bias != nullptr ? static_cast<const char*>(a->bias) + c0 * 2 : nullptr;
+  rg.out = static_cast<char*>(a->out) + c0 * 2;
+  rg.N = (int)(c1 - c0);
+  rg.ntm = (int)cdiv(a->M, bm);
+  rg.ntn = (int)cdiv(c1 - c0, bn);
+  rg.group_m = choose_group_m(rg.ntm, rg.ntn, abytes, wbytes);
+  const int64_t wgs = cdiv((int64_t)rg.ntm * rg.ntn, 8) * 8;
+  if (wgs > (int64_t)INT_MAX / 16) return QIK_ERR_SHAPE;
+  rg.wgs = (int)wgs;
+  return QIK_OK;
+}
+template <class T>
+int set_region(MxRegion& rg, const qik_mx_gemm_args* a, int64_t c0, int64_t c1) {
+  return set_region(rg, a, c0, c1, T::BM, T::BN, T::BM * T::RA, T::BN * T::RW);
+}
+
+int launch(const void* fn, dim3 grid, int threads, MxGemmParams& p, hipStream_t s) {
   void* args[] = {&p};
-  return hipLaunchKernel((const void*)rows_kernel<A8, 1, 1, FP16>, dim3((unsigned)cdiv(p.N, 16), (unsigned)gy),
-                         dim3(64 * RK), args, 0, s) == hipSuccess
-             ? QIK_OK
-             : QIK_ERR_LAUNCH;
+  return hipLaunchKernel(fn, grid, dim3((unsigned)threads), args, 0, s) == hipSuccess ? QIK_OK : QIK_ERR_LAUNCH;
 }
 
-// tile rows per group of the tile order: the group size that minimises the
-// bytes one XCD's run of tiles reads (its distinct A row blocks + W row blocks)
-int choose_group_m(int ntm, int ntn, int abytes, int wbytes) {
-  const int64_t per_xcd = std::max<int64_t>(1, ((int64_t)ntm * ntn + 7) / 8);
-  int best = 1;
-  double best_bytes = 1e300;
-  for (int gm = 1; gm <= std::min(ntm, 16); ++gm) {
-    const int64_t rows = std::min<int64_t>(gm, per_xcd);
-    const int64_t cols = std::min<int64_t>(ntn, (per_xcd + gm - 1) / gm);
-    const double bytes = (double)rows * abytes + (double)cols * wbytes;
-    if (bytes < best_bytes) {
-      best_bytes = bytes;
-      best = gm;
-    }
-  }
-  return best;
+template <class T1, class T2>
+int launch_tiles(MxGemmParams& p, const qik_mx_gemm_args* a, int64_t n1, hipStream_t s) {
+  int st = set_region<T1>(p.r[0], a, 0, n1);
+  if (st == QIK_OK) st = set_region<T2>(p.r[1], a, n1, a->N);
+  if (st != QIK_OK) return st;
+  return launch((const void*)tile_kernel<T1, T2>, dim3((unsigned)p.r[0].wgs + (unsigned)p.r[1].wgs), T1::NT, p, s);
 }
 
-template <class T, bool FP16>
-int launch_tiles(MxGemmParams& p, hipStream_t s) {
-  const int64_t ntm = cdiv(p.M, T::BM), ntn = cdiv(p.N, T::BN);
-  const int64_t grid = cdiv(ntm * ntn, 8) * 8;
-  if (grid > (int64_t)INT_MAX / 2) return QIK_ERR_SHAPE;
-  p.ntm = (int)ntm;
-  p.ntn = (int)ntn;
-  p.group_m = choose_group_m(p.ntm, p.ntn, T::BM * T::RA, T::BN * T::RW);
-  void* args[] = {&p};
-  return hipLaunchKernel((const void*)tile_kernel<T, FP16>, dim3((unsigned)grid), dim3(T::NT), args, 0, s) == hipSuccess
-             ? QIK_OK
-             : QIK_ERR_LAUNCH;
+template <class T>
+int launch_split(MxGemmParams& p, const qik_mx_gemm_args* a, hipStream_t s) {
+  int st = set_region<T>(p.r[0], a, 0, a->N);
+  if (st != QIK_OK) return st;
+  st = launch((const void*)split_kernel<T>, dim3((unsigned)p.r[0].wgs * (unsigned)p.ksplit), T::NT, p, s);
+  if (st != QIK_OK) return st;
+  return launch((const void*)join_kernel, dim3((unsigned)cdiv(a->M * (p.ldp / 4), 256)), 256, p, s);
 }
 
-enum { T256x256, T256x128, T128x256, T128x128, T64x128, T64x64, NSHAPES };
-struct TileShape {
-  int bm, bn;
-  double t0, t1;  // us of a tile: t0 + t1 per stage
+template <bool A8>
+int launch_rows(MxGemmParams& p, const qik_mx_gemm_args* a, hipStream_t s) {
+  const int st = set_region(p.r[0], a, 0, a->N, 16, 16, 0, 0);
+  if (st != QIK_OK) return st;
+  return launch((const void*)rows_kernel<A8, 1, 1>, dim3((unsigned)p.r[0].ntn, (unsigned)p.r[0].ntm), 64 * RK, p, s);
+}
+
+// Time of a tile of each shape (qik_tile.h), for A in MXFP4 and in MXFP8: fitted
+// to launches of one round on MI355X, each shape forced, 64 to 8704 rows, N x K
+// from 1024 x 1024 to 12288 x 4096 and 4096 x 12288, operands from memory.  A
+// launch that keeps all its CUs busy takes a quarter longer than its tile times
+// (the card's power limit lowers the clock: 1.7 GHz at 8192 x 8192 x 8192);
+// tiles of 64 rows, which wait more than they multiply, do not.
+enum { T256x256, T256x128, T128x256, T128x128, T192x256, T192x128, T64x128, T64x64, NSHAPES };
+static const TileShape kShapes[2][NSHAPES] = {
+    {{256, 256, 8.6, 1.22}, {256, 128, 6.15, 0.67}, {128, 256, 6.35, 0.645}, {128, 128, 4.6, 0.44, 0.4},
+     {192, 256, 7.3, 0.99}, {192, 128, 5.5, 0.575, 0.6}, {64, 128, 4.5, 0.305, 0.0}, {64, 64, 3.9, 0.25, 0.0}},
+    {{256, 256, 9.1, 1.0}, {256, 128, 6.0, 0.595}, {128, 256, 6.25, 0.56}, {128, 128, 4.45, 0.415, 0.4},
+     {192, 256, 7.7, 0.765}, {192, 128, 5.55, 0.515, 0.6}, {64, 128, 4.3, 0.29, 0.0}, {64, 64, 3.85, 0.235, 0.0}}};
+constexpr int NPAIRS = 7;
+static const int kPairs[NPAIRS][2] = {{T256x256, T256x128}, {T256x256, T128x128}, {T256x128, T128x128},
+                                      {T128x256, T128x128}, {T192x256, T192x128}, {T192x128, T128x128},
+                                      {T64x128, T64x64}};
+static const TileTable kTables[2] = {{kShapes[0], kPairs, NPAIRS, 0, 0.5, 0.5},
+                                     {kShapes[1], kPairs, NPAIRS, 0, 0.5, 0.5}};
+
+enum { SPLIT64, SPLIT128 };
+// How a product of more than a few rows is launched: slices > 1 splits K.
+struct MxPlan {
+  int pair;
+  int64_t n1;
+  bool small_first;
+  int slices, split;
 };
-static const TileShape kShapes[NSHAPES] = {{256, 256, 6.0, 1.5},   {256, 128, 6.0, 0.775}, {128, 256, 6.0, 0.81},
-                                           {128, 128, 4.6, 0.485}, {64, 128, 3.8, 0.32},   {64, 64, 3.8, 0.215}};
 
-int choose_shape(int64_t M, int64_t N, int64_t steps) {
-  int best = 0;
-  double best_t = 1e300;
-  for (int i = 0; i < NSHAPES; ++i) {
-    const TileShape& t = kShapes[i];
-    const int64_t rounds = cdiv(cdiv(cdiv(M, t.bm) * cdiv(N, t.bn), 8), 32);
-    const double us = (double)rounds * (t.t0 + t.t1 * (double)steps);
-    if (us < best_t) {
-      best_t = us;
-      best = i;
-    }
-  }
-  return best;
+MxPlan choose(int64_t M, int64_t N, int64_t K, bool a8, int cus) {
+  const GemmPlan g = choose_plan(kTables[a8], M, N, cdiv(K, a8 ? 128 : 256), cus);
+  return {g.pair, g.n1, g.small_first, 1, SPLIT64};
 }
 
-template <bool A8, bool FP16>
-int launch_shape(MxGemmParams& p, hipStream_t s) {
-  switch (choose_shape(p.M, p.N, cdiv(p.K, A8 ? 128 : 256))) {
-    case T256x256: return launch_tiles<Tile<256, 256, 2, 4, A8 ? 3 : 2, A8>, FP16>(p, s);
-    case T256x128: return launch_tiles<Tile<256, 128, 2, 4, 3, A8>, FP16>(p, s);
-    case T128x256: return launch_tiles<Tile<128, 256, 2, 4, 3, A8>, FP16>(p, s);
-    case T128x128: return launch_tiles<Tile<128, 128, 2, 4, A8 ? 4 : 3, A8>, FP16>(p, s);
-    case T64x128: return launch_tiles<Tile<64, 128, 1, 4, 4, A8>, FP16>(p, s);
-    default: return launch_tiles<Tile<64, 64, 2, 2, 4, A8>, FP16>(p, s);
+template <bool A8>
+int launch_plan(MxGemmParams& p, const qik_mx_gemm_args* a, const MxPlan& plan, float* partial, hipStream_t s) {
+  typedef Tile<256, 256, 2, 4, A8 ? 3 : 2, A8, false> C256x256;
+  typedef Tile<256, 128, 2, 4, 3, A8, true> C256x128;
+  typedef Tile<128, 256, 2, 4, 3, A8, true> C128x256;
+  typedef Tile<128, 128, 2, 4, 3, A8, true> C128x128;
+  typedef Tile<192, 256, 2, 4, A8 ? 3 : 2, A8, A8> C192x256;
+  typedef Tile<192, 128, 2, 4, 3, A8, true> C192x128;
+  typedef Tile<64, 128, 1, 4, 3, A8, true> C64x128;
+  typedef Tile<64, 64, 2, 2, 4, A8, true> C64x64;
+  if (plan.slices > 1) {
+    p.ksplit = plan.slices;
+    p.partial = partial;
+    p.ldp = cdiv(a->N, 4) * 4;
+    return plan.split == SPLIT64 ? launch_split<C64x64>(p, a, s) : launch_split<C128x128>(p, a, s);
+  }
+  p.small_first = plan.small_first ? 1 : 0;
+  switch (plan.pair) {
+    case 0: return launch_tiles<C256x256, C256x128>(p, a, plan.n1, s);
+    case 1: return launch_tiles<C256x256, C128x128>(p, a, plan.n1, s);
+    case 2: return launch_tiles<C256x128, C128x128>(p, a, plan.n1, s);
+    case 3: return launch_tiles<C128x256, C128x128>(p, a, plan.n1, s);
+    case 4: return launch_tiles<C192x256, C192x128>(p, a, plan.n1, s);
+    case 5: return launch_tiles<C192x128, C128x128>(p, a, plan.n1, s);
+    default: return launch_tiles<C64x128, C64x64>(p, a, plan.n1, s);
   }
 }
 
-int launch_gemm(const qik_mx_gemm_args* a, hipStream_t s) {
+// rows that the few-rows kernel takes
+constexpr int FEW_ROWS = 32;
+
+int64_t partial_bytes(const qik_mx_gemm_args* a) {
+  if (a->M <= FEW_ROWS) return 0;
+  const MxPlan plan = choose(a->M, a->N, a->K, a->a_format == QIK_MXFP8, device_cus());
+  return plan.slices > 1 ? (int64_t)plan.slices * a->M * cdiv(a->N, 4) * 4 * (int64_t)sizeof(float) : 0;
+}
+
+int launch_gemm(const qik_mx_gemm_args* a, float* partial, hipStream_t s) {
   MxGemmParams p = gemm_params(a);
-  const bool fp16 = a->out_dtype == QIK_DTYPE_FP16;
-  if (p.M <= 32) {
-    if (a->a_format == QIK_MXFP8) return fp16 ? launch_rows<true, true>(p, s) : launch_rows<true, false>(p, s);
-    return fp16 ? launch_rows<false, true>(p, s) : launch_rows<false, false>(p, s);
-  }
-  if (a->a_format == QIK_MXFP8) return fp16 ? launch_shape<true, true>(p, s) : launch_shape<true, false>(p, s);
-  return fp16 ? launch_shape<false, true>(p, s) : launch_shape<false, false>(p, s);
+  const bool a8 = a->a_format == QIK_MXFP8;
+  if (a->M <= FEW_ROWS) return a8 ? launch_rows<true>(p, a, s) : launch_rows<false>(p, a, s);
+  const MxPlan plan = choose(a->M, a->N, a->K, a8, device_cus());
+  return a8 ? launch_plan<true>(p, a, plan, partial, s) : launch_plan<false>(p, a, plan, partial, s);
 }
 
 inline int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -657,27 +821,32 @@ int64_t scale_bytes(const qik_mx_gemm_args* g) { return cdiv(g->M, 32) * cdiv(g-
 extern "C" {
 
 int qik_mx_gemm_workspace_size(const qik_mx_gemm_args* a, int64_t* bytes) {
+  using namespace qik_mx;
   if (bytes == nullptr) return QIK_ERR_NULL_ARG;
   *bytes = 0;
-  return qik_mx::validate_gemm(a, true);
+  const int st = validate_gemm(a, true);
+  if (st != QIK_OK || a->M == 0) return st;
+  *bytes = partial_bytes(a);
+  return QIK_OK;
 }
 
 int qik_mx_gemm(const qik_mx_gemm_args* a, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace qik_mx;
   const int st = validate_gemm(a, true);
   if (st != QIK_OK || a->M == 0) return st;
-  (void)workspace;
-  (void)workspace_bytes;
-  return launch_gemm(a, static_cast<hipStream_t>(stream));
+  const int64_t need = partial_bytes(a);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 256))) return QIK_ERR_WORKSPACE;
+  return launch_gemm(a, static_cast<float*>(workspace), static_cast<hipStream_t>(stream));
 }
 
+// workspace of a linear: the split's sums, x's codes, x's scales
 int qik_mx_linear_workspace_size(const qik_mx_linear_args* a, int64_t* bytes) {
   using namespace qik_mx;
   if (bytes == nullptr) return QIK_ERR_NULL_ARG;
   *bytes = 0;
   const int st = validate_linear(a);
-  if (st != QIK_OK) return st;
-  *bytes = code_bytes(&a->g) + scale_bytes(&a->g);
+  if (st != QIK_OK || a->g.M == 0) return st;
+  *bytes = round256(partial_bytes(&a->g)) + code_bytes(&a->g) + scale_bytes(&a->g);
   return QIK_OK;
 }
 
@@ -685,13 +854,13 @@ int qik_mx_linear(const qik_mx_linear_args* a, void* workspace, int64_t workspac
   using namespace qik_mx;
   const int st = validate_linear(a);
   if (st != QIK_OK || a->g.M == 0) return st;
-  int64_t need = 0;
-  qik_mx_linear_workspace_size(a, &need);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 256))) return QIK_ERR_WORKSPACE;
-  qik_mx_gemm_args g = a->g;
+  const int64_t sums = round256(partial_bytes(&a->g)), codes = code_bytes(&a->g);
+  const int64_t need = sums + codes + scale_bytes(&a->g);
+  if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 256)) return QIK_ERR_WORKSPACE;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  g.a = ws;
-  g.a_scales = ws + code_bytes(&g);
+  qik_mx_gemm_args g = a->g;
+  g.a = ws + sums;
+  g.a_scales = ws + sums + codes;
   g.lda = g.a_format == QIK_MXFP4 ? g.K / 2 : g.K;
   qik_mx_quant_args q;
   memset(&q, 0, sizeof(q));
@@ -699,14 +868,14 @@ int qik_mx_linear(const qik_mx_linear_args* a, void* workspace, int64_t workspac
   q.dtype = a->x_dtype;
   q.format = g.a_format;
   q.x = a->x;
-  q.codes = ws;
-  q.scales = ws + code_bytes(&g);
+  q.codes = ws + sums;
+  q.scales = ws + sums + codes;
   q.M = g.M;
   q.K = g.K;
   q.ldx = a->ldx;
   const int qs = qik_mx_quantize(&q, stream);
   if (qs != QIK_OK) return qs;
-  return launch_gemm(&g, static_cast<hipStream_t>(stream));
+  return launch_gemm(&g, reinterpret_cast<float*>(ws), static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"
