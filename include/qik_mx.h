@@ -151,7 +151,7 @@ int qik_mx_gemm(const qik_mx_gemm_args* args, void* workspace, int64_t workspace
 /* qik_mx_gemm of x quantised to g.a_format: x is [M, K] of x_dtype with row
  * stride ldx as in qik_mx_quantize; g.a, g.a_scales and g.lda are not read.
  * The workspace holds the codes and scales of x too; where the launch
- * quantises x as it loads it (few rows) no memory is needed for them. */
+ * quantises x itself (few elements) no memory is needed for them. */
 typedef struct qik_mx_linear_args {
   qik_mx_gemm_args g;
   const void* x;

@@ -8,9 +8,10 @@
 // reach LDS directly, two to four stages in flight, and the fragments of the
 // next k-step are read while the matrix cores run on the current ones.
 //
-// Few rows (`rows_kernel`): every wave takes 16 weight rows and a share of K,
-// loads the codes straight into registers and meets the others of its
-// workgroup in LDS.  It is bound by the weight's bytes.
+// Few rows (`rows_kernel`): every wave takes 16 or 32 weight rows and a share
+// of K, loads the codes straight into registers and meets the others of its
+// workgroup in LDS.  It is bound by the weight's bytes.  Of a token or a few, the
+// workgroup quantises the elements itself: one launch.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -20,14 +21,26 @@
 #include <type_traits>
 
 #include "qik_mx.h"
+#include "qik_mx_block.h"
 #include "qik_tile.h"
 
 namespace qik_mx {
 
-using namespace qik_tile;
+using qik_tile::cdiv;
+using qik_tile::choose_group_m;
+using qik_tile::choose_plan;
+using qik_tile::device_cus;
+using qik_tile::dma16;
+using qik_tile::dma4;
+using qik_tile::GemmPlan;
+using qik_tile::lds_ptr_t;
+using qik_tile::rsrc_words;
+using qik_tile::tile_origin;
+using qik_tile::TileRun;
+using qik_tile::TileShape;
+using qik_tile::TileTable;
+using qik_tile::wait_vmcnt;
 
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -532,15 +545,31 @@ __global__ void __launch_bounds__(256) join_kernel(const MxGemmParams p) {
 // of block l / 16 of the step.  W is the first operand, so a lane's 4 sums are
 // 4 consecutive columns n of row m = l % 16.
 
-constexpr int RK = 4;  // waves of a workgroup, each with its share of the 256-k chunks
+// Where the rows of A come from: codes, or elements of a type that the
+// workgroup quantises into LDS first.
+enum { SRC_CODES = -1 };  // else QIK_DTYPE_BF16, _FP16 or _FP32
 
-template <bool A8, int MB, int NB>
-__global__ void __launch_bounds__(64 * RK) rows_kernel(const MxGemmParams p) {
-  __shared__ f32x4 red[RK][NB * MB][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r = lane & 15, g = lane >> 4;
+// Most elements of A that a workgroup quantises for itself.  Every workgroup
+// does all of them, so it pays while they are few: one token, or a few of a
+// narrow layer.
+constexpr int RAW_ELEMS = 16384;
+
+// KW waves of a workgroup share K by chunks of 256; BC chunks of W are in
+// flight ahead of the ones that are multiplied.
+template <int SRC, bool A8, int MB, int NB, int KW>
+__global__ void __launch_bounds__(64 * KW) rows_kernel(const MxGemmParams p) {
+  constexpr bool RAW = SRC != SRC_CODES;
+  constexpr int BC = NB == 1 ? 4 : 2;
+  constexpr int CODE_BYTES = RAW ? RAW_ELEMS / (A8 ? 1 : 2) : 16, SCALE_BYTES = RAW ? RAW_ELEMS / 32 : 16;
+  __shared__ f32x4 red[KW][NB * MB][64];
+  __shared__ __attribute__((aligned(16))) unsigned char lcodes[CODE_BYTES];
+  __shared__ unsigned char lscales[SCALE_BYTES];
   const MxRegion& rg = p.r[0];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * (16 * NB), m0 = blockIdx.y * (16 * MB);
+  const u32x4 zero = {0u, 0u, 0u, 0u};
 
   // rows past the end repeat the last one; their sums are not stored
   const unsigned char* wr[NB];
@@ -551,13 +580,13 @@ __global__ void __launch_bounds__(64 * RK) rows_kernel(const MxGemmParams p) {
     wr[j] = rg.w + n * p.ldw;
     wsr[j] = rg.ws + (int64_t)(n >> 5) * p.C * 256 + (n & 31) * 8;
   }
-  const unsigned char* ar[MB];
-  const unsigned char* asr[MB];
+  const unsigned char* ar[MB];   // a row's codes
+  const unsigned char* asr[MB];  // its scales
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
     const int m = min(m0 + i * 16 + r, p.M - 1);
-    ar[i] = p.a + m * p.lda;
-    asr[i] = p.as + (int64_t)(m >> 5) * p.C * 256 + (m & 31) * 8;
+    ar[i] = RAW ? lcodes + m * (A8 ? p.K : p.K / 2) : p.a + m * p.lda;
+    asr[i] = RAW ? lscales + m * (p.K / 32) : p.as + (int64_t)(m >> 5) * p.C * 256 + (m & 31) * 8;
   }
 
   f32x4 acc[NB][MB];
@@ -566,62 +595,119 @@ __global__ void __launch_bounds__(64 * RK) rows_kernel(const MxGemmParams p) {
 #pragma unroll
     for (int i = 0; i < MB; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const int c0 = p.C * wave / RK, c1 = p.C * (wave + 1) / RK;
-  const u32x4 zero = {0u, 0u, 0u, 0u};
-  for (int c = c0; c < c1; ++c) {
-    u32x2 wsc[NB], asc[MB];
-    u32x4 wf[2][NB], af[2][MB][A8 ? 2 : 1];
+  const int c0 = p.C * wave / KW, c1 = p.C * (wave + 1) / KW;
+  u32x4 wf[2][BC][2][NB];
+  u32x2 wsc[2][BC][NB];
+  // a lane's blocks past K are zeros (loaded from the row's start, then cleared)
+  auto load_w = [&](const int buf, const int c) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NB; ++j) wsc[j] = *reinterpret_cast<const u32x2*>(wsr[j] + c * 256);
+    for (int b = 0; b < BC; ++b) {
+      if (c + b >= c1) break;
 #pragma unroll
-    for (int i = 0; i < MB; ++i) asc[i] = *reinterpret_cast<const u32x2*>(asr[i] + c * 256);
+      for (int s = 0; s < 2; ++s) {
+        const int k = (c + b) * 256 + s * 128 + g * 32;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      // a lane's blocks past K are zeros (loaded from the row's start, then cleared)
-      const int k = c * 256 + s * 128 + g * 32;
-#pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(wr[j] + (k < p.K ? k / 2 : 0));
-        wf[s][j] = k < p.K ? v : zero;
-      }
-#pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        if constexpr (A8) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int ka = c * 256 + s * 128 + h * 64 + g * 16;
-            const u32x4 v = *reinterpret_cast<const u32x4*>(ar[i] + (ka < p.K ? ka : 0));
-            af[s][i][h] = ka < p.K ? v : zero;
-          }
-        } else {
-          const u32x4 v = *reinterpret_cast<const u32x4*>(ar[i] + (k < p.K ? k / 2 : 0));
-          af[s][i][0] = k < p.K ? v : zero;
+        for (int j = 0; j < NB; ++j) {
+          const u32x4 v = *reinterpret_cast<const u32x4*>(wr[j] + (k < p.K ? k / 2 : 0));
+          wf[buf][b][s][j] = k < p.K ? v : zero;
         }
       }
+#pragma unroll
+      for (int j = 0; j < NB; ++j) wsc[buf][b][j] = *reinterpret_cast<const u32x2*>(wsr[j] + (c + b) * 256);
+    }
+  };
+  // what a lane holds of 16 rows of A for step s of chunk c, and its scale
+  struct AFrag {
+    u32x4 lo, hi;
+    int scale;
+  };
+  auto load_a = [&](const int i, const int c, const int s, const u32x2 asc) __attribute__((always_inline)) {
+    AFrag f;
+    const int kb = c * 256 + s * 128 + g * 32;  // the block of the lane's scale
+    if constexpr (A8) {
+      const int k = c * 256 + s * 128 + g * 16;
+      const u32x4 lo = *reinterpret_cast<const u32x4*>(ar[i] + (k < p.K ? k : 0));
+      const u32x4 hi = *reinterpret_cast<const u32x4*>(ar[i] + (k + 64 < p.K ? k + 64 : 0));
+      f.lo = k < p.K ? lo : zero;
+      f.hi = k + 64 < p.K ? hi : zero;
+    } else {
+      const u32x4 lo = *reinterpret_cast<const u32x4*>(ar[i] + (kb < p.K ? kb / 2 : 0));
+      f.lo = kb < p.K ? lo : zero;
+      f.hi = zero;
+    }
+    if constexpr (RAW) f.scale = kb < p.K ? asr[i][kb / 32] : 0;
+    else f.scale = (int)(asc[s] >> (8 * g));
+    return f;
+  };
+  auto multiply = [&](const int buf, const int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < BC; ++b) {
+      if (c + b >= c1) break;
+      AFrag a[2][MB];
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        u32x2 asc = {0u, 0u};
+        if constexpr (!RAW) asc = *reinterpret_cast<const u32x2*>(asr[i] + (c + b) * 256);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) a[s][i] = load_a(i, c + b, s, asc);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int i = 0; i < MB; ++i)
+            acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                operand(wf[buf][b][s][j], zero), operand(a[s][i].lo, a[s][i].hi), acc[j][i], FMT_E2M1,
+                A8 ? FMT_E4M3 : FMT_E2M1, 0, (int)(wsc[buf][b][j][s] >> (8 * g)), 0, a[s][i].scale);
+    }
+  };
+  load_w(0, c0);
+  if constexpr (RAW) {  // while the first weights are on their way
+    constexpr int FMT = A8 ? QIK_MXFP8 : QIK_MXFP4;
+    constexpr int IT = RAW_ELEMS / 8 / (64 * KW);
+    const int per_row = p.K / 8, total = p.M * per_row;  // vectors of 8; a multiple of 4 a row: whole quads
+    Raw8<SRC> x[IT];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int v = threadIdx.x + i * 64 * KW, m = v / per_row;
+      x[i] = Raw8<SRC>{};
+      if (v < total)
+        x[i] = load8<SRC, false>(reinterpret_cast<const char*>(p.a) + (m * p.lda + (v - m * per_row) * 8) * elem_bytes<SRC>());
     }
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
-          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              operand(wf[s][j], zero), operand(af[s][i][0], A8 ? af[s][i][A8 ? 1 : 0] : zero), acc[j][i], FMT_E2M1,
-              A8 ? FMT_E4M3 : FMT_E2M1, 0, (int)(wsc[j][s] >> (8 * g)), 0, (int)(asc[i][s] >> (8 * g)));
+    for (int i = 0; i < IT; ++i) {
+      const int v = threadIdx.x + i * 64 * KW;
+      if (v >= total) continue;
+      float f[8];
+      unpack8<SRC>(x[i], f);
+      unsigned w0, w1;
+      const unsigned byte = block_codes<FMT>(f, w0, w1);
+      store_codes<FMT>(lcodes, v, w0, w1);  // rows lie one behind the other
+      if ((v & 3) == 0) lscales[v / 4] = (unsigned char)byte;
+    }
+    __syncthreads();
   }
+  for (int c = c0; c < c1; c += 2 * BC) {
+    load_w(1, c + BC);
+    multiply(0, c);
+    load_w(0, c + 2 * BC);
+    multiply(1, c + BC);
+  }
+
 #pragma unroll
   for (int j = 0; j < NB; ++j)
 #pragma unroll
     for (int i = 0; i < MB; ++i) red[wave][j * MB + i][lane] = acc[j][i];
   __syncthreads();
-  for (int e = threadIdx.x; e < NB * MB * 256; e += 64 * RK) {
+  for (int e = threadIdx.x; e < NB * MB * 256; e += 64 * KW) {
     const int nl = e % (16 * NB), ml = e / (16 * NB);
     const int n = n0 + nl, m = m0 + ml;
     if (n >= rg.N || m >= p.M) continue;
     const int tile = (nl / 16) * MB + ml / 16, ln = (nl % 16) / 4 * 16 + ml % 16;
     float y = 0.0f;
 #pragma unroll
-    for (int k = 0; k < RK; ++k) y += red[k][tile][ln][nl % 4];  // the shares in order
+    for (int k = 0; k < KW; ++k) y += red[k][tile][ln][nl % 4];  // the shares in order
     reinterpret_cast<unsigned short*>(rg.out)[m * p.ldc + n] = round16(y + bias_at(p, rg, n), p.fp16);
   }
 }
@@ -725,11 +811,27 @@ int launch_split(MxGemmParams& p, const qik_mx_gemm_args* a, hipStream_t s) {
   return launch((const void*)join_kernel, dim3((unsigned)cdiv(a->M * (p.ldp / 4), 256)), 256, p, s);
 }
 
-template <bool A8>
-int launch_rows(MxGemmParams& p, const qik_mx_gemm_args* a, hipStream_t s) {
-  const int st = set_region(p.r[0], a, 0, a->N, 16, 16, 0, 0);
+template <int SRC, bool A8, int MB, int NB, int KW>
+int launch_rows_shape(MxGemmParams& p, const qik_mx_gemm_args* a, hipStream_t s) {
+  const int st = set_region(p.r[0], a, 0, a->N, 16 * MB, 16 * NB, 0, 0);
   if (st != QIK_OK) return st;
-  return launch((const void*)rows_kernel<A8, 1, 1>, dim3((unsigned)p.r[0].ntn, (unsigned)p.r[0].ntm), 64 * RK, p, s);
+  return launch((const void*)rows_kernel<SRC, A8, MB, NB, KW>, dim3((unsigned)p.r[0].ntn, (unsigned)p.r[0].ntm), 64 * KW, p,
+                s);
+}
+
+struct RowsPlan {
+  int nb, kw;
+};
+RowsPlan choose_rows(int64_t M, int64_t N, int64_t K) {
+  return {N > 8192 && M > 8 ? 2 : 1, N <= 8192 && K > 7 * 256 ? 8 : 4};
+}
+
+template <int SRC, bool A8, int MB>
+int launch_rows(MxGemmParams& p, const qik_mx_gemm_args* a, hipStream_t s) {
+  const RowsPlan plan = choose_rows(a->M, a->N, a->K);
+  if (plan.nb == 1)
+    return plan.kw == 4 ? launch_rows_shape<SRC, A8, MB, 1, 4>(p, a, s) : launch_rows_shape<SRC, A8, MB, 1, 8>(p, a, s);
+  return plan.kw == 4 ? launch_rows_shape<SRC, A8, MB, 2, 4>(p, a, s) : launch_rows_shape<SRC, A8, MB, 2, 8>(p, a, s);
 }
 
 // Time of a tile of each shape (qik_tile.h), for A in MXFP4 and in MXFP8: fitted
@@ -760,9 +862,31 @@ struct MxPlan {
   int slices, split;
 };
 
+// A K split pays for a launch with few tiles and a long K: S slices of 64 x 64 or
+// 128 x 128 tiles, as many as the CUs run in one round (all slices of a tile on
+// one XCD), and a second launch that joins them: 3 us, and the fp32 sums written
+// and read at about 4 TB/s (64 x 4096 x 12288 18.1 us unsplit, 12.1 in 4 slices,
+// 15.5 in 8; 203 x 2048 x 8192 13.3 and 12.5 in 2; 203 x 4096 x 12288 18.2 and
+// 19.2 in 4 of 128 x 128).
 MxPlan choose(int64_t M, int64_t N, int64_t K, bool a8, int cus) {
-  const GemmPlan g = choose_plan(kTables[a8], M, N, cdiv(K, a8 ? 128 : 256), cus);
-  return {g.pair, g.n1, g.small_first, 1, SPLIT64};
+  const int64_t steps = cdiv(K, a8 ? 128 : 256), P = std::max(1, (cus > 0 ? cus : 256) / 8);
+  const GemmPlan g = choose_plan(kTables[a8], M, N, steps, cus);
+  MxPlan plan = {g.pair, g.n1, g.small_first, 1, SPLIT64};
+  double best = 0.95 * g.t;
+  for (int which = SPLIT64; which <= SPLIT128; ++which) {
+    const TileShape& t = kShapes[a8][which == SPLIT64 ? T64x64 : T128x128];
+    const int64_t per_xcd = cdiv(cdiv(M, t.bm) * cdiv(N, t.bn), 8);
+    const int64_t most = std::min<int64_t>({P / per_xcd, 8, steps / 4});
+    for (int64_t S = 2; S <= most; ++S) {
+      const double us = t.time(cdiv(steps, S)) + 3.0 + (double)(S * M * N) * 8.0 / 4e6;
+      if (us < best) {
+        best = us;
+        plan.slices = (int)S;
+        plan.split = which;
+      }
+    }
+  }
+  return plan;
 }
 
 template <bool A8>
@@ -793,21 +917,38 @@ int launch_plan(MxGemmParams& p, const qik_mx_gemm_args* a, const MxPlan& plan, 
   }
 }
 
-// rows that the few-rows kernel takes
-constexpr int FEW_ROWS = 32;
+// Few rows: the tiles of 64 would multiply mostly padding.  From 17 rows on they
+// do better all the same where N has tiles for most CUs and K is long (32 x
+// 12288 x 8192 16.8 us against 23.2; 32 x 4096 x 8192 10.6 and 9.9).
+bool takes_rows(const qik_mx_gemm_args* a) {
+  return a->M <= 16 || (a->M <= 32 && (a->N <= 4096 || a->N * a->K <= (1 << 24)));
+}
+
+// A product of elements that each workgroup quantises for itself.
+bool takes_raw(const qik_mx_gemm_args* a) { return a->M <= 16 && a->M * a->K <= RAW_ELEMS; }
 
 int64_t partial_bytes(const qik_mx_gemm_args* a) {
-  if (a->M <= FEW_ROWS) return 0;
+  if (takes_rows(a)) return 0;
   const MxPlan plan = choose(a->M, a->N, a->K, a->a_format == QIK_MXFP8, device_cus());
   return plan.slices > 1 ? (int64_t)plan.slices * a->M * cdiv(a->N, 4) * 4 * (int64_t)sizeof(float) : 0;
 }
 
+template <bool A8>
 int launch_gemm(const qik_mx_gemm_args* a, float* partial, hipStream_t s) {
   MxGemmParams p = gemm_params(a);
-  const bool a8 = a->a_format == QIK_MXFP8;
-  if (a->M <= FEW_ROWS) return a8 ? launch_rows<true>(p, a, s) : launch_rows<false>(p, a, s);
-  const MxPlan plan = choose(a->M, a->N, a->K, a8, device_cus());
-  return a8 ? launch_plan<true>(p, a, plan, partial, s) : launch_plan<false>(p, a, plan, partial, s);
+  if (takes_rows(a)) return a->M <= 16 ? launch_rows<SRC_CODES, A8, 1>(p, a, s) : launch_rows<SRC_CODES, A8, 2>(p, a, s);
+  return launch_plan<A8>(p, a, choose(a->M, a->N, a->K, A8, device_cus()), partial, s);
+}
+int launch_gemm(const qik_mx_gemm_args* a, float* partial, hipStream_t s) {
+  return a->a_format == QIK_MXFP8 ? launch_gemm<true>(a, partial, s) : launch_gemm<false>(a, partial, s);
+}
+
+template <int SRC>
+int launch_raw(const qik_mx_linear_args* l, hipStream_t s) {
+  MxGemmParams p = gemm_params(&l->g);
+  p.a = static_cast<const unsigned char*>(l->x);
+  p.lda = l->ldx;  // elements
+  return l->g.a_format == QIK_MXFP8 ? launch_rows<SRC, true, 1>(p, &l->g, s) : launch_rows<SRC, false, 1>(p, &l->g, s);
 }
 
 inline int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -846,7 +987,7 @@ int qik_mx_linear_workspace_size(const qik_mx_linear_args* a, int64_t* bytes) {
   *bytes = 0;
   const int st = validate_linear(a);
   if (st != QIK_OK || a->g.M == 0) return st;
-  *bytes = round256(partial_bytes(&a->g)) + code_bytes(&a->g) + scale_bytes(&a->g);
+  if (!takes_raw(&a->g)) *bytes = round256(partial_bytes(&a->g)) + code_bytes(&a->g) + scale_bytes(&a->g);
   return QIK_OK;
 }
 
@@ -854,6 +995,14 @@ int qik_mx_linear(const qik_mx_linear_args* a, void* workspace, int64_t workspac
   using namespace qik_mx;
   const int st = validate_linear(a);
   if (st != QIK_OK || a->g.M == 0) return st;
+  if (takes_raw(&a->g)) {
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    switch (a->x_dtype) {
+      case QIK_DTYPE_BF16: return launch_raw<QIK_DTYPE_BF16>(a, s);
+      case QIK_DTYPE_FP16: return launch_raw<QIK_DTYPE_FP16>(a, s);
+      default: return launch_raw<QIK_DTYPE_FP32>(a, s);
+    }
+  }
   const int64_t sums = round256(partial_bytes(&a->g)), codes = code_bytes(&a->g);
   const int64_t need = sums + codes + scale_bytes(&a->g);
   if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 256)) return QIK_ERR_WORKSPACE;

@@ -330,6 +330,22 @@ def test_linear(fmt, dtype, M, K, N):
     check_product(pre, av, wv, mod.bias.double().cpu().numpy(), torch.bfloat16, fmt)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [1, 5, 16, 17, 32, 33, 65])
+def test_linear_quantises_as_quantize_mx(fmt, dtype, M):
+    """An identity weight gives back what the input was quantised to, every bit (its elements are exact in bf16)."""
+    say("identity", fmt, dtype, M)
+    for K in (32, 480, 2176):
+        w = qik.quantize_mx(torch.eye(K, device=DEV))
+        x = rows(M, K, dtype, seed=K + M)
+        # one NaN makes a row of the product NaN, so blocks that are NaN are put aside (test_linear_takes_special_rows)
+        top = 2.0 ** (15 if dtype == torch.float16 else 100)
+        x = torch.where(torch.isfinite(x), x, 1.0).float().clamp(-top, top).to(dtype).to(DEV)
+        got = qik.MXFP4Linear.from_quantized(w, None, activations=fmt)(x)
+        assert torch.equal(got, qik.quantize_mx(x, fmt).dequantize(torch.bfloat16).to(dtype))
+
+
 def test_linear_takes_special_rows():
     """Infinities and NaN poison their row, zeros and subnormals do not."""
     for fmt in FORMATS:
