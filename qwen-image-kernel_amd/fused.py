@@ -205,6 +205,63 @@ def fused_residual_rms_norm(
     in that microscaled format (an MXTensor, D a multiple of 32), with no
     rounding in between.  Asynchronous on the current stream; records no
     gradients."""
+    # one lookup per call: what depends on the operands' geometry alone (the
+    # checks, the argument struct without addresses) is prepared once per key
+    r = residual
+    key = (x.shape, x.stride(), x.dtype, x.device, weight.shape, weight.stride(), weight.dtype, weight.device, eps,
+           out_format, (x.data_ptr() | weight.data_ptr()) & 15,
+           None if r is None else (r.shape, r.stride(), r.dtype, r.device, r.data_ptr() & 15))
+    ent = _NORM_CALLS.get(key)
+    if ent is None:
+        ent = _prepare_norm(x, r, weight, eps, out_format)
+        if len(_NORM_CALLS) >= 64:
+            _NORM_CALLS.clear()
+        _NORM_CALLS[key] = ent
+    a = _lib.QikResidualRmsNormArgs.from_buffer_copy(ent.args)
+    h = scales = None
+    if ent.like:
+        out = torch.empty_like(x)
+        if r is not None:
+            a.residual = r.data_ptr()
+            h = torch.empty_like(x)
+            a.sum = h.data_ptr()
+        a.x, a.weight, a.out = x.data_ptr(), weight.data_ptr(), out.data_ptr()
+    else:
+        xs, rs, ws = (x, r, weight) if not ent.copy else _norm_copies(x, r, weight, ent.fmt)
+        out = x.new_empty(ent.out_shape, dtype=ent.out_dtype)
+        if r is not None:
+            a.residual = rs.data_ptr()
+            h = x.new_empty(x.shape)
+            a.sum = h.data_ptr()
+        if ent.fmt:
+            scales = x.new_empty(ent.scales_shape, dtype=torch.uint8)
+            a.scales = scales.data_ptr()
+        a.x, a.weight, a.out = xs.data_ptr(), ws.data_ptr(), out.data_ptr()
+    idx = ent.index
+    if idx != torch._C._cuda_getDevice():
+        with torch.cuda.device(idx):
+            _lib.check(ent.fn(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(idx)), "qik_residual_rms_norm")
+    else:
+        st = ent.fn(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(idx))
+        if st:
+            _lib.check(st, "qik_residual_rms_norm")
+    if scales is not None:
+        out = MXTensor._make(out, scales, out_format, x.shape)
+    return out if r is None else (out, h)
+
+
+class _NormCall:
+    """What one geometry of fused_residual_rms_norm needs at call time; no tensor."""
+
+    __slots__ = ("args", "fn", "index", "fmt", "like", "copy", "out_shape", "out_dtype", "scales_shape")
+
+
+# Prepared calls by the operands' geometry (shapes, strides, types, devices and
+# alignments: see fused_residual_rms_norm).
+_NORM_CALLS: dict = {}
+
+
+def _prepare_norm(x, residual, weight, eps, out_format) -> _NormCall:
     fmt = _lib.MX_NONE if out_format is None else MX_FORMATS[_check_format(out_format)]
     if x.dtype not in _NORM_DTYPES:
         raise ValueError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
@@ -224,27 +281,30 @@ def fused_residual_rms_norm(
         raise ValueError(f"weight must be [{D}] on {x.device}, got {tuple(weight.shape)} on {weight.device}")
     if weight.dtype != torch.float32 and weight.dtype != x.dtype:
         raise ValueError(f"weight must be fp32 or {x.dtype}, got {weight.dtype}")
-    x2 = _norm_rows(x, fmt)
-    r2 = None if residual is None else _norm_rows(residual, fmt)
-    if not weight.is_contiguous() or (fmt and weight.data_ptr() % 16 != 0):
-        weight = weight.clone(memory_format=torch.contiguous_format)
-    M = x2.shape[0]
-    h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    scales = None
-    if fmt:
-        out = torch.empty(_code_shape(x.shape, out_format), dtype=_CODE_DTYPE[out_format], device=x.device)
-        scales = torch.empty(_scales_shape(M, D), dtype=torch.uint8, device=x.device)
-    else:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a = _lib.QikResidualRmsNormArgs(
-        _lib.ABI_VERSION, _NORM_DTYPES[x.dtype], fmt, _NORM_DTYPES[weight.dtype], x2.data_ptr(),
-        None if r2 is None else r2.data_ptr(), weight.data_ptr(), None if h is None else h.data_ptr(), out.data_ptr(),
-        None if scales is None else scales.data_ptr(), M, D, _row_stride(x2), D if r2 is None else _row_stride(r2),
-        float(eps))
-    _on_device(x.device, _lib.load().qik_residual_rms_norm, "qik_residual_rms_norm", ctypes.byref(a))
-    if fmt:
-        out = MXTensor._make(out, scales, out_format, x.shape)
-    return out if residual is None else (out, h)
+    xs, rs, ws = _norm_copies(x, residual, weight, fmt)
+    M = xs.shape[0]
+    c = _NormCall()
+    c.fn = _lib.load().qik_residual_rms_norm
+    c.index, c.fmt = x.device.index, fmt
+    # a view of an operand at the operand's own address needs no work per call
+    c.copy = M > 0 and (xs.data_ptr() != x.data_ptr() or ws.data_ptr() != weight.data_ptr()
+                        or (rs is not None and rs.data_ptr() != residual.data_ptr()))
+    c.like = not fmt and not c.copy and x.is_contiguous()
+    c.out_shape = _code_shape(x.shape, out_format) if fmt else x.shape
+    c.out_dtype = _CODE_DTYPE[out_format] if fmt else x.dtype
+    c.scales_shape = _scales_shape(M, D) if fmt else None
+    c.args = _lib.QikResidualRmsNormArgs(
+        _lib.ABI_VERSION, _NORM_DTYPES[x.dtype], fmt, _NORM_DTYPES[weight.dtype], None, None, None, None, None, None, M, D,
+        _row_stride(xs), D if rs is None else _row_stride(rs), float(eps))
+    return c
+
+
+def _norm_copies(x, residual, weight, fmt: int):
+    """The operands as rows in a layout that the kernel takes: copies where they have another."""
+    w = weight
+    if not w.is_contiguous() or (fmt and w.data_ptr() % 16 != 0):
+        w = w.clone(memory_format=torch.contiguous_format)
+    return _norm_rows(x, fmt), None if residual is None else _norm_rows(residual, fmt), w
 
 
 def _norm_rows(t: torch.Tensor, fmt: int) -> torch.Tensor:

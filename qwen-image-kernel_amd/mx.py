@@ -34,6 +34,12 @@ _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torc
 _OUT_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 _MAX_K = 262144
 
+# argument structs without addresses, by the geometry that they were checked
+# for: (shape, format, dtype, device) here, see quantize_mx and mx_linear
+_DEQUANT_CALLS: dict = {}
+_QUANT_CALLS: dict = {}
+_PRODUCT_CALLS: dict = {}
+
 # scratch of the linears and K-split products, one per (device index, stream): see _workspace
 _WS: dict = {}
 
@@ -76,7 +82,7 @@ class MXTensor:
     ``[..., K / 32]``; ``from_block_scales`` takes them so.
     """
 
-    __slots__ = ("codes", "scales", "fmt", "shape")
+    __slots__ = ("_codes", "_scales", "_fmt", "_shape")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str):
         _check_format(fmt)
@@ -84,22 +90,22 @@ class MXTensor:
             raise ValueError(f"{fmt} codes must be {_CODE_DTYPE[fmt]}, got {codes.dtype}")
         K = codes.shape[-1] * (2 if fmt == "mxfp4" else 1)
         _check_width(K)
-        self.shape = torch.Size((*codes.shape[:-1], K))
+        shape = torch.Size((*codes.shape[:-1], K))
         if not codes.is_contiguous() or codes.data_ptr() % 16 != 0:
             codes = codes.clone(memory_format=torch.contiguous_format)
-        want = _scales_shape(_rows(self.shape), K)
+        want = _scales_shape(_rows(shape), K)
         if scales.dtype != torch.uint8 or tuple(scales.shape) != want:
             raise ValueError(f"scales must be uint8 {want}, got {scales.dtype} {tuple(scales.shape)}")
         if scales.device != codes.device:
             raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
         if not scales.is_contiguous() or scales.data_ptr() % 16 != 0:
             scales = scales.clone(memory_format=torch.contiguous_format)
-        self.codes, self.scales, self.fmt = codes, scales, fmt
+        self._codes, self._scales, self._fmt, self._shape = codes, scales, fmt, shape
 
     @staticmethod
     def _make(codes, scales, fmt, shape) -> "MXTensor":
         t = MXTensor.__new__(MXTensor)
-        t.codes, t.scales, t.fmt, t.shape = codes, scales, fmt, shape
+        t._codes, t._scales, t._fmt, t._shape = codes, scales, fmt, shape
         return t
 
     @staticmethod
@@ -127,36 +133,62 @@ class MXTensor:
         return full[:M, :K // MX_BLOCK].reshape(*self.shape[:-1], K // MX_BLOCK)
 
     @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
+
+    @property
+    def fmt(self) -> str:
+        return self._fmt
+
+    @property
+    def shape(self) -> torch.Size:
+        return self._shape
+
+    @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self._codes.device
 
     def to(self, device) -> "MXTensor":
         return MXTensor._make(self.codes.to(device), self.scales.to(device), self.fmt, self.shape)
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values, ``element * 2^(e - 127)`` rounded once to dtype (bf16, fp16 or fp32; exact in bf16 and fp32)."""
-        if dtype not in _DTYPES:
-            raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
-        if not self.codes.is_cuda:
-            raise ValueError("dequantize runs on a HIP device; move the tensor there first")
-        out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
-        a = _lib.QikMxDequantArgs(_lib.ABI_VERSION, _DTYPES[dtype], MX_FORMATS[self.fmt], 0, self.codes.data_ptr(),
-                                  self.scales.data_ptr(), out.data_ptr(), _rows(self.shape), self.shape[-1])
-        _on_device(out.device, _lib.load().qik_mx_dequantize, "qik_mx_dequantize", ctypes.byref(a))
+        codes, shape = self._codes, self._shape
+        key = (shape, self._fmt, dtype, codes.device)
+        args = _DEQUANT_CALLS.get(key)
+        if args is None:
+            if dtype not in _DTYPES:
+                raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
+            if not codes.is_cuda:
+                raise ValueError("dequantize runs on a HIP device; move the tensor there first")
+            args = _lib.QikMxDequantArgs(_lib.ABI_VERSION, _DTYPES[dtype], MX_FORMATS[self._fmt], 0, None, None, None,
+                                         _rows(shape), shape[-1])
+            if len(_DEQUANT_CALLS) >= 64:
+                _DEQUANT_CALLS.clear()
+            _DEQUANT_CALLS[key] = args
+        out = codes.new_empty(shape, dtype=dtype)
+        a = _lib.QikMxDequantArgs.from_buffer_copy(args)
+        a.codes, a.scales, a.out = codes.data_ptr(), self._scales.data_ptr(), out.data_ptr()
+        _on_device(codes.device.index, _lib.load().qik_mx_dequantize, "qik_mx_dequantize", a)
         return out
 
     def __repr__(self) -> str:
         return f"MXTensor({tuple(self.shape)}, fmt={self.fmt!r}, device={str(self.device)!r})"
 
 
-def _on_device(dev: torch.device, fn, name: str, *args) -> None:
-    """fn(*args, current stream of dev) with dev current."""
-    idx = dev.index
-    if idx != torch.cuda.current_device():
+def _on_device(idx: int, fn, name: str, args) -> None:
+    """fn(args, current stream of device idx) with that device current."""
+    if idx != torch._C._cuda_getDevice():
         with torch.cuda.device(idx):
-            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(idx)), name)
+            _lib.check(fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(idx)), name)
     else:
-        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(idx)), name)
+        st = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(idx))
+        if st:
+            _lib.check(st, name)
 
 
 def _as_rows(x: torch.Tensor) -> torch.Tensor:
@@ -177,6 +209,33 @@ def quantize_mx(x: torch.Tensor, fmt: str = "mxfp4") -> MXTensor:
 
     A CPU tensor is quantised on the CPU by the library's host routine, to the
     same bytes, so that a model can be converted on a machine without a GPU."""
+    # one lookup per call, as in fused_residual_rms_norm
+    key = (x.shape, x.stride(), x.dtype, x.device, fmt)
+    ent = _QUANT_CALLS.get(key)
+    if ent is None:
+        ent = _prepare_quant(x, fmt)
+        if len(_QUANT_CALLS) >= 64:
+            _QUANT_CALLS.clear()
+        _QUANT_CALLS[key] = ent
+    x2 = _as_rows(x) if ent.copy else x
+    codes = x.new_empty(ent.code_shape, dtype=ent.code_dtype)
+    scales = x.new_empty(ent.scales_shape, dtype=torch.uint8)
+    a = _lib.QikMxQuantArgs.from_buffer_copy(ent.args)
+    a.x, a.codes, a.scales = x2.data_ptr(), codes.data_ptr(), scales.data_ptr()
+    if ent.index is not None:
+        _on_device(ent.index, ent.fn, "qik_mx_quantize", a)
+    else:
+        _lib.check(_lib.load().qik_mx_quantize_host(ctypes.byref(a), torch.get_num_threads()), "qik_mx_quantize_host")
+    return MXTensor._make(codes, scales, fmt, x.shape)
+
+
+class _QuantCall:
+    """What one geometry of quantize_mx needs at call time; no tensor."""
+
+    __slots__ = ("args", "fn", "index", "copy", "code_shape", "code_dtype", "scales_shape")
+
+
+def _prepare_quant(x, fmt) -> _QuantCall:
     _check_format(fmt)
     if x.dtype not in _DTYPES:
         raise ValueError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
@@ -188,15 +247,14 @@ def quantize_mx(x: torch.Tensor, fmt: str = "mxfp4") -> MXTensor:
     _check_width(K)
     x2 = _as_rows(x)
     M = x2.shape[0]
-    codes = torch.empty(_code_shape(x.shape, fmt), dtype=_CODE_DTYPE[fmt], device=x.device)
-    scales = torch.empty(_scales_shape(M, K), dtype=torch.uint8, device=x.device)
-    a = _lib.QikMxQuantArgs(_lib.ABI_VERSION, _DTYPES[x.dtype], MX_FORMATS[fmt], 0, x2.data_ptr(), codes.data_ptr(),
-                            scales.data_ptr(), M, K, _row_stride(x2))
-    if x.is_cuda:
-        _on_device(x.device, _lib.load().qik_mx_quantize, "qik_mx_quantize", ctypes.byref(a))
-    else:
-        _lib.check(_lib.load().qik_mx_quantize_host(ctypes.byref(a), torch.get_num_threads()), "qik_mx_quantize_host")
-    return MXTensor._make(codes, scales, fmt, x.shape)
+    c = _QuantCall()
+    c.fn = _lib.load().qik_mx_quantize
+    c.index = x.device.index if x.is_cuda else None
+    c.copy = M > 0 and x2.data_ptr() != x.data_ptr()  # a view at x's own address needs no work per call
+    c.code_shape, c.code_dtype, c.scales_shape = _code_shape(x.shape, fmt), _CODE_DTYPE[fmt], _scales_shape(M, K)
+    c.args = _lib.QikMxQuantArgs(_lib.ABI_VERSION, _DTYPES[x.dtype], MX_FORMATS[fmt], 0, None, None, None, M, K,
+                                 _row_stride(x2))
+    return c
 
 
 def _workspace(dev: torch.device, stream: int, nbytes: int):
@@ -232,38 +290,77 @@ def mx_linear(
     """``round(a . w^T + bias)``, ``[..., N]``: the values multiplied exactly, summed in fp32, rounded once."""
     if not isinstance(a, MXTensor) or not isinstance(w, MXTensor):
         raise ValueError("mx_linear takes MXTensor operands (quantize_mx makes them)")
+    codes = a._codes
+    key = (a._shape, a._fmt, w._shape, w._fmt, codes.device, w._codes.device, out_dtype,
+           None if bias is None else (bias.shape, bias.stride(), bias.dtype, bias.device))
+    ent = _PRODUCT_CALLS.get(key)
+    if ent is None:
+        ent = _prepare_product(a, w, bias, out_dtype)
+        if len(_PRODUCT_CALLS) >= 64:
+            _PRODUCT_CALLS.clear()
+        _PRODUCT_CALLS[key] = ent
+    out = codes.new_empty(ent.shape, dtype=out_dtype)
+    if ent.args is None:
+        return out
+    g = _lib.QikMxGemmArgs.from_buffer_copy(ent.args)
+    g.a, g.a_scales, g.out = codes.data_ptr(), a._scales.data_ptr(), out.data_ptr()
+    g.w, g.w_scales = w._codes.data_ptr(), w._scales.data_ptr()
+    if bias is not None:
+        if ent.cast_bias:
+            bias = bias.reshape(-1).to(out_dtype).contiguous()
+        g.bias = bias.data_ptr()
+    idx = ent.index
+    if idx != torch._C._cuda_getDevice():
+        with torch.cuda.device(idx):
+            _launch_product(ent, g, codes.device)
+    else:
+        _launch_product(ent, g, codes.device)
+    return out
+
+
+class _ProductCall:
+    """What one geometry of mx_linear needs at call time; no tensor."""
+
+    __slots__ = ("args", "fn", "index", "shape", "ws_bytes", "cast_bias")
+
+
+def _launch_product(ent: _ProductCall, g, dev: torch.device) -> None:
+    stream = torch._C._cuda_getCurrentRawStream(ent.index)
+    ws = None if ent.ws_bytes == 0 else _workspace(dev, stream, ent.ws_bytes).data_ptr()
+    _lib.check(ent.fn(ctypes.byref(g), ws, ent.ws_bytes, stream), "qik_mx_gemm")
+
+
+def _prepare_product(a: MXTensor, w: MXTensor, bias, out_dtype) -> _ProductCall:
     if w.fmt != "mxfp4" or len(w.shape) != 2:
         raise ValueError(f"the weight must be mxfp4 [N, K], got {w.fmt} {tuple(w.shape)}")
     if a.shape[-1] != w.shape[1]:
         raise ValueError(f"shapes {tuple(a.shape)} and {tuple(w.shape)} do not multiply as A . W^T")
     if out_dtype not in _OUT_DTYPES:
         raise ValueError(f"out_dtype must be bf16 or fp16, got {out_dtype}")
-    dev = a.codes.device
+    dev = a.device
     if not a.codes.is_cuda:
         raise ValueError("mx_linear runs on a HIP device; move the operands there first")
     N, K = w.shape
     for name, t in (("w", w.codes), ("bias", bias)):
         if t is not None and t.device != dev:
             raise ValueError(f"{name} must be on {dev}")
-    if bias is not None:
-        if bias.numel() != N:
-            raise ValueError(f"bias must have {N} elements, got {bias.numel()}")
-        bias = bias.reshape(-1).to(out_dtype).contiguous()
+    if bias is not None and bias.numel() != N:
+        raise ValueError(f"bias must have {N} elements, got {bias.numel()}")
+    c = _ProductCall()
+    c.fn, c.index, c.shape = _lib.load().qik_mx_gemm, dev.index, (*a.shape[:-1], N)
+    c.cast_bias = bias is not None and (bias.dtype != out_dtype or not bias.is_contiguous())
+    c.args, c.ws_bytes = None, 0
     M = _rows(a.shape)
-    out = torch.empty((*a.shape[:-1], N), dtype=out_dtype, device=dev)
-    if out.numel() == 0:
-        return out
-    g = _gemm_args(a.fmt, w.codes, w.scales, bias, out_dtype, M, N, K)
-    g.a, g.a_scales, g.out = a.codes.data_ptr(), a.scales.data_ptr(), out.data_ptr()
-    lib = _lib.load()
+    if M == 0 or N == 0:
+        return c
+    g = _gemm_args(a.fmt, w.codes, w.scales, None, out_dtype, M, N, K)
+    g.a, g.a_scales, g.out = a.codes.data_ptr(), a.scales.data_ptr(), w.codes.data_ptr()  # the size does not go by out
+    need = ctypes.c_int64(0)
     with torch.cuda.device(dev):
-        need = ctypes.c_int64(0)
-        _lib.check(lib.qik_mx_gemm_workspace_size(ctypes.byref(g), ctypes.byref(need)), "qik_mx_gemm")
-        stream = torch._C._cuda_getCurrentRawStream(dev.index)
-        ws = _workspace(dev, stream, need.value)
-        _lib.check(lib.qik_mx_gemm(ctypes.byref(g), None if ws is None else ws.data_ptr(), need.value, stream),
-                   "qik_mx_gemm")
-    return out
+        _lib.check(_lib.load().qik_mx_gemm_workspace_size(ctypes.byref(g), ctypes.byref(need)), "qik_mx_gemm")
+    g.a = g.a_scales = g.w = g.w_scales = g.out = None
+    c.args, c.ws_bytes = g, need.value
+    return c
 
 
 class _LinearCall:
@@ -272,7 +369,7 @@ class _LinearCall:
     the buffers it was made for (with their addresses), so that it is used only
     while the module still holds exactly them and never keeps them alive."""
 
-    __slots__ = ("args", "index", "shape", "ws_bytes", "refs", "addresses", "copy", "cast_bias")
+    __slots__ = ("args", "index", "shape", "ws_bytes", "refs", "addresses", "copy", "cast_bias", "fn")
 
     def matches(self, weight, scales, bias) -> bool:
         r = self.refs
@@ -322,7 +419,8 @@ class MXFP4Linear(nn.Module):
     def forward(self, x) -> torch.Tensor:
         if isinstance(x, MXTensor):
             return mx_linear(x, self.mx_weight(), self.bias)
-        weight, scales, bias = self.weight, self.weight_scale, self.bias
+        buffers = self._buffers
+        weight, scales, bias = buffers["weight"], buffers["weight_scale"], buffers.get("bias")
         key = (x.shape, x.stride(), x.dtype, x.device, self.activations)
         calls = self.__dict__.get("_calls")
         if calls is None:
@@ -333,10 +431,10 @@ class MXFP4Linear(nn.Module):
             if len(calls) >= 8:
                 calls.clear()
             calls[key] = ent
-        out = torch.empty(ent.shape, dtype=torch.bfloat16, device=x.device)
+        out = x.new_empty(ent.shape, dtype=torch.bfloat16)
         if ent.args is not None:
             idx = ent.index
-            if idx != torch.cuda.current_device():
+            if idx != torch._C._cuda_getDevice():
                 with torch.cuda.device(idx):
                     self._launch(ent, x, out, idx)
             else:
@@ -344,7 +442,6 @@ class MXFP4Linear(nn.Module):
         return out if x.dtype == torch.bfloat16 else out.to(x.dtype)
 
     def _launch(self, ent: _LinearCall, x, out, idx: int) -> None:
-        stream = torch._C._cuda_getCurrentRawStream(idx)
         x2 = _as_rows(x) if ent.copy else x
         a = _lib.QikMxLinearArgs.from_buffer_copy(ent.args)
         a.x = x2.data_ptr()
@@ -352,9 +449,11 @@ class MXFP4Linear(nn.Module):
         if ent.cast_bias:  # the module was moved to another dtype
             bias = self.bias.to(torch.bfloat16).contiguous()
             a.g.bias = bias.data_ptr()
-        ws = _workspace(x.device, stream, ent.ws_bytes)
-        _lib.check(_lib.load().qik_mx_linear(ctypes.byref(a), None if ws is None else ws.data_ptr(), ent.ws_bytes,
-                                             stream), "qik_mx_linear")
+        stream = torch._C._cuda_getCurrentRawStream(idx)
+        ws = None if ent.ws_bytes == 0 else _workspace(x.device, stream, ent.ws_bytes).data_ptr()
+        st = ent.fn(ctypes.byref(a), ws, ent.ws_bytes, stream)
+        if st:
+            _lib.check(st, "qik_mx_linear")
 
     def _prepare(self, x, weight, scales, bias) -> _LinearCall:
         """Checks and the argument struct of one input geometry."""
@@ -376,6 +475,7 @@ class MXFP4Linear(nn.Module):
                 raise ValueError(f"{name} must be {shape}{'' if name == 'bias' else ' contiguous uint8, 16-byte aligned'}, "
                                  f"got {t.dtype} {tuple(t.shape)}")
         c = _LinearCall()
+        c.fn = _lib.load().qik_mx_linear
         c.index = x.device.index
         c.shape = (*x.shape[:-1], N)
         c.refs = (weakref.ref(weight), weakref.ref(scales), None if bias is None else weakref.ref(bias))
