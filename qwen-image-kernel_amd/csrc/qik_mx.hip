@@ -36,7 +36,6 @@ __device__ __forceinline__ int64_t scale_at(int64_t row, int block, int C) {
 // ---------------------------------------------------------------------------
 
 constexpr int QT = 256;  // threads per workgroup
-constexpr int QU = 4;    // (row, 256-k chunk) units per half wave in flight
 constexpr int MAX_K = 262144;
 
 struct QuantParams {
@@ -52,7 +51,7 @@ struct QuantParams {
 
 // Row and chunk of the unit `local` units after the workgroup's first.  The
 // row of the first is a 64-bit division of uniform values; the rest is below C
-// + 8 QU, where the product with ceil(2^32 / C) is exact (C <= 1024).
+// + 16, where the product with ceil(2^32 / C) is exact (C <= 1024).
 __device__ __forceinline__ void unit_at(const QuantParams& p, int64_t first, int local, int64_t& row, int& c) {
   const int64_t r0 = first / p.C;
   const unsigned off = (unsigned)(first - r0 * p.C) + (unsigned)local;
@@ -62,9 +61,13 @@ __device__ __forceinline__ void unit_at(const QuantParams& p, int64_t first, int
 }
 
 // 32 threads take a unit, one row's 256 elements (8 blocks, 8 scale bytes in a
-// row): 4 units per half wave, all loads ahead of the first conversion.
-// Padding rows and blocks read nothing and get a scale of 0.
-template <int DT, int FMT, bool ALIGNED>
+// row), QU units one after the other, all loads ahead of the first conversion.
+// Padding rows and blocks read nothing and get a scale of 0.  Bound by HBM: bf16
+// 4352 x 4096 to MXFP4 10.3 us (4.4 TB/s), fp32 12288 x 4096 41 us (5.5 TB/s).
+// One unit keeps the small calls short (bf16 203 x 12288 3.0 us against 3.3 with
+// two and 3.9 with four), two do better on long 16-bit ones (16000 x 3200 26.5
+// against 28.5; with four 32.0), one on fp32 (41.1, 43.4, 45.2).
+template <int DT, int FMT, bool ALIGNED, int QU>
 __global__ void __launch_bounds__(QT) quant_kernel(const QuantParams p) {
   constexpr int HW = QT / 32;
   const int hw = threadIdx.x >> 5, t = threadIdx.x & 31;
@@ -122,8 +125,9 @@ __device__ __forceinline__ float scale_value(unsigned byte) {
   return __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7fc00000u : byte << 23);
 }
 
-// The quantiser's units over the rows themselves, each read and written whole.
-template <int DT, int FMT>
+// The quantiser's units over the rows themselves, each read and written whole
+// (MXFP4 of 4352 x 4096 to bf16 9.3 us, 4.8 TB/s).
+template <int DT, int FMT, int QU>
 __global__ void __launch_bounds__(QT) dequant_kernel(const QuantParams p) {
   constexpr int HW = QT / 32;
   const int hw = threadIdx.x >> 5, t = threadIdx.x & 31;
@@ -175,10 +179,42 @@ struct NormParams {
   double eps;
 };
 
+// v of the lane that DPP control CTRL names (0.0 where there is none, or where
+// ROWS masks this lane's row of 16 off)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_move(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)u, CTRL, ROWS, 0xf, true);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(u >> 32), CTRL, ROWS, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// the sum of v over the LANES (16 or 64) lanes of a group, in each of them:
+// rotations within rows of 16, then rows 0 -> 1 and 2 -> 3, then 1 -> 2 and 3
+template <int LANES>
+__device__ __forceinline__ double lane_sum(double v) {
+  v += dpp_move<0x128, 0xf>(v);  // row_ror:8
+  v += dpp_move<0x124, 0xf>(v);
+  v += dpp_move<0x122, 0xf>(v);
+  v += dpp_move<0x121, 0xf>(v);
+  if constexpr (LANES == 64) {
+    v += dpp_move<0x142, 0xa>(v);  // row_bcast:15
+    v += dpp_move<0x143, 0xc>(v);  // row_bcast:31
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)u, 63);
+    const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(u >> 32), 63);
+    v = __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  }
+  return v;
+}
+
 // LPR threads per row, VPT vectors of 8 elements per thread: the row is read
 // once and stays in registers, packed, between the sum of squares and the
 // output.  The squares are summed in fp64 (each exact there), so the sum does
-// not depend on the order to anything that its fp32 root shows.
+// not depend on the order to anything that its fp32 root shows.  Bound by HBM:
+// bf16 4352 x 4096 with a residual 29.1 us (4.9 TB/s), to MXFP8 27.7 (4.5); rows
+// at odd addresses go slower (fp16 9001 x 1111 13.6 us, 2.9 TB/s; 1112 wide 10.1,
+// 4.0 TB/s).
 template <int DT, int FMT, bool RES, bool ALIGNED, int LPR, int VPT>
 __global__ void __launch_bounds__(LPR < 256 ? 256 : LPR) norm_kernel(const NormParams p) {
 #pragma clang fp contract(off)
@@ -231,8 +267,7 @@ __global__ void __launch_bounds__(LPR < 256 ? 256 : LPR) norm_kernel(const NormP
 #pragma unroll
     for (int k = 0; k < 8; ++k) ss = __builtin_fma((double)f[k], (double)f[k], ss);
   }
-#pragma unroll
-  for (int k = 32; k >= 1; k >>= 1) ss += __shfl_xor(ss, k);
+  ss = lane_sum<(LPR < 64 ? LPR : 64)>(ss);
   if constexpr (LPR > 64) {
     __shared__ double part[LPR / 64];
     if ((t & 63) == 0) part[t >> 6] = ss;
@@ -353,6 +388,16 @@ QuantParams unit_params(int64_t M, int64_t K, int64_t rows) {
   return p;
 }
 
+// units from which a half wave takes two (quant_kernel)
+constexpr int64_t TWO_UNITS = 65536;
+
+template <int DT, int FMT>
+const void* quant_fn(bool al, int qu) {
+  if (DT != QIK_DTYPE_FP32 && qu == 2)
+    return al ? (const void*)quant_kernel<DT, FMT, true, 2> : (const void*)quant_kernel<DT, FMT, false, 2>;
+  return al ? (const void*)quant_kernel<DT, FMT, true, 1> : (const void*)quant_kernel<DT, FMT, false, 1>;
+}
+
 template <int DT>
 int launch_quant(const qik_mx_quant_args* a, hipStream_t s) {
   QuantParams p = unit_params(a->M, a->K, cdiv(a->M, 32) * 32);
@@ -361,10 +406,9 @@ int launch_quant(const qik_mx_quant_args* a, hipStream_t s) {
   p.scales = static_cast<unsigned char*>(a->scales);
   p.ldx = a->ldx;
   const bool al = aligned_to(a->x, 16) && (a->M == 1 || a->ldx * elem_bytes<DT>() % 16 == 0);
-  const void* fn = a->format == QIK_MXFP4
-                       ? (al ? (const void*)quant_kernel<DT, QIK_MXFP4, true> : (const void*)quant_kernel<DT, QIK_MXFP4, false>)
-                       : (al ? (const void*)quant_kernel<DT, QIK_MXFP8, true> : (const void*)quant_kernel<DT, QIK_MXFP8, false>);
-  return launch(fn, cdiv(p.units, QT / 32 * QU), QT, &p, s);
+  const int qu = DT != QIK_DTYPE_FP32 && p.units >= TWO_UNITS ? 2 : 1;
+  const void* fn = a->format == QIK_MXFP4 ? quant_fn<DT, QIK_MXFP4>(al, qu) : quant_fn<DT, QIK_MXFP8>(al, qu);
+  return launch(fn, cdiv(p.units, QT / 32 * qu), QT, &p, s);
 }
 
 template <int DT>
@@ -373,9 +417,11 @@ int launch_dequant(const qik_mx_dequant_args* a, hipStream_t s) {
   p.codes = static_cast<unsigned char*>(const_cast<void*>(a->codes));
   p.scales = static_cast<unsigned char*>(const_cast<void*>(a->scales));
   p.out = static_cast<char*>(a->out);
-  const void* fn = a->format == QIK_MXFP4 ? (const void*)dequant_kernel<DT, QIK_MXFP4>
-                                          : (const void*)dequant_kernel<DT, QIK_MXFP8>;
-  return launch(fn, cdiv(p.units, QT / 32 * QU), QT, &p, s);
+  const bool two = p.units >= TWO_UNITS;
+  const void* fn = a->format == QIK_MXFP4
+                       ? (two ? (const void*)dequant_kernel<DT, QIK_MXFP4, 2> : (const void*)dequant_kernel<DT, QIK_MXFP4, 1>)
+                       : (two ? (const void*)dequant_kernel<DT, QIK_MXFP8, 2> : (const void*)dequant_kernel<DT, QIK_MXFP8, 1>);
+  return launch(fn, cdiv(p.units, QT / 32 * (two ? 2 : 1)), QT, &p, s);
 }
 
 template <int DT, int FMT, bool RES, bool ALIGNED, int LPR, int VPT>
@@ -386,12 +432,24 @@ int launch_norm_shape(const NormParams& p0, hipStream_t s) {
   return launch((const void*)norm_kernel<DT, FMT, RES, ALIGNED, LPR, VPT>, cdiv(rows, NT / LPR), NT, &p, s);
 }
 
+// The fewest lanes that hold a row in at most 64 bytes a lane of x (a wave of
+// its own needs no barrier; fp32 2048 wide 26.5 us with 256 lanes of one vector
+// against 30.5 with 64 of four, 5000 rows; bf16 4096 wide 29.1 with 256 of two
+// against 33.6 with 64 of eight), 16 of a wave for rows up to 256 (16384 rows of
+// 128 4.9 us against 10.3 with a wave each).
 template <int DT, int FMT, bool RES, bool ALIGNED>
 int launch_norm(const NormParams& p, hipStream_t s) {
+  if (p.D <= 128) return launch_norm_shape<DT, FMT, RES, ALIGNED, 16, 1>(p, s);
+  if (p.D <= 256) return launch_norm_shape<DT, FMT, RES, ALIGNED, 16, 2>(p, s);
   if (p.D <= 512) return launch_norm_shape<DT, FMT, RES, ALIGNED, 64, 1>(p, s);
   if (p.D <= 1024) return launch_norm_shape<DT, FMT, RES, ALIGNED, 64, 2>(p, s);
-  if (p.D <= 2048) return launch_norm_shape<DT, FMT, RES, ALIGNED, 64, 4>(p, s);
+  if constexpr (DT != QIK_DTYPE_FP32) {
+    if (p.D <= 1536) return launch_norm_shape<DT, FMT, RES, ALIGNED, 64, 3>(p, s);
+    if (p.D <= 2048) return launch_norm_shape<DT, FMT, RES, ALIGNED, 64, 4>(p, s);
+  }
+  if (p.D <= 2048) return launch_norm_shape<DT, FMT, RES, ALIGNED, 256, 1>(p, s);
   if (p.D <= 4096) return launch_norm_shape<DT, FMT, RES, ALIGNED, 256, 2>(p, s);
+  if (p.D <= 6144) return launch_norm_shape<DT, FMT, RES, ALIGNED, 256, 3>(p, s);
   if (p.D <= 8192) return launch_norm_shape<DT, FMT, RES, ALIGNED, 256, 4>(p, s);
   return launch_norm_shape<DT, FMT, RES, ALIGNED, 1024, 4>(p, s);
 }
