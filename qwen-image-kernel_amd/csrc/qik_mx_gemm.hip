@@ -70,6 +70,7 @@ struct MxGemmParams {
   int ksplit;        // split launches: k-slices per tile (region 0 only)
   float* partial;    // split launches: [ksplit][M][ldp] fp32 sums of each slice
   int64_t ldp;       // N rounded up to 4
+  unsigned row_magic;  // rows of elements: 2^32 / (K / 8), rounded up
 };
 
 // round to nearest even into bf16 or fp16
@@ -549,10 +550,8 @@ __global__ void __launch_bounds__(256) join_kernel(const MxGemmParams p) {
 // workgroup quantises into LDS first.
 enum { SRC_CODES = -1 };  // else QIK_DTYPE_BF16, _FP16 or _FP32
 
-// Most elements of A that a workgroup quantises for itself.  Every workgroup
-// does all of them, so it pays while they are few: one token, or a few of a
-// narrow layer.
-constexpr int RAW_ELEMS = 16384;
+// Most elements of A that a workgroup quantises for itself (takes_raw).
+constexpr int RAW_ELEMS = 32768;
 
 // KW waves of a workgroup share K by chunks of 256; BC chunks of W are in
 // flight ahead of the ones that are multiplied.
@@ -665,26 +664,29 @@ __global__ void __launch_bounds__(64 * KW) rows_kernel(const MxGemmParams p) {
   load_w(0, c0);
   if constexpr (RAW) {  // while the first weights are on their way
     constexpr int FMT = A8 ? QIK_MXFP8 : QIK_MXFP4;
-    constexpr int IT = RAW_ELEMS / 8 / (64 * KW);
+    constexpr int IT = 4;  // vectors of a thread in flight
     const int per_row = p.K / 8, total = p.M * per_row;  // vectors of 8; a multiple of 4 a row: whole quads
-    Raw8<SRC> x[IT];
+    for (int v0 = threadIdx.x; v0 < total; v0 += IT * 64 * KW) {
+      Raw8<SRC> x[IT];
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      const int v = threadIdx.x + i * 64 * KW, m = v / per_row;
-      x[i] = Raw8<SRC>{};
-      if (v < total)
-        x[i] = load8<SRC, false>(reinterpret_cast<const char*>(p.a) + (m * p.lda + (v - m * per_row) * 8) * elem_bytes<SRC>());
-    }
+      for (int i = 0; i < IT; ++i) {
+        const int v = v0 + i * 64 * KW, m = (int)__umulhi((unsigned)v, p.row_magic);
+        x[i] = Raw8<SRC>{};
+        if (v < total)
+          x[i] = load8<SRC, false>(reinterpret_cast<const char*>(p.a) +
+                                   (m * p.lda + (v - m * per_row) * 8) * elem_bytes<SRC>());
+      }
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      const int v = threadIdx.x + i * 64 * KW;
-      if (v >= total) continue;
-      float f[8];
-      unpack8<SRC>(x[i], f);
-      unsigned w0, w1;
-      const unsigned byte = block_codes<FMT>(f, w0, w1);
-      store_codes<FMT>(lcodes, v, w0, w1);  // rows lie one behind the other
-      if ((v & 3) == 0) lscales[v / 4] = (unsigned char)byte;
+      for (int i = 0; i < IT; ++i) {
+        const int v = v0 + i * 64 * KW;
+        if (v >= total) continue;
+        float f[8];
+        unpack8<SRC>(x[i], f);
+        unsigned w0, w1;
+        const unsigned byte = block_codes<FMT>(f, w0, w1);
+        store_codes<FMT>(lcodes, v, w0, w1);  // rows lie one behind the other
+        if ((v & 3) == 0) lscales[v / 4] = (unsigned char)byte;
+      }
     }
     __syncthreads();
   }
@@ -819,19 +821,24 @@ int launch_rows_shape(MxGemmParams& p, const qik_mx_gemm_args* a, hipStream_t s)
                 s);
 }
 
+// Weight rows (in 16s) and waves of a workgroup.  From 8192 columns on there is
+// a workgroup of 16 rows for every second wave slot: four waves each, and 32 rows
+// where the codes of A are worth sharing (1 x 12288 x 4096 8.4 us with 16 rows, 9.1
+// with 32; 32 x 12288 x 4096 13.5 and 12.6).  Below, eight waves share a long K (1 x
+// 4096 x 4096 4.5 us, 5.0 with four; 1 x 4096 x 12288 9.3 and 11.8), or the
+// quantising of elements, which goes by threads.
 struct RowsPlan {
   int nb, kw;
 };
-RowsPlan choose_rows(int64_t M, int64_t N, int64_t K) {
-  return {N > 8192 && M > 8 ? 2 : 1, N <= 8192 && K > 7 * 256 ? 8 : 4};
+RowsPlan choose_rows(int64_t M, int64_t N, int64_t K, bool raw) {
+  return {N > 8192 && M > 8 ? 2 : 1, N > 8192 || (!raw && K <= 7 * 256) ? 4 : 8};
 }
 
 template <int SRC, bool A8, int MB>
 int launch_rows(MxGemmParams& p, const qik_mx_gemm_args* a, hipStream_t s) {
-  const RowsPlan plan = choose_rows(a->M, a->N, a->K);
-  if (plan.nb == 1)
-    return plan.kw == 4 ? launch_rows_shape<SRC, A8, MB, 1, 4>(p, a, s) : launch_rows_shape<SRC, A8, MB, 1, 8>(p, a, s);
-  return plan.kw == 4 ? launch_rows_shape<SRC, A8, MB, 2, 4>(p, a, s) : launch_rows_shape<SRC, A8, MB, 2, 8>(p, a, s);
+  const RowsPlan plan = choose_rows(a->M, a->N, a->K, SRC != SRC_CODES);
+  if (plan.nb == 2) return launch_rows_shape<SRC, A8, MB, 2, 4>(p, a, s);
+  return plan.kw == 4 ? launch_rows_shape<SRC, A8, MB, 1, 4>(p, a, s) : launch_rows_shape<SRC, A8, MB, 1, 8>(p, a, s);
 }
 
 // Time of a tile of each shape (qik_tile.h), for A in MXFP4 and in MXFP8: fitted
@@ -924,23 +931,40 @@ bool takes_rows(const qik_mx_gemm_args* a) {
   return a->M <= 16 || (a->M <= 32 && (a->N <= 4096 || a->N * a->K <= (1 << 24)));
 }
 
-// A product of elements that each workgroup quantises for itself.
-bool takes_raw(const qik_mx_gemm_args* a) { return a->M <= 16 && a->M * a->K <= RAW_ELEMS; }
+// A linear whose workgroups each quantise all of x for themselves saves a
+// launch: 2 us in a graph, 4 us of host time in a loop of calls.  It costs what a
+// CU's workgroups quantise, about 2.5 us for 32768 elements (in a graph 1 x 4096
+// x 4096 4.8 us against 6.5, 32 x 4096 x 1024 5.8 / 5.7, 4 x 12288 x 4096 11.1 /
+// 10.9, 17 x 5001 x 1504 6.7 / 6.3 and with MXFP8 9.1 / 6.6; called in a loop the
+// last takes 9 against 11.6).
+bool takes_raw(const qik_mx_gemm_args* a) {
+  if (!takes_rows(a) || a->M * a->K > RAW_ELEMS) return false;
+  const int64_t wgs = cdiv(a->N, 16 * choose_rows(a->M, a->N, a->K, true).nb);
+  return cdiv(wgs, 256) * a->M * a->K <= 2 * RAW_ELEMS;
+}
 
-int64_t partial_bytes(const qik_mx_gemm_args* a) {
-  if (takes_rows(a)) return 0;
-  const MxPlan plan = choose(a->M, a->N, a->K, a->a_format == QIK_MXFP8, device_cus());
-  return plan.slices > 1 ? (int64_t)plan.slices * a->M * cdiv(a->N, 4) * 4 * (int64_t)sizeof(float) : 0;
+// How a call is launched, and the bytes of its slices' sums.
+struct Launch {
+  bool rows;  // the few-rows kernel, else by plan
+  MxPlan plan;
+  int64_t partial_bytes;
+};
+Launch plan_launch(const qik_mx_gemm_args* a) {
+  Launch l = {takes_rows(a), {0, 0, false, 1, SPLIT64}, 0};
+  if (l.rows) return l;
+  l.plan = choose(a->M, a->N, a->K, a->a_format == QIK_MXFP8, device_cus());
+  if (l.plan.slices > 1) l.partial_bytes = (int64_t)l.plan.slices * a->M * cdiv(a->N, 4) * 4 * (int64_t)sizeof(float);
+  return l;
 }
 
 template <bool A8>
-int launch_gemm(const qik_mx_gemm_args* a, float* partial, hipStream_t s) {
+int launch_gemm(const qik_mx_gemm_args* a, const Launch& l, float* partial, hipStream_t s) {
   MxGemmParams p = gemm_params(a);
-  if (takes_rows(a)) return a->M <= 16 ? launch_rows<SRC_CODES, A8, 1>(p, a, s) : launch_rows<SRC_CODES, A8, 2>(p, a, s);
-  return launch_plan<A8>(p, a, choose(a->M, a->N, a->K, A8, device_cus()), partial, s);
+  if (l.rows) return a->M <= 16 ? launch_rows<SRC_CODES, A8, 1>(p, a, s) : launch_rows<SRC_CODES, A8, 2>(p, a, s);
+  return launch_plan<A8>(p, a, l.plan, partial, s);
 }
-int launch_gemm(const qik_mx_gemm_args* a, float* partial, hipStream_t s) {
-  return a->a_format == QIK_MXFP8 ? launch_gemm<true>(a, partial, s) : launch_gemm<false>(a, partial, s);
+int launch_gemm(const qik_mx_gemm_args* a, const Launch& l, float* partial, hipStream_t s) {
+  return a->a_format == QIK_MXFP8 ? launch_gemm<true>(a, l, partial, s) : launch_gemm<false>(a, l, partial, s);
 }
 
 template <int SRC>
@@ -948,7 +972,12 @@ int launch_raw(const qik_mx_linear_args* l, hipStream_t s) {
   MxGemmParams p = gemm_params(&l->g);
   p.a = static_cast<const unsigned char*>(l->x);
   p.lda = l->ldx;  // elements
-  return l->g.a_format == QIK_MXFP8 ? launch_rows<SRC, true, 1>(p, &l->g, s) : launch_rows<SRC, false, 1>(p, &l->g, s);
+  // v / (K / 8) = umulhi(v, magic) for v < RAW_ELEMS / 8 and K / 8 from 4 to 4096:
+  // the product is off by less than v (K / 8) / 2^32 < 1 / (K / 8)
+  p.row_magic = (unsigned)((((uint64_t)1 << 32) + p.K / 8 - 1) / (p.K / 8));
+  if (l->g.a_format == QIK_MXFP8)
+    return p.M <= 16 ? launch_rows<SRC, true, 1>(p, &l->g, s) : launch_rows<SRC, true, 2>(p, &l->g, s);
+  return p.M <= 16 ? launch_rows<SRC, false, 1>(p, &l->g, s) : launch_rows<SRC, false, 2>(p, &l->g, s);
 }
 
 inline int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -967,7 +996,7 @@ int qik_mx_gemm_workspace_size(const qik_mx_gemm_args* a, int64_t* bytes) {
   *bytes = 0;
   const int st = validate_gemm(a, true);
   if (st != QIK_OK || a->M == 0) return st;
-  *bytes = partial_bytes(a);
+  *bytes = plan_launch(a).partial_bytes;
   return QIK_OK;
 }
 
@@ -975,9 +1004,11 @@ int qik_mx_gemm(const qik_mx_gemm_args* a, void* workspace, int64_t workspace_by
   using namespace qik_mx;
   const int st = validate_gemm(a, true);
   if (st != QIK_OK || a->M == 0) return st;
-  const int64_t need = partial_bytes(a);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 256))) return QIK_ERR_WORKSPACE;
-  return launch_gemm(a, static_cast<float*>(workspace), static_cast<hipStream_t>(stream));
+  const Launch l = plan_launch(a);
+  if (l.partial_bytes > 0 &&
+      (workspace == nullptr || workspace_bytes < l.partial_bytes || !aligned_to(workspace, 256)))
+    return QIK_ERR_WORKSPACE;
+  return launch_gemm(a, l, static_cast<float*>(workspace), static_cast<hipStream_t>(stream));
 }
 
 // workspace of a linear: the split's sums, x's codes, x's scales
@@ -987,7 +1018,7 @@ int qik_mx_linear_workspace_size(const qik_mx_linear_args* a, int64_t* bytes) {
   *bytes = 0;
   const int st = validate_linear(a);
   if (st != QIK_OK || a->g.M == 0) return st;
-  if (!takes_raw(&a->g)) *bytes = round256(partial_bytes(&a->g)) + code_bytes(&a->g) + scale_bytes(&a->g);
+  if (!takes_raw(&a->g)) *bytes = round256(plan_launch(&a->g).partial_bytes) + code_bytes(&a->g) + scale_bytes(&a->g);
   return QIK_OK;
 }
 
@@ -1003,7 +1034,8 @@ int qik_mx_linear(const qik_mx_linear_args* a, void* workspace, int64_t workspac
       default: return launch_raw<QIK_DTYPE_FP32>(a, s);
     }
   }
-  const int64_t sums = round256(partial_bytes(&a->g)), codes = code_bytes(&a->g);
+  const Launch l = plan_launch(&a->g);
+  const int64_t sums = round256(l.partial_bytes), codes = code_bytes(&a->g);
   const int64_t need = sums + codes + scale_bytes(&a->g);
   if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 256)) return QIK_ERR_WORKSPACE;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
@@ -1024,7 +1056,7 @@ int qik_mx_linear(const qik_mx_linear_args* a, void* workspace, int64_t workspac
   q.ldx = a->ldx;
   const int qs = qik_mx_quantize(&q, stream);
   if (qs != QIK_OK) return qs;
-  return launch_gemm(&g, reinterpret_cast<float*>(ws), static_cast<hipStream_t>(stream));
+  return launch_gemm(&g, l, reinterpret_cast<float*>(ws), static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"
