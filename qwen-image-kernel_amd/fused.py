@@ -207,9 +207,9 @@ def fused_residual_rms_norm(
     gradients."""
     # one lookup per call: what depends on the operands' geometry alone (the
     # checks, the argument struct without addresses) is prepared once per key
-    r = residual
+    r, eps = residual, float(eps)
     key = (x.shape, x.stride(), x.dtype, x.device, weight.shape, weight.stride(), weight.dtype, weight.device, eps,
-           out_format, (x.data_ptr() | weight.data_ptr()) & 15,
+           out_format, x.data_ptr() & 15, weight.data_ptr() & 15,
            None if r is None else (r.shape, r.stride(), r.dtype, r.device, r.data_ptr() & 15))
     ent = _NORM_CALLS.get(key)
     if ent is None:
@@ -295,7 +295,7 @@ def _prepare_norm(x, residual, weight, eps, out_format) -> _NormCall:
     c.scales_shape = _scales_shape(M, D) if fmt else None
     c.args = _lib.QikResidualRmsNormArgs(
         _lib.ABI_VERSION, _NORM_DTYPES[x.dtype], fmt, _NORM_DTYPES[weight.dtype], None, None, None, None, None, None, M, D,
-        _row_stride(xs), D if rs is None else _row_stride(rs), float(eps))
+        _row_stride(xs), D if rs is None else _row_stride(rs), eps)
     return c
 
 

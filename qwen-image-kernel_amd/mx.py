@@ -40,9 +40,6 @@ _DEQUANT_CALLS: dict = {}
 _QUANT_CALLS: dict = {}
 _PRODUCT_CALLS: dict = {}
 
-# scratch of the linears and K-split products, one per (device index, stream): see _workspace
-_WS: dict = {}
-
 
 def _check_format(fmt: str) -> str:
     if fmt not in MX_FORMATS:
@@ -257,24 +254,6 @@ def _prepare_quant(x, fmt) -> _QuantCall:
     return c
 
 
-def _workspace(dev: torch.device, stream: int, nbytes: int):
-    """Scratch of at least nbytes on this stream (None for 0).  One per (device,
-    stream), grown as needed: calls on one stream run in order, so they share
-    it.  Under graph capture a fresh one from the graph's pool, so that two
-    graphs replayed on different streams never share memory."""
-    if nbytes <= 0:
-        return None
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    key = (dev.index, stream)
-    ws = _WS.get(key)
-    if ws is None or ws.numel() < nbytes:
-        if len(_WS) >= 64:
-            _WS.clear()
-        ws = _WS[key] = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    return ws
-
-
 def _gemm_args(a_fmt: str, w_codes, w_scales, bias, out_dtype, M: int, N: int, K: int) -> _lib.QikMxGemmArgs:
     return _lib.QikMxGemmArgs(_lib.ABI_VERSION, _OUT_DTYPES[out_dtype], MX_FORMATS[a_fmt], 0, None, None,
                               w_codes.data_ptr(), w_scales.data_ptr(), None if bias is None else bias.data_ptr(), None,
@@ -312,9 +291,9 @@ def mx_linear(
     idx = ent.index
     if idx != torch._C._cuda_getDevice():
         with torch.cuda.device(idx):
-            _launch_product(ent, g, codes.device)
+            _launch(ent, "qik_mx_gemm", g, codes)
     else:
-        _launch_product(ent, g, codes.device)
+        _launch(ent, "qik_mx_gemm", g, codes)
     return out
 
 
@@ -324,10 +303,14 @@ class _ProductCall:
     __slots__ = ("args", "fn", "index", "shape", "ws_bytes", "cast_bias")
 
 
-def _launch_product(ent: _ProductCall, g, dev: torch.device) -> None:
-    stream = torch._C._cuda_getCurrentRawStream(ent.index)
-    ws = None if ent.ws_bytes == 0 else _workspace(dev, stream, ent.ws_bytes).data_ptr()
-    _lib.check(ent.fn(ctypes.byref(g), ws, ent.ws_bytes, stream), "qik_mx_gemm")
+def _launch(ent, name: str, args, like: torch.Tensor) -> None:
+    """The launch on the current stream of like's device, with scratch of its
+    own: two threads that share a stream, or two graphs, never share memory."""
+    ws = like.new_empty(ent.ws_bytes, dtype=torch.uint8) if ent.ws_bytes else None
+    st = ent.fn(ctypes.byref(args), None if ws is None else ws.data_ptr(), ent.ws_bytes,
+                torch._C._cuda_getCurrentRawStream(ent.index))
+    if st:
+        _lib.check(st, name)
 
 
 def _prepare_product(a: MXTensor, w: MXTensor, bias, out_dtype) -> _ProductCall:
@@ -436,12 +419,12 @@ class MXFP4Linear(nn.Module):
             idx = ent.index
             if idx != torch._C._cuda_getDevice():
                 with torch.cuda.device(idx):
-                    self._launch(ent, x, out, idx)
+                    self._launch(ent, x, out)
             else:
-                self._launch(ent, x, out, idx)
+                self._launch(ent, x, out)
         return out if x.dtype == torch.bfloat16 else out.to(x.dtype)
 
-    def _launch(self, ent: _LinearCall, x, out, idx: int) -> None:
+    def _launch(self, ent: _LinearCall, x, out) -> None:
         x2 = _as_rows(x) if ent.copy else x
         a = _lib.QikMxLinearArgs.from_buffer_copy(ent.args)
         a.x = x2.data_ptr()
@@ -449,11 +432,7 @@ class MXFP4Linear(nn.Module):
         if ent.cast_bias:  # the module was moved to another dtype
             bias = self.bias.to(torch.bfloat16).contiguous()
             a.g.bias = bias.data_ptr()
-        stream = torch._C._cuda_getCurrentRawStream(idx)
-        ws = None if ent.ws_bytes == 0 else _workspace(x.device, stream, ent.ws_bytes).data_ptr()
-        st = ent.fn(ctypes.byref(a), ws, ent.ws_bytes, stream)
-        if st:
-            _lib.check(st, "qik_mx_linear")
+        _launch(ent, "qik_mx_linear", a, x)
 
     def _prepare(self, x, weight, scales, bias) -> _LinearCall:
         """Checks and the argument struct of one input geometry."""

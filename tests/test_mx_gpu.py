@@ -482,6 +482,47 @@ def test_two_streams_at_once():
             assert torch.equal(o[0], want[k][0]) and torch.equal(o[1], want[k][1])
 
 
+def test_two_threads_on_one_stream():
+    """Two threads call linears of two sizes on the same stream: neither reads the other's scratch."""
+    import threading
+    say("threads")
+    mods = [qik.MXFP4Linear.from_linear(torch.nn.Linear(1056, 512, device=DEV), f) for f in FORMATS]
+    xs = [torch.randn(M, 1056, device=DEV).bfloat16() for M in (150, 400)]
+    want = [m(x).clone() for m, x in zip(mods, xs)]
+    got = [[], []]
+
+    def work(k):
+        for _ in range(200):
+            got[k].append(mods[k](xs[k]))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert len(got[k]) == 200 and all(torch.equal(o, want[k]) for o in got[k])
+
+
+def test_norm_prepared_calls_go_by_each_operand():
+    """Operands of one geometry, now x and now the weight at an odd address: the one that is copied changes."""
+    say("norm alignments")
+    base = torch.randn(16 * 512 + 64, device=DEV).bfloat16()
+    wbase = torch.rand(300, device=DEV) + 0.5
+    for off_x, off_w in ((1, 0), (0, 1), (0, 0), (1, 1), (0, 1), (1, 0)):
+        x = base[off_x:].as_strided((16, 256), (512, 1))
+        w = wbase[off_w:off_w + 256]
+        for fmt in (None, "mxfp8"):
+            y = qik.fused_residual_rms_norm(x, x, w, EPS, fmt)
+            z = qik.fused_residual_rms_norm(x.contiguous(), x.contiguous(), w.clone(), EPS, fmt)
+            assert torch.equal(y[1], z[1])
+            if fmt is None:
+                assert torch.equal(y[0], z[0])
+            else:
+                assert torch.equal(y[0].codes.view(torch.uint8), z[0].codes.view(torch.uint8))
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_nothing_beside_the_outputs_is_written(fmt):
     """Outputs in the middle of a filled buffer: the rest of it keeps its bytes (rows past the end, columns past N)."""
