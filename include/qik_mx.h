@@ -121,8 +121,9 @@ int qik_residual_rms_norm(const qik_residual_rms_norm_args* args, void* stream);
  * rounding to nearest even into out_dtype.  A block whose scale is 255 makes
  * its row's outputs NaN.  a: rows of a_format (row stride lda bytes), w: rows
  * of MXFP4 (ldw bytes); both row strides multiples of 16 and at least a row,
- * 16-byte aligned; scales in the layout above, 16-byte aligned.  bias [N] and
- * out (row stride ldc elements, >= N) in out_dtype, aligned to an element.
+ * 16-byte aligned; scales in the layout above, 16-byte aligned.  bias [N]
+ * (4-byte aligned) and out (row stride ldc elements, >= N; aligned to an element)
+ * in out_dtype.
  * 0 <= M < 2^31 (0: nothing is launched), 1 <= N < 2^31, K a multiple of 32,
  * 32 <= K <= 262144. */
 typedef struct qik_mx_gemm_args {

@@ -117,9 +117,13 @@ struct Tile {
   static constexpr int WI = BN * RW / (1024 * NW);
   static constexpr int SI = (SBLK + NW - 1) / NW;     // 256-byte copies
   static constexpr int COPIES = AI + WI + SI;
+  static constexpr int BIAS_AT = NS * STAGE;          // behind the stages: the columns' bias, 16 bits each
+  static constexpr int BIAS_COPIES = (BN * 2 + 255) / 256;
+  static constexpr int LDS = BIAS_AT + 256 * BIAS_COPIES;
   static_assert(NW == 4 || NW == 8, "one or two waves per SIMD");
   static_assert(NS >= 2 && (NS - 1) * COPIES < 64, "the prologue's copies fit the vmcnt field");
-  static_assert(NS * STAGE <= 160 * 1024, "the stages fit LDS");
+  static_assert(LDS <= 160 * 1024, "the stages and the bias fit LDS");
+  static_assert(BIAS_COPIES <= NW, "one copy of bias per wave");
   static_assert(AI * 1024 * NW == BM * RA && WI * 1024 * NW == BN * RW, "whole copies per wave");
   static_assert(MI * 32 == WM && NJ * 32 == WN, "whole MFMA blocks per wave");
   static_assert((BN & (BN - 1)) == 0, "the output staging's swizzle needs a power of two");
@@ -140,15 +144,23 @@ __device__ __forceinline__ void store_tile(const MxGemmParams& p, const MxRegion
   constexpr int RB = T::BN * 2;  // bytes of a staged row
   constexpr int CPR = RB / 16;   // 16-byte chunks per row
   constexpr int RPI = 64 / CPR;  // rows per store instruction
+  // the bias was copied in whole dwords: an odd last element is read here
+  const bool odd_end = (rg.N & 1) != 0 && n0 + T::BN >= rg.N;
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < T::NJ; ++j) {
 #pragma unroll
     for (int qd = 0; qd < 4; ++qd) {
       const int nl = wn * T::WN + j * 32 + qd * 8 + (lane >> 5) * 4;
+      const u32x2 braw = *reinterpret_cast<const u32x2*>(lds + T::BIAS_AT + nl * 2);
       float bv[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bv[e] = bias_at(p, rg, n0 + nl + e);
+      for (int e = 0; e < 4; ++e) bv[e] = widen16((unsigned short)(braw[e / 2] >> (16 * (e % 2))), p.fp16);
+      if (odd_end && n0 + nl <= rg.N - 1 && n0 + nl + 4 > rg.N - 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n0 + nl + e == rg.N - 1) bv[e] = bias_at(p, rg, rg.N - 1);
+      }
 #pragma unroll
       for (int i = 0; i < T::MI; ++i) {
         const int ml = wm * T::WM + i * 32 + (lane & 31);
@@ -341,7 +353,14 @@ __device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion&
 #pragma unroll
     for (int i = 0; i < T::MI; ++i) acc[j][i] = f32x16{};
 
-  // prologue: every stage in flight, stage 0 published, its first fragments read
+  // prologue: the bias (zeros without one), then every stage in flight, stage 0
+  // published, its first fragments read
+  if constexpr (!SPLIT) {
+    const int b = wave % T::BIAS_COPIES;
+    const u32x4 rb = rsrc_words(reinterpret_cast<const unsigned char*>(rg.bias) + n0 * 2,
+                                rg.bias != nullptr ? (uint32_t)(nrows / 2 * 4) : 0u);
+    dma4(rb, lds0 + (uint32_t)(T::BIAS_AT + b * 256), (uint32_t)(b * 256 + lane * 4));
+  }
 #pragma unroll
   for (int s0 = 0; s0 < T::NS; ++s0) {
     const Step sc = prepare(kb + s0, s0);
@@ -488,7 +507,7 @@ template <class T1, class T2>
 __global__ void __launch_bounds__(T1::NT) __attribute__((amdgpu_waves_per_eu(T1::NW / 4, T1::NW / 4)))
 tile_kernel(const MxGemmParams p) {
   static_assert(T1::NT == T2::NT, "one workgroup size per launch");
-  constexpr int L1 = T1::NS * T1::STAGE, L2 = T2::NS * T2::STAGE;
+  constexpr int L1 = T1::LDS, L2 = T2::LDS;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[L1 > L2 ? L1 : L2];
   const int bx = blockIdx.x;
   const int off0 = p.small_first ? p.r[1].wgs : 0;  // first workgroup of each region
@@ -502,7 +521,7 @@ tile_kernel(const MxGemmParams p) {
 template <class T>
 __global__ void __launch_bounds__(T::NT) __attribute__((amdgpu_waves_per_eu(T::NW / 4, T::NW / 4)))
 split_kernel(const MxGemmParams p) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[T::NS * T::STAGE];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[T::LDS];
   const int wgs = p.r[0].wgs;
   gemm_tile<T, true>(p, p.r[0], blockIdx.x % wgs, lds, blockIdx.x / wgs);
 }
@@ -735,7 +754,7 @@ int validate_gemm(const qik_mx_gemm_args* a, bool with_a) {
   if (a->M == 0) return QIK_OK;
   if (a->w == nullptr || a->w_scales == nullptr || a->out == nullptr) return QIK_ERR_NULL_ARG;
   if (!aligned_to(a->w, 16) || !aligned_to(a->w_scales, 16) || a->ldw % 16 != 0) return QIK_ERR_ALIGN;
-  if (!aligned_to(a->out, 2) || !aligned_to(a->bias, 2)) return QIK_ERR_ALIGN;
+  if (!aligned_to(a->out, 2) || !aligned_to(a->bias, 4)) return QIK_ERR_ALIGN;
   if (with_a) {
     if (a->a == nullptr || a->a_scales == nullptr) return QIK_ERR_NULL_ARG;
     if (!aligned_to(a->a, 16) || !aligned_to(a->a_scales, 16) || a->lda % 16 != 0) return QIK_ERR_ALIGN;

@@ -287,6 +287,8 @@ def mx_linear(
     if bias is not None:
         if ent.cast_bias:
             bias = bias.reshape(-1).to(out_dtype).contiguous()
+        if bias.data_ptr() % 4 != 0:
+            bias = bias.clone()
         g.bias = bias.data_ptr()
     idx = ent.index
     if idx != torch._C._cuda_getDevice():
@@ -429,8 +431,8 @@ class MXFP4Linear(nn.Module):
         a = _lib.QikMxLinearArgs.from_buffer_copy(ent.args)
         a.x = x2.data_ptr()
         a.g.out = out.data_ptr()
-        if ent.cast_bias:  # the module was moved to another dtype
-            bias = self.bias.to(torch.bfloat16).contiguous()
+        if ent.cast_bias:  # not bf16 (the module was moved to another dtype), or not as the kernel reads it
+            bias = self.bias.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
             a.g.bias = bias.data_ptr()
         _launch(ent, "qik_mx_linear", a, x)
 
@@ -460,14 +462,15 @@ class MXFP4Linear(nn.Module):
         c.refs = (weakref.ref(weight), weakref.ref(scales), None if bias is None else weakref.ref(bias))
         c.addresses = (weight.data_ptr(), scales.data_ptr(), None if bias is None else bias.data_ptr())
         c.args, c.ws_bytes = None, 0
-        c.cast_bias = bias is not None and (bias.dtype != torch.bfloat16 or not bias.is_contiguous())
+        c.cast_bias = bias is not None and (bias.dtype != torch.bfloat16 or not bias.is_contiguous() or bias.data_ptr() % 4 != 0)
         x2 = _as_rows(x)
         # a view of x with x's own address needs no work per call
         c.copy = x2.data_ptr() != x.data_ptr()
         M = x2.shape[0]
         if M == 0:
             return c
-        a = _lib.QikMxLinearArgs(_gemm_args(self.activations, weight, scales, bias, torch.bfloat16, M, N, K),
+        a = _lib.QikMxLinearArgs(_gemm_args(self.activations, weight, scales, None if c.cast_bias else bias,
+                                            torch.bfloat16, M, N, K),
                                  x2.data_ptr(), _row_stride(x2), _DTYPES[x.dtype], 0)
         a.g.out = x2.data_ptr()  # any address: the size does not go by it
         need = ctypes.c_int64(0)

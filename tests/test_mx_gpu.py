@@ -292,6 +292,25 @@ def test_poisoned_blocks_reach_only_their_rows(fmt, M):
     assert torch.equal(torch.isnan(out), nan)
 
 
+@pytest.mark.parametrize("M", [1, 20, 40, 300])
+def test_bias_layouts(M):
+    """Biases at odd addresses, strided, of another type, of odd length."""
+    say("bias", M)
+    K = 288
+    a, av = tensors(M, K, "mxfp4", 1)
+    for N in (1, 2, 63, 64, 65, 127, 257, 513):
+        w, wv = tensors(N, K, "mxfp4", N)
+        full = torch.randn(2 * N + 2, device=DEV) * 50
+        for b in (full.bfloat16()[1:N + 1], full.bfloat16()[:2 * N:2], full[:N], full.half()[1:N + 1], full[:N].view(N, 1)):
+            want = b.reshape(-1).to(torch.bfloat16).double().cpu().numpy()
+            check_product(qik.mx_linear(a, w, b), av, wv, want, torch.bfloat16)
+    mod = qik.MXFP4Linear.from_quantized(w, full.bfloat16()[1:N + 1])
+    mod.bias = full.bfloat16()[1:N + 1]
+    x = torch.randn(M, K, device=DEV).bfloat16()
+    same = qik.MXFP4Linear.from_quantized(w, full.bfloat16()[1:N + 1])
+    assert torch.equal(mod(x), same(x))
+
+
 def test_product_shapes_of_many_dimensions():
     a, av = tensors(24, 96, "mxfp4", 1)
     a3 = qik.MXTensor(a.codes.view(2, 3, 4, 48), a.scales, "mxfp4")

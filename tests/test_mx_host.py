@@ -272,7 +272,7 @@ def test_dequantise_status_codes(kw, code):
     (dict(ldw=16), -5), (dict(ldw=2 ** 24), -5), (dict(ldc=7), -5), (dict(a_format=_lib.MXFP8), -5), (dict(a=None), -1),
     (dict(a_scales=None), -1), (dict(w=None), -1), (dict(w_scales=None), -1), (dict(out=None), -1), (dict(a=AT + 8), -8),
     (dict(w=AT + 8), -8), (dict(a_scales=AT + 8), -8), (dict(w_scales=AT + 8), -8), (dict(lda=40), -8), (dict(ldw=40), -8),
-    (dict(out=AT + 1), -8), (dict(bias=AT + 1), -8), (dict(M=0, a=None), 0)])
+    (dict(out=AT + 1), -8), (dict(bias=AT + 1), -8), (dict(bias=AT + 2), -8), (dict(M=0, a=None), 0)])
 def test_gemm_status_codes(kw, code):
     lib = _lib.load()
     n = ctypes.c_int64(-1)
