@@ -402,11 +402,10 @@ class MXFP4Linear(nn.Module):
         return MXTensor(self.weight, self.weight_scale, "mxfp4")
 
     def forward(self, x) -> torch.Tensor:
-        if isinstance(x, MXTensor):
-            return mx_linear(x, self.mx_weight(), self.bias)
         buffers = self._buffers
         weight, scales, bias = buffers["weight"], buffers["weight_scale"], buffers.get("bias")
-        key = (x.shape, x.stride(), x.dtype, x.device, self.activations)
+        mx = isinstance(x, MXTensor)
+        key = (x._shape, x._fmt, x._codes.device) if mx else (x.shape, x.stride(), x.dtype, x.device, self.activations)
         calls = self.__dict__.get("_calls")
         if calls is None:
             calls = self.__dict__["_calls"] = {}
@@ -416,7 +415,8 @@ class MXFP4Linear(nn.Module):
             if len(calls) >= 8:
                 calls.clear()
             calls[key] = ent
-        out = x.new_empty(ent.shape, dtype=torch.bfloat16)
+        rows = x._codes if mx else x
+        out = rows.new_empty(ent.shape, dtype=torch.bfloat16)
         if ent.args is not None:
             idx = ent.index
             if idx != torch._C._cuda_getDevice():
@@ -424,26 +424,32 @@ class MXFP4Linear(nn.Module):
                     self._launch(ent, x, out)
             else:
                 self._launch(ent, x, out)
-        return out if x.dtype == torch.bfloat16 else out.to(x.dtype)
+        return out if mx or x.dtype == torch.bfloat16 else out.to(x.dtype)
 
     def _launch(self, ent: _LinearCall, x, out) -> None:
-        x2 = _as_rows(x) if ent.copy else x
-        a = _lib.QikMxLinearArgs.from_buffer_copy(ent.args)
-        a.x = x2.data_ptr()
-        a.g.out = out.data_ptr()
+        if isinstance(x, MXTensor):
+            a = g = _lib.QikMxGemmArgs.from_buffer_copy(ent.args)
+            g.a, g.a_scales = x._codes.data_ptr(), x._scales.data_ptr()
+        else:
+            x2 = _as_rows(x) if ent.copy else x
+            a = _lib.QikMxLinearArgs.from_buffer_copy(ent.args)
+            a.x = x2.data_ptr()
+            g = a.g
+        g.out = out.data_ptr()
         if ent.cast_bias:  # not bf16 (the module was moved to another dtype), or not as the kernel reads it
             bias = self.bias.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
-            a.g.bias = bias.data_ptr()
-        _launch(ent, "qik_mx_linear", a, x)
+            g.bias = bias.data_ptr()
+        _launch(ent, "MXFP4Linear", a, out)
 
     def _prepare(self, x, weight, scales, bias) -> _LinearCall:
         """Checks and the argument struct of one input geometry."""
         N, K = self.out_features, self.in_features
-        if x.dtype not in _DTYPES:
+        mx = isinstance(x, MXTensor)
+        if not mx and x.dtype not in _DTYPES:
             raise ValueError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
-        if x.dim() < 1 or x.shape[-1] != K:
+        if len(x.shape) < 1 or x.shape[-1] != K:
             raise ValueError(f"x must be [..., {K}], got {tuple(x.shape)}")
-        if not x.is_cuda:
+        if x.device.type != "cuda":
             raise ValueError("MXFP4Linear runs on a HIP device; move its input and the module there first")
         for name, t, shape in (("weight", weight, (N, K // 2)), ("weight_scale", scales, _scales_shape(N, K)),
                                ("bias", bias, (N,))):
@@ -455,27 +461,30 @@ class MXFP4Linear(nn.Module):
                                                                or t.data_ptr() % 16 != 0)):
                 raise ValueError(f"{name} must be {shape}{'' if name == 'bias' else ' contiguous uint8, 16-byte aligned'}, "
                                  f"got {t.dtype} {tuple(t.shape)}")
+        lib = _lib.load()
         c = _LinearCall()
-        c.fn = _lib.load().qik_mx_linear
+        c.fn = lib.qik_mx_gemm if mx else lib.qik_mx_linear
         c.index = x.device.index
         c.shape = (*x.shape[:-1], N)
         c.refs = (weakref.ref(weight), weakref.ref(scales), None if bias is None else weakref.ref(bias))
         c.addresses = (weight.data_ptr(), scales.data_ptr(), None if bias is None else bias.data_ptr())
-        c.args, c.ws_bytes = None, 0
+        c.args, c.ws_bytes, c.copy = None, 0, False
         c.cast_bias = bias is not None and (bias.dtype != torch.bfloat16 or not bias.is_contiguous() or bias.data_ptr() % 4 != 0)
-        x2 = _as_rows(x)
-        # a view of x with x's own address needs no work per call
-        c.copy = x2.data_ptr() != x.data_ptr()
-        M = x2.shape[0]
+        M = _rows(x.shape)
         if M == 0:
             return c
-        a = _lib.QikMxLinearArgs(_gemm_args(self.activations, weight, scales, None if c.cast_bias else bias,
-                                            torch.bfloat16, M, N, K),
-                                 x2.data_ptr(), _row_stride(x2), _DTYPES[x.dtype], 0)
-        a.g.out = x2.data_ptr()  # any address: the size does not go by it
+        a = _gemm_args(x.fmt if mx else self.activations, weight, scales, None if c.cast_bias else bias, torch.bfloat16, M, N, K)
+        a.out = weight.data_ptr()  # any address: the size does not go by it
+        if mx:
+            a.a, a.a_scales, size = x.codes.data_ptr(), x.scales.data_ptr(), lib.qik_mx_gemm_workspace_size
+        else:
+            x2 = _as_rows(x)
+            c.copy = x2.data_ptr() != x.data_ptr()  # a view at x's own address needs no work per call
+            a = _lib.QikMxLinearArgs(a, x2.data_ptr(), _row_stride(x2), _DTYPES[x.dtype], 0)
+            size = lib.qik_mx_linear_workspace_size
         need = ctypes.c_int64(0)
         with torch.cuda.device(x.device):
-            _lib.check(_lib.load().qik_mx_linear_workspace_size(ctypes.byref(a), ctypes.byref(need)), "qik_mx_linear")
+            _lib.check(size(ctypes.byref(a), ctypes.byref(need)), "MXFP4Linear")
         c.args, c.ws_bytes = a, need.value
         return c
 

@@ -292,6 +292,113 @@ def test_poisoned_blocks_reach_only_their_rows(fmt, M):
     assert torch.equal(torch.isnan(out), nan)
 
 
+def launch_of(M, N, K, fmt):
+    """Bytes of scratch that a product takes: more than none where K is split."""
+    import ctypes
+    from qwen_image_kernel_amd import _lib
+    at = 1 << 20
+    g = _lib.QikMxGemmArgs(_lib.ABI_VERSION, 0, {"mxfp4": 1, "mxfp8": 2}[fmt], 0, at, at, at, at, None, at, M, N, K,
+                           K // 2 if fmt == "mxfp4" else K, K // 2, N)
+    n = ctypes.c_int64()
+    assert _lib.load().qik_mx_gemm_workspace_size(ctypes.byref(g), ctypes.byref(n)) == 0
+    return n.value
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(40, 48, 12288), (64, 333, 8192), (130, 257, 12320), (200, 192, 12288)])
+def test_split_products(fmt, M, N, K):
+    """K split over workgroups: the values, and the same bits again, eager and replayed, with other work in between."""
+    say("split", fmt, M, N, K)
+    assert launch_of(M, N, K, fmt) > 0
+    a, av = tensors(M, K, fmt, M)
+    w, wv = tensors(N, K, "mxfp4", N)
+    b = torch.randn(N, device=DEV).bfloat16()
+    want = qik.mx_linear(a, w, b)
+    check_product(want, av, wv, b.double().cpu().numpy(), torch.bfloat16, fmt)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        qik.mx_linear(a, w, b)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = qik.mx_linear(a, w, b)
+    for _ in range(4):
+        got.zero_()
+        graph.replay()
+        again = qik.mx_linear(a, w, b)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(again, want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(16, 8200, 288), (9, 8233, 96), (32, 8300, 96), (20, 9000, 2048), (31, 4100, 4128),
+                                   (2, 33, 262144), (40, 33, 262144)])
+def test_few_rows_wide_and_long(fmt, M, N, K):
+    """Few rows into many columns, the two widths of the few-rows kernel, and the longest K."""
+    say("wide", fmt, M, N, K)
+    g = torch.Generator(device=DEV).manual_seed(N)
+    x = torch.randn(M, K, generator=g, device=DEV)
+    a, w = qik.quantize_mx(x, fmt), qik.quantize_mx(torch.randn(N, K, generator=g, device=DEV) / 8, "mxfp4")
+    av, wv = a.dequantize(torch.float32).double(), w.dequantize(torch.float32).double()
+    want = av @ wv.t().contiguous()
+    acc = (K + 1) * 2.0 ** -23 * (av.abs() @ wv.abs().t().contiguous())
+    if fmt == "mxfp8":
+        top = [torch.nn.functional.pad(t.abs(), (0, -K % 128)).unflatten(1, (-1, 128)).amax(-1) for t in (av, wv)]
+        acc += 128 * 2.0 ** -13 * (top[0] @ top[1].t().contiguous())
+    tol = acc + 2.0 ** -8 * (want.abs() + acc)
+    for got in (qik.mx_linear(a, w), qik.MXFP4Linear.from_quantized(w, None, fmt)(x)):
+        err = (got.double() - want).abs()
+        assert (err <= tol).all(), (err / tol).max().item()
+
+
+def test_offsets_past_32_bits():
+    """Rows, codes, weights and outputs whose last bytes lie past 2^31 and 2^32."""
+    say("offsets: quantise and back, norm")
+    M, K = 33000, 65536  # 2.2e9 elements
+    tail = torch.randn(40, K, device=DEV).bfloat16()
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device=DEV)
+    x[-40:] = tail
+    for fmt in FORMATS:
+        t, u = qik.quantize_mx(x, fmt), qik.quantize_mx(tail, fmt)
+        assert torch.equal(t.codes[-40:].view(torch.uint8), u.codes.view(torch.uint8))
+        assert torch.equal(t.block_scales()[-40:], u.block_scales())
+        assert torch.equal(t.dequantize()[-40:], u.dequantize())
+        del t
+    x = x.view(2 * M, K // 2)
+    w = torch.rand(K // 2, device=DEV)
+    rows_, small = tail.view(80, K // 2), None
+    for fmt in (None, "mxfp4"):
+        y, h = qik.fused_residual_rms_norm(x, x, w, EPS, fmt)
+        small, hs = qik.fused_residual_rms_norm(rows_, rows_, w, EPS, fmt)
+        assert torch.equal(h[-80:], hs)
+        assert torch.equal(y[-80:], small) if fmt is None else torch.equal(y.codes[-80:], small.codes)
+    del x, y, h
+    say("offsets: weights")
+    N, K = 70016, 65536  # 2.3e9 bytes of codes
+    codes = torch.zeros(N, K // 2, dtype=torch.uint8, device=DEV)
+    bs = torch.full((N, K // 32), 127, dtype=torch.uint8, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    codes[-70:] = torch.randint(0, 256, (70, K // 2), generator=g, device=DEV, dtype=torch.uint8)
+    w = qik.MXTensor.from_block_scales(codes, bs, "mxfp4")
+    part = qik.MXTensor.from_block_scales(codes[-70:].clone(), bs[-70:].clone(), "mxfp4")
+    for M in (1, 70):
+        a = qik.quantize_mx(torch.randn(M, K, generator=g, device=DEV))
+        av, wv = a.dequantize(torch.float32).double(), part.dequantize(torch.float32).double()
+        got = qik.mx_linear(a, w)
+        assert (got[:, :-70] == 0).all()
+        check_product(got[:, -70:], av.cpu().numpy(), wv.cpu().numpy(), None, torch.bfloat16)
+    del w, codes, bs, got
+    say("offsets: outputs")
+    M, N, K = 40000, 60000, 32  # 2.4e9 outputs
+    a = qik.quantize_mx(torch.randn(M, K, generator=g, device=DEV))
+    w = qik.quantize_mx(torch.randn(N, K, generator=g, device=DEV))
+    got = qik.mx_linear(a, w)
+    av, wv = (t.dequantize(torch.float32).double().cpu().numpy() for t in (a, w))
+    check_product(got[-33:], av[-33:], wv, None, torch.bfloat16)
+    check_product(got[:, -5:], av, wv[-5:], None, torch.bfloat16)
+
+
 @pytest.mark.parametrize("M", [1, 20, 40, 300])
 def test_bias_layouts(M):
     """Biases at odd addresses, strided, of another type, of odd length."""
@@ -499,6 +606,31 @@ def test_two_streams_at_once():
     for k in range(2):
         for o in got[k]:
             assert torch.equal(o[0], want[k][0]) and torch.equal(o[1], want[k][1])
+
+
+def test_projections_of_the_attention_processor():
+    """The processor's projections as MXFP4Linear: the layer is what its products, norms and attention give one by one."""
+    from types import SimpleNamespace
+    say("processor")
+    S, H, D = 300, 4, 128
+    dim = H * D
+    g = torch.Generator(device=DEV).manual_seed(5)
+    net = torch.nn.ModuleDict({"qkv": torch.nn.Linear(dim, 3 * dim), "out": torch.nn.Linear(dim, dim)}).to(DEV)
+    assert qik.convert_linears_mxfp4(net) == ["qkv", "out"]
+    ones = SimpleNamespace(weight=torch.rand(D, generator=g, device=DEV) + 0.5, eps=EPS)
+    attn = SimpleNamespace(heads=H, fused_qkv=net["qkv"], to_out=[net["out"], torch.nn.Identity()], norm_q=ones, norm_k=ones)
+    x = torch.randn(1, S, dim, generator=g, device=DEV).bfloat16()
+    ang = torch.rand(S, D // 2, generator=g, device=DEV)
+    freqs = torch.polar(torch.ones_like(ang), ang)
+    got = qik.QwenImage21KernelProcessor()(attn, x, rotary_emb=freqs)
+
+    def product(mod, t):
+        return qik.mx_linear(qik.quantize_mx(t), mod.mx_weight(), mod.bias)
+
+    q, k, v = product(net["qkv"], x).unflatten(-1, (3 * H, D)).chunk(3, dim=-2)
+    q, k = (qik.fused_rms_norm_rope(t, ones.weight, freqs, EPS) for t in (q, k))
+    o = qik.block_causal_flash_attention(q, k, v, None, None, uniform_full=True)
+    assert torch.equal(got, product(net["out"], o.flatten(2, 3)))
 
 
 def test_two_threads_on_one_stream():
