@@ -26,6 +26,9 @@ namespace qik_mx {
 inline bool aligned_to(const void* ptr, uintptr_t a) { return (reinterpret_cast<uintptr_t>(ptr) % a) == 0; }
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// a launch's workgroups in order: a grid of 2^32 threads or more has rows (launch)
+__device__ __forceinline__ int64_t block_index() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // byte offset of (row, block) in the scales; C = ceil(K / 256)
 __device__ __forceinline__ int64_t scale_at(int64_t row, int block, int C) {
   return ((row >> 5) * C + (block >> 3)) * 256 + (row & 31) * 8 + (block & 7);
@@ -71,7 +74,7 @@ template <int DT, int FMT, bool ALIGNED, int QU>
 __global__ void __launch_bounds__(QT) quant_kernel(const QuantParams p) {
   constexpr int HW = QT / 32;
   const int hw = threadIdx.x >> 5, t = threadIdx.x & 31;
-  const int64_t first = (int64_t)blockIdx.x * (HW * QU);
+  const int64_t first = block_index() * (HW * QU);
   Raw8<DT> raw[QU];
   int64_t row[QU];
   int v[QU];  // 8-element vector within the row
@@ -131,7 +134,7 @@ template <int DT, int FMT, int QU>
 __global__ void __launch_bounds__(QT) dequant_kernel(const QuantParams p) {
   constexpr int HW = QT / 32;
   const int hw = threadIdx.x >> 5, t = threadIdx.x & 31;
-  const int64_t first = (int64_t)blockIdx.x * (HW * QU);
+  const int64_t first = block_index() * (HW * QU);
   unsigned w0[QU], w1[QU], byte[QU];
   int64_t at[QU];  // element offset, or -1
 #pragma unroll
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(LPR < 256 ? 256 : LPR) norm_kernel(const NormP
   constexpr int NT = LPR < 256 ? 256 : LPR;
   constexpr int EB = elem_bytes<DT>();
   const int t = threadIdx.x % LPR;
-  const int64_t row = (int64_t)blockIdx.x * (NT / LPR) + threadIdx.x / LPR;
+  const int64_t row = block_index() * (NT / LPR) + threadIdx.x / LPR;
   if constexpr (FMT != QIK_MX_NONE) {
     // scales of padding rows (up to 32 ceil(M / 32)) and padding blocks
     if (row >= ((p.M + 31) & ~(int64_t)31)) return;
@@ -371,10 +374,12 @@ int validate_norm(const qik_residual_rms_norm_args* a) {
 }
 
 int launch(const void* fn, int64_t grid, int threads, void* params, hipStream_t s) {
-  if (grid > (int64_t)INT_MAX) return QIK_ERR_SHAPE;
+  const int64_t gy = cdiv(grid * threads, UINT_MAX);  // below 2^32 threads in x
+  const int64_t gx = cdiv(grid, gy);                  // the last row's surplus is behind the last row of the data
+  if (gy > 65535) return QIK_ERR_SHAPE;
   void* args[] = {params};
-  return hipLaunchKernel(fn, dim3((unsigned)grid), dim3((unsigned)threads), args, 0, s) == hipSuccess ? QIK_OK
-                                                                                                    : QIK_ERR_LAUNCH;
+  const dim3 g((unsigned)gx, (unsigned)gy);
+  return hipLaunchKernel(fn, g, dim3((unsigned)threads), args, 0, s) == hipSuccess ? QIK_OK : QIK_ERR_LAUNCH;
 }
 
 QuantParams unit_params(int64_t M, int64_t K, int64_t rows) {

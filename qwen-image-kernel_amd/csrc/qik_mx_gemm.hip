@@ -745,7 +745,7 @@ int validate_gemm(const qik_mx_gemm_args* a, bool with_a) {
   if (a->abi_version != QIK_ABI_VERSION || a->reserved0 != 0) return QIK_ERR_ABI_VERSION;
   if (a->out_dtype != QIK_DTYPE_BF16 && a->out_dtype != QIK_DTYPE_FP16) return QIK_ERR_DTYPE;
   if (a->a_format != QIK_MXFP4 && a->a_format != QIK_MXFP8) return QIK_ERR_DTYPE;
-  if (a->M < 0 || a->M > INT_MAX || a->N < 1 || a->N > INT_MAX) return QIK_ERR_SHAPE;
+  if (a->M < 0 || a->M > ((int64_t)1 << 30) || a->N < 1 || a->N >= ((int64_t)1 << 28)) return QIK_ERR_SHAPE;
   if (a->K < 32 || a->K > 262144 || a->K % 32 != 0) return QIK_ERR_SHAPE;
   const int64_t row_a = a->a_format == QIK_MXFP4 ? a->K / 2 : a->K;
   // a tile's rows must be addressable by a 31-bit buffer offset
@@ -811,6 +811,7 @@ int set_region(MxRegion& rg, const qik_mx_gemm_args* a, int64_t c0, int64_t c1) 
 }
 
 int launch(const void* fn, dim3 grid, int threads, MxGemmParams& p, hipStream_t s) {
+  if ((uint64_t)grid.x * (unsigned)threads >> 32 != 0) return QIK_ERR_SHAPE;  // more than a launch holds
   void* args[] = {&p};
   return hipLaunchKernel(fn, grid, dim3((unsigned)threads), args, 0, s) == hipSuccess ? QIK_OK : QIK_ERR_LAUNCH;
 }

@@ -500,6 +500,41 @@ def test_linear_module_moves_copies_and_reloads():
     assert fresh(x[:0]).shape == (0, 64) and fresh(x[0]).shape == (64,)
 
 
+def test_linear_takes_a_bias_set_later():
+    x = torch.randn(5, 64, device=DEV).bfloat16()
+    for mod in (qik.MXFP4Linear(64, 40), qik.MXFP4Linear.from_quantized(qik.quantize_mx(torch.zeros(40, 64)))):
+        mod = mod.to(DEV)
+        assert (mod(x) == 0).all() and (mod(qik.quantize_mx(x)) == 0).all()
+        b = torch.randn(40, device=DEV)
+        for bias in (b.bfloat16(), torch.nn.Parameter(b), None):
+            mod.bias = bias
+            want = torch.zeros(5, 40, device=DEV).bfloat16() if bias is None else b.bfloat16().expand(5, 40)
+            assert torch.equal(mod(x), want) and torch.equal(mod(qik.quantize_mx(x)), want)
+
+
+def test_launches_of_more_than_2_to_32_threads():
+    say("grids: quantise and back")
+    M, K = 2 ** 27 + 40, 32
+    x = torch.ones(M, K, dtype=torch.bfloat16, device=DEV)
+    x[-40:] = tail = torch.randn(40, K, device=DEV).bfloat16()
+    t, u = qik.quantize_mx(x), qik.quantize_mx(tail)
+    assert (t.codes[:-40] == 0x66).all() and torch.equal(t.codes[-40:], u.codes)
+    assert (t.block_scales()[:-40] == 125).all() and torch.equal(t.block_scales()[-40:], u.block_scales())
+    del x
+    y = t.dequantize()
+    assert (y[:-40] == 1).all() and torch.equal(y[-40:], u.dequantize())
+    del t, y
+    say("grids: norm")
+    M, D = 2 ** 28 + 40, 8
+    x = torch.ones(M, D, dtype=torch.bfloat16, device=DEV)
+    x[-40:] = tail = torch.randn(40, D, device=DEV).bfloat16()
+    w = torch.ones(D, device=DEV)
+    y, h = qik.fused_residual_rms_norm(x, x, w, 0.0)
+    assert (y[:-40] == 1).all() and (h[:-40] == 2).all()
+    for a, b in zip((y, h), qik.fused_residual_rms_norm(tail, tail, w, 0.0)):
+        assert torch.equal(a[-40:], b)
+
+
 def test_refusals_on_the_device():
     x = torch.zeros(4, 64, device=DEV)
     w = torch.ones(64, device=DEV)

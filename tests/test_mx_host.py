@@ -281,6 +281,12 @@ def test_gemm_status_codes(kw, code):
     assert code == 0 or n.value == 0
 
 
+@pytest.mark.parametrize("kw", [
+    dict(M=2 ** 30 + 1), dict(N=2 ** 28, ldc=2 ** 28), dict(M=2 ** 30, N=2 ** 20, ldc=2 ** 20)])
+def test_products_beyond_a_launch_are_refused(kw):
+    assert _lib.load().qik_mx_gemm(ctypes.byref(gemm_args(**kw)), None, 0, None) == -5
+
+
 @pytest.mark.parametrize("kw,code", [
     (dict(x_dtype=3), -3), (dict(reserved0=1), -2), (dict(ldx=63), -5), (dict(x=None), -1), (dict(x=AT + 1), -8)])
 def test_linear_status_codes(kw, code):
