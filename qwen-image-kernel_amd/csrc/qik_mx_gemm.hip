@@ -841,17 +841,18 @@ int launch_rows_shape(MxGemmParams& p, const qik_mx_gemm_args* a, hipStream_t s)
                 s);
 }
 
-// Weight rows (in 16s) and waves of a workgroup.  From 8192 columns on there is
-// a workgroup of 16 rows for every second wave slot: four waves each, and 32 rows
-// where the codes of A are worth sharing (1 x 12288 x 4096 8.4 us with 16 rows, 9.1
-// with 32; 32 x 12288 x 4096 13.5 and 12.6).  Below, eight waves share a long K (1 x
-// 4096 x 4096 4.5 us, 5.0 with four; 1 x 4096 x 12288 9.3 and 11.8), or the
-// quantising of elements, which goes by threads.
+// Weight rows (in 16s) and waves of a workgroup.  Past 8192 columns there is a
+// workgroup of 16 rows for every second wave slot: four waves each (1 x 12288 x
+// 4096 7.8 us, 9.3 with eight), and 32 rows where the codes of A are worth sharing
+// (1 x 12288 x 4096 7.8 us with 16 rows, 8.2 with 32; 16 x 24576 x 4096 18.1 and
+// 13.9).  Below, eight waves share a long K (1 x 4096 x 12288 8.6 us, 11.2 with
+// four; 1 x 4096 x 1536 3.0 and 3.1, x 1024 2.8 and 2.7), or the quantising of
+// elements, which goes by threads.
 struct RowsPlan {
   int nb, kw;
 };
 RowsPlan choose_rows(int64_t M, int64_t N, int64_t K, bool raw) {
-  return {N > 8192 && M > 8 ? 2 : 1, N > 8192 || (!raw && K <= 7 * 256) ? 4 : 8};
+  return {N > 8192 && M > 8 ? 2 : 1, N > 8192 || (!raw && K <= 4 * 256) ? 4 : 8};
 }
 
 template <int SRC, bool A8, int MB>
@@ -892,9 +893,10 @@ struct MxPlan {
 // A K split pays for a launch with few tiles and a long K: S slices of 64 x 64 or
 // 128 x 128 tiles, as many as the CUs run in one round (all slices of a tile on
 // one XCD), and a second launch that joins them: 3 us, and the fp32 sums written
-// and read at about 4 TB/s (64 x 4096 x 12288 18.1 us unsplit, 12.1 in 4 slices,
-// 15.5 in 8; 203 x 2048 x 8192 13.3 and 12.5 in 2; 203 x 4096 x 12288 18.2 and
-// 19.2 in 4 of 128 x 128).
+// and read at about 4 TB/s (64 x 4096 x 12288 16.6 us unsplit, 12.8 in 4 slices,
+// 15.7 in 8; 200 x 1024 x 8192 12.5 and 10.6 in 4; 203 x 2048 x 8192 12.7 and 12.8
+// in 2, with MXFP8 rows 19.4 and 16.6; 203 x 4096 x 12288 17.4 and 18.6 in 4 of
+// 128 x 128).
 MxPlan choose(int64_t M, int64_t N, int64_t K, bool a8, int cus) {
   const int64_t steps = cdiv(K, a8 ? 128 : 256), P = std::max(1, (cus > 0 ? cus : 256) / 8);
   const GemmPlan g = choose_plan(kTables[a8], M, N, steps, cus);
@@ -944,11 +946,17 @@ int launch_plan(MxGemmParams& p, const qik_mx_gemm_args* a, const MxPlan& plan, 
   }
 }
 
-// Few rows: the tiles of 64 would multiply mostly padding.  From 17 rows on they
-// do better all the same where N has tiles for most CUs and K is long (32 x
-// 12288 x 8192 16.8 us against 23.2; 32 x 4096 x 8192 10.6 and 9.9).
+// Few rows: the tiles of 64 would multiply mostly padding.  They do better all
+// the same where K is so long that splitting it over workgroups pays (us, rows
+// then tiles: 1 x 4096 x 16384 10.9 / 11.7 and x 32768 18.8 / 18.2; 32 x 4096 x
+// 8192 9.3 / 10.5 and x 12288 12.5 / 11.8, with MXFP8 rows x 4096 7.5 / 10.0 and x
+// 8192 12.8 / 12.4), and where N has tiles for most CUs and K is long (16 x 8192 x
+// 8192 11.7 / 12.9, 16 x 12288 x 8192 15.8 / 13.2; 32 x 5120 x 2048 5.4 / 6.2, 32 x
+// 12288 x 4096 11.8 / 8.9).
 bool takes_rows(const qik_mx_gemm_args* a) {
-  return a->M <= 16 || (a->M <= 32 && (a->N <= 4096 || a->N * a->K <= (1 << 24)));
+  if (a->M <= 8) return a->K <= 16384;
+  if (a->M <= 16) return a->K <= 16384 && a->N * a->K <= ((int64_t)1 << 26);
+  return a->M <= 32 && (a->N <= 4096 ? a->K <= (a->a_format == QIK_MXFP8 ? 6144 : 8192) : a->N * a->K <= (1 << 24));
 }
 
 // A linear whose workgroups each quantise all of x for themselves saves a
@@ -958,7 +966,7 @@ bool takes_rows(const qik_mx_gemm_args* a) {
 // 10.9, 17 x 5001 x 1504 6.7 / 6.3 and with MXFP8 9.1 / 6.6; called in a loop the
 // last takes 9 against 11.6).
 bool takes_raw(const qik_mx_gemm_args* a) {
-  if (!takes_rows(a) || a->M * a->K > RAW_ELEMS) return false;
+  if (a->M * a->K > RAW_ELEMS || (a->M > 16 && !takes_rows(a))) return false;
   const int64_t wgs = cdiv(a->N, 16 * choose_rows(a->M, a->N, a->K, true).nb);
   return cdiv(wgs, 256) * a->M * a->K <= 2 * RAW_ELEMS;
 }
