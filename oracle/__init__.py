@@ -25,6 +25,9 @@ qwen-image-kernel reference repository):
 * ``rms_rope``  -- per-head RMSNorm + RoPE (triton_fused.py:28-105): an fp32 restatement
                    in the HIP kernel's operation order, and the stock torch composition
                    the reference tests against (tests/test_fused.py:21-33).
+* ``mx``        -- the microscaled formats and the operators on them (no counterpart in
+                   the reference): quantiser, scale layout, product and residual RMSNorm
+                   from their definitions, in fp64.
 
 How each function is pinned is stated in its docstring; the tests under
 ``tests/test_oracle_*.py`` hold the checks.

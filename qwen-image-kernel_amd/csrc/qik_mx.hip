@@ -215,8 +215,8 @@ __device__ __forceinline__ double lane_sum(double v) {
 // once and stays in registers, packed, between the sum of squares and the
 // output.  The squares are summed in fp64 (each exact there), so the sum does
 // not depend on the order to anything that its fp32 root shows.  Bound by HBM:
-// bf16 4352 x 4096 with a residual 29.1 us (4.9 TB/s), to MXFP8 27.7 (4.5); rows
-// at odd addresses go slower (fp16 9001 x 1111 13.6 us, 2.9 TB/s; 1112 wide 10.1,
+// bf16 4352 x 4096 with a residual 28.4 us (5.0 TB/s), to MXFP8 27.1 (4.6); rows
+// at odd addresses go slower (fp16 9001 x 1111 11.8 us, 3.4 TB/s; 1112 wide 10.0,
 // 4.0 TB/s).
 template <int DT, int FMT, bool RES, bool ALIGNED, int LPR, int VPT>
 __global__ void __launch_bounds__(LPR < 256 ? 256 : LPR) norm_kernel(const NormParams p) {

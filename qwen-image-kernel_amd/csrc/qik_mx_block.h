@@ -50,29 +50,52 @@ __device__ __forceinline__ void store8(char* p, const Raw8<DT>& r) {
     else *reinterpret_cast<u32x4_u*>(p + 16 * i) = r.w[i];
   }
 }
-// the first n < 8 elements at p, the rest zero
+typedef u32x2 u32x2_u __attribute__((aligned(2)));
+typedef unsigned u32_u __attribute__((aligned(2)));
+
+// The first n < 8 elements at p, the rest zero, in pieces of 4, 2 and 1: a wave
+// issues each piece of a row's end for one lane of it, and element by element
+// they cost a tenth of the call (fp16 9001 x 1111 13.4 us, in pieces 11.8).
 template <int DT>
 __device__ __forceinline__ Raw8<DT> load_part(const char* p, int n) {
+  constexpr int EB = elem_bytes<DT>();
+  const bool h4 = (n & 4) != 0, h2 = (n & 2) != 0, h1 = (n & 1) != 0;
   Raw8<DT> r = {};
-#pragma unroll
-  for (int i = 0; i < 7; ++i) {
-    if constexpr (DT == QIK_DTYPE_FP32) {
-      if (i < n) r.w[i / 4][i % 4] = reinterpret_cast<const unsigned*>(p)[i];
-    } else {
-      if (i < n) r.w[0][i / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[i] << (16 * (i % 2));
-    }
+  if constexpr (DT == QIK_DTYPE_FP32) {
+    u32x4 a = {};
+    u32x2 b = {};
+    unsigned c = 0u;
+    if (h4) a = *reinterpret_cast<const u32x4_u*>(p);
+    if (h2) b = *reinterpret_cast<const u32x2_u*>(p + (n & 4) * EB);
+    if (h1) c = *reinterpret_cast<const unsigned*>(p + (n & 6) * EB);
+    const u32x4 rest = h2 ? u32x4{b.x, b.y, c, 0u} : u32x4{c, 0u, 0u, 0u};
+    r.w[0] = h4 ? a : rest;
+    r.w[1] = h4 ? rest : u32x4{};
+  } else {
+    u32x2 a = {};
+    unsigned b = 0u, c = 0u;
+    if (h4) a = *reinterpret_cast<const u32x2_u*>(p);
+    if (h2) b = *reinterpret_cast<const u32_u*>(p + (n & 4) * EB);
+    if (h1) c = *reinterpret_cast<const unsigned short*>(p + (n & 6) * EB);
+    const u32x2 rest = h2 ? u32x2{b, c} : u32x2{c, 0u};
+    r.w[0] = h4 ? u32x4{a.x, a.y, rest.x, rest.y} : u32x4{rest.x, rest.y, 0u, 0u};
   }
   return r;
 }
 template <int DT>
 __device__ __forceinline__ void store_part(char* p, const Raw8<DT>& r, int n) {
-#pragma unroll
-  for (int i = 0; i < 7; ++i) {
-    if constexpr (DT == QIK_DTYPE_FP32) {
-      if (i < n) reinterpret_cast<unsigned*>(p)[i] = r.w[i / 4][i % 4];
-    } else {
-      if (i < n) reinterpret_cast<unsigned short*>(p)[i] = (unsigned short)(r.w[0][i / 2] >> (16 * (i % 2)));
-    }
+  constexpr int EB = elem_bytes<DT>();
+  const bool h4 = (n & 4) != 0, h2 = (n & 2) != 0;
+  if constexpr (DT == QIK_DTYPE_FP32) {
+    const u32x4 rest = h4 ? r.w[1] : r.w[0];
+    if (h4) *reinterpret_cast<u32x4_u*>(p) = r.w[0];
+    if (h2) *reinterpret_cast<u32x2_u*>(p + (n & 4) * EB) = u32x2{rest.x, rest.y};
+    if (n & 1) *reinterpret_cast<unsigned*>(p + (n & 6) * EB) = h2 ? rest.z : rest.x;
+  } else {
+    const u32x2 rest = h4 ? u32x2{r.w[0].z, r.w[0].w} : u32x2{r.w[0].x, r.w[0].y};
+    if (h4) *reinterpret_cast<u32x2_u*>(p) = u32x2{r.w[0].x, r.w[0].y};
+    if (h2) *reinterpret_cast<u32_u*>(p + (n & 4) * EB) = rest.x;
+    if (n & 1) *reinterpret_cast<unsigned short*>(p + (n & 6) * EB) = (unsigned short)(h2 ? rest.y : rest.x);
   }
 }
 

@@ -962,8 +962,8 @@ bool takes_rows(const qik_mx_gemm_args* a) {
 // A linear whose workgroups each quantise all of x for themselves saves a
 // launch: 2 us in a graph, 4 us of host time in a loop of calls.  It costs what a
 // CU's workgroups quantise, about 2.5 us for 32768 elements (in a graph 1 x 4096
-// x 4096 4.8 us against 6.5, 32 x 4096 x 1024 5.8 / 5.7, 4 x 12288 x 4096 11.1 /
-// 10.9, 17 x 5001 x 1504 6.7 / 6.3 and with MXFP8 9.1 / 6.6; called in a loop the
+// x 4096 4.2 us against 5.9, 32 x 4096 x 1024 5.6 / 5.4, 4 x 12288 x 4096 10.1 /
+// 10.2, 17 x 5001 x 1504 6.2 / 5.8 and with MXFP8 8.5 / 7.1; called in a loop the
 // last takes 9 against 11.6).
 bool takes_raw(const qik_mx_gemm_args* a) {
   if (a->M * a->K > RAW_ELEMS || (a->M > 16 && !takes_rows(a))) return false;
