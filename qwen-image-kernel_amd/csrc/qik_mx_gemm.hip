@@ -250,9 +250,9 @@ __device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion&
   constexpr int WROWS = 1024 / T::RW;  // rows of a copy of W
   uint32_t aoff[T::AI], woff[T::WI];
 #pragma unroll
-  for (int i = 0; i < T::AI; ++i) aoff[i] = (uint32_t)((arow + 8 * T::NW * i) * (int)p.lda + achunk);
+  for (int i = 0; i < T::AI; ++i) aoff[i] = (uint32_t)((arow + 8 * T::NW * i) * (int)p.lda);
 #pragma unroll
-  for (int i = 0; i < T::WI; ++i) woff[i] = (uint32_t)((wrow + WROWS * T::NW * i) * (int)p.ldw + wchunk);
+  for (int i = 0; i < T::WI; ++i) woff[i] = (uint32_t)((wrow + WROWS * T::NW * i) * (int)p.ldw);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
   const unsigned char* abase = p.a + (int64_t)m0 * p.lda;
   const unsigned char* wbase = rg.w + (int64_t)n0 * p.ldw;
@@ -264,41 +264,55 @@ __device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion&
   const int kb = SPLIT ? (int)((int64_t)nkall * slice / p.ksplit) : 0;
   const int nk = SPLIT ? (int)((int64_t)nkall * (slice + 1) / p.ksplit) : nkall;  // end of the stages
 
-  // The copies of one step: past the end of K a lane's chunk would read the
-  // next row, so its offset gets the top bit (out of range: zeros); a step at
-  // or past the end gets empty resources, so that every step issues the same
-  // copies and the waits stay uniform.
+  // The copies of one step.  Resources hold for all of them (rows past the
+  // tile's last are out of range: zeros) and only lanes' offsets move on: with
+  // one wave per SIMD the instructions of a stage are what a small tile waits
+  // for, and resources made anew each step were a third of them.  Past the end of
+  // K, or of the slice, a lane's chunk would read the next row, so its offset
+  // gets the top bit (out of range); every step issues the same copies, so the
+  // waits stay uniform.  Scales past the end are of other blocks and meet no code.
+  const int rowa = T::A8 ? p.K : p.K / 2, roww = p.K / 2;
+  const u32x4 ra = rsrc_words(abase, (uint32_t)((mrows - 1) * (int)p.lda + rowa));
+  const u32x4 rw = rsrc_words(wbase, (uint32_t)((nrows - 1) * (int)p.ldw + roww));
+  const uint32_t aend = (uint32_t)min(rowa, nk * T::RA), wend = (uint32_t)min(roww, nk * T::RW);
+  u32x4 rs[T::SI];
+  uint32_t soff[T::SI], sdst[T::SI];
+#pragma unroll
+  for (int i = 0; i < T::SI; ++i) {
+    // the surplus waves of the last round copy the last group again
+    const int b = min(wave + T::NW * i, T::SBLK - 1);
+    const bool of_a = b < T::BM / 32;
+    rs[i] = rsrc_words(of_a ? asbase : wsbase, (uint32_t)((of_a ? agroups : wgroups) * group));
+    soff[i] = (uint32_t)((of_a ? b : b - T::BM / 32) * group + lane * 4);
+    sdst[i] = (uint32_t)(T::S_AT + b * 256);
+  }
   struct Step {
-    u32x4 ra, rw, sa, sw;
-    uint32_t st;
-    uint32_t adead, wdead;
+    uint32_t st;        // LDS address of the stage
+    uint32_t ka, kw;    // offset of the lane's chunk in its row, or out of range
+    uint32_t ks;        // of the stage's scales in a row group's
   };
   auto prepare = [&](const int kt, const int stage) __attribute__((always_inline)) {
     Step sc;
-    const int ka = kt * T::RA, kw = kt * T::RW, ks = (T::A8 ? kt >> 1 : kt) * 256;
-    const int la = (T::A8 ? p.K : p.K / 2) - ka, lw = p.K / 2 - kw;
-    const bool in = kt < nk;
-    sc.ra = rsrc_words(abase + ka, in ? (uint32_t)((mrows - 1) * (int)p.lda + min(T::RA, la)) : 0u);
-    sc.rw = rsrc_words(wbase + kw, in ? (uint32_t)((nrows - 1) * (int)p.ldw + min(T::RW, lw)) : 0u);
-    sc.sa = rsrc_words(asbase + ks, in ? (uint32_t)(agroups * group - ks) : 0u);
-    sc.sw = rsrc_words(wsbase + ks, in ? (uint32_t)(wgroups * group - ks) : 0u);
     sc.st = lds0 + (uint32_t)(stage * T::STAGE);
-    sc.adead = (la < T::RA && achunk >= la) ? 0x80000000u : 0u;
-    sc.wdead = (lw < T::RW && wchunk >= lw) ? 0x80000000u : 0u;
+    sc.ka = (uint32_t)(kt * T::RA + achunk);
+    sc.ka = sc.ka < aend ? sc.ka : 0x80000000u;
+    sc.kw = sc.ka;
+    if constexpr (T::A8) {
+      sc.kw = (uint32_t)(kt * T::RW + wchunk);
+      sc.kw = sc.kw < wend ? sc.kw : 0x80000000u;
+    }
+    sc.ks = (uint32_t)((T::A8 ? kt >> 1 : kt) * 256);
     return sc;
   };
   auto issue = [&](const Step& sc, const int i) __attribute__((always_inline)) {
     if (i < T::AI) {
-      dma16(sc.ra, sc.st + (uint32_t)((wave + T::NW * i) * 1024), aoff[i] | sc.adead);
+      dma16(ra, sc.st + (uint32_t)((wave + T::NW * i) * 1024), aoff[i] + sc.ka);
     } else if (i < T::AI + T::WI) {
       const int k = i - T::AI;
-      dma16(sc.rw, sc.st + (uint32_t)(T::W_AT + (wave + T::NW * k) * 1024), woff[k] | sc.wdead);
+      dma16(rw, sc.st + (uint32_t)(T::W_AT + (wave + T::NW * k) * 1024), woff[k] + sc.kw);
     } else {
-      // the surplus waves of the last round copy the last group again
-      const int b = min(wave + T::NW * (i - T::AI - T::WI), T::SBLK - 1);
-      const bool of_a = b < T::BM / 32;
-      const uint32_t off = (uint32_t)((of_a ? b : b - T::BM / 32) * group + lane * 4);
-      dma4(of_a ? sc.sa : sc.sw, sc.st + (uint32_t)(T::S_AT + b * 256), off);
+      const int k = i - T::AI - T::WI;
+      dma4(rs[k], sc.st + sdst[k], soff[k] + sc.ks);
     }
   };
 
