@@ -19,6 +19,7 @@
 #include <limits.h>
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "qik_mx.h"
 #include "qik_mx_block.h"
@@ -30,8 +31,8 @@ using qik_tile::cdiv;
 using qik_tile::choose_group_m;
 using qik_tile::choose_plan;
 using qik_tile::device_cus;
-using qik_tile::dma16;
-using qik_tile::dma4;
+using qik_tile::dma16_at;
+using qik_tile::dma4_at;
 using qik_tile::GemmPlan;
 using qik_tile::lds_ptr_t;
 using qik_tile::rsrc_words;
@@ -92,6 +93,30 @@ __device__ __forceinline__ i32x8 operand(u32x4 lo, u32x4 hi) {
 // ---------------------------------------------------------------------------
 // Tiles
 // ---------------------------------------------------------------------------
+
+template <int I>
+using num = std::integral_constant<int, I>;
+
+// f(num<0>) .. f(num<N - 1>)
+template <class F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+  (f(num<I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+  each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+// f(num<(kt - kb) % U>, kt) for kt of [kb, nk), nk > kb
+template <class F, int... I>
+__device__ __forceinline__ void stages_of(int kt, const int nk, F&& f, std::integer_sequence<int, I...>) {
+  while (((f(num<I>{}, kt), ++kt < nk) && ...)) {
+  }
+}
+template <int U, class F>
+__device__ __forceinline__ void stages(const int kb, const int nk, F&& f) {
+  stages_of(kb, nk, f, std::make_integer_sequence<int, U>{});
+}
 
 // Tile shape BM x BN, WGM x WGN waves, NS stages.  A stage holds 128 bytes of
 // every A row (256 k of MXFP4, 128 of MXFP8), the W codes of the same k (128 or
@@ -277,6 +302,7 @@ __device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion&
   const uint32_t aend = (uint32_t)min(rowa, nk * T::RA), wend = (uint32_t)min(roww, nk * T::RW);
   u32x4 rs[T::SI];
   uint32_t soff[T::SI], sdst[T::SI];
+  const uint32_t cdst = lds0 + (uint32_t)wave * 1024;
 #pragma unroll
   for (int i = 0; i < T::SI; ++i) {
     // the surplus waves of the last round copy the last group again
@@ -284,16 +310,14 @@ __device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion&
     const bool of_a = b < T::BM / 32;
     rs[i] = rsrc_words(of_a ? asbase : wsbase, (uint32_t)((of_a ? agroups : wgroups) * group));
     soff[i] = (uint32_t)((of_a ? b : b - T::BM / 32) * group + lane * 4);
-    sdst[i] = (uint32_t)(T::S_AT + b * 256);
+    sdst[i] = lds0 + (uint32_t)(T::S_AT + b * 256);
   }
   struct Step {
-    uint32_t st;        // LDS address of the stage
     uint32_t ka, kw;    // offset of the lane's chunk in its row, or out of range
     uint32_t ks;        // of the stage's scales in a row group's
   };
-  auto prepare = [&](const int kt, const int stage) __attribute__((always_inline)) {
+  auto prepare = [&](const int kt) __attribute__((always_inline)) {
     Step sc;
-    sc.st = lds0 + (uint32_t)(stage * T::STAGE);
     sc.ka = (uint32_t)(kt * T::RA + achunk);
     sc.ka = sc.ka < aend ? sc.ka : 0x80000000u;
     sc.kw = sc.ka;
@@ -304,30 +328,40 @@ __device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion&
     sc.ks = (uint32_t)((T::A8 ? kt >> 1 : kt) * 256);
     return sc;
   };
-  auto issue = [&](const Step& sc, const int i) __attribute__((always_inline)) {
-    if (i < T::AI) {
-      dma16(ra, sc.st + (uint32_t)((wave + T::NW * i) * 1024), aoff[i] + sc.ka);
-    } else if (i < T::AI + T::WI) {
-      const int k = i - T::AI;
-      dma16(rw, sc.st + (uint32_t)(T::W_AT + (wave + T::NW * k) * 1024), woff[k] + sc.kw);
-    } else {
-      const int k = i - T::AI - T::WI;
-      dma4(rs[k], sc.st + sdst[k], soff[k] + sc.ks);
-    }
+  // copies [C0, C1) of the step into stage ST
+  auto issue = [&](auto st_tag, const Step& sc, auto c0_tag, auto c1_tag) __attribute__((always_inline)) {
+    constexpr int ST = decltype(st_tag)::value * T::STAGE, C0 = decltype(c0_tag)::value, C1 = decltype(c1_tag)::value;
+    auto copy = [&](auto i_tag) __attribute__((always_inline)) {
+      constexpr int i = C0 + decltype(i_tag)::value;
+      if constexpr (i < T::AI) {
+        dma16_at<ST + T::NW * i * 1024>(ra, cdst, aoff[i] + sc.ka);
+      } else if constexpr (i < T::AI + T::WI) {
+        constexpr int k = i - T::AI;
+        dma16_at<ST + T::W_AT + T::NW * k * 1024>(rw, cdst, woff[k] + sc.kw);
+      } else {
+        constexpr int k = i - T::AI - T::WI;
+        dma4_at<ST>(rs[k], sdst[k], soff[k] + sc.ks);
+      }
+    };
+    each<C1 - C0>(copy);
   };
 
-  // fragment reads: lane l reads row l % 32 of a 32-row block
+  // fragment reads: lane l reads row l % 32 of a 32-row block; the offsets hold
+  // the wave's place, so that a stage and a block are an instruction's constant
   const int frow = lane & 31, half = lane >> 5;
   constexpr int ACH = T::A8 ? 2 : 1;  // chunks of an A fragment
   uint32_t fa_off[T::KS][ACH], fw_off[T::KS];
 #pragma unroll
   for (int s = 0; s < T::KS; ++s) {
     const int c0 = T::A8 ? 4 * s + half : 4 * half + s;
-    fa_off[s][0] = (uint32_t)(frow * 128 + ((c0 ^ ((frow >> 1) & 7)) * 16));
-    if constexpr (T::A8) fa_off[s][ACH - 1] = (uint32_t)(frow * 128 + (((c0 + 2) ^ ((frow >> 1) & 7)) * 16));
-    fw_off[s] = T::A8 ? (uint32_t)(frow * 64 + (((2 * s + half) ^ ((frow >> 2) & 3)) * 16)) : fa_off[s][0];
+    const uint32_t r0 = (uint32_t)((wm * T::WM + frow) * 128);
+    fa_off[s][0] = r0 + (uint32_t)((c0 ^ ((frow >> 1) & 7)) * 16);
+    if constexpr (T::A8) fa_off[s][ACH - 1] = r0 + (uint32_t)(((c0 + 2) ^ ((frow >> 1) & 7)) * 16);
+    fw_off[s] = (uint32_t)((wn * T::WN + frow) * T::RW) +
+                (uint32_t)(T::A8 ? ((2 * s + half) ^ ((frow >> 2) & 3)) * 16 : (c0 ^ ((frow >> 1) & 7)) * 16);
   }
-  const uint32_t sc_off = (uint32_t)(T::S_AT + frow * 8 + (T::A8 ? 0 : half * 4));
+  const uint32_t sc_off = (uint32_t)(frow * 8 + (T::A8 ? 0 : half * 4));
+  const uint32_t sa_off = sc_off + (uint32_t)(wm * T::MI * 256), sw_off = sc_off + (uint32_t)(wn * T::NJ * 256);
 
   // fragments in two buffers, of a k-step each, or of a whole stage (T::WS)
   constexpr int SLOTS = T::WS ? T::KS : 1;
@@ -340,16 +374,16 @@ __device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion&
     const int slot = T::WS ? s : 0;
     if (r < T::MI * ACH) {
       const int f = r / ACH;
-      fa[buf][slot][f][r % ACH] = *reinterpret_cast<const u32x4*>(st + (wm * T::WM + f * 32) * T::RA + fa_off[s][r % ACH]);
+      fa[buf][slot][f][r % ACH] = *reinterpret_cast<const u32x4*>(st + f * 32 * T::RA + fa_off[s][r % ACH]);
     } else {
       const int f = r - T::MI * ACH;
-      fw[buf][slot][f] = *reinterpret_cast<const u32x4*>(st + T::W_AT + (wn * T::WN + f * 32) * T::RW + fw_off[s]);
+      fw[buf][slot][f] = *reinterpret_cast<const u32x4*>(st + T::W_AT + f * 32 * T::RW + fw_off[s]);
     }
   };
   auto read_scale = [&](const int stage, const int odd, const int r) __attribute__((always_inline)) {
-    const int b = r < T::MI ? wm * T::MI + r : T::BM / 32 + wn * T::NJ + r - T::MI;
-    const unsigned char* at = lds + stage * T::STAGE + b * 256 + sc_off;
-    const int v = *reinterpret_cast<const int*>(at + (T::A8 ? odd * 4 : 0));
+    const int b = r < T::MI ? r : T::BM / 32 + r - T::MI;
+    const unsigned char* at = lds + stage * T::STAGE + T::S_AT + b * 256;
+    const int v = *reinterpret_cast<const int*>(at + (r < T::MI ? sa_off : sw_off) + (T::A8 ? odd * 4 : 0));
     if (r < T::MI) nsa[r] = v;
     else nsw[r - T::MI] = v;
   };
@@ -373,14 +407,11 @@ __device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion&
     const int b = wave % T::BIAS_COPIES;
     const u32x4 rb = rsrc_words(reinterpret_cast<const unsigned char*>(rg.bias) + n0 * 2,
                                 rg.bias != nullptr ? (uint32_t)(nrows / 2 * 4) : 0u);
-    dma4(rb, lds0 + (uint32_t)(T::BIAS_AT + b * 256), (uint32_t)(b * 256 + lane * 4));
+    dma4_at<T::BIAS_AT>(rb, lds0 + (uint32_t)(b * 256), (uint32_t)(b * 256 + lane * 4));
   }
-#pragma unroll
-  for (int s0 = 0; s0 < T::NS; ++s0) {
-    const Step sc = prepare(kb + s0, s0);
-#pragma unroll
-    for (int c = 0; c < T::COPIES; ++c) issue(sc, c);
-  }
+  each<T::NS>([&](auto s_tag) __attribute__((always_inline)) {
+    issue(s_tag, prepare(kb + decltype(s_tag)::value), num<0>{}, num<T::COPIES>{});
+  });
   wait_vmcnt<(T::NS - 1) * T::COPIES>();
   __syncthreads();
 #pragma unroll
@@ -399,7 +430,7 @@ __device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion&
         FMT_E2M1, T::A8 ? FMT_E4M3 : FMT_E2M1, OP, sw[j], OP, sa[i]);
   };
 
-  int st = 0;  // LDS stage of step kt
+  // The loops are unrolled over the stages: a stage's LDS addresses are constants.
   if constexpr (!T::WS) {
     // k-step S of a stage on fragments S % 2, with the reads of the next k-step
     // into the others between its MFMAs.  The last one (COPY) issues its first
@@ -409,16 +440,16 @@ __device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion&
     // the next stage and the copies of the stage after next into this one's
     // memory.
     constexpr int PRE = 2 < NMF ? 2 : 1;
-    auto kstep = [&](auto s_tag, const int stage, const int next, const int next_odd, const Step& sc)
-        __attribute__((always_inline)) {
+    auto kstep = [&](auto s_tag, auto st_tag, const int next_odd, const Step& sc) __attribute__((always_inline)) {
       constexpr int S = decltype(s_tag)::value;
+      constexpr int stage = decltype(st_tag)::value, next = (stage + 1) % T::NS;
       constexpr bool COPY = S == T::KS - 1;
       // reads (and copies) after MFMAs [R0, R0 + H)
       constexpr int R0 = COPY ? (NMF > PRE ? PRE : PRE - 1) : 0;
       constexpr int H = COPY ? NMF - R0 : (NMF >= 2 ? NMF / 2 : 1);
       constexpr int RD = NRD + (COPY ? NSR : 0);
-#pragma unroll
-      for (int idx = 0; idx < NMF; ++idx) {
+      each<NMF>([&](auto idx_tag) __attribute__((always_inline)) {
+        constexpr int idx = decltype(idx_tag)::value;
         mfma(s_tag, idx, S % 2);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (COPY) {
@@ -434,48 +465,42 @@ __device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion&
             if (r < NRD) read_frag(COPY ? next : stage, COPY ? 0 : S + 1, r, (S + 1) % 2);
             else read_scale(next, next_odd, r - NRD);
           }
-          if constexpr (COPY) {
-#pragma unroll
-            for (int c = (idx - R0) * T::COPIES / H; c < (idx - R0 + 1) * T::COPIES / H; ++c) issue(sc, c);
-          }
+          if constexpr (COPY && idx >= R0 && idx < R0 + H)
+            issue(st_tag, sc, num<(idx - R0) * T::COPIES / H>{}, num<(idx - R0 + 1) * T::COPIES / H>{});
         }
         __builtin_amdgcn_sched_barrier(0);
-      }
+      });
     };
-    for (int kt = kb; kt < nk; ++kt) {
+    stages<T::NS>(kb, nk, [&](auto st_tag, const int kt) __attribute__((always_inline)) {
       const Step none = {};
-      const int nst = st + 1 == T::NS ? 0 : st + 1;
       take_scales();
-      kstep(std::integral_constant<int, 0>{}, st, nst, 0, none);
+      kstep(num<0>{}, st_tag, 0, none);
       if constexpr (T::KS == 4) {
-        kstep(std::integral_constant<int, 1>{}, st, nst, 0, none);
-        kstep(std::integral_constant<int, 2>{}, st, nst, 0, none);
+        kstep(num<1>{}, st_tag, 0, none);
+        kstep(num<2>{}, st_tag, 0, none);
       }
       __builtin_amdgcn_sched_barrier(0);
-      const Step sc = prepare(kt + T::NS, st);
-      kstep(std::integral_constant<int, T::KS - 1>{}, st, nst, (kt + 1) & 1, sc);
-      st = nst;
-    }
+      const Step sc = prepare(kt + T::NS);
+      kstep(num<T::KS - 1>{}, st_tag, (kt + 1) & 1, sc);
+    });
   } else {
     // A tile of few MFMAs per k-step is bound by the latency of its fragment
     // reads (about 130 cycles a k-step at one MFMA of 32), so a whole stage of
     // fragments is read at a time, one stage ahead: all MFMAs of a stage run on
     // registers, and the stage's memory is free for the copies of the stage NS
     // later as soon as the barrier says that every wave has its fragments.
-    auto stage_step = [&](auto buf_tag, const int kt) __attribute__((always_inline)) {
-      constexpr int BUF = decltype(buf_tag)::value;
+    auto stage_step = [&](auto u_tag, const int kt) __attribute__((always_inline)) {
+      constexpr int BUF = decltype(u_tag)::value % 2, st = decltype(u_tag)::value % T::NS, nst = (st + 1) % T::NS;
       constexpr int TOTAL = T::KS * NMF;
       constexpr int PRE = TOTAL / 4 < 2 ? 1 : 2;
       constexpr int H = TOTAL - PRE;  // MFMAs with reads and copies beside them
       constexpr int RD = T::KS * NRD + NSR;
-      const int nst = st + 1 == T::NS ? 0 : st + 1;
       take_scales();
-      const Step sc = prepare(kt + T::NS, st);
+      const Step sc = prepare(kt + T::NS);
       auto run = [&](auto s_tag) __attribute__((always_inline)) {
         constexpr int S = decltype(s_tag)::value;
-#pragma unroll
-        for (int i = 0; i < NMF; ++i) {
-          const int idx = S * NMF + i;
+        each<NMF>([&](auto i_tag) __attribute__((always_inline)) {
+          constexpr int i = decltype(i_tag)::value, idx = S * NMF + i;
           mfma(s_tag, i, BUF);
           __builtin_amdgcn_sched_barrier(0);
           if (idx == PRE - 1) {
@@ -483,31 +508,21 @@ __device__ __forceinline__ void gemm_tile(const MxGemmParams& p, const MxRegion&
             __syncthreads();
             __builtin_amdgcn_sched_barrier(0);
           }
-          if (idx >= PRE - 1 && idx < PRE - 1 + H) {
-            const int q = idx - (PRE - 1);
+          if constexpr (idx >= PRE - 1 && idx < PRE - 1 + H) {
+            constexpr int q = idx - (PRE - 1);
 #pragma unroll
             for (int r = q * RD / H; r < (q + 1) * RD / H; ++r) {
               if (r < T::KS * NRD) read_frag(nst, r / NRD, r % NRD, BUF ^ 1);
               else read_scale(nst, (kt + 1) & 1, r - T::KS * NRD);
             }
-#pragma unroll
-            for (int c = q * T::COPIES / H; c < (q + 1) * T::COPIES / H; ++c) issue(sc, c);
+            issue(num<st>{}, sc, num<q * T::COPIES / H>{}, num<(q + 1) * T::COPIES / H>{});
           }
           __builtin_amdgcn_sched_barrier(0);
-        }
+        });
       };
-      run(std::integral_constant<int, 0>{});
-      run(std::integral_constant<int, 1>{});
-      if constexpr (T::KS == 4) {
-        run(std::integral_constant<int, 2>{});
-        run(std::integral_constant<int, 3>{});
-      }
-      st = nst;
+      each<T::KS>(run);
     };
-    for (int kt = kb; kt < nk; kt += 2) {
-      stage_step(std::integral_constant<int, 0>{}, kt);
-      if (kt + 1 < nk) stage_step(std::integral_constant<int, 1>{}, kt + 1);
-    }
+    stages<T::NS % 2 == 0 ? T::NS : 2 * T::NS>(kb, nk, stage_step);  // both buffers' turns too
   }
   wait_vmcnt<0>();  // the copies of the steps past the end still land in their stages
   if constexpr (SPLIT) store_partial<T>(p, rg, m0, n0, acc, slice, wave, lane);

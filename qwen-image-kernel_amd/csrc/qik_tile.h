@@ -24,10 +24,17 @@ __device__ __forceinline__ void dma16(u32x4 rsrc, uint32_t lds_addr, uint32_t vo
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :: "s"(lds_addr), "v"(voff), "s"(rsrc) : "m0");
 }
-// the same with 4 bytes a lane: 256 contiguous bytes of LDS
-__device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t lds_addr, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-               :: "s"(lds_addr), "v"(voff), "s"(rsrc) : "m0");
+// The same to LDS byte lds_addr + AT, and with 4 bytes a lane: 256 contiguous
+// bytes of LDS.
+template <uint32_t AT>
+__device__ __forceinline__ void dma16_at(u32x4 rsrc, uint32_t lds_addr, uint32_t voff) {
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(lds_addr), "v"(voff), "s"(rsrc), "i"(AT) : "m0", "scc");
+}
+template <uint32_t AT>
+__device__ __forceinline__ void dma4_at(u32x4 rsrc, uint32_t lds_addr, uint32_t voff) {
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :: "s"(lds_addr), "v"(voff), "s"(rsrc), "i"(AT) : "m0", "scc");
 }
 #pragma clang diagnostic pop
 
