@@ -899,10 +899,10 @@ int launch_rows(MxGemmParams& p, const qik_mx_gemm_args* a, hipStream_t s) {
 // tiles of 64 rows, which wait more than they multiply, do not.
 enum { T256x256, T256x128, T128x256, T128x128, T192x256, T192x128, T64x128, T64x64, NSHAPES };
 static const TileShape kShapes[2][NSHAPES] = {
-    {{256, 256, 8.6, 1.22}, {256, 128, 6.15, 0.67}, {128, 256, 6.35, 0.645}, {128, 128, 4.6, 0.44, 0.4},
-     {192, 256, 7.3, 0.99}, {192, 128, 5.5, 0.575, 0.6}, {64, 128, 4.5, 0.305, 0.0}, {64, 64, 3.9, 0.25, 0.0}},
-    {{256, 256, 9.1, 1.0}, {256, 128, 6.0, 0.595}, {128, 256, 6.25, 0.56}, {128, 128, 4.45, 0.415, 0.4},
-     {192, 256, 7.7, 0.765}, {192, 128, 5.55, 0.515, 0.6}, {64, 128, 4.3, 0.29, 0.0}, {64, 64, 3.85, 0.235, 0.0}}};
+    {{256, 256, 8.75, 1.16}, {256, 128, 6.25, 0.58, 1.4}, {128, 256, 6.35, 0.55, 1.4}, {128, 128, 4.35, 0.37, 0.7},
+     {192, 256, 7.5, 0.965}, {192, 128, 5.45, 0.495, 0.9}, {64, 128, 4.15, 0.29, 0.0}, {64, 64, 3.75, 0.18, 0.0}},
+    {{256, 256, 9.15, 0.93}, {256, 128, 5.9, 0.525, 1.2}, {128, 256, 5.95, 0.505, 1.2}, {128, 128, 4.05, 0.335, 0.6},
+     {192, 256, 7.8, 0.705}, {192, 128, 5.1, 0.445, 0.8}, {64, 128, 3.65, 0.27, 0.0}, {64, 64, 3.45, 0.165, 0.0}}};
 constexpr int NPAIRS = 7;
 static const int kPairs[NPAIRS][2] = {{T256x256, T256x128}, {T256x256, T128x128}, {T256x128, T128x128},
                                       {T128x256, T128x128}, {T192x256, T192x128}, {T192x128, T128x128},
