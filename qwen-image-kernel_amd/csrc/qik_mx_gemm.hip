@@ -872,16 +872,16 @@ int launch_rows_shape(MxGemmParams& p, const qik_mx_gemm_args* a, hipStream_t s)
 
 // Weight rows (in 16s) and waves of a workgroup.  Past 8192 columns there is a
 // workgroup of 16 rows for every second wave slot: four waves each (1 x 12288 x
-// 4096 7.8 us, 9.3 with eight), and 32 rows where the codes of A are worth sharing
-// (1 x 12288 x 4096 7.8 us with 16 rows, 8.2 with 32; 16 x 24576 x 4096 18.1 and
-// 13.9).  Below, eight waves share a long K (1 x 4096 x 12288 8.6 us, 11.2 with
+// 4096 7.8 us, 9.3 with eight), and past 16384, or where they are to be quantised,
+// 32 rows that share the codes of A (9 x 24576 x 1024 6.7 us with 16 rows, 5.7 with
+// 32; 16 x 12288 x 1024 3.8 and 4.2).  Below, eight waves share a long K (1 x 4096 x 12288 8.6 us, 11.2 with
 // four; 1 x 4096 x 1536 3.0 and 3.1, x 1024 2.8 and 2.7), or the quantising of
 // elements, which goes by threads.
 struct RowsPlan {
   int nb, kw;
 };
 RowsPlan choose_rows(int64_t M, int64_t N, int64_t K, bool raw) {
-  return {N > 8192 && M > 8 ? 2 : 1, N > 8192 || (!raw && K <= 4 * 256) ? 4 : 8};
+  return {M > 8 && N > (raw ? 8192 : 16384) ? 2 : 1, N > 8192 || (!raw && K <= 4 * 256) ? 4 : 8};
 }
 
 template <int SRC, bool A8, int MB>
@@ -903,10 +903,9 @@ static const TileShape kShapes[2][NSHAPES] = {
      {192, 256, 7.5, 0.965}, {192, 128, 5.45, 0.495, 0.9}, {64, 128, 4.15, 0.29, 0.0}, {64, 64, 3.75, 0.18, 0.0}},
     {{256, 256, 9.15, 0.93}, {256, 128, 5.9, 0.525, 1.2}, {128, 256, 5.95, 0.505, 1.2}, {128, 128, 4.05, 0.335, 0.6},
      {192, 256, 7.8, 0.705}, {192, 128, 5.1, 0.445, 0.8}, {64, 128, 3.65, 0.27, 0.0}, {64, 64, 3.45, 0.165, 0.0}}};
-constexpr int NPAIRS = 7;
-static const int kPairs[NPAIRS][2] = {{T256x256, T256x128}, {T256x256, T128x128}, {T256x128, T128x128},
-                                      {T128x256, T128x128}, {T192x256, T192x128}, {T192x128, T128x128},
-                                      {T64x128, T64x64}};
+constexpr int NPAIRS = 5;
+static const int kPairs[NPAIRS][2] = {{T256x256, T256x128}, {T256x256, T128x128}, {T128x256, T128x128},
+                                      {T192x256, T192x128}, {T64x128, T64x64}};
 static const TileTable kTables[2] = {{kShapes[0], kPairs, NPAIRS, 0, 0.5, 0.5},
                                      {kShapes[1], kPairs, NPAIRS, 0, 0.5, 0.5}};
 
@@ -922,10 +921,9 @@ struct MxPlan {
 // A K split pays for a launch with few tiles and a long K: S slices of 64 x 64 or
 // 128 x 128 tiles, as many as the CUs run in one round (all slices of a tile on
 // one XCD), and a second launch that joins them: 3 us, and the fp32 sums written
-// and read at about 4 TB/s (64 x 4096 x 12288 16.6 us unsplit, 12.8 in 4 slices,
-// 15.7 in 8; 200 x 1024 x 8192 12.5 and 10.6 in 4; 203 x 2048 x 8192 12.7 and 12.8
-// in 2, with MXFP8 rows 19.4 and 16.6; 203 x 4096 x 12288 17.4 and 18.6 in 4 of
-// 128 x 128).
+// and read at about 4 TB/s (64 x 4096 x 12288 13.0 us unsplit, 12.2 in 4 slices,
+// 14.8 in 8, with MXFP8 rows 19.8, 12.6 and 15.7; 200 x 1024 x 8192 with MXFP8 rows
+// 13.9 and 10.8 in 4; 203 x 4096 x 12288 14.0 and 22.0 in 4 of 128 x 128).
 MxPlan choose(int64_t M, int64_t N, int64_t K, bool a8, int cus) {
   const int64_t steps = cdiv(K, a8 ? 128 : 256), P = std::max(1, (cus > 0 ? cus : 256) / 8);
   const GemmPlan g = choose_plan(kTables[a8], M, N, steps, cus);
@@ -967,25 +965,25 @@ int launch_plan(MxGemmParams& p, const qik_mx_gemm_args* a, const MxPlan& plan, 
   switch (plan.pair) {
     case 0: return launch_tiles<C256x256, C256x128>(p, a, plan.n1, s);
     case 1: return launch_tiles<C256x256, C128x128>(p, a, plan.n1, s);
-    case 2: return launch_tiles<C256x128, C128x128>(p, a, plan.n1, s);
-    case 3: return launch_tiles<C128x256, C128x128>(p, a, plan.n1, s);
-    case 4: return launch_tiles<C192x256, C192x128>(p, a, plan.n1, s);
-    case 5: return launch_tiles<C192x128, C128x128>(p, a, plan.n1, s);
+    case 2: return launch_tiles<C128x256, C128x128>(p, a, plan.n1, s);
+    case 3: return launch_tiles<C192x256, C192x128>(p, a, plan.n1, s);
     default: return launch_tiles<C64x128, C64x64>(p, a, plan.n1, s);
   }
 }
 
 // Few rows: the tiles of 64 would multiply mostly padding.  They do better all
-// the same where K is so long that splitting it over workgroups pays (us, rows
-// then tiles: 1 x 4096 x 16384 10.9 / 11.7 and x 32768 18.8 / 18.2; 32 x 4096 x
-// 8192 9.3 / 10.5 and x 12288 12.5 / 11.8, with MXFP8 rows x 4096 7.5 / 10.0 and x
-// 8192 12.8 / 12.4), and where N has tiles for most CUs and K is long (16 x 8192 x
-// 8192 11.7 / 12.9, 16 x 12288 x 8192 15.8 / 13.2; 32 x 5120 x 2048 5.4 / 6.2, 32 x
-// 12288 x 4096 11.8 / 8.9).
+// the same where N has tiles for most CUs and K is long, or where K is so long
+// that splitting it over workgroups pays (us, rows then tiles: 1 x 4096 x 12288
+// 8.6 / 10.1, 8 x 512 x 16384 8.6 / 7.6, 8 x 12288 x 2048 5.7 / 6.0 and x 4096 8.4 /
+// 7.9; 16 x 4096 x 8192 7.4 / 9.7 and with MXFP8 rows x 12288 11.9 / 11.3, 16 x
+// 12288 x 1024 4.1 / 4.5 and x 2048 6.5 / 6.1; 32 x 4096 x 6144 7.6 / 7.9 and x 8192
+// 9.4 / 9.0, with MXFP8 rows x 4096 7.3 / 8.0 and x 6144 10.3 / 9.8, 32 x 5120 x
+// 2048 5.3 / 4.8).
 bool takes_rows(const qik_mx_gemm_args* a) {
-  if (a->M <= 8) return a->K <= 16384;
-  if (a->M <= 16) return a->K <= 16384 && a->N * a->K <= ((int64_t)1 << 26);
-  return a->M <= 32 && (a->N <= 4096 ? a->K <= (a->a_format == QIK_MXFP8 ? 6144 : 8192) : a->N * a->K <= (1 << 24));
+  const bool narrow = a->N <= 4096;
+  if (a->M <= 8) return narrow ? a->K <= 12288 : a->N * a->K <= (1 << 25);
+  if (a->M <= 16) return narrow ? a->K <= 8192 : a->N * a->K <= (1 << 24);
+  return a->M <= 32 && narrow && a->K <= (a->a_format == QIK_MXFP8 ? 4096 : 6144);
 }
 
 // A linear whose workgroups each quantise all of x for themselves saves a
@@ -995,7 +993,7 @@ bool takes_rows(const qik_mx_gemm_args* a) {
 // 10.2, 17 x 5001 x 1504 6.2 / 5.8 and with MXFP8 8.5 / 7.1; called in a loop the
 // last takes 9 against 11.6).
 bool takes_raw(const qik_mx_gemm_args* a) {
-  if (a->M * a->K > RAW_ELEMS || (a->M > 16 && !takes_rows(a))) return false;
+  if (a->M * a->K > RAW_ELEMS || (a->M > 16 && (a->M > 32 || a->N * a->K > (1 << 24)))) return false;
   const int64_t wgs = cdiv(a->N, 16 * choose_rows(a->M, a->N, a->K, true).nb);
   return cdiv(wgs, 256) * a->M * a->K <= 2 * RAW_ELEMS;
 }

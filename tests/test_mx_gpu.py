@@ -334,7 +334,9 @@ def test_split_products(fmt, M, N, K):
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("M,N,K", [(16, 8200, 288), (9, 8233, 96), (32, 8300, 96), (20, 9000, 2048), (31, 4100, 4128),
                                    (2, 33, 262144), (40, 33, 262144), (16, 40, 16384), (16, 40, 16416), (1, 65, 32768),
-                                   (3, 65, 16416), (9, 8300, 8192), (20, 64, 6144), (20, 64, 6176), (32, 64, 8224)])
+                                   (3, 65, 16416), (9, 8300, 8192), (20, 64, 6144), (20, 64, 6176), (32, 64, 8224), (20, 64, 4128),
+                                   (8, 70, 12288), (8, 70, 12320), (16, 70, 8224), (9, 16500, 992), (12, 9000, 1888),
+                                   (5, 8200, 4128)])
 def test_few_rows_wide_and_long(fmt, M, N, K):
     """Few rows into many columns, the two widths of the few-rows kernel, and the longest K."""
     say("wide", fmt, M, N, K)
