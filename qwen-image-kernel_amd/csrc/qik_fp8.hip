@@ -1077,7 +1077,7 @@ static const int kPairs[NPAIRS][2] = {{T256x256, T256x128}, {T256x128, T128x128}
 
 inline int64_t steps_of(int64_t K) { return cdiv(K, 128); }  // 128-k-byte steps
 
-// The clock under load (TileTable): from 24 steps (K = 3072) on the matrix cores run long
+// The clock under load (TileTable): from 24 steps of 128 k on the matrix cores run long
 // enough that the clock follows it: the tile times hold with three quarters of the CUs
 // busy, and with all of them busy a tile takes 14% longer.  (Quantiser + GEMM,
 // the weights of six layers in turn: time / makespan from the tile times, the

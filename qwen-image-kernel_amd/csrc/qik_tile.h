@@ -204,8 +204,8 @@ inline GemmPlan choose_plan(const TileTable& tb, int64_t M, int64_t N, int64_t s
     }
   }
   // the small tiles first when that is estimated no slower (measured on the fp8
-  // product: 1-2% faster at 4352 x 9216 x 3072 and 4352 x 12288 x 3072, whose makespans are
-  // equal either way; 12% slower at 1543 x 9232 x 1104, whose is not)
+  // product: 1-2% faster where the makespans are equal either way, as at 4352 rows
+  // into 9216 and 12288 columns; 12% slower at 1543 x 9232 x 1104, whose are not)
   const TileShape& s1 = tb.shapes[tb.pairs[best.pair][0]];
   const TileShape& s2 = tb.shapes[tb.pairs[best.pair][1]];
   const int64_t t1 = cdiv(M, s1.bm) * cdiv(best.n1, s1.bn);
