@@ -731,3 +731,28 @@ def test_nothing_beside_the_outputs_is_written(fmt):
         assert lib.qik_mx_gemm(ctypes.byref(g), ws.data_ptr(), n.value, torch.cuda.current_stream().cuda_stream) == 0
         check_product(buf[1:M + 1, :N], av, wv, None, torch.bfloat16, fmt)
         assert (buf[0] == 3).all() and (buf[M + 1] == 3).all() and (buf[:, N:] == 3).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(1, 40, 288), (20, 70, 1504), (40, 33, 32), (70, 129, 96), (64, 100, 12320), (300, 260, 544),
+                                   (1000, 520, 1056), (1300, 1100, 416)])
+def test_rows_with_bytes_between_them(fmt, M, N, K):
+    """Row strides of the codes beyond a row: what lies between the rows reaches no output, nor does what lies behind."""
+    import ctypes
+    from qwen_image_kernel_amd import _lib, mx
+    say("strides", fmt, M, N, K)
+    lib = _lib.load()
+    a, w = tensors(M, K, fmt, 1)[0], tensors(N, K, "mxfp4", 2)[0]
+    want = qik.mx_linear(a, w)
+    for pa, pw in ((16, 0), (0, 48), (80, 144)):
+        ca, cw = (torch.full((t.shape[0], t.codes.shape[1] + p), 0x7f, dtype=torch.uint8, device=DEV)
+                  for t, p in ((a, pa), (w, pw)))  # 0x7f: NaN in E4M3, 6 and -6 in E2M1
+        ca[:, :a.codes.shape[1]], cw[:, :w.codes.shape[1]] = a.codes.view(torch.uint8), w.codes
+        out = torch.full((M, N), 3.0, dtype=torch.bfloat16, device=DEV)
+        g = mx._gemm_args(fmt, cw, w.scales, None, torch.bfloat16, M, N, K)
+        g.a, g.a_scales, g.out, g.lda, g.ldw = ca.data_ptr(), a.scales.data_ptr(), out.data_ptr(), ca.shape[1], cw.shape[1]
+        n = ctypes.c_int64()
+        assert lib.qik_mx_gemm_workspace_size(ctypes.byref(g), ctypes.byref(n)) == 0
+        ws = torch.empty(max(n.value, 1), dtype=torch.uint8, device=DEV)
+        assert lib.qik_mx_gemm(ctypes.byref(g), ws.data_ptr(), n.value, torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out, want)
