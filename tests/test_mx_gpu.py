@@ -756,3 +756,29 @@ def test_rows_with_bytes_between_them(fmt, M, N, K):
         ws = torch.empty(max(n.value, 1), dtype=torch.uint8, device=DEV)
         assert lib.qik_mx_gemm(ctypes.byref(g), ws.data_ptr(), n.value, torch.cuda.current_stream().cuda_stream) == 0
         assert torch.equal(out, want)
+
+
+# every pair of tile shapes and each of the two alone, both orders, and the K split of 128 x 128 tiles, on 256 CUs;
+# from two stages of K to more than a loop's turn
+LAUNCHES = [(8202, 1813, 288), (7454, 1644, 288), (403, 11316, 288), (8202, 1350, 288), (810, 13702, 288), (5083, 3937, 288),
+            (1087, 13702, 1312), (8202, 143, 288), (602, 8490, 288), (810, 7009, 1824), (268, 11316, 1824), (8202, 908, 1824),
+            (7454, 1108, 288), (2597, 9344, 288), (8202, 71, 800), (8202, 1813, 1824), (2597, 71, 19424), (2597, 71, 12928)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", LAUNCHES)
+def test_product_of_every_launch(fmt, M, N, K):
+    say("launch", fmt, M, N, K)
+    g = torch.Generator(device=DEV).manual_seed(M + N)
+    a = qik.quantize_mx(torch.randn(M, K, generator=g, device=DEV), fmt)
+    w = qik.quantize_mx(torch.randn(N, K, generator=g, device=DEV), "mxfp4")
+    b = torch.randn(N, generator=g, device=DEV).bfloat16()
+    av, wv = a.dequantize(torch.float32).double(), w.dequantize(torch.float32).double()
+    want = av @ wv.t().contiguous() + b.double()
+    acc = (K + 1) * 2.0 ** -23 * (av.abs() @ wv.abs().t().contiguous() + b.double().abs())
+    if fmt == "mxfp8":  # the cut of a step's products, as in test_product_of_larger_tiles
+        top = [torch.nn.functional.pad(t.abs(), (0, -K % 128)).unflatten(1, (-1, 128)).amax(-1) for t in (av, wv)]
+        acc += 128 * 2.0 ** -13 * (top[0] @ top[1].t().contiguous())
+    err = (qik.mx_linear(a, w, b).double() - want).abs()
+    tol = acc + 2.0 ** -8 * (want.abs() + acc)
+    assert (err <= tol).all(), (err / tol).max().item()
