@@ -1,4 +1,5 @@
-// Element conversions on the host, for the quantisers of data in host memory.
+// Host-side helpers: element conversions for the quantisers of data in host
+// memory, and a launch's grid.
 #ifndef QIK_HOST_H
 #define QIK_HOST_H
 
@@ -56,6 +57,18 @@ inline unsigned char host_e4m3fn(float q) {
   // move the exponent from bias 127 to bias 7
   const uint32_t r = a + 0x7ffffu + ((a >> 20) & 1u);
   return sign | (unsigned char)((r >> 20) - (120u << 3));
+}
+
+// `workgroups` of `threads` as a grid of x * y workgroups, less than y of them
+// surplus, with fewer than 2^32 threads in x (a launch's limit) and y at most
+// 65535; false where no such grid holds them.
+inline bool split_grid(int64_t workgroups, int threads, unsigned* x, unsigned* y) {
+  const int64_t most = UINT32_MAX / threads;  // workgroups in x
+  const int64_t rows = (workgroups + most - 1) / most;
+  if (workgroups < 1 || rows > 65535) return false;
+  *x = (unsigned)((workgroups + rows - 1) / rows);
+  *y = (unsigned)rows;
+  return true;
 }
 
 }  // namespace qik_host

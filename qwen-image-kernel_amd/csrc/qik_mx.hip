@@ -374,12 +374,10 @@ int validate_norm(const qik_residual_rms_norm_args* a) {
 }
 
 int launch(const void* fn, int64_t grid, int threads, void* params, hipStream_t s) {
-  const int64_t gy = cdiv(grid * threads, UINT_MAX);  // below 2^32 threads in x
-  const int64_t gx = cdiv(grid, gy);                  // the last row's surplus is behind the last row of the data
-  if (gy > 65535) return QIK_ERR_SHAPE;
+  unsigned gx, gy;  // the surplus workgroups are behind the last row of the data
+  if (!qik_host::split_grid(grid, threads, &gx, &gy)) return QIK_ERR_SHAPE;
   void* args[] = {params};
-  const dim3 g((unsigned)gx, (unsigned)gy);
-  return hipLaunchKernel(fn, g, dim3((unsigned)threads), args, 0, s) == hipSuccess ? QIK_OK : QIK_ERR_LAUNCH;
+  return hipLaunchKernel(fn, dim3(gx, gy), dim3((unsigned)threads), args, 0, s) == hipSuccess ? QIK_OK : QIK_ERR_LAUNCH;
 }
 
 QuantParams unit_params(int64_t M, int64_t K, int64_t rows) {
