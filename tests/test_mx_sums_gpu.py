@@ -13,6 +13,8 @@ import torch
 from oracle import mx as om
 
 import qwen_image_kernel_amd as qik
+from mx_exact import exact_operands
+from test_mx_host import FORMATS
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +71,32 @@ def test_product_of_e4m3_is_the_cut_sum(M, N, K):
                         torch.from_numpy(bias).to(torch.float16).to(DEV), torch.float16)
     err = np.abs(got.double().cpu().numpy() - want)
     assert (err <= tol).all(), ((err / tol).max(), (err / tol)[row].max())
+
+
+def check_exact(M, N, K, fmt):
+    """mx_linear in both types, and MXFP4Linear of the values, give the exact sums rounded once."""
+    (ca, sa, a), (cw, sw, w), bias = exact_operands(M, N, K, fmt, M + N + K)
+    ta, tw = tensor(ca, sa, fmt), tensor(cw, sw, "mxfp4")
+    av, wv, bv = (torch.from_numpy(t.astype(np.float64)).to(DEV) for t in (a, w, bias))
+    assert (av.abs() @ wv.abs().t().contiguous() + bv.abs()).max() <= 2 ** 24
+    want = (av @ wv.t().contiguous() + bv).float()
+    for dtype in (torch.bfloat16, torch.float16):  # the bias is whole numbers up to 128: exact in both
+        got = qik.mx_linear(ta, tw, bv.to(dtype), dtype)
+        assert torch.equal(got, want.to(dtype)), ((got != want.to(dtype)).sum().item(), dtype)
+    mod = qik.MXFP4Linear.from_quantized(tw, bv, fmt)
+    for x in (av.bfloat16(), ta):  # up to 12: exact in bf16, and in both formats whatever the block's scale
+        assert torch.equal(mod(x), want.bfloat16())
+
+
+# few rows in the few-rows kernel's forms, with one launch and with two; few rows in tiles; K split over 64 x 64 and
+# 128 x 128 tiles; the longest K in each; ends of K inside a stage
+LONG = [(1, 40, 4096), (1, 65, 32768), (2, 33, 262144), (8, 70, 12288), (8, 70, 12320), (9, 8300, 8192), (16, 40, 16384),
+        (16, 40, 16416), (16, 70, 8224), (20, 64, 6144), (20, 64, 6176), (31, 300, 4128), (32, 64, 8224), (40, 33, 262144),
+        (64, 333, 8192), (130, 257, 12320), (200, 192, 12288), (300, 70, 65568), (2597, 71, 19424)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", LONG)
+def test_long_products_are_the_exact_sums(fmt, M, N, K):
+    say("exact", fmt, M, N, K)
+    check_exact(M, N, K, fmt)
