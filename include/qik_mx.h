@@ -153,6 +153,16 @@ typedef struct qik_mx_gemm_args {
 int qik_mx_gemm_workspace_size(const qik_mx_gemm_args* args, int64_t* bytes);
 int qik_mx_gemm(const qik_mx_gemm_args* args, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* The launch qik_mx_gemm makes for an M x N x K product with A in a_format on a
+ * device with `cus` compute units (0: 256), host only, no device involved, for
+ * tests and tooling.  Few rows: plan[0..5] = rows and columns of a workgroup, its
+ * waves, 0, 0, 0, and *n1 = N.  Tiles: plan[0..5] = big tile rows and columns,
+ * small tile rows and columns, 1 when the small tiles' workgroups come first in
+ * blockIdx order, the K slices (1: no split); *n1 = the columns [0, n1) that the
+ * big tiles cover (N for a split, which runs one tile shape).  QIK_ERR_SHAPE and
+ * QIK_ERR_DTYPE as for a qik_mx_gemm of packed rows, M at least 1. */
+int qik_mx_gemm_plan(int64_t M, int64_t N, int64_t K, int32_t a_format, int32_t cus, int32_t* plan, int64_t* n1);
+
 /* qik_mx_gemm of x quantised to g.a_format: x is [M, K] of x_dtype with row
  * stride ldx as in qik_mx_quantize; g.a, g.a_scales and g.lda are not read.
  * The workspace holds the codes and scales of x too; where the launch

@@ -352,6 +352,9 @@ MX_EXPORTS = (
      (ctypes.POINTER(QikMxGemmArgs), ctypes.POINTER(ctypes.c_int64))),
     ("qik_mx_gemm", ctypes.c_int,
      (ctypes.POINTER(QikMxGemmArgs), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p)),
+    ("qik_mx_gemm_plan", ctypes.c_int,
+     (ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+      ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int64))),
     ("qik_mx_linear_workspace_size", ctypes.c_int,
      (ctypes.POINTER(QikMxLinearArgs), ctypes.POINTER(ctypes.c_int64))),
     ("qik_mx_linear", ctypes.c_int,

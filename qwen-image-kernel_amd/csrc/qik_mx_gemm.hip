@@ -768,14 +768,17 @@ __global__ void __launch_bounds__(64 * KW) rows_kernel(const MxGemmParams p) {
 
 inline bool aligned_to(const void* ptr, uintptr_t a) { return (reinterpret_cast<uintptr_t>(ptr) % a) == 0; }
 
+inline bool known_sizes(int64_t M, int64_t N, int64_t K) {
+  return M >= 0 && M <= ((int64_t)1 << 30) && N >= 1 && N < ((int64_t)1 << 28) && K >= 32 && K <= 262144 && K % 32 == 0;
+}
+
 // with_a: a, a_scales and lda are checked too
 int validate_gemm(const qik_mx_gemm_args* a, bool with_a) {
   if (a == nullptr) return QIK_ERR_NULL_ARG;
   if (a->abi_version != QIK_ABI_VERSION || a->reserved0 != 0) return QIK_ERR_ABI_VERSION;
   if (a->out_dtype != QIK_DTYPE_BF16 && a->out_dtype != QIK_DTYPE_FP16) return QIK_ERR_DTYPE;
   if (a->a_format != QIK_MXFP4 && a->a_format != QIK_MXFP8) return QIK_ERR_DTYPE;
-  if (a->M < 0 || a->M > ((int64_t)1 << 30) || a->N < 1 || a->N >= ((int64_t)1 << 28)) return QIK_ERR_SHAPE;
-  if (a->K < 32 || a->K > 262144 || a->K % 32 != 0) return QIK_ERR_SHAPE;
+  if (!known_sizes(a->M, a->N, a->K)) return QIK_ERR_SHAPE;
   const int64_t row_a = a->a_format == QIK_MXFP4 ? a->K / 2 : a->K;
   // a tile's rows must be addressable by a 31-bit buffer offset
   if (a->ldw < a->K / 2 || a->ldw > INT_MAX / 256 || a->ldc < a->N || a->ldc > ((int64_t)1 << 40)) return QIK_ERR_SHAPE;
@@ -979,11 +982,11 @@ int launch_plan(MxGemmParams& p, const qik_mx_gemm_args* a, const MxPlan& plan, 
 // 12288 x 1024 4.1 / 4.5 and x 2048 6.5 / 6.1; 32 x 4096 x 6144 7.6 / 7.9 and x 8192
 // 9.4 / 9.0, with MXFP8 rows x 4096 7.3 / 8.0 and x 6144 10.3 / 9.8, 32 x 5120 x
 // 2048 5.3 / 4.8).
-bool takes_rows(const qik_mx_gemm_args* a) {
-  const bool narrow = a->N <= 4096;
-  if (a->M <= 8) return narrow ? a->K <= 12288 : a->N * a->K <= (1 << 25);
-  if (a->M <= 16) return narrow ? a->K <= 8192 : a->N * a->K <= (1 << 24);
-  return a->M <= 32 && narrow && a->K <= (a->a_format == QIK_MXFP8 ? 4096 : 6144);
+bool takes_rows(int64_t M, int64_t N, int64_t K, bool a8) {
+  const bool narrow = N <= 4096;
+  if (M <= 8) return narrow ? K <= 12288 : N * K <= (1 << 25);
+  if (M <= 16) return narrow ? K <= 8192 : N * K <= (1 << 24);
+  return M <= 32 && narrow && K <= (a8 ? 4096 : 6144);
 }
 
 // A linear whose workgroups each quantise all of x for themselves saves a
@@ -1004,13 +1007,15 @@ struct Launch {
   MxPlan plan;
   int64_t partial_bytes;
 };
-Launch plan_launch(const qik_mx_gemm_args* a) {
-  Launch l = {takes_rows(a), {0, 0, false, 1, SPLIT64}, 0};
+Launch plan_launch(int64_t M, int64_t N, int64_t K, int32_t a_format, int cus) {
+  const bool a8 = a_format == QIK_MXFP8;
+  Launch l = {takes_rows(M, N, K, a8), {0, 0, false, 1, SPLIT64}, 0};
   if (l.rows) return l;
-  l.plan = choose(a->M, a->N, a->K, a->a_format == QIK_MXFP8, device_cus());
-  if (l.plan.slices > 1) l.partial_bytes = (int64_t)l.plan.slices * a->M * cdiv(a->N, 4) * 4 * (int64_t)sizeof(float);
+  l.plan = choose(M, N, K, a8, cus);
+  if (l.plan.slices > 1) l.partial_bytes = (int64_t)l.plan.slices * M * cdiv(N, 4) * 4 * (int64_t)sizeof(float);
   return l;
 }
+Launch plan_launch(const qik_mx_gemm_args* a) { return plan_launch(a->M, a->N, a->K, a->a_format, device_cus()); }
 
 template <bool A8>
 int launch_gemm(const qik_mx_gemm_args* a, const Launch& l, float* partial, hipStream_t s) {
@@ -1064,6 +1069,31 @@ int qik_mx_gemm(const qik_mx_gemm_args* a, void* workspace, int64_t workspace_by
       (workspace == nullptr || workspace_bytes < l.partial_bytes || !aligned_to(workspace, 256)))
     return QIK_ERR_WORKSPACE;
   return launch_gemm(a, l, static_cast<float*>(workspace), static_cast<hipStream_t>(stream));
+}
+
+int qik_mx_gemm_plan(int64_t M, int64_t N, int64_t K, int32_t a_format, int32_t cus, int32_t* plan, int64_t* n1) {
+  using namespace qik_mx;
+  if (plan == nullptr || n1 == nullptr) return QIK_ERR_NULL_ARG;
+  if (a_format != QIK_MXFP4 && a_format != QIK_MXFP8) return QIK_ERR_DTYPE;
+  if (!known_sizes(M, N, K) || M < 1) return QIK_ERR_SHAPE;
+  const Launch l = plan_launch(M, N, K, a_format, cus > 0 ? cus : 256);
+  const TileShape* shapes = kShapes[a_format == QIK_MXFP8];
+  *n1 = N;
+  if (l.rows) {
+    const RowsPlan r = choose_rows(M, N, K, false);
+    const int32_t v[6] = {M <= 16 ? 16 : 32, 16 * r.nb, r.kw, 0, 0, 0};
+    memcpy(plan, v, sizeof(v));
+  } else if (l.plan.slices > 1) {
+    const TileShape& t = shapes[l.plan.split == SPLIT64 ? T64x64 : T128x128];
+    const int32_t v[6] = {t.bm, t.bn, t.bm, t.bn, 0, l.plan.slices};
+    memcpy(plan, v, sizeof(v));
+  } else {
+    const TileShape &t1 = shapes[kPairs[l.plan.pair][0]], &t2 = shapes[kPairs[l.plan.pair][1]];
+    const int32_t v[6] = {t1.bm, t1.bn, t2.bm, t2.bn, l.plan.small_first ? 1 : 0, 1};
+    memcpy(plan, v, sizeof(v));
+    *n1 = l.plan.n1;
+  }
+  return QIK_OK;
 }
 
 // workspace of a linear: the split's sums, x's codes, x's scales

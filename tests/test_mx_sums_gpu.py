@@ -13,8 +13,9 @@ import torch
 from oracle import mx as om
 
 import qwen_image_kernel_amd as qik
-from mx_exact import exact_operands
+from mx_exact import CODES, SIGN, exact_operands
 from test_mx_host import FORMATS
+from test_mx_sums_host import LAUNCHES, kind
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +101,29 @@ LONG = [(1, 40, 4096), (1, 65, 32768), (2, 33, 262144), (8, 70, 12288), (8, 70, 
 def test_long_products_are_the_exact_sums(fmt, M, N, K):
     say("exact", fmt, M, N, K)
     check_exact(M, N, K, fmt)
+
+
+def device_rows(M, K, fmt, scales, g):
+    """exact_rows on the device: an MXTensor and its float64 values."""
+    m = torch.randint(-3, 4, (M, K), generator=g, device=DEV, dtype=torch.int8)
+    e = torch.randint(0, scales, (M, K // 32), generator=g, device=DEV, dtype=torch.uint8)
+    c = torch.from_numpy(CODES[fmt]).to(DEV)[m.abs().int()] + (m < 0).to(torch.uint8) * SIGN[fmt]
+    c = c.view(torch.float8_e4m3fn) if fmt == "mxfp8" else c[:, 0::2] | (c[:, 1::2] << 4)
+    return (qik.MXTensor.from_block_scales(c, e + 127, fmt),
+            m.double() * torch.exp2(e.double()).repeat_interleave(32, 1))
+
+
+@pytest.mark.parametrize("fmt,shape", [(f, s) for f in LAUNCHES for s in LAUNCHES[f]])
+def test_every_launch_gives_the_exact_sums(fmt, shape):
+    say("launch", fmt, shape)
+    M, N, K = shape
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    assert kind(*shape, fmt, cus) == LAUNCHES[fmt][shape]
+    g = torch.Generator(device=DEV).manual_seed(M + N + K)
+    (a, av), (w, wv) = device_rows(M, K, fmt, 3, g), device_rows(N, K, "mxfp4", 2, g)
+    b = torch.randint(-128, 129, (N,), generator=g, device=DEV).double()
+    assert (av.abs().amax(0) @ wv.abs().amax(0) + 128).item() <= 2 ** 24
+    want = (av @ wv.t().contiguous() + b).float()
+    for dtype in (torch.bfloat16, torch.float16):
+        got = qik.mx_linear(a, w, b.to(dtype), dtype)
+        assert torch.equal(got, want.to(dtype)), ((got != want.to(dtype)).sum().item(), dtype)
