@@ -449,8 +449,9 @@ int launch_norm(const NormParams& p, hipStream_t s) {
   if constexpr (DT != QIK_DTYPE_FP32) {
     if (p.D <= 1536) return launch_norm_shape<DT, FMT, RES, ALIGNED, 64, 3>(p, s);
     if (p.D <= 2048) return launch_norm_shape<DT, FMT, RES, ALIGNED, 64, 4>(p, s);
+  } else {
+    if (p.D <= 2048) return launch_norm_shape<DT, FMT, RES, ALIGNED, 256, 1>(p, s);
   }
-  if (p.D <= 2048) return launch_norm_shape<DT, FMT, RES, ALIGNED, 256, 1>(p, s);
   if (p.D <= 4096) return launch_norm_shape<DT, FMT, RES, ALIGNED, 256, 2>(p, s);
   if (p.D <= 6144) return launch_norm_shape<DT, FMT, RES, ALIGNED, 256, 3>(p, s);
   if (p.D <= 8192) return launch_norm_shape<DT, FMT, RES, ALIGNED, 256, 4>(p, s);

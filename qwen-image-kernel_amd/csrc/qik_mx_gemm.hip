@@ -890,8 +890,15 @@ RowsPlan choose_rows(int64_t M, int64_t N, int64_t K, bool raw) {
 template <int SRC, bool A8, int MB>
 int launch_rows(MxGemmParams& p, const qik_mx_gemm_args* a, hipStream_t s) {
   const RowsPlan plan = choose_rows(a->M, a->N, a->K, SRC != SRC_CODES);
-  if (plan.nb == 2) return launch_rows_shape<SRC, A8, MB, 2, 4>(p, a, s);
-  return plan.kw == 4 ? launch_rows_shape<SRC, A8, MB, 1, 4>(p, a, s) : launch_rows_shape<SRC, A8, MB, 1, 8>(p, a, s);
+  // more than 16 rows of codes come here with up to 4096 columns (takes_rows), so
+  // never in pairs of 16; of elements past 8192 columns always in pairs
+  if constexpr (MB == 1 || SRC != SRC_CODES) {
+    if (plan.nb == 2) return launch_rows_shape<SRC, A8, MB, 2, 4>(p, a, s);
+  }
+  if constexpr (MB == 1 || SRC == SRC_CODES) {
+    if (plan.kw == 4) return launch_rows_shape<SRC, A8, MB, 1, 4>(p, a, s);
+  }
+  return launch_rows_shape<SRC, A8, MB, 1, 8>(p, a, s);
 }
 
 // Time of a tile of each shape (qik_tile.h), for A in MXFP4 and in MXFP8: fitted

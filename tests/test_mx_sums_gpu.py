@@ -127,3 +127,23 @@ def test_every_launch_gives_the_exact_sums(fmt, shape):
     for dtype in (torch.bfloat16, torch.float16):
         got = qik.mx_linear(a, w, b.to(dtype), dtype)
         assert torch.equal(got, want.to(dtype)), ((got != want.to(dtype)).sum().item(), dtype)
+
+
+# one row and more in each width of the kernel that quantises its own rows, narrow outputs and wide ones
+ONE_LAUNCH = [(1, 40, 4096), (1, 9000, 1056), (8, 9000, 512), (12, 9000, 512), (16, 300, 2048), (20, 9000, 512), (31, 8200, 96),
+              (17, 5001, 1504), (32, 70, 1024)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", ONE_LAUNCH)
+def test_linears_of_one_launch_give_the_exact_sums(fmt, M, N, K):
+    say("one launch", fmt, M, N, K)
+    g = torch.Generator(device=DEV).manual_seed(M + N + K)
+    (_, av), (w, wv) = device_rows(M, K, fmt, 3, g), device_rows(N, K, "mxfp4", 2, g)
+    b = torch.randint(-128, 129, (N,), generator=g, device=DEV).double()
+    want = (av @ wv.t().contiguous() + b).float().bfloat16()
+    mod = qik.MXFP4Linear.from_quantized(w, b, fmt)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        got = mod(av.to(dtype))
+        assert got.dtype == dtype and torch.equal(got, want.to(dtype))
+    assert all(c.ws_bytes == 0 for c in mod._calls.values())  # no codes in memory: one launch
