@@ -47,6 +47,12 @@ def _check_format(fmt: str) -> str:
     return fmt
 
 
+def _check_out_dtype(dtype: torch.dtype | None) -> torch.dtype | None:
+    if dtype is not None and dtype not in _OUT_DTYPES:
+        raise ValueError(f"out_dtype must be bf16, fp16 or None, got {dtype}")
+    return dtype
+
+
 def _check_width(K: int) -> None:
     if K < MX_BLOCK or K % MX_BLOCK != 0 or K > _MAX_K:
         raise ValueError(f"the last dimension must be a multiple of {MX_BLOCK} up to {_MAX_K}, got {K}")
@@ -358,7 +364,7 @@ class _LinearCall:
     the buffers it was made for (with their addresses), so that it is used only
     while the module still holds exactly them and never keeps them alive."""
 
-    __slots__ = ("args", "index", "shape", "ws_bytes", "refs", "addresses", "copy", "cast_bias", "fn")
+    __slots__ = ("args", "index", "shape", "out_dtype", "ws_bytes", "refs", "addresses", "copy", "cast_bias", "fn")
 
     def matches(self, weight, scales, bias) -> bool:
         r = self.refs
@@ -375,14 +381,19 @@ class MXFP4Linear(nn.Module):
     ``forward`` takes a tensor (bf16, fp16 or fp32 ``[..., in_features]``), which
     it quantises to ``activations`` ("mxfp4": both operands in 4 bits, the
     matrix cores' fastest form; "mxfp8": 8-bit activations, closer to the
-    input), or an ``MXTensor`` of either format.  The result has the input's
-    dtype, bf16 for an ``MXTensor``; it is summed in fp32 and rounded to bf16
-    once.  Buffers: ``weight`` uint8 ``[out, in / 2]``, ``weight_scale`` uint8
-    ``[ceil(out / 32), ceil(in / 256), 256]`` (the layout of
-    ``MXTensor.scales``), ``bias`` bf16 ``[out]`` or None.  ``in_features`` is a
-    multiple of 32."""
+    input), or an ``MXTensor`` of either format.  The result is summed in fp32
+    and rounded once: into ``out_dtype`` (bf16 or fp16) where that is set; else
+    into bf16, and then it is cast to the input's dtype (bf16 for an
+    ``MXTensor``), so an fp16 model keeps fp16's three further bits, and saves
+    the cast, with ``out_dtype=torch.float16``.  Buffers: ``weight`` uint8 ``[out,
+    in / 2]``, ``weight_scale`` uint8 ``[ceil(out / 32), ceil(in / 256), 256]``
+    (the layout of ``MXTensor.scales``), ``bias`` ``[out]`` in ``out_dtype`` or
+    bf16, or None.  ``in_features`` is a multiple of 32."""
 
-    def __init__(self, in_features: int, out_features: int, bias: bool = False, activations: str = "mxfp4"):
+    out_dtype: torch.dtype | None = None
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = False, activations: str = "mxfp4",
+                 out_dtype: torch.dtype | None = None):
         super().__init__()
         _check_width(in_features)
         if out_features < 1:
@@ -390,13 +401,14 @@ class MXFP4Linear(nn.Module):
         self.in_features = in_features
         self.out_features = out_features
         self.activations = _check_format(activations)
+        self.out_dtype = _check_out_dtype(out_dtype)
         self.register_buffer("weight", torch.zeros(out_features, in_features // 2, dtype=torch.uint8))
         self.register_buffer("weight_scale", torch.zeros(_scales_shape(out_features, in_features), dtype=torch.uint8))
-        self.register_buffer("bias", torch.zeros(out_features, dtype=torch.bfloat16) if bias else None)
+        self.register_buffer("bias", torch.zeros(out_features, dtype=out_dtype or torch.bfloat16) if bias else None)
 
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, "
-                f"activations={self.activations}")
+                f"activations={self.activations}{'' if self.out_dtype is None else f', out_dtype={self.out_dtype}'}")
 
     def mx_weight(self) -> MXTensor:
         """The weight as an MXTensor on the module's buffers."""
@@ -407,7 +419,9 @@ class MXFP4Linear(nn.Module):
         weight, scales = buffers["weight"], buffers["weight_scale"]
         bias = buffers["bias"] if "bias" in buffers else self.bias  # set to a parameter, say
         mx = isinstance(x, MXTensor)
-        key = (x._shape, x._fmt, x._codes.device) if mx else (x.shape, x.stride(), x.dtype, x.device, self.activations)
+        want = self.out_dtype
+        key = ((x._shape, x._fmt, x._codes.device, want) if mx
+               else (x.shape, x.stride(), x.dtype, x.device, self.activations, want))
         calls = self.__dict__.get("_calls")
         if calls is None:
             calls = self.__dict__["_calls"] = {}
@@ -418,7 +432,7 @@ class MXFP4Linear(nn.Module):
                 calls.clear()
             calls[key] = ent
         rows = x._codes if mx else x
-        out = rows.new_empty(ent.shape, dtype=torch.bfloat16)
+        out = rows.new_empty(ent.shape, dtype=ent.out_dtype)
         if ent.args is not None:
             idx = ent.index
             if idx != torch._C._cuda_getDevice():
@@ -426,7 +440,7 @@ class MXFP4Linear(nn.Module):
                     self._launch(ent, x, out)
             else:
                 self._launch(ent, x, out)
-        return out if mx or x.dtype == torch.bfloat16 else out.to(x.dtype)
+        return out if mx or want is not None or x.dtype == torch.bfloat16 else out.to(x.dtype)
 
     def _launch(self, ent: _LinearCall, x, out) -> None:
         if isinstance(x, MXTensor):
@@ -438,8 +452,8 @@ class MXFP4Linear(nn.Module):
             a.x = x2.data_ptr()
             g = a.g
         g.out = out.data_ptr()
-        if ent.cast_bias:  # not bf16 (the module was moved to another dtype), or not as the kernel reads it
-            bias = self.bias.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
+        if ent.cast_bias:  # of another dtype than the output (the module was moved, say), or not as the kernel reads it
+            bias = self.bias.to(ent.out_dtype).clone(memory_format=torch.contiguous_format)
             g.bias = bias.data_ptr()
         _launch(ent, "MXFP4Linear", a, out)
 
@@ -468,14 +482,15 @@ class MXFP4Linear(nn.Module):
         c.fn = lib.qik_mx_gemm if mx else lib.qik_mx_linear
         c.index = x.device.index
         c.shape = (*x.shape[:-1], N)
+        c.out_dtype = out_dtype = _check_out_dtype(self.out_dtype) or torch.bfloat16
         c.refs = (weakref.ref(weight), weakref.ref(scales), None if bias is None else weakref.ref(bias))
         c.addresses = (weight.data_ptr(), scales.data_ptr(), None if bias is None else bias.data_ptr())
         c.args, c.ws_bytes, c.copy = None, 0, False
-        c.cast_bias = bias is not None and (bias.dtype != torch.bfloat16 or not bias.is_contiguous() or bias.data_ptr() % 4 != 0)
+        c.cast_bias = bias is not None and (bias.dtype != out_dtype or not bias.is_contiguous() or bias.data_ptr() % 4 != 0)
         M = _rows(x.shape)
         if M == 0:
             return c
-        a = _gemm_args(x.fmt if mx else self.activations, weight, scales, None if c.cast_bias else bias, torch.bfloat16, M, N, K)
+        a = _gemm_args(x.fmt if mx else self.activations, weight, scales, None if c.cast_bias else bias, out_dtype, M, N, K)
         a.out = weight.data_ptr()  # any address: the size does not go by it
         if mx:
             a.a, a.a_scales, size = x.codes.data_ptr(), x.scales.data_ptr(), lib.qik_mx_gemm_workspace_size
@@ -503,7 +518,8 @@ class MXFP4Linear(nn.Module):
         return state
 
     @staticmethod
-    def from_quantized(weight: MXTensor, bias: torch.Tensor | None = None, activations: str = "mxfp4") -> "MXFP4Linear":
+    def from_quantized(weight: MXTensor, bias: torch.Tensor | None = None, activations: str = "mxfp4",
+                       out_dtype: torch.dtype | None = None) -> "MXFP4Linear":
         """From an MXFP4 weight ``[out, in]`` and a bias; the module takes the weight's buffers as they are."""
         if not isinstance(weight, MXTensor) or weight.fmt != "mxfp4" or len(weight.shape) != 2:
             raise ValueError("the weight must be an mxfp4 MXTensor [out, in]")
@@ -513,28 +529,31 @@ class MXFP4Linear(nn.Module):
         mod = MXFP4Linear.__new__(MXFP4Linear)
         nn.Module.__init__(mod)
         mod.in_features, mod.out_features, mod.activations = K, N, _check_format(activations)
+        mod.out_dtype = _check_out_dtype(out_dtype)
         mod.register_buffer("weight", weight.codes)
         mod.register_buffer("weight_scale", weight.scales)
         if bias is not None:
-            bias = bias.detach().to(device=weight.device, dtype=torch.bfloat16).clone()
+            bias = bias.detach().to(device=weight.device, dtype=out_dtype or torch.bfloat16).clone()
         mod.register_buffer("bias", bias)
         return mod
 
     @staticmethod
-    def from_linear(linear: nn.Linear, activations: str = "mxfp4") -> "MXFP4Linear":
+    def from_linear(linear: nn.Linear, activations: str = "mxfp4",
+                    out_dtype: torch.dtype | None = None) -> "MXFP4Linear":
         """Convert a loaded nn.Linear (weights on the CPU or a HIP device)."""
         w = linear.weight.data
         w = w if w.dtype in _DTYPES else w.float()
         bias = None if linear.bias is None else linear.bias.data
-        return MXFP4Linear.from_quantized(quantize_mx(w, "mxfp4"), bias, activations)
+        return MXFP4Linear.from_quantized(quantize_mx(w, "mxfp4"), bias, activations, out_dtype)
 
 
 def convert_linears_mxfp4(module: nn.Module, skip_patterns: tuple[str, ...] = (), prefix: str = "",
-                          activations: str = "mxfp4") -> list[str]:
+                          activations: str = "mxfp4", out_dtype: torch.dtype | None = None) -> list[str]:
     """Replace every nn.Linear below `module` whose in_features is a multiple of
     32 with MXFP4Linear in place; returns the converted names, skipping names
     that contain a skip pattern (the counterpart of convert_linears_fp8)."""
     _check_format(activations)
+    _check_out_dtype(out_dtype)
     converted = []
     for name, child in list(module.named_children()):
         full = f"{prefix}.{name}" if prefix else name
@@ -542,8 +561,8 @@ def convert_linears_mxfp4(module: nn.Module, skip_patterns: tuple[str, ...] = ()
             continue
         if isinstance(child, nn.Linear):
             if child.in_features % MX_BLOCK == 0 and MX_BLOCK <= child.in_features <= _MAX_K:
-                setattr(module, name, MXFP4Linear.from_linear(child, activations))
+                setattr(module, name, MXFP4Linear.from_linear(child, activations, out_dtype))
                 converted.append(full)
         else:
-            converted.extend(convert_linears_mxfp4(child, skip_patterns, full, activations))
+            converted.extend(convert_linears_mxfp4(child, skip_patterns, full, activations, out_dtype))
     return converted

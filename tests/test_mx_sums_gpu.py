@@ -147,3 +147,54 @@ def test_linears_of_one_launch_give_the_exact_sums(fmt, M, N, K):
         got = mod(av.to(dtype))
         assert got.dtype == dtype and torch.equal(got, want.to(dtype))
     assert all(c.ws_bytes == 0 for c in mod._calls.values())  # no codes in memory: one launch
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(1, 40, 4096), (17, 33, 1504), (70, 129, 96), (64, 333, 8192), (300, 520, 352)])
+def test_linear_rounds_once_into_its_out_dtype(fmt, M, N, K):
+    """Exact sums, so the result is theirs in the type asked for, whatever the input's; a bias with more bits than bf16
+    has keeps them."""
+    say("out dtype", fmt, M, N, K)
+    g = torch.Generator(device=DEV).manual_seed(M + N + K)
+    (a, av), (w, wv) = device_rows(M, K, fmt, 3, g), device_rows(N, K, "mxfp4", 2, g)
+    b = torch.randint(-2047, 2048, (N,), generator=g, device=DEV).double()  # exact in fp16, half of them not in bf16
+    sums = av @ wv.t().contiguous()
+    lin = torch.nn.Linear(K, N, device=DEV)
+    lin.weight.data, lin.bias.data = wv.float(), b.float()
+    want = (sums + b).half()
+    assert not torch.equal(want, (sums + b.bfloat16().double()).bfloat16().half())
+    for mod in (qik.MXFP4Linear.from_quantized(w, b, fmt, torch.float16),
+                qik.MXFP4Linear.from_linear(lin, fmt, out_dtype=torch.float16)):
+        for x in (av.half(), av.bfloat16(), av.float(), a):
+            got = mod(x)
+            assert got.dtype == torch.float16 and torch.equal(got, want)
+        assert mod.bias.dtype == torch.float16 and mod(av[:0].half()).dtype == torch.float16
+    # an attribute: set, changed and taken back on a module in use
+    mod = qik.MXFP4Linear.from_quantized(w, b, fmt)
+    rounded = (sums + b.bfloat16().double()).float().bfloat16()
+    x = av.half()
+    assert torch.equal(mod(x), rounded.half())
+    mod.out_dtype = torch.float16
+    assert torch.equal(mod(x), (sums + b.bfloat16().double()).half())
+    mod.out_dtype = torch.bfloat16
+    assert torch.equal(mod(x), rounded) and torch.equal(mod(a), rounded)
+    mod.out_dtype = None
+    assert torch.equal(mod(x), rounded.half()) and torch.equal(mod(a), rounded)
+    mod.out_dtype = torch.float32
+    with pytest.raises(ValueError, match="out_dtype"):
+        mod(x)
+
+
+def test_fp16_linear_is_within_fp16_of_its_sums():
+    """Random data through convert_linears_mxfp4: half a step of fp16 and the fp32 sums' rounding (K + 1 additions of a
+    step, 2^-23, of the magnitudes' sum each)."""
+    say("fp16 net")
+    torch.manual_seed(1)
+    net = torch.nn.Sequential(torch.nn.Linear(544, 96)).to(DEV).half()
+    assert qik.convert_linears_mxfp4(net, out_dtype=torch.float16) == ["0"]
+    x = torch.randn(200, 544, device=DEV).half()
+    got = net(x)
+    a, w = qik.quantize_mx(x).dequantize(torch.float32).double(), net[0].mx_weight().dequantize(torch.float32).double()
+    want, mag = a @ w.t().contiguous() + net[0].bias.double(), a.abs() @ w.abs().t().contiguous() + net[0].bias.double().abs()
+    acc = 545 * 2.0 ** -23 * mag
+    assert got.dtype == torch.float16 and ((got.double() - want).abs() <= acc + 2.0 ** -11 * (want.abs() + acc) + 2.0 ** -25).all()

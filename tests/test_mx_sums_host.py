@@ -5,7 +5,9 @@ import ctypes
 
 import numpy as np
 import pytest
+import torch
 
+import qwen_image_kernel_amd as qik
 from qwen_image_kernel_amd import _lib
 
 from mx_exact import exact_operands, exact_sums
@@ -140,3 +142,26 @@ def test_plan_checks():
         assert call(*bad, 1) == -5, bad
     assert lib.qik_mx_gemm_plan(1, 1, 32, 1, 0, None, ctypes.byref(n1)) == -1
     assert lib.qik_mx_gemm_plan(1, 1, 32, 1, 0, got, None) == -1
+
+
+@pytest.mark.parametrize("call", [
+    lambda d: qik.MXFP4Linear(64, 8, out_dtype=d), lambda d: qik.MXFP4Linear.from_linear(torch.nn.Linear(64, 8), out_dtype=d),
+    lambda d: qik.MXFP4Linear.from_quantized(qik.quantize_mx(torch.zeros(4, 32)), out_dtype=d),
+    lambda d: qik.convert_linears_mxfp4(torch.nn.Sequential(torch.nn.Linear(64, 8)), out_dtype=d)])
+def test_out_dtype_of_a_linear(call):
+    for d in (torch.float32, torch.uint8, "fp16"):
+        with pytest.raises(ValueError, match="out_dtype"):
+            call(d)
+    call(torch.bfloat16), call(torch.float16), call(None)
+
+
+def test_bias_is_kept_in_the_out_dtype():
+    lin = torch.nn.Linear(64, 8).half()
+    lin.bias.data += 1
+    for d in (torch.float16, torch.bfloat16, None):
+        mod = qik.MXFP4Linear.from_linear(lin, out_dtype=d)
+        assert mod.bias.dtype == (d or torch.bfloat16) and torch.equal(mod.bias, lin.bias.data.to(mod.bias.dtype))
+        assert qik.MXFP4Linear(64, 8, bias=True, out_dtype=d).bias.dtype == mod.bias.dtype
+        fresh = qik.MXFP4Linear(64, 8, bias=True, out_dtype=d)
+        fresh.load_state_dict(mod.state_dict())
+        assert torch.equal(fresh.bias, mod.bias)
