@@ -361,8 +361,9 @@ def _prepare_product(a: MXTensor, w: MXTensor, bias, out_dtype) -> _ProductCall:
 class _LinearCall:
     """What one MXFP4Linear input geometry needs at call time: the argument
     struct without the addresses of x and the output, and weak references to
-    the buffers it was made for (with their addresses), so that it is used only
-    while the module still holds exactly them and never keeps them alive."""
+    the buffers it was made for (with their addresses and the bias's dtype, which
+    its ``.data`` may change at one address), so that it is used only while the
+    module still holds exactly them and never keeps them alive."""
 
     __slots__ = ("args", "index", "shape", "out_dtype", "ws_bytes", "refs", "addresses", "copy", "cast_bias", "fn")
 
@@ -372,7 +373,13 @@ class _LinearCall:
             return False
         if (r[2] is None) != (bias is None) or (bias is not None and r[2]() is not bias):
             return False
-        return self.addresses == (weight.data_ptr(), scales.data_ptr(), None if bias is None else bias.data_ptr())
+        return self.addresses == _addresses(weight, scales, bias)
+
+
+def _addresses(weight, scales, bias):
+    if bias is None:
+        return weight.data_ptr(), scales.data_ptr()
+    return weight.data_ptr(), scales.data_ptr(), bias.data_ptr(), bias.dtype
 
 
 class MXFP4Linear(nn.Module):
@@ -484,7 +491,7 @@ class MXFP4Linear(nn.Module):
         c.shape = (*x.shape[:-1], N)
         c.out_dtype = out_dtype = _check_out_dtype(self.out_dtype) or torch.bfloat16
         c.refs = (weakref.ref(weight), weakref.ref(scales), None if bias is None else weakref.ref(bias))
-        c.addresses = (weight.data_ptr(), scales.data_ptr(), None if bias is None else bias.data_ptr())
+        c.addresses = _addresses(weight, scales, bias)
         c.args, c.ws_bytes, c.copy = None, 0, False
         c.cast_bias = bias is not None and (bias.dtype != out_dtype or not bias.is_contiguous() or bias.data_ptr() % 4 != 0)
         M = _rows(x.shape)

@@ -23,3 +23,17 @@ def test_norm_of_one_workgroup_less_than_two_full_rows_of_a_grid():
     x[-40:] = -3
     y = qik.fused_residual_rms_norm(x, None, torch.ones(1, device=DEV), 0.0)
     assert (y[:-40] == 1).all() and (y[-40:] == -1).all()
+
+
+@pytest.mark.parametrize("M", [1, 200])
+def test_linear_follows_its_bias_to_another_dtype(M):
+    """The bias's data replaced by another dtype's at the same address, which a prepared call must notice."""
+    say("bias dtype", M)
+    mod = qik.MXFP4Linear(64, 40, bias=True).to(DEV)
+    x = torch.randn(M, 64, device=DEV).bfloat16()
+    b = torch.randn(40, device=DEV).half()
+    mod.bias.data = b.view(torch.bfloat16)
+    assert torch.equal(mod(x), mod.bias.expand(M, 40)) and torch.equal(mod(qik.quantize_mx(x)), mod.bias.expand(M, 40))
+    mod.bias.data = mod.bias.data.view(torch.float16)
+    assert mod.bias.data_ptr() == b.data_ptr()
+    assert torch.equal(mod(x), b.bfloat16().expand(M, 40)) and torch.equal(mod(qik.quantize_mx(x)), b.bfloat16().expand(M, 40))
