@@ -422,9 +422,11 @@ class MXFP4Linear(nn.Module):
         return MXTensor(self.weight, self.weight_scale, "mxfp4")
 
     def forward(self, x) -> torch.Tensor:
-        buffers = self._buffers
-        weight, scales = buffers["weight"], buffers["weight_scale"]
-        bias = buffers["bias"] if "bias" in buffers else self.bias  # set to a parameter, say
+        try:
+            buffers = self._buffers
+            weight, scales, bias = buffers["weight"], buffers["weight_scale"], buffers["bias"]
+        except KeyError:  # one of them was set to a parameter, say
+            weight, scales, bias = self.weight, self.weight_scale, self.bias
         mx = isinstance(x, MXTensor)
         want = self.out_dtype
         key = ((x._shape, x._fmt, x._codes.device, want) if mx

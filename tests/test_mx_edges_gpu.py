@@ -37,3 +37,16 @@ def test_linear_follows_its_bias_to_another_dtype(M):
     mod.bias.data = mod.bias.data.view(torch.float16)
     assert mod.bias.data_ptr() == b.data_ptr()
     assert torch.equal(mod(x), b.bfloat16().expand(M, 40)) and torch.equal(mod(qik.quantize_mx(x)), b.bfloat16().expand(M, 40))
+
+
+def test_linear_whose_tensors_are_parameters():
+    """Weight, scales and bias set to parameters (frozen, as loaders that know no buffers make them)."""
+    say("parameters")
+    ref = qik.MXFP4Linear.from_linear(torch.nn.Linear(288, 40, device=DEV))
+    x = torch.randn(5, 288, device=DEV).bfloat16()
+    want = ref(x)
+    for names in (["weight"], ["weight_scale"], ["weight", "weight_scale", "bias"]):
+        mod = qik.MXFP4Linear.from_quantized(ref.mx_weight(), ref.bias)
+        for n in names:
+            setattr(mod, n, torch.nn.Parameter(getattr(mod, n), requires_grad=False))
+        assert torch.equal(mod(x), want) and torch.equal(mod(qik.quantize_mx(x)), ref(qik.quantize_mx(x)))

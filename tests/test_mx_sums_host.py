@@ -165,3 +165,10 @@ def test_bias_is_kept_in_the_out_dtype():
         fresh = qik.MXFP4Linear(64, 8, bias=True, out_dtype=d)
         fresh.load_state_dict(mod.state_dict())
         assert torch.equal(fresh.bias, mod.bias)
+
+
+def test_linear_finds_tensors_that_are_parameters():
+    mod = qik.MXFP4Linear(64, 8)
+    mod.weight = torch.nn.Parameter(mod.weight, requires_grad=False)
+    with pytest.raises(ValueError, match="HIP device"):  # the refusal of a host tensor, not a lookup's error
+        mod(torch.zeros(2, 64))
