@@ -15,7 +15,9 @@ kernels:
 * the causal lengths: ``build_prefix_lengths`` (qik_build_prefix_lengths).
 
 The projections (``to_q/k/v`` or ``fused_qkv``, ``to_out``) are the caller's
-modules, called as the reference calls them.
+modules, called as the reference calls them.  ``hidden_states`` is what they
+take: with ``MXFP4Linear`` projections also the ``MXTensor`` that
+``fused_residual_rms_norm`` writes, quantised once for Q, K and V.
 """
 
 from __future__ import annotations

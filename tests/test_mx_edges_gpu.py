@@ -1,5 +1,7 @@
 """Microscaled operators at edges of what their calls allow."""
 
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -50,3 +52,44 @@ def test_linear_whose_tensors_are_parameters():
         for n in names:
             setattr(mod, n, torch.nn.Parameter(getattr(mod, n), requires_grad=False))
         assert torch.equal(mod(x), want) and torch.equal(mod(qik.quantize_mx(x)), ref(qik.quantize_mx(x)))
+
+
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+def test_processor_takes_the_norms_microscaled_output(fmt, fused):
+    """A layer whose residual norm writes the projections' input in their format: the processor's hidden_states are
+    that MXTensor, read by one projection or by three."""
+    say("processor", fmt, fused)
+    B, S, H, D = 2, 150, 4, 128
+    dim = H * D
+    g = torch.Generator(device=DEV).manual_seed(6)
+    torch.manual_seed(6)
+    names = ["qkv", "out"] if fused else ["q", "k", "v", "out"]
+    net = torch.nn.ModuleDict({n: torch.nn.Linear(dim, 3 * dim if n == "qkv" else dim) for n in names}).to(DEV)
+    assert qik.convert_linears_mxfp4(net, activations=fmt) == names
+    norm = SimpleNamespace(weight=torch.rand(D, generator=g, device=DEV) + 0.5, eps=1e-6)
+    attn = SimpleNamespace(heads=H, to_out=[net["out"], torch.nn.Identity()], norm_q=norm, norm_k=norm)
+    if fused:
+        attn.fused_qkv = net["qkv"]
+    else:
+        attn.to_q, attn.to_k, attn.to_v = net["q"], net["k"], net["v"]
+    x, res = (torch.randn(B, S, dim, generator=g, device=DEV).bfloat16() for _ in range(2))
+    w = torch.rand(dim, generator=g, device=DEV) + 0.5
+    ang = torch.rand(S, D // 2, generator=g, device=DEV)
+    freqs = torch.polar(torch.ones_like(ang), ang)
+    y, h = qik.fused_residual_rms_norm(x, res, w, 1e-6, out_format=fmt)
+    got = qik.QwenImage21KernelProcessor()(attn, y, rotary_emb=freqs)
+    assert got.shape == (B, S, dim) and got.dtype == torch.bfloat16
+
+    def product(mod, t):
+        t = t if isinstance(t, qik.MXTensor) else qik.quantize_mx(t, fmt)
+        return qik.mx_linear(t, mod.mx_weight(), mod.bias)
+
+    if fused:
+        q, k, v = product(net["qkv"], y).unflatten(-1, (3 * H, D)).chunk(3, dim=-2)
+    else:
+        q, k, v = (product(net[n], y).unflatten(-1, (H, D)) for n in "qkv")
+    q, k = (qik.fused_rms_norm_rope(t, norm.weight, freqs, norm.eps) for t in (q, k))
+    o = qik.block_causal_flash_attention(q, k, v, None, None, uniform_full=True)
+    assert torch.equal(got, product(net["out"], o.flatten(2, 3)))
+    assert torch.equal(h, (x.float() + res.float()).bfloat16())
