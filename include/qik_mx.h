@@ -70,8 +70,11 @@ int qik_mx_quantize(const qik_mx_quant_args* args, void* stream);
  * bytes.  `threads` host threads at most (< 1 means 1). Blocking. */
 int qik_mx_quantize_host(const qik_mx_quant_args* args, int32_t threads);
 
-/* out[m, k] = element * 2^(e - 127), rounded once to nearest even into dtype
- * (exact in bf16 and fp32); NaN where e is 255.  out: row stride K, 16-byte
+/* out[m, k] = element * 2^(e - 127), rounded once to nearest even into dtype; NaN
+ * where e is 255.  Exact in fp32 and bf16 but past their range: infinity from
+ * 2^128 on (e from 253 in MXFP4, 247 in MXFP8; qik_mx_quantize writes none of
+ * them but 255), and in bf16 MXFP8 values that are no multiple of its least
+ * subnormal, 2^-133 (e below 3).  out: row stride K, 16-byte
  * aligned; codes and scales as qik_mx_quantize writes them. */
 typedef struct qik_mx_dequant_args {
   int32_t abi_version;        /* QIK_ABI_VERSION                                     */

@@ -100,8 +100,9 @@ __global__ void __launch_bounds__(QT) quant_kernel(const QuantParams p) {
   }
 }
 
-// the values of 8 codes of MXFP4 (w0) or MXFP8 times s (exact in fp32: a
-// product below the normals is a subnormal with bits to spare)
+// the values of 8 codes of MXFP4 (w0) or MXFP8 times s: exact in fp32 (a product
+// below the normals, 2^-136 at least, is a subnormal with bits to spare) up to
+// its overflow
 template <int FMT>
 __device__ __forceinline__ void values8(unsigned w0, unsigned w1, float s, float (&f)[8]) {
   f32x2 d[4];

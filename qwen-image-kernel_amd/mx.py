@@ -159,7 +159,8 @@ class MXTensor:
         return MXTensor._make(self.codes.to(device), self.scales.to(device), self.fmt, self.shape)
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The values, ``element * 2^(e - 127)`` rounded once to dtype (bf16, fp16 or fp32; exact in bf16 and fp32)."""
+        """The values, ``element * 2^(e - 127)`` rounded once to dtype (bf16, fp16 or fp32): exact in bf16 and fp32
+        except past their range, infinity from 2^128 on and MXFP8 values of scale bytes below 3 in bf16's subnormals."""
         codes, shape = self._codes, self._shape
         key = (shape, self._fmt, dtype, codes.device)
         args = _DEQUANT_CALLS.get(key)

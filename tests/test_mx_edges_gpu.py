@@ -93,3 +93,24 @@ def test_processor_takes_the_norms_microscaled_output(fmt, fused):
     o = qik.block_causal_flash_attention(q, k, v, None, None, uniform_full=True)
     assert torch.equal(got, product(net["out"], o.flatten(2, 3)))
     assert torch.equal(h, (x.float() + res.float()).bfloat16())
+
+
+def test_dequantised_values_past_a_types_range():
+    """Exact in bf16 and fp32 up to infinity from 2^128 on, and to bf16's least subnormal, 2^-133."""
+    def value(code, e, fmt, dtype):
+        codes = torch.full((1, 32 if fmt == "mxfp8" else 16), code, dtype=torch.uint8, device=DEV)
+        scale = torch.full((1, 1), e, dtype=torch.uint8, device=DEV)
+        t = qik.MXTensor.from_block_scales(codes.view(torch.float8_e4m3fn) if fmt == "mxfp8" else codes, scale, fmt)
+        return t.dequantize(dtype)[0, 0].item()
+
+    tiny = 2.0 ** -133
+    for code, e, exact, rounded in ((1, 0, 2.0 ** -136, 0.0), (15, 0, 15 * 2.0 ** -136, 2 * tiny), (1, 2, 2.0 ** -134, 0.0),
+                                    (3, 2, 1.5 * tiny, 2 * tiny), (1, 3, tiny, tiny), (7, 3, 7 * tiny, 7 * tiny)):
+        assert value(code, e, "mxfp8", torch.float32) == exact and value(code, e, "mxfp8", torch.bfloat16) == rounded
+    assert value(0x11, 0, "mxfp4", torch.bfloat16) == 2.0 ** -128  # 0.5 of the least scale
+    for dtype in (torch.bfloat16, torch.float32):
+        assert value(0x7e, 246, "mxfp8", dtype) == 448 * 2.0 ** 119 and value(0x7e, 247, "mxfp8", dtype) == float("inf")
+        assert value(0x77, 252, "mxfp4", dtype) == 6 * 2.0 ** 125 and value(0xff, 253, "mxfp4", dtype) == float("-inf")
+    # the largest values quantise to no larger a scale
+    big = torch.full((1, 32), torch.finfo(torch.float32).max, device=DEV)
+    assert qik.quantize_mx(big, "mxfp4").block_scales().item() == 252 and qik.quantize_mx(big, "mxfp8").block_scales().item() == 246
