@@ -6,7 +6,8 @@
 // 32 elements of a block are in the four lanes of a quad, whose largest
 // magnitude takes two cross-lane moves, and the elements are converted by
 // gfx950's packed fp4 / fp8 conversions.  Contraction is off, so every fp32
-// operation rounds on its own and a plain restatement reproduces every bit.
+// operation rounds on its own and a plain restatement reproduces every bit (the
+// norm's but for the order of its fp64 sum, norm_kernel).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -214,11 +215,13 @@ __device__ __forceinline__ double lane_sum(double v) {
 
 // LPR threads per row, VPT vectors of 8 elements per thread: the row is read
 // once and stays in registers, packed, between the sum of squares and the
-// output.  The squares are summed in fp64 (each exact there), so the sum does
-// not depend on the order to anything that its fp32 root shows.  Bound by HBM:
-// bf16 4352 x 4096 with a residual 28.4 us (5.0 TB/s), to MXFP8 27.1 (4.6); rows
-// at odd addresses go slower (fp16 9001 x 1111 11.8 us, 3.4 TB/s; 1112 wide 10.0,
-// 4.0 TB/s).
+// output.  The squares are summed in fp64: each is exact there, and the sum off
+// by some sixty roundings of 2^-53 at most, so another order changes r only where 1
+// / sqrt lies that close to the middle of two fp32 numbers, and then by one step
+// of fp32.  Bound by
+// HBM: operands from memory, bf16 4352 x 4096 with a residual 29.0 us (4.9 TB/s),
+// to MXFP8 28.0 (4.5), to MXFP4 26.2 (4.4); rows at odd addresses go slower (fp16
+// 9001 x 1111 15.2 us, 2.6 TB/s; 1112 wide 13.1, 3.1 TB/s).
 template <int DT, int FMT, bool RES, bool ALIGNED, int LPR, int VPT>
 __global__ void __launch_bounds__(LPR < 256 ? 256 : LPR) norm_kernel(const NormParams p) {
 #pragma clang fp contract(off)
