@@ -369,18 +369,12 @@ class _LinearCall:
     __slots__ = ("args", "index", "shape", "out_dtype", "ws_bytes", "refs", "addresses", "copy", "cast_bias", "fn")
 
     def matches(self, weight, scales, bias) -> bool:
-        r = self.refs
-        if r[0]() is not weight or r[1]() is not scales:
+        r, at = self.refs, self.addresses
+        if r[0]() is not weight or r[1]() is not scales or at[0] != weight.data_ptr() or at[1] != scales.data_ptr():
             return False
-        if (r[2] is None) != (bias is None) or (bias is not None and r[2]() is not bias):
-            return False
-        return self.addresses == _addresses(weight, scales, bias)
-
-
-def _addresses(weight, scales, bias):
-    if bias is None:
-        return weight.data_ptr(), scales.data_ptr()
-    return weight.data_ptr(), scales.data_ptr(), bias.data_ptr(), bias.dtype
+        if bias is None or r[2] is None:
+            return bias is None and r[2] is None
+        return r[2]() is bias and at[2] == bias.data_ptr() and at[3] is bias.dtype
 
 
 class MXFP4Linear(nn.Module):
@@ -494,7 +488,7 @@ class MXFP4Linear(nn.Module):
         c.shape = (*x.shape[:-1], N)
         c.out_dtype = out_dtype = _check_out_dtype(self.out_dtype) or torch.bfloat16
         c.refs = (weakref.ref(weight), weakref.ref(scales), None if bias is None else weakref.ref(bias))
-        c.addresses = _addresses(weight, scales, bias)
+        c.addresses = (weight.data_ptr(), scales.data_ptr(), *((bias.data_ptr(), bias.dtype) if bias is not None else ()))
         c.args, c.ws_bytes, c.copy = None, 0, False
         c.cast_bias = bias is not None and (bias.dtype != out_dtype or not bias.is_contiguous() or bias.data_ptr() % 4 != 0)
         M = _rows(x.shape)
