@@ -66,8 +66,9 @@ __device__ __forceinline__ void unit_at(const QuantParams& p, int64_t first, int
 
 // 32 threads take a unit, one row's 256 elements (8 blocks, 8 scale bytes in a
 // row), QU units one after the other, all loads ahead of the first conversion.
-// Padding rows and blocks read nothing and get a scale of 0.  Bound by HBM: bf16
-// 4352 x 4096 to MXFP4 10.3 us (4.4 TB/s), fp32 12288 x 4096 41 us (5.5 TB/s).
+// Padding rows and blocks read nothing and get a scale of 0.  Bound by HBM:
+// from memory bf16 4352 x 4096 to MXFP4 13.1 us (3.4 TB/s; 10.4 where the 256 MB
+// cache holds a part), fp32 12288 x 4096 41.6 us (5.5 TB/s).
 // One unit keeps the small calls short (bf16 203 x 12288 3.0 us against 3.3 with
 // two and 3.9 with four), two do better on long 16-bit ones (16000 x 3200 26.5
 // against 28.5; with four 32.0), one on fp32 (41.1, 43.4, 45.2).
@@ -131,7 +132,8 @@ __device__ __forceinline__ float scale_value(unsigned byte) {
 }
 
 // The quantiser's units over the rows themselves, each read and written whole
-// (MXFP4 of 4352 x 4096 to bf16 9.3 us, 4.8 TB/s).
+// (MXFP4 of 4352 x 4096 to bf16 12.2 us from memory, 3.7 TB/s; 9.3 where the 256 MB
+// cache holds a part).
 template <int DT, int FMT, int QU>
 __global__ void __launch_bounds__(QT) dequant_kernel(const QuantParams p) {
   constexpr int HW = QT / 32;

@@ -997,11 +997,13 @@ bool takes_rows(int64_t M, int64_t N, int64_t K, bool a8) {
 }
 
 // A linear whose workgroups each quantise all of x for themselves saves a
-// launch: 2 us in a graph, 4 us of host time in a loop of calls.  It costs what a
-// CU's workgroups quantise, about 2.5 us for 32768 elements (in a graph 1 x 4096
-// x 4096 4.2 us against 5.9, 32 x 4096 x 1024 5.6 / 5.4, 4 x 12288 x 4096 10.1 /
-// 10.2, 17 x 5001 x 1504 6.2 / 5.8 and with MXFP8 8.5 / 7.1; called in a loop the
-// last takes 9 against 11.6).
+// launch: up to 2 us in a graph, 4 us of host time in a loop of calls.  It costs
+// what a CU's workgroups quantise, about 2.5 us for 32768 elements.  One launch and
+// two, called in a loop: 1 x 4096 x 4096 7.6 / 11.4 us, 32 x 4096 x 1024 7.5 / 12.0,
+// 4 x 12288 x 4096 9.7 / 11.8, 17 x 5001 x 1504 7.5 / 12.1, with MXFP8 8.3 / 12.1; in
+// a graph 4.3 / 5.9, 5.4 / 5.7, 10.4 / 9.9, 6.2 / 7.2 and 8.7 / 7.8.  The limits go
+// by the loop; a graph of the third and the last would do 5 and 12% better with
+// two.
 bool takes_raw(const qik_mx_gemm_args* a) {
   if (a->M * a->K > RAW_ELEMS || (a->M > 16 && (a->M > 32 || a->N * a->K > (1 << 24)))) return false;
   const int64_t wgs = cdiv(a->N, 16 * choose_rows(a->M, a->N, a->K, true).nb);
