@@ -114,3 +114,32 @@ def test_dequantised_values_past_a_types_range():
     # the largest values quantise to no larger a scale
     big = torch.full((1, 32), torch.finfo(torch.float32).max, device=DEV)
     assert qik.quantize_mx(big, "mxfp4").block_scales().item() == 252 and qik.quantize_mx(big, "mxfp8").block_scales().item() == 246
+
+
+@pytest.mark.parametrize("M", [3, 90])
+def test_linear_with_a_cast_bias_is_captured(M):
+    """An fp16 result with a bias in bf16, cast within the call: captured, replayed between eager calls, with the bias
+    changed in place in between."""
+    say("captured cast", M)
+    torch.manual_seed(2)
+    mod = qik.MXFP4Linear.from_linear(torch.nn.Linear(1056, 300, device=DEV))
+    mod.out_dtype = torch.float16
+    x = torch.randn(M, 1056, device=DEV).half()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        mod(x)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = mod(x)
+    for i in range(4):
+        mod.bias.fill_(float(i))
+        got.zero_()
+        graph.replay()
+        want = mod(x)
+        torch.cuda.synchronize()
+        assert got.dtype == torch.float16 and torch.equal(got, want)
+        if i:
+            assert not torch.equal(want, before)
+        before = want.clone()
