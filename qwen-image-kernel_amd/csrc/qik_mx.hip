@@ -220,10 +220,9 @@ __device__ __forceinline__ double lane_sum(double v) {
 // output.  The squares are summed in fp64: each is exact there, and the sum off
 // by some sixty roundings of 2^-53 at most, so another order changes r only where 1
 // / sqrt lies that close to the middle of two fp32 numbers, and then by one step
-// of fp32.  Bound by
-// HBM: operands from memory, bf16 4352 x 4096 with a residual 29.0 us (4.9 TB/s),
-// to MXFP8 28.0 (4.5), to MXFP4 26.2 (4.4); rows at odd addresses go slower (fp16
-// 9001 x 1111 15.2 us, 2.6 TB/s; 1112 wide 13.1, 3.1 TB/s).
+// of fp32.  Bound by HBM: operands from memory, bf16 4352 x 4096 with a residual
+// 29.0 us (4.9 TB/s), to MXFP8 28.0 (4.5), to MXFP4 26.2 (4.4); rows at odd
+// addresses go slower (fp16 9001 x 1111 15.2 us, 2.6 TB/s; 1112 wide 13.1, 3.1).
 template <int DT, int FMT, bool RES, bool ALIGNED, int LPR, int VPT>
 __global__ void __launch_bounds__(LPR < 256 ? 256 : LPR) norm_kernel(const NormParams p) {
 #pragma clang fp contract(off)

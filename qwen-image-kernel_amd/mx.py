@@ -33,6 +33,7 @@ _CODE_DTYPE = {"mxfp4": torch.uint8, "mxfp8": torch.float8_e4m3fn}
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
 _OUT_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 _MAX_K = 262144
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 # argument structs without addresses, by the geometry that they were checked
 # for: (shape, format, dtype, device) here, see quantize_mx and mx_linear
@@ -186,11 +187,11 @@ class MXTensor:
 
 def _on_device(idx: int, fn, name: str, args) -> None:
     """fn(args, current stream of device idx) with that device current."""
-    if idx != torch._C._cuda_getDevice():
+    if idx != _current_device():
         with torch.cuda.device(idx):
-            _lib.check(fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(idx)), name)
+            _lib.check(fn(ctypes.byref(args), _raw_stream(idx)), name)
     else:
-        st = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(idx))
+        st = fn(ctypes.byref(args), _raw_stream(idx))
         if st:
             _lib.check(st, name)
 
@@ -302,7 +303,7 @@ def mx_linear(
             bias = bias.clone()
         g.bias = bias.data_ptr()
     idx = ent.index
-    if idx != torch._C._cuda_getDevice():
+    if idx != _current_device():
         with torch.cuda.device(idx):
             _launch(ent, "qik_mx_gemm", g, codes)
     else:
@@ -321,7 +322,7 @@ def _launch(ent, name: str, args, like: torch.Tensor) -> None:
     own: two threads that share a stream, or two graphs, never share memory."""
     ws = like.new_empty(ent.ws_bytes, dtype=torch.uint8) if ent.ws_bytes else None
     st = ent.fn(ctypes.byref(args), None if ws is None else ws.data_ptr(), ent.ws_bytes,
-                torch._C._cuda_getCurrentRawStream(ent.index))
+                _raw_stream(ent.index))
     if st:
         _lib.check(st, name)
 
@@ -362,19 +363,21 @@ def _prepare_product(a: MXTensor, w: MXTensor, bias, out_dtype) -> _ProductCall:
 class _LinearCall:
     """What one MXFP4Linear input geometry needs at call time: the argument
     struct without the addresses of x and the output, and weak references to
-    the buffers it was made for (with their addresses and the bias's dtype, which
-    its ``.data`` may change at one address), so that it is used only while the
-    module still holds exactly them and never keeps them alive."""
+    the buffers it was made for (with their addresses and layout, which ``.data``
+    may change), so that it is used only while the module still holds exactly
+    them and never keeps them alive."""
 
-    __slots__ = ("args", "index", "shape", "out_dtype", "ws_bytes", "refs", "addresses", "copy", "cast_bias", "fn")
+    __slots__ = ("args", "index", "shape", "out_dtype", "ws_bytes", "refs", "layout", "copy", "cast_bias", "fn")
 
     def matches(self, weight, scales, bias) -> bool:
-        r, at = self.refs, self.addresses
-        if r[0]() is not weight or r[1]() is not scales or at[0] != weight.data_ptr() or at[1] != scales.data_ptr():
+        r, was = self.refs, self.layout
+        if (r[0]() is not weight or r[1]() is not scales or was[0] != weight.data_ptr() or was[1] != weight.nbytes
+                or was[2] != scales.data_ptr() or was[3] != scales.nbytes):
             return False
         if bias is None or r[2] is None:
             return bias is None and r[2] is None
-        return r[2]() is bias and at[2] == bias.data_ptr() and at[3] is bias.dtype
+        return (r[2]() is bias and was[4] == bias.data_ptr() and was[5] == bias.nbytes
+                and was[6] is bias.dtype and was[7] is bias.is_contiguous())
 
 
 class MXFP4Linear(nn.Module):
@@ -438,28 +441,30 @@ class MXFP4Linear(nn.Module):
         rows = x._codes if mx else x
         out = rows.new_empty(ent.shape, dtype=ent.out_dtype)
         if ent.args is not None:
-            idx = ent.index
-            if idx != torch._C._cuda_getDevice():
-                with torch.cuda.device(idx):
-                    self._launch(ent, x, out)
+            # the structs of both launches are prepared, only addresses of x and out change
+            if mx:
+                a = g = _lib.QikMxGemmArgs.from_buffer_copy(ent.args)
+                g.a, g.a_scales = x._codes.data_ptr(), x._scales.data_ptr()
             else:
-                self._launch(ent, x, out)
+                x2 = _as_rows(x) if ent.copy else x
+                a = _lib.QikMxLinearArgs.from_buffer_copy(ent.args)
+                a.x = x2.data_ptr()
+                g = a.g
+            g.out = out.data_ptr()
+            if ent.cast_bias:  # of another dtype than the output (the module was moved, say), or not as the kernel reads it
+                bias = bias.to(ent.out_dtype).clone(memory_format=torch.contiguous_format)
+                g.bias = bias.data_ptr()
+            idx = ent.index
+            if idx != _current_device():
+                with torch.cuda.device(idx):
+                    _launch(ent, "MXFP4Linear", a, out)
+            elif ent.ws_bytes:
+                _launch(ent, "MXFP4Linear", a, out)
+            else:
+                st = ent.fn(ctypes.byref(a), None, 0, _raw_stream(idx))
+                if st:
+                    _lib.check(st, "MXFP4Linear")
         return out if mx or want is not None or x.dtype == torch.bfloat16 else out.to(x.dtype)
-
-    def _launch(self, ent: _LinearCall, x, out) -> None:
-        if isinstance(x, MXTensor):
-            a = g = _lib.QikMxGemmArgs.from_buffer_copy(ent.args)
-            g.a, g.a_scales = x._codes.data_ptr(), x._scales.data_ptr()
-        else:
-            x2 = _as_rows(x) if ent.copy else x
-            a = _lib.QikMxLinearArgs.from_buffer_copy(ent.args)
-            a.x = x2.data_ptr()
-            g = a.g
-        g.out = out.data_ptr()
-        if ent.cast_bias:  # of another dtype than the output (the module was moved, say), or not as the kernel reads it
-            bias = self.bias.to(ent.out_dtype).clone(memory_format=torch.contiguous_format)
-            g.bias = bias.data_ptr()
-        _launch(ent, "MXFP4Linear", a, out)
 
     def _prepare(self, x, weight, scales, bias) -> _LinearCall:
         """Checks and the argument struct of one input geometry."""
@@ -488,7 +493,9 @@ class MXFP4Linear(nn.Module):
         c.shape = (*x.shape[:-1], N)
         c.out_dtype = out_dtype = _check_out_dtype(self.out_dtype) or torch.bfloat16
         c.refs = (weakref.ref(weight), weakref.ref(scales), None if bias is None else weakref.ref(bias))
-        c.addresses = (weight.data_ptr(), scales.data_ptr(), *((bias.data_ptr(), bias.dtype) if bias is not None else ()))
+        c.layout = (weight.data_ptr(), weight.nbytes, scales.data_ptr(), scales.nbytes)
+        if bias is not None:
+            c.layout += (bias.data_ptr(), bias.nbytes, bias.dtype, bias.is_contiguous())
         c.args, c.ws_bytes, c.copy = None, 0, False
         c.cast_bias = bias is not None and (bias.dtype != out_dtype or not bias.is_contiguous() or bias.data_ptr() % 4 != 0)
         M = _rows(x.shape)

@@ -143,3 +143,28 @@ def test_linear_with_a_cast_bias_is_captured(M):
         if i:
             assert not torch.equal(want, before)
         before = want.clone()
+
+
+@pytest.mark.parametrize("M", [1, 200])
+def test_linear_follows_its_tensors_to_another_layout(M):
+    """Data of another stride or size at the same address, which a prepared call must notice: a strided bias is read as
+    it lies, a weight, scales or bias of another size is refused."""
+    say("layout", M)
+    x = torch.randn(M, 64, device=DEV).bfloat16()
+    base = torch.randn(80, device=DEV).bfloat16()
+    for arg in (x, qik.quantize_mx(x)):
+        mod = qik.MXFP4Linear(64, 40, bias=True).to(DEV)
+        mod.bias.data = base[:40]
+        assert torch.equal(mod(arg), base[:40].expand(M, 40))
+        mod.bias.data = base[::2]
+        assert mod.bias.data_ptr() == base.data_ptr() and torch.equal(mod(arg), base[::2].expand(M, 40))
+        mod.bias.data = base[:40]
+        assert torch.equal(mod(arg), base[:40].expand(M, 40))
+        for name in ("bias", "weight", "weight_scale"):
+            t = getattr(mod, name)
+            whole = t.data
+            t.data = whole[:1]
+            with pytest.raises(ValueError, match=name):
+                mod(arg)
+            t.data = whole
+            assert torch.equal(mod(arg), base[:40].expand(M, 40))
