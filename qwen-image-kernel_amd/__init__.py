@@ -9,7 +9,8 @@ Drop-in for the attention path of qwen_image_kernel: ``block_causal_flash_attent
 layer's projections (fp8.py:63) on the fp8 matrix cores (include/qik_fp8.h).
 Beside them, with no counterpart in the reference: microscaled tensors and the
 4-bit ``MXFP4Linear`` (mx.py), and the residual RMSNorm that feeds it
-(include/qik_mx.h).
+(include/qik_mx.h); the prefix slab in 4 bits, ``MXKVCache``, which the
+attention reads in place (include/qik_mx_attn.h).
 The package directory is ``qwen-image-kernel_amd/``; the top-level module
 ``qwen_image_kernel_amd.py`` imports it under this name.
 """
@@ -22,8 +23,9 @@ from .attention import (  # noqa: F401
 )
 from .fp8 import FP8Linear, fp8_linear, quantize_tensorwise, quantize_weight_tensorwise  # noqa: F401
 from .fused import fused_residual_rms_norm, fused_rms_norm_rope  # noqa: F401
-from .kv_cache import FP8_E4M3_MAX, ContiguousKVCache  # noqa: F401
+from .kv_cache import FP8_E4M3_MAX, ContiguousKVCache, MXKVCache  # noqa: F401
 from .mx import MXFP4Linear, MXTensor, convert_linears_mxfp4, mx_linear, quantize_mx  # noqa: F401
+from .mx_slab import MXSlab  # noqa: F401
 from .processors import QwenImage21KernelProcessor  # noqa: F401
 
 __all__ = [
@@ -33,6 +35,8 @@ __all__ = [
     "block_shape",
     "ContiguousKVCache",
     "FP8_E4M3_MAX",
+    "MXKVCache",
+    "MXSlab",
     "fused_rms_norm_rope",
     "QwenImage21KernelProcessor",
     "FP8Linear",

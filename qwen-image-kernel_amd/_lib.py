@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI declared in include/qik_attn.h, qik_ops.h, qik_fp8.h and qik_mx.h.
+"""ctypes binding of the C ABI declared in include/qik_attn.h, qik_ops.h, qik_fp8.h, qik_mx.h and qik_mx_attn.h.
 
 The shared library is built in-tree (``lib/libqik_attn.so`` next to this file)
 by ``build.py``.  There is no fallback: if the library is missing or fails to
@@ -277,6 +277,71 @@ class QikMxLinearArgs(ctypes.Structure):
     ]
 
 
+class QikMxSlab(ctypes.Structure):
+    """Mirror of ``struct qik_mx_slab`` (include/qik_mx_attn.h)."""
+
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("stride_codes", _i64x3),
+        ("stride_scales", _i64x3),
+    ]
+
+
+class QikMxSlabStoreArgs(ctypes.Structure):
+    """Mirror of ``struct qik_mx_slab_store_args`` (include/qik_mx_attn.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_dst", QikMxSlab),
+        ("v_dst", QikMxSlab),
+        ("at", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("arrivals", ctypes.c_void_p),
+        ("B", ctypes.c_int64),
+        ("S", ctypes.c_int64),
+        ("H", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("capacity", ctypes.c_int64),
+        ("stride_k", _i64x3),
+        ("stride_v", _i64x3),
+    ]
+
+
+class QikMxSlabLoadArgs(ctypes.Structure):
+    """Mirror of ``struct qik_mx_slab_load_args`` (include/qik_mx_attn.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("k_src", QikMxSlab),
+        ("v_src", QikMxSlab),
+        ("lengths", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("B", ctypes.c_int64),
+        ("P", ctypes.c_int64),
+        ("H", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+    ]
+
+
+class QikMxAttnArgs(ctypes.Structure):
+    """Mirror of ``struct qik_mx_attn_args`` (include/qik_mx_attn.h)."""
+
+    _fields_ = [
+        ("a", QikAttnArgs),
+        ("k_slab", QikMxSlab),
+        ("v_slab", QikMxSlab),
+        ("lengths", ctypes.c_void_p),
+        ("HKV", ctypes.c_int64),
+        ("stride_lengths_b", ctypes.c_int64),
+    ]
+
+
 # (name, restype, argtypes) of every entry point of qik_attn.h, qik_ops.h and qik_fp8.h
 EXPORTS = (
     ("qik_abi_version", ctypes.c_int, ()),
@@ -361,6 +426,19 @@ MX_EXPORTS = (
      (ctypes.POINTER(QikMxLinearArgs), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p)),
 )
 
+# of qik_mx_attn.h
+MX_ATTN_EXPORTS = (
+    ("qik_mx_slab_store", ctypes.c_int, (ctypes.POINTER(QikMxSlabStoreArgs), ctypes.c_void_p)),
+    ("qik_mx_slab_load", ctypes.c_int, (ctypes.POINTER(QikMxSlabLoadArgs), ctypes.c_void_p)),
+    ("qik_mx_attn_validate", ctypes.c_int, (ctypes.POINTER(QikMxAttnArgs),)),
+    ("qik_mx_attn_workspace_size", ctypes.c_int, (ctypes.POINTER(QikMxAttnArgs), ctypes.POINTER(ctypes.c_int64))),
+    ("qik_mx_attn_fwd", ctypes.c_int,
+     (ctypes.POINTER(QikMxAttnArgs), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p)),
+    ("qik_mx_attn_plan", ctypes.c_int,
+     (ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+      ctypes.c_int32, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32))),
+)
+
 _lock = threading.Lock()
 _lib = None
 
@@ -379,7 +457,7 @@ def load() -> ctypes.CDLL:
                 "run __graft_entry__.build() or python -m qwen_image_kernel_amd.build"
             )
         lib = ctypes.CDLL(LIB_PATH)
-        for name, restype, argtypes in EXPORTS + MX_EXPORTS:
+        for name, restype, argtypes in EXPORTS + MX_EXPORTS + MX_ATTN_EXPORTS:
             fn = getattr(lib, name)
             fn.restype = restype
             fn.argtypes = list(argtypes)

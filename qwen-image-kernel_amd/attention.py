@@ -19,6 +19,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .mx_slab import MXSlab
 
 __all__ = [
     "block_causal_flash_attention",
@@ -139,6 +140,12 @@ def block_causal_flash_attention(
     With ``cache_v_scale`` the cache V is fp8e4m3fn dequantised per (b, h) as
     bf16(fp32(v) * scale).  Semantics: triton_attention.py:171-260.
 
+    ``cache_k`` and ``cache_v`` may be ``MXSlab`` (a 4-bit slab, such as
+    ``MXKVCache`` layers give): then key and value may have fewer heads than
+    query (query head h reads head h // (H / HKV)), prefix_lengths may be [B, SQ],
+    a slab's ``lengths`` say how many of its rows each batch entry has, and keys
+    that key_valid hides may hold anything (see mx_attention.py).
+
     ``debug_tiles`` (keyword only, not in the reference) receives the number of
     KV tiles visited per (b, h, row block), int32 [B*H*cdiv(SQ, BM)].
 
@@ -148,6 +155,10 @@ def block_causal_flash_attention(
     tiles) with a zeroed workspace kept per (device, stream); False runs
     ``qik_attn_fwd``, one workgroup per row block.
     """
+    if isinstance(cache_k, MXSlab) or isinstance(cache_v, MXSlab):
+        if debug_tiles is not None or not split_tail or cache_v_scale is not None:
+            raise ValueError("a 4-bit slab takes no debug_tiles, split_tail=False or cache_v_scale")
+        return mx_attention.mx_slab_attention(query, key, value, prefix_lengths, key_valid, cache_k, cache_v, uniform_full)
     assert query.dtype in (torch.bfloat16, torch.float16), "fp16/bf16 only"
     B, SQ, H, D = query.shape
     if cache_k is not None:
@@ -433,3 +444,6 @@ def tile_schedule(
     )
     _lib.check(st, "qik_attn_tile_schedule")
     return out[: -(-SQ // bm)]
+
+
+from . import mx_attention  # noqa: E402  (it uses the workspaces above)

@@ -8,11 +8,13 @@ half-written file.
 
 from __future__ import annotations
 
+import concurrent.futures
 import glob
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
@@ -27,7 +29,6 @@ HIPCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     # keep hipcc from forming packed-fp32 VALU ops (v_pk_*_f32)
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     # every device atomic here is issued by one thread; the atomic optimizer's
@@ -55,22 +56,39 @@ def sources() -> list[str]:
 
 
 def build(verbose: bool = False) -> str:
-    """Compile the HIP sources into lib/libqik_attn.so and return its path."""
+    """Compile the HIP sources into lib/libqik_attn.so and return its path.
+
+    Every source is an object of its own, compiled side by side: the attention
+    kernels alone take two minutes."""
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = f"{LIB_PATH}.tmp{os.getpid()}"
-    cmd = [hipcc(), *HIPCC_FLAGS, f"-I{INCLUDE}", *sources(), "-o", tmp,
-           f"-Wl,-rpath,{os.path.join(ROCM, 'lib')}"]
+    with tempfile.TemporaryDirectory(prefix="qik_build_") as objs:
+        def compile_one(src: str) -> str:
+            obj = os.path.join(objs, os.path.basename(src) + ".o")
+            _run([hipcc(), *HIPCC_FLAGS, "-c", f"-I{INCLUDE}", src, "-o", obj], verbose)
+            return obj
+
+        with concurrent.futures.ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+            built = list(pool.map(compile_one, sources()))
+        try:
+            _run([hipcc(), "--offload-arch=gfx950", "-shared", *built, "-o", tmp,
+                  f"-Wl,-rpath,{os.path.join(ROCM, 'lib')}"], verbose)
+        except RuntimeError:
+            if os.path.exists(tmp):
+                os.remove(tmp)
+            raise
+    os.replace(tmp, LIB_PATH)
+    return LIB_PATH
+
+
+def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        if os.path.exists(tmp):
-            os.remove(tmp)
         raise RuntimeError(f"hipcc failed ({res.returncode}):\n{res.stderr}")
     if verbose and res.stderr.strip():
         print(res.stderr, file=sys.stderr)
-    os.replace(tmp, LIB_PATH)
-    return LIB_PATH
 
 
 if __name__ == "__main__":

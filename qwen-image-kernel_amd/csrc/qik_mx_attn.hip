@@ -1,0 +1,584 @@
+// The 4-bit prefix slab and the attention over it: the entry points of
+// include/qik_mx_attn.h.  The slab's store and load are byte movers (a thread
+// takes eight elements of a row, a quad of lanes a block of 32); the attention
+// runs the kernel of qik_mx_rows.h for few query rows and that of
+// qik_attn_kernel.h, in its 4-bit instance, for others.
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <string.h>
+#include <limits.h>
+#include <algorithm>
+#include <atomic>
+
+#include "qik_mx_attn.h"
+#include "qik_mx_block.h"
+#include "qik_host.h"
+#include "qik_attn_kernel.h"
+#include "qik_attn_launch.h"
+#include "qik_mx_rows.h"
+
+namespace qik_mx_slabs {
+
+using qik_mx::u32x2;
+using qik_mx::u32x4;
+
+constexpr int THREADS = 256;
+constexpr int UNITS = 4;  // rows of a thread, their loads issued before any of them is used
+
+struct StoreParams {
+  const char* src[2];            // K, V
+  unsigned char* codes[2];
+  unsigned char* scales[2];
+  int64_t ss[2][3];              // source b, s, h in bytes
+  int64_t sc[2][3], se[2][3];    // codes, scales: b, p, h in bytes
+  const int32_t* at;
+  int32_t* lengths;
+  unsigned* arrivals;            // the word that counts workgroups where lengths == at
+  int rows;                      // B * H * S
+  int B, S, H;
+  int capacity;
+};
+
+// Rows in the slab's order (b, h, s), so that a wave writes runs of whole rows;
+// blockIdx.y: K or V.
+template <int D, bool FP16>
+__global__ void __launch_bounds__(THREADS) slab_store_kernel(const StoreParams p) {
+  constexpr int DT = FP16 ? QIK_DTYPE_FP16 : QIK_DTYPE_BF16;
+  constexpr int TPR = D / 8;             // threads of a row
+  constexpr int RPB = THREADS / TPR;     // rows of a pass
+  const int which = blockIdx.y;
+  const int t = (int)threadIdx.x % TPR;
+  const int row0 = (int)blockIdx.x * (RPB * UNITS) + (int)threadIdx.x / TPR;
+  qik_mx::Raw8<DT> raw[UNITS];
+  int64_t to_c[UNITS], to_e[UNITS];
+  bool on[UNITS];
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const int row = min(row0 + u * RPB, p.rows - 1);
+    const unsigned bh = (unsigned)row / (unsigned)p.S;
+    const int s = row - (int)bh * p.S;
+    const int b = (int)(bh / (unsigned)p.H), h = (int)bh - b * p.H;
+    const int64_t at = (p.at == nullptr ? 0 : (int64_t)p.at[b]) + s;
+    on[u] = row0 + u * RPB < p.rows && at >= 0 && at < p.capacity;
+    raw[u] = qik_mx::load8<DT, true>(p.src[which] + b * p.ss[which][0] + s * p.ss[which][1] + h * p.ss[which][2] + t * 16);
+    to_c[u] = b * p.sc[which][0] + at * p.sc[which][1] + h * p.sc[which][2];
+    to_e[u] = b * p.se[which][0] + at * p.se[which][1] + h * p.se[which][2];
+  }
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    float f[8];
+    qik_mx::unpack8<DT>(raw[u], f);
+    unsigned w0, w1;
+    const unsigned byte = qik_mx::block_codes<QIK_MXFP4>(f, w0, w1);
+    if (!on[u]) continue;
+    *reinterpret_cast<unsigned*>(p.codes[which] + to_c[u] + 4 * t) = w0;
+    if ((t & 3) == 0) p.scales[which][to_e[u] + t / 4] = (unsigned char)byte;
+  }
+  if (p.lengths == nullptr) return;
+  // the lengths behind the new rows.  Where they are what `at` was, they change
+  // once every workgroup has read it: the last to arrive writes them
+  if (p.arrivals != nullptr) {
+    __shared__ int last;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const unsigned all = gridDim.x * gridDim.y;
+      last = qik::g_fetch_add(p.arrivals, 1u) == all - 1u ? 1 : 0;
+      if (last) qik::g_store(p.arrivals, 0u);
+    }
+    __syncthreads();
+    if (last == 0) return;
+  } else if (blockIdx.x != 0 || blockIdx.y != 0) {
+    return;
+  }
+  for (int b = (int)threadIdx.x; b < p.B; b += THREADS) {
+    const int64_t n = (p.at == nullptr ? 0 : (int64_t)p.at[b]) + p.S;
+    p.lengths[b] = (int32_t)min(max(n, (int64_t)0), (int64_t)p.capacity);
+  }
+}
+
+struct LoadParams {
+  const unsigned char* codes[2];
+  const unsigned char* scales[2];
+  char* out[2];
+  int64_t sc[2][3], se[2][3];
+  const int32_t* lengths;
+  int64_t rows;
+  int B, P, H;
+};
+
+// Rows in the slab's order; out is [B, P, H, D] contiguous.
+template <int D, bool FP16>
+__global__ void __launch_bounds__(THREADS) slab_load_kernel(const LoadParams p) {
+  constexpr int TPR = D / 8;
+  constexpr int RPB = THREADS / TPR;
+  const int which = blockIdx.z;
+  const int t = (int)threadIdx.x % TPR;
+  const int64_t row0 = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (RPB * UNITS) + (int)threadIdx.x / TPR;
+  unsigned code[UNITS], e[UNITS];
+  int64_t to[UNITS];
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const int64_t row = min(row0 + u * RPB, p.rows - 1);
+    const int64_t bh = row / p.P;
+    const int s = (int)(row - bh * p.P);
+    const int b = (int)(bh / p.H), h = (int)(bh - (int64_t)b * p.H);
+    const bool in = p.lengths == nullptr || s < p.lengths[b];
+    code[u] = 0u;
+    e[u] = 127u;
+    if (in) {
+      code[u] = *reinterpret_cast<const unsigned*>(p.codes[which] + b * p.sc[which][0] + s * p.sc[which][1] + h * p.sc[which][2] + 4 * t);
+      e[u] = p.scales[which][b * p.se[which][0] + s * p.se[which][1] + h * p.se[which][2] + t / 4];
+    }
+    to[u] = (((int64_t)b * p.P + s) * p.H + h) * (D * 2) + t * 16;
+  }
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u)
+    if (row0 + u * RPB < p.rows)
+      *reinterpret_cast<u32x4*>(p.out[which] + to[u]) =
+          qik::dequant_fp4x8<FP16>(code[u], __uint_as_float(e[u] << 23));
+}
+
+typedef void (*store_fn)(StoreParams);
+typedef void (*load_fn)(LoadParams);
+template <bool FP16>
+store_fn pick_store(int64_t D) {
+  switch (D) {
+    case 32: return slab_store_kernel<32, FP16>;
+    case 64: return slab_store_kernel<64, FP16>;
+    case 128: return slab_store_kernel<128, FP16>;
+    default: return slab_store_kernel<256, FP16>;
+  }
+}
+template <bool FP16>
+load_fn pick_load(int64_t D) {
+  switch (D) {
+    case 32: return slab_load_kernel<32, FP16>;
+    case 64: return slab_load_kernel<64, FP16>;
+    case 128: return slab_load_kernel<128, FP16>;
+    default: return slab_load_kernel<256, FP16>;
+  }
+}
+
+// Layout rules of one slab of rows [B, P, H, D].
+int slab_status(const qik_mx_slab& s, int64_t B, int64_t P, int64_t H, int64_t D) {
+  if (s.codes == nullptr || s.scales == nullptr) return QIK_ERR_NULL_ARG;
+  const int64_t eb = D / 32;
+  if (!qik::aligned_to(s.codes, 16) || !qik::aligned_to(s.scales, (uintptr_t)eb)) return QIK_ERR_ALIGN;
+  if (!qik::stride_ok(s.stride_codes, B, P, H, 16) || !qik::stride_ok(s.stride_scales, B, P, H, eb)) return QIK_ERR_ALIGN;
+  if (P > 1 && (s.stride_codes[1] < D / 2 || s.stride_scales[1] < eb)) return QIK_ERR_ALIGN;
+  const int64_t lim = ((int64_t)1 << 31) / qik::BN;  // a tile's byte offsets are 31 bits
+  if (P > 1 && (s.stride_codes[1] >= lim || s.stride_scales[1] >= lim)) return QIK_ERR_SHAPE;
+  return QIK_OK;
+}
+
+}  // namespace qik_mx_slabs
+
+namespace qik {
+
+typedef void (*mx_kernel_fn)(MxParams);
+typedef void (*rows_kernel_fn)(RowsParams);
+
+template <int D, bool FP16, bool KV>
+void pick_mx(Kernels* k) {
+  mx_kernel_fn f = attn_fwd_kernel<D, FP16, SlabKV::MX, KV, 1, false>;
+  k->one = reinterpret_cast<const void*>(f);
+  if constexpr (D <= 128) {
+    f = attn_fwd_kernel<D, FP16, SlabKV::MX, KV, 1, true>;
+    k->pieces = reinterpret_cast<const void*>(f);
+    f = attn_fwd_kernel<D, FP16, SlabKV::MX, KV, 2, false>;
+    k->groups = reinterpret_cast<const void*>(f);
+  }
+}
+template <int D>
+void pick_mx(bool fp16, bool kv, Kernels* k) {
+  if (fp16) kv ? pick_mx<D, true, true>(k) : pick_mx<D, true, false>(k);
+  else kv ? pick_mx<D, false, true>(k) : pick_mx<D, false, false>(k);
+}
+template <int D>
+rows_kernel_fn pick_rows(bool fp16, bool kv) {
+  if (fp16) return kv ? mx_rows_kernel<D, true, true> : mx_rows_kernel<D, true, false>;
+  return kv ? mx_rows_kernel<D, false, true> : mx_rows_kernel<D, false, false>;
+}
+
+std::atomic<int> g_mx_slots[16][MAX_DEVICES];
+
+Kernels mx_kernels_of(const qik_attn_args* a) {
+  const bool fp16 = a->dtype == QIK_DTYPE_FP16;
+  const bool kv = (a->flags & QIK_HAS_KEY_VALID) != 0;
+  Kernels k = {nullptr, nullptr, nullptr, nullptr};
+  int di = 3;
+  switch (a->D) {
+    case 32: pick_mx<32>(fp16, kv, &k); di = 0; break;
+    case 64: pick_mx<64>(fp16, kv, &k); di = 1; break;
+    case 128: pick_mx<128>(fp16, kv, &k); di = 2; break;
+    default: pick_mx<256>(fp16, kv, &k); break;
+  }
+  k.slots = g_mx_slots[4 * di + (fp16 ? 2 : 0) + (kv ? 1 : 0)];
+  return k;
+}
+
+rows_kernel_fn rows_kernel_of(const qik_attn_args* a) {
+  const bool fp16 = a->dtype == QIK_DTYPE_FP16;
+  const bool kv = (a->flags & QIK_HAS_KEY_VALID) != 0;
+  switch (a->D) {
+    case 32: return pick_rows<32>(fp16, kv);
+    case 64: return pick_rows<64>(fp16, kv);
+    case 128: return pick_rows<128>(fp16, kv);
+    default: return pick_rows<256>(fp16, kv);
+  }
+}
+
+int max_splits_d(int64_t D, int rows) {
+  switch (D) {
+    case 32: return rows_max_splits<32>(rows);
+    case 64: return rows_max_splits<64>(rows);
+    case 128: return rows_max_splits<128>(rows);
+    default: return rows_max_splits<256>(rows);
+  }
+}
+int rows_slot_d(int64_t D, int rows) {
+  switch (D) {
+    case 32: return rows_slot<32>(rows);
+    case 64: return rows_slot<64>(rows);
+    case 128: return rows_slot<128>(rows);
+    default: return rows_slot<256>(rows);
+  }
+}
+
+// The kernel of few rows, its row tiles and its slices of the keys.
+struct RowsPlan {
+  bool few;
+  int nrt, nsplit;
+};
+
+constexpr int FEW_ROWS = 64;
+
+RowsPlan rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, int cus) {
+  RowsPlan r = {false, 0, 0};
+  const int64_t R = SQ * (H / HKV);
+  if (R > FEW_ROWS) return r;
+  r.few = true;
+  r.nrt = (int)cdiv64(R, ROWS_M);
+  const int64_t items = B * HKV * r.nrt;
+  const int64_t steps = cdiv64(P, ROWS_N) + cdiv64(SN, ROWS_N);
+  int64_t n = std::max<int64_t>(1, 2 * (int64_t)std::max(cus, 1) / items);
+  n = std::min(n, std::max<int64_t>(1, steps / ROWS_WAVES));
+  n = std::min<int64_t>(n, max_splits_d(D, (int)std::min<int64_t>(R, ROWS_M)));
+  r.nsplit = (int)n;
+  return r;
+}
+
+int64_t rows_ws_bytes(const RowsPlan& r, int64_t B, int64_t HKV, int64_t D, int64_t R) {
+  if (r.nsplit <= 1) return 0;
+  return QIK_ATTN_WS_CTL_BYTES + B * HKV * r.nrt * r.nsplit * rows_slot_d(D, (int)std::min<int64_t>(R, ROWS_M)) * 4;
+}
+
+struct MxLaunch {
+  RowsPlan rows;
+  Launch many;
+  int64_t ws_bytes;
+};
+
+bool no_work(const qik_attn_args& a) { return a.B == 0 || a.H == 0 || a.SQ == 0; }
+
+int plan_mx(const qik_mx_attn_args* x, MxLaunch* l) {
+  const qik_attn_args& a = x->a;
+  l->ws_bytes = 0;
+  const int64_t G = a.H / x->HKV;
+  l->rows = rows_plan(a.B, a.SQ, a.SN, a.P, a.H, x->HKV, a.D, device_cus());
+  if (l->rows.few) {
+    l->ws_bytes = rows_ws_bytes(l->rows, a.B, x->HKV, a.D, a.SQ * G);
+    return QIK_OK;
+  }
+  const int st = plan_launch(a.B * x->HKV, a.SQ * G, a.D, (a.flags & QIK_UNIFORM_L) != 0, mx_kernels_of(&a), true, &l->many);
+  l->ws_bytes = l->many.ws_bytes;
+  return st;
+}
+
+}  // namespace qik
+
+extern "C" {
+
+int qik_mx_slab_store(const qik_mx_slab_store_args* a, void* stream) {
+  if (a == nullptr) return QIK_ERR_NULL_ARG;
+  if (a->abi_version != QIK_ABI_VERSION) return QIK_ERR_ABI_VERSION;
+  if (a->dtype != QIK_DTYPE_BF16 && a->dtype != QIK_DTYPE_FP16) return QIK_ERR_DTYPE;
+  if (a->D != 32 && a->D != 64 && a->D != 128 && a->D != 256) return QIK_ERR_HEAD_DIM;
+  if (a->B < 0 || a->S < 0 || a->H < 0 || a->capacity < 0 || a->B > INT_MAX || a->S > INT_MAX || a->H > INT_MAX ||
+      a->capacity > INT_MAX)
+    return QIK_ERR_SHAPE;
+  if (a->B == 0 || a->S == 0 || a->H == 0) return QIK_OK;
+  if (a->B * a->H > INT_MAX || a->B * a->H > INT_MAX / a->S) return QIK_ERR_SHAPE;
+  if (a->k == nullptr || a->v == nullptr) return QIK_ERR_NULL_ARG;
+  if (!qik::aligned_to(a->k, 16) || !qik::aligned_to(a->v, 16) || !qik::stride_ok(a->stride_k, a->B, a->S, a->H, 8) ||
+      !qik::stride_ok(a->stride_v, a->B, a->S, a->H, 8))
+    return QIK_ERR_ALIGN;
+  int st = qik_mx_slabs::slab_status(a->k_dst, a->B, a->capacity, a->H, a->D);
+  if (st == QIK_OK) st = qik_mx_slabs::slab_status(a->v_dst, a->B, a->capacity, a->H, a->D);
+  if (st != QIK_OK) return st;
+  const bool grow = a->lengths != nullptr && a->lengths == a->at;
+  if (grow && a->arrivals == nullptr) return QIK_ERR_NULL_ARG;
+
+  qik_mx_slabs::StoreParams p;
+  memset(&p, 0, sizeof(p));
+  const void* src[2] = {a->k, a->v};
+  const qik_mx_slab* dst[2] = {&a->k_dst, &a->v_dst};
+  const int64_t* st_in[2] = {a->stride_k, a->stride_v};
+  for (int w = 0; w < 2; ++w) {
+    p.src[w] = static_cast<const char*>(src[w]);
+    p.codes[w] = static_cast<unsigned char*>(dst[w]->codes);
+    p.scales[w] = static_cast<unsigned char*>(dst[w]->scales);
+    for (int i = 0; i < 3; ++i) {
+      p.ss[w][i] = st_in[w][i] * 2;
+      p.sc[w][i] = dst[w]->stride_codes[i];
+      p.se[w][i] = dst[w]->stride_scales[i];
+    }
+  }
+  p.at = a->at;
+  p.lengths = a->lengths;
+  p.arrivals = grow ? a->arrivals : nullptr;
+  p.rows = (int)(a->B * a->H * a->S);
+  p.B = (int)a->B;
+  p.S = (int)a->S;
+  p.H = (int)a->H;
+  p.capacity = (int)a->capacity;
+  const int rows_wg = qik_mx_slabs::THREADS / (int)(a->D / 8) * qik_mx_slabs::UNITS;
+  const unsigned grid = (unsigned)(((int64_t)p.rows + rows_wg - 1) / rows_wg);
+  const auto fn = a->dtype == QIK_DTYPE_FP16 ? qik_mx_slabs::pick_store<true>(a->D) : qik_mx_slabs::pick_store<false>(a->D);
+  void* kargs[] = {&p};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3(grid, 2), dim3(qik_mx_slabs::THREADS), kargs, 0,
+                                       static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? QIK_OK : QIK_ERR_LAUNCH;
+}
+
+int qik_mx_slab_load(const qik_mx_slab_load_args* a, void* stream) {
+  if (a == nullptr) return QIK_ERR_NULL_ARG;
+  if (a->abi_version != QIK_ABI_VERSION) return QIK_ERR_ABI_VERSION;
+  if (a->dtype != QIK_DTYPE_BF16 && a->dtype != QIK_DTYPE_FP16) return QIK_ERR_DTYPE;
+  if (a->D != 32 && a->D != 64 && a->D != 128 && a->D != 256) return QIK_ERR_HEAD_DIM;
+  if (a->B < 0 || a->P < 0 || a->H < 0 || a->B > INT_MAX || a->P > INT_MAX || a->H > INT_MAX) return QIK_ERR_SHAPE;
+  if (a->B == 0 || a->P == 0 || a->H == 0) return QIK_OK;
+  if (a->B * a->H > INT_MAX) return QIK_ERR_SHAPE;
+  if (a->k == nullptr || a->v == nullptr) return QIK_ERR_NULL_ARG;
+  if (!qik::aligned_to(a->k, 16) || !qik::aligned_to(a->v, 16)) return QIK_ERR_ALIGN;
+  int st = qik_mx_slabs::slab_status(a->k_src, a->B, a->P, a->H, a->D);
+  if (st == QIK_OK) st = qik_mx_slabs::slab_status(a->v_src, a->B, a->P, a->H, a->D);
+  if (st != QIK_OK) return st;
+
+  qik_mx_slabs::LoadParams p;
+  memset(&p, 0, sizeof(p));
+  const qik_mx_slab* src[2] = {&a->k_src, &a->v_src};
+  void* out[2] = {a->k, a->v};
+  for (int w = 0; w < 2; ++w) {
+    p.codes[w] = static_cast<const unsigned char*>(src[w]->codes);
+    p.scales[w] = static_cast<const unsigned char*>(src[w]->scales);
+    p.out[w] = static_cast<char*>(out[w]);
+    for (int i = 0; i < 3; ++i) {
+      p.sc[w][i] = src[w]->stride_codes[i];
+      p.se[w][i] = src[w]->stride_scales[i];
+    }
+  }
+  p.lengths = a->lengths;
+  p.rows = a->B * a->H * a->P;
+  p.B = (int)a->B;
+  p.P = (int)a->P;
+  p.H = (int)a->H;
+  const int64_t rows_wg = qik_mx_slabs::THREADS / (a->D / 8) * qik_mx_slabs::UNITS;
+  unsigned gx, gy;
+  if (!qik_host::split_grid((p.rows + rows_wg - 1) / rows_wg, qik_mx_slabs::THREADS, &gx, &gy)) return QIK_ERR_SHAPE;
+  const auto fn = a->dtype == QIK_DTYPE_FP16 ? qik_mx_slabs::pick_load<true>(a->D) : qik_mx_slabs::pick_load<false>(a->D);
+  void* kargs[] = {&p};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3(gx, gy, 2), dim3(qik_mx_slabs::THREADS), kargs, 0,
+                                       static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? QIK_OK : QIK_ERR_LAUNCH;
+}
+
+int qik_mx_attn_validate(const qik_mx_attn_args* x) {
+  if (x == nullptr) return QIK_ERR_NULL_ARG;
+  const qik_attn_args& a = x->a;
+  if (a.abi_version != QIK_ABI_VERSION || a.reserved0 != 0 || a.reserved1 != 0) return QIK_ERR_ABI_VERSION;
+  if (a.dtype != QIK_DTYPE_BF16 && a.dtype != QIK_DTYPE_FP16) return QIK_ERR_DTYPE;
+  if (a.D != 32 && a.D != 64 && a.D != 128 && a.D != 256) return QIK_ERR_HEAD_DIM;
+  const int64_t lim = (int64_t)INT_MAX;
+  if (a.B < 0 || a.SQ < 0 || a.SN < 0 || a.P < 0 || a.H < 0 || x->HKV < 0) return QIK_ERR_SHAPE;
+  if (a.SQ > lim || a.SN > lim || a.P > lim || a.H > lim || a.P + a.SN > lim || a.B > lim) return QIK_ERR_SHAPE;
+  if ((a.flags & ~(QIK_HAS_CACHE | QIK_HAS_KEY_VALID | QIK_UNIFORM_L)) != 0) return QIK_ERR_SHAPE;
+  const bool has_cache = (a.flags & QIK_HAS_CACHE) != 0;
+  const bool has_kv = (a.flags & QIK_HAS_KEY_VALID) != 0;
+  const bool uniform = (a.flags & QIK_UNIFORM_L) != 0;
+  if (has_cache != (a.P > 0) || a.k_cache != nullptr || a.v_cache != nullptr) return QIK_ERR_CACHE;
+  if (a.v_scale != nullptr) return QIK_ERR_FP8_SCALE;
+  if (has_kv != (a.key_valid != nullptr) || a.debug_tiles != nullptr) return QIK_ERR_NULL_ARG;
+  if (qik::no_work(a)) return QIK_OK;
+  if (x->HKV < 1 || a.H % x->HKV != 0) return QIK_ERR_SHAPE;
+  // row blocks of a KV head's rows, and all of them
+  const int64_t G = a.H / x->HKV;
+  if (a.SQ > lim / G) return QIK_ERR_SHAPE;
+  const int64_t tiles = qik::cdiv64(a.SQ * G, qik::ROWS_M);
+  if (a.B > lim / x->HKV || a.B * x->HKV > lim / tiles) return QIK_ERR_SHAPE;
+
+  if (a.q == nullptr || a.out == nullptr) return QIK_ERR_NULL_ARG;
+  if (a.SN > 0 && (a.k_new == nullptr || a.v_new == nullptr)) return QIK_ERR_NULL_ARG;
+  if (!uniform && a.prefix_lengths == nullptr) return QIK_ERR_NULL_ARG;
+  if (!qik::aligned_to(a.q, 16) || !qik::aligned_to(a.out, 16)) return QIK_ERR_ALIGN;
+  if (!qik::stride_ok(a.stride_q, a.B, a.SQ, a.H, 8) || !qik::stride_ok(a.stride_out, a.B, a.SQ, a.H, 8)) return QIK_ERR_ALIGN;
+  if (a.SN > 0) {
+    if (!qik::aligned_to(a.k_new, 16) || !qik::aligned_to(a.v_new, 16)) return QIK_ERR_ALIGN;
+    if (!qik::stride_ok(a.stride_k_new, a.B, a.SN, x->HKV, 8) || !qik::stride_ok(a.stride_v_new, a.B, a.SN, x->HKV, 8))
+      return QIK_ERR_ALIGN;
+    const int64_t tile_lim = ((int64_t)1 << 31) / qik::BN;
+    if (a.SN > 1 && (a.stride_k_new[1] < a.D || a.stride_v_new[1] < a.D)) return QIK_ERR_ALIGN;
+    if (a.stride_k_new[1] * 2 >= tile_lim || a.stride_v_new[1] * 2 >= tile_lim) return QIK_ERR_SHAPE;
+  }
+  if (has_cache) {
+    int st = qik_mx_slabs::slab_status(x->k_slab, a.B, a.P, x->HKV, a.D);
+    if (st == QIK_OK) st = qik_mx_slabs::slab_status(x->v_slab, a.B, a.P, x->HKV, a.D);
+    if (st != QIK_OK) return st;
+  }
+  return QIK_OK;
+}
+
+int qik_mx_attn_workspace_size(const qik_mx_attn_args* x, int64_t* bytes) {
+  if (bytes == nullptr) return QIK_ERR_NULL_ARG;
+  *bytes = 0;
+  const int st = qik_mx_attn_validate(x);
+  if (st != QIK_OK || qik::no_work(x->a)) return st;
+  qik::MxLaunch l;
+  const int pst = qik::plan_mx(x, &l);
+  if (pst == QIK_OK) *bytes = l.ws_bytes;
+  return pst;
+}
+
+int qik_mx_attn_fwd(const qik_mx_attn_args* x, void* ws, int64_t ws_bytes, void* stream) {
+  const int st = qik_mx_attn_validate(x);
+  if (st != QIK_OK || qik::no_work(x->a)) return st;
+  const qik_attn_args& a = x->a;
+  qik::MxLaunch l;
+  const int pst = qik::plan_mx(x, &l);
+  if (pst != QIK_OK) return pst;
+  if (l.ws_bytes > 0 && (ws == nullptr || !qik::aligned_to(ws, 256) || ws_bytes < l.ws_bytes)) return QIK_ERR_WORKSPACE;
+  const int64_t G = a.H / x->HKV;
+  const float qk_scale = a.sm_scale * 1.44269504088896340736f;
+  const bool cache = a.P > 0;
+  const int64_t none[3] = {0, 0, 0};
+  const int64_t* kc = cache ? x->k_slab.stride_codes : none;
+  const int64_t* vc = cache ? x->v_slab.stride_codes : none;
+  const int64_t* ks = cache ? x->k_slab.stride_scales : none;
+  const int64_t* vs = cache ? x->v_slab.stride_scales : none;
+  const void* fn;
+  void* kargs[1];
+  unsigned grid, threads;
+  qik::RowsParams r;
+  qik::MxParams p;
+  if (l.rows.few) {
+    memset(&r, 0, sizeof(r));
+    r.q = static_cast<const char*>(a.q);
+    r.k_new = static_cast<const char*>(a.k_new);
+    r.v_new = static_cast<const char*>(a.v_new);
+    if (cache) {
+      r.k_codes = static_cast<const char*>(x->k_slab.codes);
+      r.v_codes = static_cast<const char*>(x->v_slab.codes);
+      r.k_scales = static_cast<const char*>(x->k_slab.scales);
+      r.v_scales = static_cast<const char*>(x->v_slab.scales);
+      r.lengths = x->lengths;
+    }
+    r.L = a.prefix_lengths;
+    r.key_valid = a.key_valid;
+    r.out = static_cast<char*>(a.out);
+    if (l.ws_bytes > 0) {
+      r.ctl = static_cast<unsigned*>(ws);
+      r.part = reinterpret_cast<float*>(static_cast<char*>(ws) + QIK_ATTN_WS_CTL_BYTES);
+    }
+    for (int i = 0; i < 3; ++i) {
+      r.sq[i] = a.stride_q[i];
+      r.skn[i] = a.stride_k_new[i];
+      r.svn[i] = a.stride_v_new[i];
+      r.so[i] = a.stride_out[i];
+      r.skc[i] = kc[i];
+      r.svc[i] = vc[i];
+      r.sks[i] = ks[i];
+      r.svs[i] = vs[i];
+    }
+    r.svalid_b = a.stride_valid_b;
+    r.sL_b = x->stride_lengths_b;
+    r.R = (int)(a.SQ * G);
+    r.SN = (int)a.SN;
+    r.P = (int)a.P;
+    r.HKV = (int)x->HKV;
+    r.G = (int)G;
+    r.KV = (int)(a.P + a.SN);
+    r.uniform = (a.flags & QIK_UNIFORM_L) ? 1 : 0;
+    r.nrt = l.rows.nrt;
+    r.nsplit = l.rows.nsplit;
+    r.prow = std::min(r.R, qik::ROWS_M);
+    r.qk_scale = qk_scale;
+    fn = reinterpret_cast<const void*>(qik::rows_kernel_of(&a));
+    grid = (unsigned)(a.B * x->HKV * l.rows.nrt * l.rows.nsplit);
+    threads = qik::ROWS_THREADS;
+    kargs[0] = &r;
+  } else {
+    if (l.many.grid == 0) return QIK_OK;
+    memset(&p, 0, sizeof(p));
+    p.q = static_cast<const char*>(a.q);
+    p.k_new = static_cast<const char*>(a.k_new);
+    p.v_new = static_cast<const char*>(a.v_new);
+    if (cache) {
+      p.k_cache = static_cast<const char*>(x->k_slab.codes);
+      p.v_cache = static_cast<const char*>(x->v_slab.codes);
+      p.k_scales = static_cast<const uint8_t*>(x->k_slab.scales);
+      p.v_scales = static_cast<const uint8_t*>(x->v_slab.scales);
+      p.lengths = x->lengths;
+    }
+    p.L = a.prefix_lengths;
+    p.key_valid = a.key_valid;
+    p.out = static_cast<char*>(a.out);
+    if (l.ws_bytes > 0) {
+      p.ctl = static_cast<unsigned*>(ws);
+      p.ws_slots = static_cast<char*>(ws) + l.many.ctl_bytes;
+    }
+    for (int i = 0; i < 3; ++i) {
+      p.sq[i] = a.stride_q[i];
+      p.skn[i] = a.stride_k_new[i];
+      p.svn[i] = a.stride_v_new[i];
+      p.so[i] = a.stride_out[i];
+      p.skc[i] = kc[i];
+      p.svc[i] = vc[i];
+      p.sks[i] = ks[i];
+      p.svs[i] = vs[i];
+    }
+    p.svalid_b = a.stride_valid_b;
+    p.sL_b = x->stride_lengths_b;
+    p.SQ = (int)(a.SQ * G);
+    p.SN = (int)a.SN;
+    p.P = (int)a.P;
+    p.H = (int)x->HKV;
+    p.KV = (int)(a.P + a.SN);
+    p.has_cache = cache ? 1 : 0;
+    p.has_key_valid = (a.flags & QIK_HAS_KEY_VALID) ? 1 : 0;
+    p.uniform = (a.flags & QIK_UNIFORM_L) ? 1 : 0;
+    p.qk_scale = qk_scale;
+    p.plan = l.many.plan;
+    p.G = (int)G;
+    fn = l.many.fn;
+    grid = (unsigned)l.many.grid;
+    threads = (unsigned)l.many.threads;
+    kargs[0] = &p;
+  }
+  const hipError_t e = hipLaunchKernel(fn, dim3(grid), dim3(threads), kargs, 0, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? QIK_OK : QIK_ERR_LAUNCH;
+}
+
+int qik_mx_attn_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, int32_t cus,
+                     int32_t* few, int32_t* row_tiles, int32_t* splits) {
+  if (few == nullptr || row_tiles == nullptr || splits == nullptr) return QIK_ERR_NULL_ARG;
+  if (B < 1 || SQ < 1 || SN < 0 || P < 0 || HKV < 1 || H < HKV || H % HKV != 0 || cus < 1) return QIK_ERR_SHAPE;
+  if (D != 32 && D != 64 && D != 128 && D != 256) return QIK_ERR_HEAD_DIM;
+  const qik::RowsPlan r = qik::rows_plan(B, SQ, SN, P, H, HKV, D, cus);
+  *few = r.few ? 1 : 0;
+  *row_tiles = r.nrt;
+  *splits = r.nsplit;
+  return QIK_OK;
+}
+
+}  // extern "C"

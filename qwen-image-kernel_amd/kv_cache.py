@@ -18,6 +18,11 @@ reference's own CPU-runnable case) runs those torch ops.
 Difference from the reference: the prefix length of each layer is also kept on
 the host, so ``get()``/``views()`` do not synchronise the device
 (the reference reads ``int(lengths[layer])``, kv_cache.py:49, 56).
+
+``MXKVCache`` (no counterpart in the reference) is a slab with K and V in 4
+bits, 272 bytes a token and head at D = 128 where the bf16 slab has 1024 and the
+fp8-V one 768, with a length for each batch entry and tokens appended behind it
+(include/qik_mx_attn.h).
 """
 
 from __future__ import annotations
@@ -28,11 +33,16 @@ import torch
 
 from . import _lib
 from .attention import _kernel_layout
+from .mx_slab import _DTYPES, HEAD_DIMS, MXSlab, slab_values
 
 FP8_E4M3_MAX = 448.0
 
 
-class _LayerView:
+class _SlabLayer:
+    """A layer whose store copies what it is given (a cache that keeps the tensors themselves is none)."""
+
+
+class _LayerView(_SlabLayer):
     """Per-layer store/get interface compatible with the stock cache."""
 
     def __init__(self, cache: "ContiguousKVCache", layer: int):
@@ -235,4 +245,180 @@ class ContiguousKVCache:
         return ws.data_ptr()
 
     def get_layer(self, i: int) -> _LayerView:
+        return self.layers[i]
+
+
+class _MXLayerView(_SlabLayer):
+    """One layer of an ``MXKVCache``: store / append / get / views."""
+
+    def __init__(self, cache: "MXKVCache", layer: int):
+        self._c = cache
+        self._layer = layer
+
+    def store(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        """k, v ``[B, P, H, D]`` post-RoPE become rows 0 .. P - 1 of every batch entry, whose length is then P."""
+        c = self._c
+        P = self._check(k, v)
+        if P > c.capacity:
+            raise ValueError(f"prefix of {P} tokens exceeds the slab capacity {c.capacity}")
+        if P == 0 or k.numel() == 0:
+            c.lengths[self._layer].fill_(P)
+        else:
+            self._launch(k, v, None, False)
+        c._host_lengths[self._layer], c._exact[self._layer] = P, True
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, at: torch.Tensor | int | None = None) -> None:
+        """k, v ``[B, S, H, D]`` become rows ``at[b]`` .. ``at[b] + S - 1`` of batch entry b, whose length is then
+        ``at[b] + S``, clamped to 0 .. capacity.
+
+        ``at``: None (behind each entry's present length), an int, or an int32
+        ``[B]`` device tensor, which must not overlap the layer's ``lengths``
+        unless it is them.  Rows past the capacity are not written; where the
+        host knows the lengths (they came from ``store``, or from appends with
+        None or an int outside of graph capture) that is a ValueError instead."""
+        c = self._c
+        S = self._check(k, v)
+        n, exact = c._host_lengths[self._layer], c._exact[self._layer]
+        lengths = c.lengths[self._layer]
+        if isinstance(at, torch.Tensor):
+            if tuple(at.shape) != (c.batch_size,) or at.dtype != torch.int32 or at.device != lengths.device:
+                raise ValueError(f"at must be int32 [{c.batch_size}] on {lengths.device}, "
+                                 f"got {at.dtype} {tuple(at.shape)} on {at.device}")
+            first, last = lengths.data_ptr(), lengths.data_ptr() + 4 * c.batch_size
+            if not at.is_contiguous() or (at.data_ptr() != first and first - 4 * c.batch_size < at.data_ptr() < last):
+                at = at.clone(memory_format=torch.contiguous_format)
+            n, exact = c.capacity, False
+        elif at is not None:
+            at = int(at)
+            if at < 0 or at + S > c.capacity:
+                raise ValueError(f"{S} tokens at {at} exceed the slab capacity {c.capacity}")
+            lengths.fill_(at)
+            n, exact = at + S, True
+            at = lengths
+        else:
+            if exact and n + S > c.capacity:
+                raise ValueError(f"{S} tokens behind {n} exceed the slab capacity {c.capacity}")
+            n, at = min(n + S, c.capacity), lengths
+            if torch.cuda.is_current_stream_capturing():
+                # a replay grows the entries further than the host sees
+                n, exact = c.capacity, False
+        if k.numel():
+            self._launch(k, v, at, at.data_ptr() == lengths.data_ptr())
+        elif at.data_ptr() != lengths.data_ptr():
+            lengths.copy_((at + S).clamp_(0, c.capacity))
+        elif S:
+            lengths.add_(S).clamp_(0, c.capacity)
+        c._host_lengths[self._layer], c._exact[self._layer] = n, exact
+
+    def _check(self, k: torch.Tensor, v: torch.Tensor) -> int:
+        c = self._c
+        H, D = c.num_heads, c.head_dim
+        if k.shape != v.shape or k.dim() != 4 or tuple(k.shape[2:]) != (H, D):
+            raise ValueError(f"k, v must be [B, P, {H}, {D}] matching the slab, got {tuple(k.shape)}, {tuple(v.shape)}")
+        if k.shape[0] != c.batch_size:
+            raise ValueError(f"batch {k.shape[0]} != slab batch {c.batch_size}")
+        return k.shape[1]
+
+    def _launch(self, k, v, at, grow: bool) -> None:
+        c = self._c
+        i, dev = self._layer, c.lengths.device
+        k, v = (_kernel_layout(t if t.stride(-1) == 1 else t.contiguous())
+                for t in (k.to(device=dev, dtype=c.dtype), v.to(device=dev, dtype=c.dtype)))
+        gkey = (i, k.shape, k.stride(), v.stride())
+        a = c._args_cache.get(gkey)
+        if a is None:
+            B, S, H, D = k.shape
+            full = self._slabs(c.capacity)
+            a = _lib.QikMxSlabStoreArgs(_lib.ABI_VERSION, _DTYPES[c.dtype], None, None, full[0].struct(), full[1].struct(),
+                                        None, c.lengths[i].data_ptr(), None, B, S, H, D, c.capacity,
+                                        _lib._i64x3(*k.stride()[:3]), _lib._i64x3(*v.stride()[:3]))
+            if len(c._args_cache) >= 4 * max(c.num_layers, 1):
+                c._args_cache.clear()
+            c._args_cache[gkey] = a
+        a = _lib.QikMxSlabStoreArgs.from_buffer_copy(a)
+        a.k, a.v = k.data_ptr(), v.data_ptr()
+        if at is not None:
+            a.at = at.data_ptr()
+            if grow:
+                a.arrivals = c._arrivals.data_ptr() + 4 * i
+        idx = dev.index
+        fn = _lib.load().qik_mx_slab_store
+        if idx != torch.cuda.current_device():
+            with torch.cuda.device(idx):
+                st = fn(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(idx))
+        else:
+            st = fn(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(idx))
+        if st:
+            _lib.check(st, "qik_mx_slab_store")
+
+    def _slabs(self, P: int) -> tuple[MXSlab, MXSlab]:
+        c, i = self._c, self._layer
+        hit = c._views.get((i, P))
+        if hit is None:
+            hit = tuple(MXSlab(codes[i, :, :, :P].transpose(1, 2), scales[i, :, :, :P].transpose(1, 2), c.lengths[i])
+                        for codes, scales in ((c.k_codes, c.k_scales), (c.v_codes, c.v_scales)))
+            if len(c._views) >= 4 * max(c.num_layers, 1):
+                c._views.clear()
+            c._views[(i, P)] = hit
+        return hit
+
+    def get(self):
+        """(k, v): the values of the layer's rows, ``[B, P, H, D]`` in the cache's dtype, zeros behind each entry's
+        length; P as in ``views()``."""
+        return slab_values(*self._slabs(self._c._host_lengths[self._layer]), self._c.dtype)
+
+    def views(self, P: int | None = None):
+        """(k, v, None) for block_causal_flash_attention: ``MXSlab`` views of the first P rows, with the entries'
+        lengths.  P by default is the longest length as far as the host knows it (the capacity after an append whose
+        places only the device knows); fewer rows plan a call for fewer keys, and leave out what lies behind them."""
+        c = self._c
+        if P is None:
+            P = c._host_lengths[self._layer]
+        elif not 0 <= P <= c.capacity:
+            raise ValueError(f"{P} rows of a slab of {c.capacity}")
+        return (*self._slabs(P), None)
+
+
+class MXKVCache:
+    """Single-slab prefix KV cache with K and V in MXFP4: one allocation per buffer for all layers.
+
+    Codes ``k_codes``, ``v_codes`` uint8 ``[L, B, H, P_max, D / 2]`` and block
+    scales ``k_scales``, ``v_scales`` uint8 ``[L, B, H, P_max, D / 32]``, the
+    format of ``quantize_mx`` (an infinity or NaN makes its block NaN);
+    ``lengths`` int32 ``[L, B]``, kept on the device by ``store`` and ``append``.  A
+    program may lower lengths itself (an entry that ends and starts anew);
+    they grow through ``append`` alone.  ``num_heads`` counts the keys' heads,
+    which may be fewer than the queries'.  HIP devices only."""
+
+    def __init__(
+        self,
+        num_layers: int,
+        batch: int,
+        prefix_max: int,
+        num_heads: int,
+        head_dim: int,
+        device: torch.device | str = "cuda",
+        dtype: torch.dtype = torch.bfloat16,
+    ):
+        if torch.device(device).type != "cuda":
+            raise ValueError(f"a 4-bit slab lives on a HIP device, got {device}")
+        if dtype not in _DTYPES:
+            raise ValueError(f"the model's dtype must be bfloat16 or float16, got {dtype}")
+        if head_dim not in HEAD_DIMS:
+            raise ValueError(f"the head dim must be one of {HEAD_DIMS}, got {head_dim}")
+        self.num_layers, self.batch_size, self.capacity = num_layers, batch, prefix_max
+        self.num_heads, self.head_dim, self.dtype = num_heads, head_dim, dtype
+        shape = (num_layers, batch, num_heads, prefix_max)
+        self.k_codes, self.v_codes = (torch.zeros(*shape, head_dim // 2, dtype=torch.uint8, device=device) for _ in range(2))
+        self.k_scales, self.v_scales = (torch.zeros(*shape, head_dim // 32, dtype=torch.uint8, device=device)
+                                        for _ in range(2))
+        self.lengths = torch.zeros(num_layers, batch, dtype=torch.int32, device=device)
+        self._arrivals = torch.zeros(num_layers, dtype=torch.int32, device=device)
+        self._host_lengths = [0] * num_layers   # no entry of the layer is longer
+        self._exact = [True] * num_layers       # ... and every one is that long, if the program changed none
+        self._args_cache: dict = {}             # store geometry -> argument struct
+        self._views: dict = {}                  # (layer, rows) -> MXSlab views
+        self.layers = [_MXLayerView(self, i) for i in range(num_layers)]
+
+    def get_layer(self, i: int) -> _MXLayerView:
         return self.layers[i]

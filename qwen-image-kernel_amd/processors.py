@@ -26,7 +26,7 @@ import torch
 
 from .attention import block_causal_flash_attention, build_prefix_lengths
 from .fused import _rms_rope_qk
-from .kv_cache import _LayerView
+from .kv_cache import _SlabLayer
 
 __all__ = ["QwenImage21KernelProcessor", "_build_prefix_lengths"]
 
@@ -78,12 +78,12 @@ class QwenImage21KernelProcessor:
 
         if kv_cache_mode == "extract" and layer_cache is not None and cache_write_slice is not None:
             k_pre, v_pre = key[:, cache_write_slice], value[:, cache_write_slice]
-            if not isinstance(layer_cache, _LayerView):
+            if not isinstance(layer_cache, _SlabLayer):
                 # a cache that keeps the tensors it is given (the stock get()-only
                 # cache) gets copies, as processors.py:83-84 hands it, so that it
                 # does not pin the whole K/V (or fused QKV output) of the layer
                 k_pre, v_pre = k_pre.clone(), v_pre.clone()
-            # ContiguousKVCache copies into its slab: the slices are read in place
+            # the slabs copy into their buffers: the slices are read in place
             layer_cache.store(k_pre, v_pre)
 
         if segments is not None:
