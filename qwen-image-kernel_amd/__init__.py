@@ -10,7 +10,8 @@ layer's projections (fp8.py:63) on the fp8 matrix cores (include/qik_fp8.h).
 Beside them, with no counterpart in the reference: microscaled tensors and the
 4-bit ``MXFP4Linear`` (mx.py), and the residual RMSNorm that feeds it
 (include/qik_mx.h); the prefix slab in 4 bits, ``MXKVCache``, which the
-attention reads in place (include/qik_mx_attn.h).
+attention reads in place (include/qik_mx_attn.h); and rotary positions on several
+axes for Q and K, with their gradient (include/qik_rope.h).
 The package directory is ``qwen-image-kernel_amd/``; the top-level module
 ``qwen_image_kernel_amd.py`` imports it under this name.
 """
@@ -26,6 +27,7 @@ from .fused import fused_residual_rms_norm, fused_rms_norm_rope  # noqa: F401
 from .kv_cache import FP8_E4M3_MAX, ContiguousKVCache, MXKVCache  # noqa: F401
 from .mx import MXFP4Linear, MXTensor, convert_linears_mxfp4, mx_linear, quantize_mx  # noqa: F401
 from .mx_slab import MXSlab  # noqa: F401
+from .rope import AxialRope, fused_qk_norm_rope  # noqa: F401
 from .processors import QwenImage21KernelProcessor  # noqa: F401
 
 __all__ = [
@@ -38,6 +40,8 @@ __all__ = [
     "MXKVCache",
     "MXSlab",
     "fused_rms_norm_rope",
+    "AxialRope",
+    "fused_qk_norm_rope",
     "QwenImage21KernelProcessor",
     "FP8Linear",
     "fp8_linear",

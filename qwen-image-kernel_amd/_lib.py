@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI declared in include/qik_attn.h, qik_ops.h, qik_fp8.h, qik_mx.h and qik_mx_attn.h.
+"""ctypes binding of the C ABI declared in include/qik_attn.h, qik_ops.h, qik_fp8.h, qik_mx.h, qik_mx_attn.h
+and qik_rope.h.
 
 The shared library is built in-tree (``lib/libqik_attn.so`` next to this file)
 by ``build.py``.  There is no fallback: if the library is missing or fails to
@@ -342,6 +343,45 @@ class QikMxAttnArgs(ctypes.Structure):
     ]
 
 
+class QikRopeTensor(ctypes.Structure):
+    """Mirror of ``struct qik_rope_tensor`` (include/qik_rope.h)."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("dy", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p),
+        ("dw", ctypes.c_void_p),
+        ("H", ctypes.c_int64),
+        ("stride_x", _i64x3),
+        ("stride_out", _i64x3),
+        ("stride_dy", _i64x3),
+        ("eps", ctypes.c_float),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
+class QikAxialRopeArgs(ctypes.Structure):
+    """Mirror of ``struct qik_axial_rope_args`` (include/qik_rope.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("halves", ctypes.c_int32),
+        ("naxes", ctypes.c_int32),
+        ("positions", ctypes.c_void_p),
+        ("freq", ctypes.c_void_p),
+        ("axis", ctypes.c_void_p),
+        ("stride_pos_b", ctypes.c_int64),
+        ("stride_pos_a", ctypes.c_int64),
+        ("B", ctypes.c_int64),
+        ("S", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("t", QikRopeTensor * 2),
+    ]
+
+
 # (name, restype, argtypes) of every entry point of qik_attn.h, qik_ops.h and qik_fp8.h
 EXPORTS = (
     ("qik_abi_version", ctypes.c_int, ()),
@@ -439,6 +479,15 @@ MX_ATTN_EXPORTS = (
       ctypes.c_int32, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32))),
 )
 
+# of qik_rope.h
+ROPE_EXPORTS = (
+    ("qik_axial_rope", ctypes.c_int, (ctypes.POINTER(QikAxialRopeArgs), ctypes.c_void_p)),
+    ("qik_axial_rope_bwd_workspace_size", ctypes.c_int,
+     (ctypes.POINTER(QikAxialRopeArgs), ctypes.POINTER(ctypes.c_int64))),
+    ("qik_axial_rope_bwd", ctypes.c_int,
+     (ctypes.POINTER(QikAxialRopeArgs), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p)),
+)
+
 _lock = threading.Lock()
 _lib = None
 
@@ -457,7 +506,7 @@ def load() -> ctypes.CDLL:
                 "run __graft_entry__.build() or python -m qwen_image_kernel_amd.build"
             )
         lib = ctypes.CDLL(LIB_PATH)
-        for name, restype, argtypes in EXPORTS + MX_EXPORTS + MX_ATTN_EXPORTS:
+        for name, restype, argtypes in EXPORTS + MX_EXPORTS + MX_ATTN_EXPORTS + ROPE_EXPORTS:
             fn = getattr(lib, name)
             fn.restype = restype
             fn.argtypes = list(argtypes)

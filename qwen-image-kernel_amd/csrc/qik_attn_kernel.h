@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(NTHREADS * KSPLIT, (KSPLIT == 1 && D <= 128) ?
       const int n_in = (seg0 ? slab_keys() : p.SN) - row0;
       char* kd = kst[stage];
       char* vdst = vst[stage];
-      if (MX && seg0) {
+      if (seg0) {
         if constexpr (MX) {
           const int kss = (int)p.sks[1], vss = (int)p.svs[1];
           const auto rk = make_rsrc(kcb + (int64_t)row0 * kcs, tile_bytes(n_in, kcs, D / 2));
@@ -641,22 +641,22 @@ __global__ void __launch_bounds__(NTHREADS * KSPLIT, (KSPLIT == 1 && D <= 128) ?
               vexp[i] = __builtin_amdgcn_raw_buffer_load_b8(rvs, (uint32_t)(lane * vss + blk), 0, 0);
             }
           }
-        }
-      } else if (seg0) {
-        dma_tile<D>(kcb + (int64_t)row0 * kcs, kcs, n_in, kd, wave, lane, koff_c);
-        if constexpr (V_FP8) {
-          const char* tb = vcb + (int64_t)row0 * vcs;
-          const auto rs = make_rsrc(tb, tile_bytes(n_in, vcs, D));
-#pragma unroll
-          for (int i = 0; i < F8_LOADS; ++i) {
-            const int qd = i * NTHREADS + tid;
-            const int row = qd / CH8, c16 = qd % CH8;
-            if (F8_CHUNKS >= NTHREADS || qd < F8_CHUNKS)
-              f8reg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                        rs, (uint32_t)(row * vcs + c16 * 16), 0, 0));
-          }
         } else {
-          dma_tile<D>(vcb + (int64_t)row0 * vcs, vcs, n_in, vdst, wave, lane, voff_c);
+          dma_tile<D>(kcb + (int64_t)row0 * kcs, kcs, n_in, kd, wave, lane, koff_c);
+          if constexpr (V_FP8) {
+            const char* tb = vcb + (int64_t)row0 * vcs;
+            const auto rs = make_rsrc(tb, tile_bytes(n_in, vcs, D));
+#pragma unroll
+            for (int i = 0; i < F8_LOADS; ++i) {
+              const int qd = i * NTHREADS + tid;
+              const int row = qd / CH8, c16 = qd % CH8;
+              if (F8_CHUNKS >= NTHREADS || qd < F8_CHUNKS)
+                f8reg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                          rs, (uint32_t)(row * vcs + c16 * 16), 0, 0));
+            }
+          } else {
+            dma_tile<D>(vcb + (int64_t)row0 * vcs, vcs, n_in, vdst, wave, lane, voff_c);
+          }
         }
       } else {
         dma_tile<D>(knb + (int64_t)row0 * kns, kns, n_in, kd, wave, lane, koff_new);
@@ -672,8 +672,11 @@ __global__ void __launch_bounds__(NTHREADS * KSPLIT, (KSPLIT == 1 && D <= 128) ?
         const auto rs = make_rsrc(reinterpret_cast<const char*>(p.key_valid) + b * p.svalid_b + kv0,
                                   __builtin_amdgcn_readfirstlane(min(n_in, BN)));
         // (with a 4-bit slab every wave holds the tile's bytes: it writes rows that are masked as zeros)
-        if (MX) kvbyte = __builtin_amdgcn_raw_buffer_load_b8(rs, (uint32_t)lane, 0, 0);
-        else if (tid < BN) kvbyte = __builtin_amdgcn_raw_buffer_load_b8(rs, (uint32_t)tid, 0, 0);
+        if constexpr (MX) {
+          kvbyte = __builtin_amdgcn_raw_buffer_load_b8(rs, (uint32_t)lane, 0, 0);
+        } else {
+          if (tid < BN) kvbyte = __builtin_amdgcn_raw_buffer_load_b8(rs, (uint32_t)tid, 0, 0);
+        }
       }
     };
 
@@ -833,7 +836,7 @@ __global__ void __launch_bounds__(NTHREADS * KSPLIT, (KSPLIT == 1 && D <= 128) ?
     // 4-bit slab with a key mask: the fresh keys' V rows that the mask hides
     // become zeros once this wave's copies have landed (each wave its own rows,
     // before the barrier that hands the tile on): 0 x NaN would reach every row
-    auto scrub_tile = [&](int g, int stage) {
+    [[maybe_unused]] auto scrub_tile = [&](int g, int stage) {
       if constexpr (MX && KV) {
         const uint64_t hidden = __ballot(kvbyte == 0u);
         if (g < run0 || hidden == 0) return;
@@ -970,7 +973,9 @@ __global__ void __launch_bounds__(NTHREADS * KSPLIT, (KSPLIT == 1 && D <= 128) ?
       finish_tile(g0, 0);
     }
     wait_copies();
-    if (g0 < g1) scrub_tile(g0, 0);
+    if constexpr (MX && KV) {
+      if (g0 < g1) scrub_tile(g0, 0);
+    }
     __syncthreads();
 
     for (int g = g0; g < g1; g += 2) {
@@ -979,14 +984,18 @@ __global__ void __launch_bounds__(NTHREADS * KSPLIT, (KSPLIT == 1 && D <= 128) ?
       compute_tile(g, 0);
       if (g + 1 < g1) finish_tile(g + 1, 1);
       wait_copies();
-      if (g + 1 < g1) scrub_tile(g + 1, 1);
+      if constexpr (MX && KV) {
+        if (g + 1 < g1) scrub_tile(g + 1, 1);
+      }
       tile_sync();
       if (g + 1 < g1) {
         if (g + 2 < g1) issue_tile(g + 2, 0);
         compute_tile(g + 1, 1);
         if (g + 2 < g1) finish_tile(g + 2, 0);
         wait_copies();
-        if (g + 2 < g1) scrub_tile(g + 2, 0);
+        if constexpr (MX && KV) {
+          if (g + 2 < g1) scrub_tile(g + 2, 0);
+        }
         tile_sync();
       }
     }

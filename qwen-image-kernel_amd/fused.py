@@ -18,6 +18,9 @@ the input dtype.  Differences from the reference, both on the safe side:
 ``fused_residual_rms_norm`` is the norm between a layer's linears: the residual
 added, RMSNorm over the last dimension, the result in the element type or
 microscaled for ``MXFP4Linear`` (qik_residual_rms_norm, include/qik_mx.h).
+
+With an ``AxialRope`` in the place of ``freqs_cis`` the angles come from positions
+on several axes (rope.py).
 """
 
 from __future__ import annotations
@@ -30,6 +33,7 @@ from . import _lib
 from .mx import _DTYPES as _NORM_DTYPES
 from .mx import MX_FORMATS, MXTensor, _as_rows, _check_format, _check_width, _CODE_DTYPE, _code_shape, _on_device, \
     _row_stride, _scales_shape
+from .rope import AxialRope, fused_qk_norm_rope, norm_rope
 
 __all__ = ["fused_rms_norm_rope", "fused_residual_rms_norm"]
 
@@ -57,10 +61,15 @@ def _cos_sin(freqs_cis: torch.Tensor, device: torch.device):
 def fused_rms_norm_rope(
     x: torch.Tensor,           # [B, S, H, D] bf16 (or fp16)
     weight: torch.Tensor,      # [D] fp32
-    freqs_cis: torch.Tensor,   # complex [S, D/2]
+    freqs_cis: torch.Tensor | AxialRope,   # complex [S, D/2], or positions on several axes
     eps: float,
 ) -> torch.Tensor:
-    """RMSNorm over D per (b, s, h), then complex RoPE by position s; returns [B, S, H, D]."""
+    """RMSNorm over D per (b, s, h), then complex RoPE by position s; returns [B, S, H, D].
+
+    With an AxialRope the result is rounded once, weight may be None (no norm),
+    and gradients are recorded."""
+    if isinstance(freqs_cis, AxialRope):
+        return norm_rope(x, weight, freqs_cis, eps)
     # One lookup per call: everything that only depends on the geometry, the
     # weight and freqs_cis tensors (and their in-place versions) and eps is
     # checked and prepared once per key -- the argument struct with the
@@ -86,6 +95,11 @@ def _rms_rope_qk(query, key, norm_q, norm_k, freqs_cis):
     """fused_rms_norm_rope of a layer's Q and K (``norm_q`` and ``norm_k`` carry
     ``weight`` and ``eps``), in one launch when both are of one dtype, head dim
     and device, else in two."""
+    if isinstance(freqs_cis, AxialRope):
+        if query.dtype != key.dtype or query.shape[3] != key.shape[3]:
+            return (norm_rope(query, norm_q.weight, freqs_cis, norm_q.eps),
+                    norm_rope(key, norm_k.weight, freqs_cis, norm_k.eps))
+        return fused_qk_norm_rope(query, key, norm_q.weight, norm_k.weight, freqs_cis, norm_q.eps, norm_k.eps)
     if query.dtype != key.dtype or query.shape[-1] != key.shape[-1] or query.device != key.device:
         return (fused_rms_norm_rope(query, norm_q.weight, freqs_cis, norm_q.eps),
                 fused_rms_norm_rope(key, norm_k.weight, freqs_cis, norm_k.eps))
