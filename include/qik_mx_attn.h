@@ -93,7 +93,7 @@ int qik_mx_slab_load(const qik_mx_slab_load_args* args, void* stream);
  * they are: exact in bf16, rounded to fp16 as in qik_mx_slab_load.
  *
  * Few query rows (a token's, or some tokens') run a kernel of their own, which
- * splits the keys over the device; others the kernel of qik_attn_fwd_ws, with
+ * cuts the keys into pieces of one length, one a workgroup; others the kernel of qik_attn_fwd_ws, with
  * the slab's tiles turned into the element type on their way into LDS.  The
  * workspace is qik_attn_fwd_ws's kind: at least qik_mx_attn_workspace_size
  * bytes, 256-byte aligned, its first QIK_ATTN_WS_CTL_BYTES zero before its first
@@ -112,10 +112,10 @@ int qik_mx_attn_workspace_size(const qik_mx_attn_args* args, int64_t* bytes);
 int qik_mx_attn_fwd(const qik_mx_attn_args* args, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Host only: which kernel a call of this shape takes on a device of `cus`
- * compute units.  few: 1 for the kernel of few rows; row_tiles, splits: its
- * workgroups for each (b, KV head). */
+ * compute units.  few: 1 for the kernel of few rows; row_tiles: 16-row tiles of
+ * each (b, KV head)'s rows there; pieces: workgroups that share its keys. */
 int qik_mx_attn_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, int32_t cus,
-                     int32_t* few, int32_t* row_tiles, int32_t* splits);
+                     int32_t* few, int32_t* row_tiles, int32_t* pieces);
 
 #ifdef __cplusplus
 }

@@ -195,10 +195,14 @@ void pick_mx(bool fp16, bool kv, Kernels* k) {
   if (fp16) kv ? pick_mx<D, true, true>(k) : pick_mx<D, true, false>(k);
   else kv ? pick_mx<D, false, true>(k) : pick_mx<D, false, false>(k);
 }
-template <int D>
+template <int D, int MT>
 rows_kernel_fn pick_rows(bool fp16, bool kv) {
-  if (fp16) return kv ? mx_rows_kernel<D, true, true> : mx_rows_kernel<D, true, false>;
-  return kv ? mx_rows_kernel<D, false, true> : mx_rows_kernel<D, false, false>;
+  if (fp16) return kv ? mx_rows_kernel<D, true, true, MT> : mx_rows_kernel<D, true, false, MT>;
+  return kv ? mx_rows_kernel<D, false, true, MT> : mx_rows_kernel<D, false, false, MT>;
+}
+template <int D>
+rows_kernel_fn pick_rows(bool fp16, bool kv, int mt) {
+  return mt == 1 ? pick_rows<D, 1>(fp16, kv) : pick_rows<D, 2>(fp16, kv);
 }
 
 std::atomic<int> g_mx_slots[16][MAX_DEVICES];
@@ -218,61 +222,79 @@ Kernels mx_kernels_of(const qik_attn_args* a) {
   return k;
 }
 
-rows_kernel_fn rows_kernel_of(const qik_attn_args* a) {
+rows_kernel_fn rows_kernel_of(const qik_attn_args* a, int mt) {
   const bool fp16 = a->dtype == QIK_DTYPE_FP16;
   const bool kv = (a->flags & QIK_HAS_KEY_VALID) != 0;
   switch (a->D) {
-    case 32: return pick_rows<32>(fp16, kv);
-    case 64: return pick_rows<64>(fp16, kv);
-    case 128: return pick_rows<128>(fp16, kv);
-    default: return pick_rows<256>(fp16, kv);
+    case 32: return pick_rows<32>(fp16, kv, mt);
+    case 64: return pick_rows<64>(fp16, kv, mt);
+    case 128: return pick_rows<128>(fp16, kv, mt);
+    default: return pick_rows<256>(fp16, kv, mt);
   }
 }
 
-int max_splits_d(int64_t D, int rows) {
-  switch (D) {
-    case 32: return rows_max_splits<32>(rows);
-    case 64: return rows_max_splits<64>(rows);
-    case 128: return rows_max_splits<128>(rows);
-    default: return rows_max_splits<256>(rows);
-  }
-}
-int rows_slot_d(int64_t D, int rows) {
-  switch (D) {
-    case 32: return rows_slot<32>(rows);
-    case 64: return rows_slot<64>(rows);
-    case 128: return rows_slot<128>(rows);
-    default: return rows_slot<256>(rows);
-  }
-}
-
-// The kernel of few rows, its row tiles and its slices of the keys.
+// The kernel of few rows (qik_mx_rows.h): 16-row tiles of an item, items for a KV
+// head's rows, steps of a piece and pieces of an item at most.
 struct RowsPlan {
   bool few;
-  int nrt, nsplit;
+  int mt, nrt, steps, pieces;
+  int row_bits;  // log2 of the rows a piece keeps in the workspace
 };
 
-constexpr int FEW_ROWS = 64;
+// What a call lasts, in us, from measurements at D = 128 on 256 CUs (P 1000 to
+// 131072, 64 to 2048 rows of 1 to 24 KV heads).  Of the kernel of few rows: a
+// wave's step takes 1.4 us with two tiles and eight waves on a CU, 1.9 with one
+// and sixteen; a piece 4 beside its steps; the merge 2, and 1 more for 100 KB of
+// pieces, which one workgroup reads.  Of the other: 10 and its KV tiles, which
+// run no faster than a row block's on as many CUs as it can be split over.
+double rows_cost(const RowsPlan& r, int64_t items, int64_t T, int64_t pieces, int64_t slots, int waves, int64_t D) {
+  const double step = r.mt == 1 ? 1.9 : 1.4;
+  const double merge = pieces > 1 ? 2.0 + (double)pieces * (4 << r.row_bits) * (double)D * 1e-5 : 0.0;
+  return (double)cdiv64(items * pieces, slots) * (step * (double)cdiv64(T, pieces * waves) + 4.0) + merge;
+}
+double many_cost(int64_t blocks, int64_t T, int cus) {
+  return 10.0 + (double)T * std::max(0.455, 1.23 * (double)blocks / cus);
+}
 
 RowsPlan rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, int cus) {
-  RowsPlan r = {false, 0, 0};
-  const int64_t R = SQ * (H / HKV);
-  if (R > FEW_ROWS) return r;
-  r.few = true;
-  r.nrt = (int)cdiv64(R, ROWS_M);
-  const int64_t items = B * HKV * r.nrt;
-  const int64_t steps = cdiv64(P, ROWS_N) + cdiv64(SN, ROWS_N);
-  int64_t n = std::max<int64_t>(1, 2 * (int64_t)std::max(cus, 1) / items);
-  n = std::min(n, std::max<int64_t>(1, steps / ROWS_WAVES));
-  n = std::min<int64_t>(n, max_splits_d(D, (int)std::min<int64_t>(R, ROWS_M)));
-  r.nsplit = (int)n;
+  RowsPlan r = {false, 0, 0, 0, 0, 0};
+  const int64_t G = H / HKV, R = SQ * G;
+  r.mt = R <= ROWS_M ? 1 : 2;
+  const int64_t nrt = cdiv64(R, r.mt * ROWS_M);
+  // limits of the kernel: its grid has the entries in z, the heads and row tiles
+  // in y, and it divides by multiplication
+  if (B > 65535 || HKV > 65535 / nrt || G > INT_MAX / R || HKV * nrt > INT_MAX / HKV) return r;
+  r.nrt = (int)nrt;
+  cus = std::max(cus, 1);
+  const int waves = rows_waves((int)D, r.mt);
+  const int64_t slots = (int64_t)cus * (r.mt == 1 && D <= 128 ? 2 : 1);  // resident workgroups
+  const int64_t T = std::max<int64_t>(cdiv64(P, ROWS_N) + cdiv64(SN, ROWS_N), 1);
+  const int64_t items = B * HKV * nrt;
+  while ((1 << r.row_bits) < std::min<int64_t>(R, r.mt * ROWS_M)) ++r.row_bits;
+  // pieces that fill the slots once, twice ... or none; every wave of a piece has
+  // a step, and an item that is cut a word of the control words
+  const int64_t most = items > QIK_ATTN_WS_CTL_BYTES / 4 ? 1 : std::max<int64_t>(T / waves, 1);
+  int64_t best = 1;
+  double cost = rows_cost(r, items, T, 1, slots, waves, D);
+  for (int64_t k = 1; k <= 4; ++k) {
+    const int64_t n = std::min(std::max<int64_t>(k * slots / items, 1), most);
+    const double c = rows_cost(r, items, T, n, slots, waves, D);
+    if (c < cost) cost = c, best = n;
+  }
+  r.steps = (int)cdiv64(T, best);
+  r.pieces = (int)cdiv64(T, r.steps);
+  const int64_t T64 = cdiv64(P, BN) + cdiv64(SN, BN);
+  r.few = r.mt == 1 || cost < many_cost(B * HKV * cdiv64(R, BM), T64, cus);
   return r;
 }
 
-int64_t rows_ws_bytes(const RowsPlan& r, int64_t B, int64_t HKV, int64_t D, int64_t R) {
-  if (r.nsplit <= 1) return 0;
-  return QIK_ATTN_WS_CTL_BYTES + B * HKV * r.nrt * r.nsplit * rows_slot_d(D, (int)std::min<int64_t>(R, ROWS_M)) * 4;
+int64_t rows_ws_bytes(const RowsPlan& r, int64_t B, int64_t HKV, int64_t D) {
+  if (r.pieces <= 1) return 0;
+  return QIK_ATTN_WS_CTL_BYTES + B * HKV * r.nrt * r.pieces * rows_slot((int)D, 1 << r.row_bits);
 }
+
+// ceil(2^32 / d) for the kernel's quotient, 0 for 1
+unsigned reciprocal(int64_t d) { return d == 1 ? 0u : (unsigned)((((int64_t)1 << 32) + d - 1) / d); }
 
 struct MxLaunch {
   RowsPlan rows;
@@ -288,7 +310,7 @@ int plan_mx(const qik_mx_attn_args* x, MxLaunch* l) {
   const int64_t G = a.H / x->HKV;
   l->rows = rows_plan(a.B, a.SQ, a.SN, a.P, a.H, x->HKV, a.D, device_cus());
   if (l->rows.few) {
-    l->ws_bytes = rows_ws_bytes(l->rows, a.B, x->HKV, a.D, a.SQ * G);
+    l->ws_bytes = rows_ws_bytes(l->rows, a.B, x->HKV, a.D);
     return QIK_OK;
   }
   const int st = plan_launch(a.B * x->HKV, a.SQ * G, a.D, (a.flags & QIK_UNIFORM_L) != 0, mx_kernels_of(&a), true, &l->many);
@@ -468,7 +490,8 @@ int qik_mx_attn_fwd(const qik_mx_attn_args* x, void* ws, int64_t ws_bytes, void*
   const int64_t* vs = cache ? x->v_slab.stride_scales : none;
   const void* fn;
   void* kargs[1];
-  unsigned grid, threads;
+  dim3 grid;
+  unsigned threads;
   qik::RowsParams r;
   qik::MxParams p;
   if (l.rows.few) {
@@ -509,13 +532,14 @@ int qik_mx_attn_fwd(const qik_mx_attn_args* x, void* ws, int64_t ws_bytes, void*
     r.G = (int)G;
     r.KV = (int)(a.P + a.SN);
     r.uniform = (a.flags & QIK_UNIFORM_L) ? 1 : 0;
-    r.nrt = l.rows.nrt;
-    r.nsplit = l.rows.nsplit;
-    r.prow = std::min(r.R, qik::ROWS_M);
+    r.steps = l.rows.steps;
+    r.by_G = qik::reciprocal(G);
+    r.by_HKV = qik::reciprocal(x->HKV);
+    r.row_bits = l.rows.row_bits;
     r.qk_scale = qk_scale;
-    fn = reinterpret_cast<const void*>(qik::rows_kernel_of(&a));
-    grid = (unsigned)(a.B * x->HKV * l.rows.nrt * l.rows.nsplit);
-    threads = qik::ROWS_THREADS;
+    fn = reinterpret_cast<const void*>(qik::rows_kernel_of(&a, l.rows.mt));
+    grid = dim3((unsigned)l.rows.pieces, (unsigned)(x->HKV * l.rows.nrt), (unsigned)a.B);
+    threads = 64u * (unsigned)qik::rows_waves((int)a.D, l.rows.mt);
     kargs[0] = &r;
   } else {
     if (l.many.grid == 0) return QIK_OK;
@@ -561,23 +585,23 @@ int qik_mx_attn_fwd(const qik_mx_attn_args* x, void* ws, int64_t ws_bytes, void*
     p.plan = l.many.plan;
     p.G = (int)G;
     fn = l.many.fn;
-    grid = (unsigned)l.many.grid;
+    grid = dim3((unsigned)l.many.grid);
     threads = (unsigned)l.many.threads;
     kargs[0] = &p;
   }
-  const hipError_t e = hipLaunchKernel(fn, dim3(grid), dim3(threads), kargs, 0, static_cast<hipStream_t>(stream));
+  const hipError_t e = hipLaunchKernel(fn, grid, dim3(threads), kargs, 0, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? QIK_OK : QIK_ERR_LAUNCH;
 }
 
 int qik_mx_attn_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, int32_t cus,
-                     int32_t* few, int32_t* row_tiles, int32_t* splits) {
-  if (few == nullptr || row_tiles == nullptr || splits == nullptr) return QIK_ERR_NULL_ARG;
+                     int32_t* few, int32_t* row_tiles, int32_t* pieces) {
+  if (few == nullptr || row_tiles == nullptr || pieces == nullptr) return QIK_ERR_NULL_ARG;
   if (B < 1 || SQ < 1 || SN < 0 || P < 0 || HKV < 1 || H < HKV || H % HKV != 0 || cus < 1) return QIK_ERR_SHAPE;
   if (D != 32 && D != 64 && D != 128 && D != 256) return QIK_ERR_HEAD_DIM;
   const qik::RowsPlan r = qik::rows_plan(B, SQ, SN, P, H, HKV, D, cus);
   *few = r.few ? 1 : 0;
-  *row_tiles = r.nrt;
-  *splits = r.nsplit;
+  *row_tiles = r.mt * r.nrt;
+  *pieces = r.pieces;
   return QIK_OK;
 }
 

@@ -2,23 +2,32 @@
 // token's heads, or some tokens', against a cache of any length.
 //
 // The mathematics is the tile loop's of qik_attn_kernel.h (S^T = K.Q^T, online
-// softmax in the exp2 domain with a lazy reference point, O^T = V^T.P^T on
-// v_mfma_f32_32x32x16), but such a call is bound by the slab's bytes: 17/32 of
-// a byte per element of K and V, each read once.  So:
-//   * a workgroup holds up to 32 query rows of one (b, KV head) -- the query heads
-//     that share the KV head times the query positions -- and one slice of its
-//     keys; its four waves take the slice's steps of 32 keys in turn, each with
-//     its own softmax state, and never wait for each other before the end;
+// softmax in the exp2 domain with a lazy reference point, O^T = V^T.P^T), but such
+// a call is bound by the slab's bytes: 17/32 of a byte per element of K and V,
+// each read once.  So:
+//   * an item is 16 or 32 query rows of one (b, KV head) -- the query heads that
+//     share the KV head times the query positions -- and its keys in steps of
+//     32.  Items are cut into pieces of the same number of steps, one a
+//     workgroup, so that sequences of any lengths fill the device evenly (a
+//     piece behind an item's last key ends at once);
+//   * a workgroup's waves take its steps in turn, each with its own softmax state
+//     and its own LDS, and never wait for each other before the end;
+//   * a call lasts some microseconds, so that its instructions' way from memory
+//     shows: the loop's and the merge's code stands once, what can be a loop is
+//     one, and what can be divided on the host is;
+//   * the products are v_mfma_f32_16x16x32: with 16 rows a lane holds half of the
+//     scores and accumulators that a 32-row tile has;
 //   * K goes from memory to the matrix cores through registers alone.  The
 //     order of the head dim inside a dot product is free, as long as Q has the
-//     same: lane (key, half) holds its key's half row, 16 to 64 contiguous bytes
-//     of codes, and every 4 bytes become one operand;
+//     same: lane (key, quarter) holds a quarter of its key's row, 4 to 32
+//     contiguous bytes of codes, and every 4 bytes become one operand;
 //   * V is turned into the element type in registers and goes through the
 //     wave's own LDS, whose transpose read gives the V^T operand;
-//   * the next step's codes are loaded before the present step is computed;
-//   * the slices of a (b, KV head) leave their (m, l, O) in the workspace, and
-//     the last to arrive combines them in slice order, so that the result does
-//     not depend on which one that is.
+//   * the next step's codes are loaded as soon as this step's have been turned,
+//     before its softmax;
+//   * the pieces of a cut item leave their (m, l, O) in the workspace, and the
+//     last to arrive combines them in the order of the keys, so that the result
+//     does not depend on which one that is.
 #ifndef QIK_MX_ROWS_H
 #define QIK_MX_ROWS_H
 
@@ -26,10 +35,11 @@
 
 namespace qik {
 
-constexpr int ROWS_WAVES = 4;
 constexpr int ROWS_N = 32;        // keys of a step
-constexpr int ROWS_M = 32;        // query rows of a workgroup
-constexpr int ROWS_THREADS = ROWS_WAVES * 64;
+constexpr int ROWS_M = 16;        // query rows of a tile; an item has one or two tiles
+
+// Waves of a workgroup; two workgroups share a CU (one at D = 256 or with two tiles).
+constexpr int rows_waves(int D, int mt) { return D > 128 && mt > 1 ? 4 : 8; }
 
 struct RowsParams {
   const char* q;
@@ -43,85 +53,120 @@ struct RowsParams {
   const int32_t* L;
   const uint8_t* key_valid;
   char* out;
-  unsigned* ctl;             // arrivals per item, zero between launches (nsplit > 1)
-  float* part;               // per (item, slice): rows x D accumulators, then rows (m, l)
+  unsigned* ctl;             // arrivals per item, zero between launches
+  float* part;               // per (item, piece): rows x D accumulators, then rows (m, l)
   int64_t sq[3], skn[3], svn[3], so[3];  // b, s, h in elements
   int64_t skc[3], svc[3], sks[3], svs[3];  // b, p, h in bytes
   int64_t svalid_b, sL_b;
   int R;                     // query rows of a KV head: SQ * G, row r is head r % G of position r / G
   int SN, P, HKV, G, KV;
   int uniform;
-  int nrt, nsplit;           // row tiles of a KV head, slices of its keys
-  int prow;                  // rows a slice keeps in the workspace: min(R, ROWS_M)
+  int steps;                 // of a piece
+  unsigned by_G, by_HKV;     // ceil(2^32 / G), ceil(2^32 / HKV): see quotient
+  int row_bits;              // log2 of the rows a piece keeps in the workspace, a power of two
   float qk_scale;
 };
 
-// LDS bytes of one wave: its V step, and at the end its share of O (half of the
-// head dim at a time)
+// LDS bytes of one wave: its V step, and at the end its share of a tile's O
 template <int D>
-constexpr int rows_wave_lds() { return D * 2 * ROWS_N > 4096 ? D * 2 * ROWS_N : 4096; }
-// the merge keeps (m, l) of every slice and row there, beside 16 bytes a thread
-template <int D>
-constexpr int rows_max_splits(int rows) { return (ROWS_WAVES * rows_wave_lds<D>() - 16 * ROWS_THREADS) / 8 / rows; }
-// fp32 values a slice of `rows` rows keeps in the workspace: O, then (m, l) of each row
-template <int D>
-__host__ __device__ constexpr int rows_slot(int rows) { return (rows * (D + 2) + 3) / 4 * 4; }
+constexpr int rows_wave_lds() { return D * 2 * ROWS_N; }
+static_assert(ROWS_N * 2 == ROWS_M * 4, "a wave's O of 16 rows in fp32 takes the room of a step's V");
+// bytes a piece of `rows` rows keeps in the workspace: O, then (m, l) of each row
+__host__ __device__ constexpr int rows_slot(int D, int rows) { return (rows * (D + 2) + 3) / 4 * 16; }
 
-template <int D, bool FP16, bool KV>
-__global__ void __launch_bounds__(ROWS_THREADS, D <= 128 ? 2 : 1) mx_rows_kernel(const RowsParams p) {
+template <bool FP16>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (FP16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// x of the four lanes l, l ^ 16, l ^ 32, l ^ 48 together
+__device__ __forceinline__ float quad_max(float x) {
+  const unsigned u = __float_as_uint(pair_max(x));
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  const unsigned u = __float_as_uint(pair_sum(x));
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// n / d by ceil(2^32 / d) (0 for d = 1): exact while n * d < 2^32
+__device__ __forceinline__ int quotient(int n, unsigned by) { return by == 0u ? n : (int)__umulhi((unsigned)n, by); }
+
+// MT: 16-row tiles of an item.
+template <int D, bool FP16, bool KV, int MT>
+__global__ void __launch_bounds__(64 * rows_waves(D, MT), D <= 128 && MT == 1 ? 4 : 1) mx_rows_kernel(const RowsParams p) {
+  constexpr int ROWS_WAVES = rows_waves(D, MT);
+  constexpr int ROWS_THREADS = 64 * ROWS_WAVES;
   constexpr int CH = D / 8;
   constexpr int ROWB = D * 2;
-  constexpr int KSTEPS = D / 16;
-  constexpr int DBLK = D / 32;
+  constexpr int KSTEPS = D / 32;              // products of a 16-key block of S^T
+  constexpr int DBLK = D / 16;                // 16-row blocks of O^T
   constexpr float TAU = 8.0f;
-  constexpr int WORDS = D / 16;               // 4-byte words of codes in half a row
-  constexpr int NB = D >= 64 ? D / 64 : 1;    // blocks (scale bytes) of half a row
+  constexpr int WORDS = D / 32;               // 4-byte words of codes in a quarter row
+  constexpr int NB = D / 128 > 0 ? D / 128 : 1;  // scale bytes of a quarter row
   constexpr int WLDS = rows_wave_lds<D>();
+  constexpr int ROWS = MT * ROWS_M;
   __shared__ u32x4 lds[ROWS_WAVES * WLDS / 16];
-  __shared__ float sm[ROWS_WAVES][ROWS_M], sl[ROWS_WAVES][ROWS_M];
+  __shared__ float sm[ROWS_WAVES][ROWS], sl[ROWS_WAVES][ROWS], smax[ROWS];
   __shared__ int slast;
 
   const int tid = (int)threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hf = lane >> 5, l32 = lane & 31;
+  const int g = lane >> 4, l16 = lane & 15;
   char* const vS = reinterpret_cast<char*>(lds) + wave * WLDS;
 
-  // workgroup -> (row tile, slice, batch entry, KV head): the row tiles of one
-  // slice are a multiple of the slices apart, so they share an XCD's L2 when
-  // that is a multiple of the XCDs
-  const int per = (int)(gridDim.x / (unsigned)p.nrt);
-  const int rt = (int)blockIdx.x / per;
-  const int rest = (int)blockIdx.x - rt * per;
-  const int bh = rest / p.nsplit;
-  const int slice = rest - bh * p.nsplit;
-  const int b = bh / p.HKV;
-  const int h = bh - b * p.HKV;
-
-  const int m = rt * ROWS_M + l32;
-  const bool live = m < p.R;
-  const int mrd = live ? m : p.R - 1;
-  const int tok = (int)((unsigned)mrd / (unsigned)p.G);
-  const int head = h * p.G + (mrd - tok * p.G);
-  const int rows = min(p.R - rt * ROWS_M, ROWS_M);
-
+  // ---- the item and its steps [t0, t1): the slab's, then the fresh keys'
+  const int b = (int)blockIdx.z, hr = (int)blockIdx.y;
+  const int rt = quotient(hr, p.by_HKV);
+  const int h = hr - rt * p.HKV;
+  const int row_first = rt * ROWS;
+  const int rows = min(p.R - row_first, ROWS);
   int Pc = p.P;
-  if (p.lengths != nullptr) Pc = __builtin_amdgcn_readfirstlane(min(max(gload_i32(p.lengths + b), 0), p.P));
-  int Lrow = p.KV - 1, Lmax = p.KV - 1, Lmin = p.KV - 1;
-  if (!p.uniform) {
-    const int Lraw = gload_i32(p.L + b * p.sL_b + tok);
-    Lrow = live ? Lraw : -1;
-    Lmax = wave_reduce_i32<true>(Lrow);
-    Lmin = wave_reduce_i32<false>(live ? Lraw : INT_MAX);
-  }
+  if (p.lengths != nullptr)
+    Pc = min(max(*((const __attribute__((address_space(4))) int32_t*)(p.lengths + b)), 0), p.P);
+  const int slab = cdiv_i(Pc, ROWS_N);
+  const int T = slab + cdiv_i(p.SN, ROWS_N);
+  const int t0 = (int)blockIdx.x * p.steps;
+  if (t0 >= T && t0 > 0) return;
+  const int pieces = max((T + p.steps - 1) / p.steps, 1);
+  const int s1 = p.P;  // absolute index of the first fresh key
 
-  // Q as the B operand: lane holds Q[m, hf * D/2 + 8j .. + 8], the order in
-  // which the codes of half a row come
-  u32x4 qreg[KSTEPS];
-  {
-    const char* qr = p.q + (b * p.sq[0] + (int64_t)tok * p.sq[1] + head * p.sq[2]) * 2 + hf * D;
+  // Q as the B operand: lane holds Q[m, g * D/4 + 8j .. + 8], the order in which
+  // the codes of a quarter row come; and each row's causal length
+  u32x4 qreg[MT][KSTEPS];
+  int Lrow[MT];
+  int Lmax = p.KV - 1, Lmin = p.KV - 1;
+  if (!p.uniform) Lmax = -1, Lmin = INT_MAX;
 #pragma unroll
-    for (int j = 0; j < KSTEPS; ++j) qreg[j] = gload16(qr + 16 * j);
+  for (int mt = 0; mt < MT; ++mt) {
+    const int m = row_first + mt * ROWS_M + l16;
+    const bool live = m < p.R;
+    const int mrd = live ? m : p.R - 1;
+    const int tok = quotient(mrd, p.by_G);
+    const int head = h * p.G + (mrd - tok * p.G);
+    const char* qr = p.q + (b * p.sq[0] + (int64_t)tok * p.sq[1] + head * p.sq[2]) * 2 + g * (D / 2);
+#pragma unroll
+    for (int j = 0; j < KSTEPS; ++j) qreg[mt][j] = gload16(qr + 16 * j);
+    Lrow[mt] = p.KV - 1;
+    if (!p.uniform) {
+      const int Lraw = gload_i32(p.L + b * p.sL_b + tok);
+      Lrow[mt] = live ? Lraw : -1;
+      Lmax = max(Lmax, Lrow[mt]);
+      Lmin = min(Lmin, live ? Lraw : INT_MAX);
+    }
+  }
+  // the steps that a row sees
+  int t1 = min(T, t0 + p.steps);
+  if (!p.uniform) {
+    Lmax = wave_reduce_i32<true>(Lmax);
+    Lmin = wave_reduce_i32<false>(Lmin);
+    t1 = min(t1, Lmax >= s1 ? slab + (Lmax - s1) / ROWS_N + 1 : min(slab, Lmax >= 0 ? Lmax / ROWS_N + 1 : 0));
   }
 
   const char* const kcb = p.k_codes + b * p.skc[0] + h * p.skc[2];
@@ -132,20 +177,12 @@ __global__ void __launch_bounds__(ROWS_THREADS, D <= 128 ? 2 : 1) mx_rows_kernel
   const char* const vnb = p.v_new + (b * p.svn[0] + h * p.svn[2]) * 2;
   const int kcs = (int)p.skc[1], vcs = (int)p.svc[1], kss = (int)p.sks[1], vss = (int)p.svs[1];
   const int kns = (int)(p.skn[1] * 2), vns = (int)(p.svn[1] * 2);
-  const int s1 = p.P;  // absolute index of the first fresh key
 
-  // steps: the slab's, then the fresh keys'; this slice's, dealt to the waves in turn
-  const int run0 = Lmax >= 0 ? min(cdiv_i(Pc, ROWS_N), Lmax / ROWS_N + 1) : 0;
-  const int run1 = Lmax >= s1 ? min(cdiv_i(p.SN, ROWS_N), (Lmax - s1) / ROWS_N + 1) : 0;
-  const int T = run0 + run1;
-  const int t0 = (int)((int64_t)T * slice / p.nsplit);
-  const int t1 = (int)((int64_t)T * (slice + 1) / p.nsplit);
-
-  // a step's codes of this lane's key (l32) and half row (hf), and its scale bytes
+  // a step's codes of this lane's two keys (l16 and l16 + 16) and quarter row
+  // (g), and their scale bytes
   struct Step {
-    unsigned kc[WORDS], vc[WORDS];
-    unsigned ks, vs;
-    unsigned valid;
+    unsigned kc[2][WORDS], vc[2][WORDS];
+    unsigned ks[2], vs[2], valid[2];
   };
   auto rows_bytes = [](int n_in, int stride, int bytes) {
     const int n = min(n_in, ROWS_N);
@@ -159,24 +196,25 @@ __global__ void __launch_bounds__(ROWS_THREADS, D <= 128 ? 2 : 1) mx_rows_kernel
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[4 * i + e] = v[e];
       }
-    } else {
+    } else if constexpr (WORDS == 2) {
       const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, 0));
       w[0] = v[0];
       w[1] = v[1];
+    } else {
+      w[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
     }
   };
   auto load_scales = [&](const __amdgpu_buffer_rsrc_t rs, uint32_t row) -> unsigned {
-    if constexpr (NB == 4) return __builtin_amdgcn_raw_buffer_load_b32(rs, row + 4 * hf, 0, 0);
-    if constexpr (NB == 2) return __builtin_amdgcn_raw_buffer_load_b16(rs, row + 2 * hf, 0, 0);
-    return __builtin_amdgcn_raw_buffer_load_b8(rs, row + (D == 32 ? 0 : hf), 0, 0);
+    if constexpr (NB == 2) return __builtin_amdgcn_raw_buffer_load_b16(rs, row + 2 * g, 0, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b8(rs, row + g * (D / 4) / 32, 0, 0);
   };
-  auto load_valid = [&](int kv0, int n_in) -> unsigned {
+  auto load_valid = [&](int kv0, int n_in, unsigned (&valid)[2]) {
     if constexpr (KV) {
       const auto rs = make_rsrc(reinterpret_cast<const char*>(p.key_valid) + b * p.svalid_b + kv0,
                                 __builtin_amdgcn_readfirstlane(min(n_in, ROWS_N)));
-      return __builtin_amdgcn_raw_buffer_load_b8(rs, (uint32_t)l32, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) valid[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, (uint32_t)(l16 + 16 * i), 0, 0);
     }
-    return 1u;
   };
   auto load_step = [&](int t, Step& s) {
     const int row0 = t * ROWS_N, n_in = Pc - row0;
@@ -184,276 +222,295 @@ __global__ void __launch_bounds__(ROWS_THREADS, D <= 128 ? 2 : 1) mx_rows_kernel
     const auto rv = make_rsrc(vcb + (int64_t)row0 * vcs, rows_bytes(n_in, vcs, D / 2));
     const auto rks = make_rsrc(ksb + (int64_t)row0 * kss, rows_bytes(n_in, kss, D / 32));
     const auto rvs = make_rsrc(vsb + (int64_t)row0 * vss, rows_bytes(n_in, vss, D / 32));
-    load_words(s.kc, rk, (uint32_t)(l32 * kcs + hf * (D / 4)));
-    s.ks = load_scales(rks, (uint32_t)(l32 * kss));
-    load_words(s.vc, rv, (uint32_t)(l32 * vcs + hf * (D / 4)));
-    s.vs = load_scales(rvs, (uint32_t)(l32 * vss));
-    s.valid = load_valid(row0, n_in);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      load_words(s.kc[i], rk, (uint32_t)((l16 + 16 * i) * kcs + g * (D / 8)));
+      s.ks[i] = load_scales(rks, (uint32_t)((l16 + 16 * i) * kss));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      load_words(s.vc[i], rv, (uint32_t)((l16 + 16 * i) * vcs + g * (D / 8)));
+      s.vs[i] = load_scales(rvs, (uint32_t)((l16 + 16 * i) * vss));
+    }
+    load_valid(row0, n_in, s.valid);
   };
   // 2^(byte - 127) of word j's block
   auto scale_of = [](unsigned bytes, int j) { return __uint_as_float(((bytes >> (8 * (j / 4))) & 0xffu) << 23); };
 
-  float m_run = -INFINITY, l_run = 0.0f;
-  f32x16 oacc[DBLK];
+  float m_run[MT], l_run[MT];
+  f32x4 oacc[MT][DBLK];
 #pragma unroll
-  for (int db = 0; db < DBLK; ++db) oacc[db] = f32x16{};
-
-  const int j16 = lane & 15;
-  const int rq = 4 * hf + (j16 >> 2);
-  const int colq = 16 * ((lane >> 4) & 1) + 4 * (j16 & 3);
-  int voffs[2][DBLK];
+  for (int mt = 0; mt < MT; ++mt) {
+    m_run[mt] = -INFINITY;
+    l_run[mt] = 0.0f;
 #pragma unroll
-  for (int db = 0; db < DBLK; ++db) {
-    const int col = db * 32 + colq;
-    voffs[0][db] = rq * ROWB + (((col >> 3) ^ swz<CH>(rq)) << 4) + ((col & 7) << 1);
-    voffs[1][db] = (rq + 8) * ROWB + (((col >> 3) ^ swz<CH>(rq + 8)) << 4) + ((col & 7) << 1);
+    for (int db = 0; db < DBLK; ++db) oacc[mt][db] = f32x4{};
   }
-  auto put_v = [&](int j, u32x4 v) {
-    *reinterpret_cast<u32x4*>(vS + l32 * ROWB + (((hf * WORDS + j) ^ swz<CH>(l32)) << 4)) = v;
+
+  // V^T operand: the transpose read gives lane l16 column 16 db + l16 of four
+  // rows; rows 4g .. 4g + 3 and the same 16 on, whose chunks swz leaves at the
+  // same places
+  const int rq = 4 * g + (l16 >> 2);
+  int voffs[DBLK];
+#pragma unroll
+  for (int db = 0; db < DBLK; ++db)
+    voffs[db] = rq * ROWB + (((2 * db + ((l16 & 3) >> 1)) ^ swz<CH>(rq)) << 4) + 8 * (l16 & 1);
+  auto put_v = [&](int i, int j, u32x4 v) {
+    const int key = l16 + 16 * i;
+    *reinterpret_cast<u32x4*>(vS + key * ROWB + (((g * WORDS + j) ^ swz<CH>(key)) << 4)) = v;
   };
 
-  // softmax and PV of one step: sa holds S^T (lane: row l32, keys 8(i/4) + 4hf
-  // + i%4), the wave's LDS its V
-  auto finish_step = [&](f32x16& sa, int kv0, int n_in, unsigned valid) {
+  // softmax and PV of one step: sa holds S^T (lane: row l16, keys 16s + 4g + i),
+  // the wave's LDS its V
+  auto finish_step = [&](f32x4 (&sa)[MT][2], int kv0, int n_in, const unsigned (&valid)[2]) {
     [[maybe_unused]] unsigned vm = ~0u;
-    if constexpr (KV) vm = (unsigned)__ballot(valid != 0u);
-    if (!(n_in >= ROWS_N && kv0 + ROWS_N - 1 <= Lmin && (!KV || vm == ~0u))) {
-      const int lim = min(Lrow - kv0, n_in - 1) - 4 * hf;
-      const unsigned mine = vm >> (4 * hf);
+    if constexpr (KV) vm = ((unsigned)__ballot(valid[0] != 0u) & 0xffffu) | ((unsigned)__ballot(valid[1] != 0u) << 16);
+    const bool masked = !(n_in >= ROWS_N && kv0 + ROWS_N - 1 <= Lmin && (!KV || vm == ~0u));
+    u32x4 pb[MT];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int na = 8 * (i >> 2) + (i & 3);
-        bool ok = na <= lim;
-        if constexpr (KV) ok = ok && ((mine >> na) & 1u) != 0;
-        sa[i] = ok ? sa[i] : -INFINITY;
+    for (int mt = 0; mt < MT; ++mt) {
+      if (masked) {
+        const int lim = min(Lrow[mt] - kv0, n_in - 1) - 4 * g;
+        const unsigned mine = vm >> (4 * g);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            bool ok = 16 * s + i <= lim;
+            if constexpr (KV) ok = ok && ((mine >> (16 * s + i)) & 1u) != 0;
+            sa[mt][s][i] = ok ? sa[mt][s][i] : -INFINITY;
+          }
       }
+      float mx = sa[mt][0][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sa[mt][e / 4][e % 4]);
+      mx = quad_max(mx) * p.qk_scale;
+      if (__any(mx > m_run[mt] + TAU)) {
+        const float m_new = fmaxf(m_run[mt], mx);
+        const float alpha = (m_new == -INFINITY) ? 1.0f : __builtin_amdgcn_exp2f(m_run[mt] - m_new);
+        l_run[mt] *= alpha;
+#pragma unroll
+        for (int db = 0; db < DBLK; ++db)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) oacc[mt][db][i] *= alpha;
+        m_run[mt] = m_new;
+      }
+      const float m_safe = (m_run[mt] == -INFINITY) ? 0.0f : m_run[mt];
+      float rs = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sa[mt][e / 4][e % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(sa[mt][e / 4][e % 4], p.qk_scale, -m_safe));
+        rs += sa[mt][e / 4][e % 4];
+      }
+      l_run[mt] += rs;
+      pb[mt] = u32x4{pack2<FP16>(sa[mt][0][0], sa[mt][0][1]), pack2<FP16>(sa[mt][0][2], sa[mt][0][3]),
+                     pack2<FP16>(sa[mt][1][0], sa[mt][1][1]), pack2<FP16>(sa[mt][1][2], sa[mt][1][3])};
     }
-    float mx = sa[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sa[i]);
-    mx = pair_max(mx) * p.qk_scale;
-    if (__any(mx > m_run + TAU)) {
-      const float m_new = fmaxf(m_run, mx);
-      const float alpha = (m_new == -INFINITY) ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-      l_run *= alpha;
-#pragma unroll
-      for (int db = 0; db < DBLK; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) oacc[db][i] *= alpha;
-      m_run = m_new;
-    }
-    const float m_safe = (m_run == -INFINITY) ? 0.0f : m_run;
-    float rs = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      sa[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sa[i], p.qk_scale, -m_safe));
-      rs += sa[i];
-    }
-    l_run += rs;
     // the wave's own LDS stores are done in order before its reads; the empty
     // asm keeps the compiler from moving either across
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      u32x4 pb;
-      pb.x = pack2<FP16>(sa[8 * s + 0], sa[8 * s + 1]);
-      pb.y = pack2<FP16>(sa[8 * s + 2], sa[8 * s + 3]);
-      pb.z = pack2<FP16>(sa[8 * s + 4], sa[8 * s + 5]);
-      pb.w = pack2<FP16>(sa[8 * s + 6], sa[8 * s + 7]);
+    for (int db = 0; db < DBLK; ++db) {
+      const u32x2 w0 = __builtin_bit_cast(u32x2, lds_read_tr16(vS + voffs[db]));
+      const u32x2 w1 = __builtin_bit_cast(u32x2, lds_read_tr16(vS + voffs[db] + 16 * ROWB));
 #pragma unroll
-      for (int db = 0; db < DBLK; ++db) {
-        const u32x2 w0 = __builtin_bit_cast(u32x2, lds_read_tr16(vS + voffs[0][db] + 16 * s * ROWB));
-        const u32x2 w1 = __builtin_bit_cast(u32x2, lds_read_tr16(vS + voffs[1][db] + 16 * s * ROWB));
-        oacc[db] = mfma32<FP16>(u32x4{w0.x, w0.y, w1.x, w1.y}, pb, oacc[db]);
-      }
+      for (int mt = 0; mt < MT; ++mt)
+        oacc[mt][db] = mfma16<FP16>(u32x4{w0.x, w0.y, w1.x, w1.y}, pb[mt], oacc[mt][db]);
     }
     asm volatile("" ::: "memory");
   };
 
-  // ---- the slab's steps
-  const int e0 = min(t1, run0);
+  Step cur = {};
   int t = t0 + wave;
-  Step next;
-  if (t < e0) load_step(t, next);
-  for (; t < e0; t += ROWS_WAVES) {
-    const Step cur = next;
-    if (t + ROWS_WAVES < e0) load_step(t + ROWS_WAVES, next);
-    const int n_in = Pc - t * ROWS_N;
-    f32x16 sa = f32x16{};
-#pragma unroll
-    for (int j = 0; j < KSTEPS; ++j) sa = mfma32<FP16>(dequant_fp4x8<FP16>(cur.kc[j], scale_of(cur.ks, j)), qreg[j], sa);
-    const bool on = !KV || cur.valid != 0u;  // a hidden key's V counts as zeros, whatever it held
-#pragma unroll
-    for (int j = 0; j < WORDS; ++j) put_v(j, dequant_fp4x8<FP16>(on ? cur.vc[j] : 0u, on ? scale_of(cur.vs, j) : 1.0f));
-    finish_step(sa, t * ROWS_N, n_in, cur.valid);
-  }
-  // ---- the fresh keys'
+  if (t < min(t1, slab)) load_step(t, cur);
   for (; t < t1; t += ROWS_WAVES) {
-    const int row0 = (t - run0) * ROWS_N, n_in = p.SN - row0;
-    const auto rk = make_rsrc(knb + (int64_t)row0 * kns, rows_bytes(n_in, kns, ROWB));
-    const auto rv = make_rsrc(vnb + (int64_t)row0 * vns, rows_bytes(n_in, vns, ROWB));
-    const unsigned valid = load_valid(s1 + row0, n_in);
-    f32x16 sa = f32x16{};
-    u32x4 kw[KSTEPS];
+    f32x4 sa[MT][2];
+    int kv0 = t * ROWS_N, n_in = Pc - kv0;
+    unsigned valid[2] = {cur.valid[0], cur.valid[1]};
+    if (t < slab) {
 #pragma unroll
-    for (int j = 0; j < KSTEPS; ++j)
-      kw[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, (uint32_t)(l32 * kns + hf * D + 16 * j), 0, 0));
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < KSTEPS; ++j) sa = mfma32<FP16>(kw[j], qreg[j], sa);
-    const bool on = !KV || valid != 0u;
+        for (int j = 0; j < KSTEPS; ++j) {
+          const u32x4 kw = dequant_fp4x8<FP16>(cur.kc[i][j], scale_of(cur.ks[i], j));
 #pragma unroll
-    for (int j = 0; j < KSTEPS; ++j) {
-      const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, (uint32_t)(l32 * vns + hf * D + 16 * j), 0, 0));
-      put_v(j, on ? w : u32x4{0u, 0u, 0u, 0u});
+          for (int mt = 0; mt < MT; ++mt) sa[mt][i] = mfma16<FP16>(kw, qreg[mt][j], j == 0 ? f32x4{} : sa[mt][i]);
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool on = !KV || valid[i] != 0u;  // a hidden key's V counts as zeros, whatever it held
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j)
+          put_v(i, j, dequant_fp4x8<FP16>(on ? cur.vc[i][j] : 0u, on ? scale_of(cur.vs[i], j) : 1.0f));
+      }
+      if (t + ROWS_WAVES < min(t1, slab)) load_step(t + ROWS_WAVES, cur);
+    } else {
+      // fresh keys
+      const int row0 = (t - slab) * ROWS_N;
+      kv0 = s1 + row0;
+      n_in = p.SN - row0;
+      const auto rk = make_rsrc(knb + (int64_t)row0 * kns, rows_bytes(n_in, kns, ROWB));
+      const auto rv = make_rsrc(vnb + (int64_t)row0 * vns, rows_bytes(n_in, vns, ROWB));
+      load_valid(kv0, n_in, valid);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < KSTEPS; ++j) {
+          const u32x4 kw = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                         rk, (uint32_t)((l16 + 16 * i) * kns + g * (D / 2) + 16 * j), 0, 0));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) sa[mt][i] = mfma16<FP16>(kw, qreg[mt][j], j == 0 ? f32x4{} : sa[mt][i]);
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool on = !KV || valid[i] != 0u;
+#pragma unroll
+        for (int j = 0; j < KSTEPS; ++j) {
+          const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                        rv, (uint32_t)((l16 + 16 * i) * vns + g * (D / 2) + 16 * j), 0, 0));
+          put_v(i, j, on ? w : u32x4{0u, 0u, 0u, 0u});
+        }
+      }
     }
-    finish_step(sa, s1 + row0, n_in, valid);
+    finish_step(sa, kv0, n_in, valid);
   }
 
-  // ---- the waves' states become the slice's: m and l through LDS, then O in
-  // halves of the head dim, each wave's rows in its own LDS, added in wave order
-  const float l_tot = pair_sum(l_run);
-  if (hf == 0) {
-    sm[wave][l32] = m_run;
-    sl[wave][l32] = l_tot;
-  }
+  // ---- the waves' states become the piece's: m through LDS, then O tile by
+  // tile and l, scaled to the rows' largest m, each wave's in its own LDS, and
+  // added in wave order
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+    if (g == 0) sm[wave][mt * ROWS_M + l16] = m_run[mt];
   __syncthreads();
-  float M = sm[0][l32];
-#pragma unroll
-  for (int w = 1; w < ROWS_WAVES; ++w) M = fmaxf(M, sm[w][l32]);
-  const float a = (m_run == -INFINITY) ? 0.0f : __builtin_amdgcn_exp2f(m_run - M);
-  // l of the slice's row r, and of its reference point
-  auto row_l = [&](int r, float* mrow) {
-    float mm = sm[0][r], ll = 0.0f;
-#pragma unroll
-    for (int w = 1; w < ROWS_WAVES; ++w) mm = fmaxf(mm, sm[w][r]);
-#pragma unroll
-    for (int w = 0; w < ROWS_WAVES; ++w)
-      ll += sl[w][r] * (sm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][r] - mm));
-    *mrow = mm;
-    return ll;
-  };
   // 1 / l, 0 for a row without keys, NaN for a NaN
   auto inverse = [](float l) {
     const bool pos = l > 0.0f;
     return (1.0f / (pos ? l : 1.0f)) * (pos ? 1.0f : l - l);
   };
-  auto out_row = [&](int r) {
-    const int mm = rt * ROWS_M + r;
-    const int tk = (int)((unsigned)mm / (unsigned)p.G);
-    const int hd = h * p.G + (mm - tk * p.G);
-    return p.out + (b * p.so[0] + (int64_t)tk * p.so[1] + hd * p.so[2]) * 2;
-  };
-  constexpr int DH = DBLK > 1 ? DBLK / 2 : 1;  // blocks of a pass
-  constexpr int C4 = DH * 8;                   // four-element pieces of a row in a pass
+  constexpr int C4 = D / 4;                    // four-element pieces of a row
   constexpr int SC1 = 16;                      // cache policy: device scope
-  const int item = rt * (per / p.nsplit) + bh;
-  const int slot = rows_slot<D>(p.prow) * 4;   // bytes of a slice
-  const bool whole = p.nsplit == 1;
-  // the item's slots (less than 2^31 bytes: rows_max_splits)
-  const auto slots = make_rsrc(reinterpret_cast<const char*>(p.part) + (int64_t)item * p.nsplit * slot, whole ? 0 : p.nsplit * slot);
+  // the output of piece c of the item's row r
+  auto put_out = [&](int r, int c, f32x4 v, float l) {
+    const float inv = inverse(l);
+    const int m = row_first + r;
+    const int tok = quotient(m, p.by_G);
+    const int head = h * p.G + (m - tok * p.G);
+    gstore8(p.out + (b * p.so[0] + (int64_t)tok * p.so[1] + head * p.so[2]) * 2 + c * 8,
+            u32x2{pack2<FP16>(v[0] * inv, v[1] * inv), pack2<FP16>(v[2] * inv, v[3] * inv)});
+  };
+  const int item = b * (int)gridDim.y + hr;
+  const int slot = rows_slot(D, 1 << p.row_bits);  // bytes of a piece
+  const int ml_at = (D * 4) << p.row_bits;         // of its (m, l)
+  // the item's pieces (gridDim.x at most, less than 2^31 bytes)
+  const auto slots = make_rsrc(reinterpret_cast<const char*>(p.part) + (int64_t)item * (int)gridDim.x * slot,
+                               pieces == 1 ? 0 : pieces * slot);
+  const uint32_t mine = (uint32_t)((int)blockIdx.x * slot);
+  auto piece_at = [](int r, int c) { return r * (D * 4) + ((c ^ (r & (C4 - 1) & 15)) << 4); };
 #pragma unroll
-  for (int d0 = 0; d0 < DBLK; d0 += DH) {
-    if (l32 < rows) {
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r0 = mt * ROWS_M;
+    float M = sm[0][r0 + l16];
 #pragma unroll
-      for (int db = 0; db < DH; ++db)
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const int c = db * 8 + 2 * q4 + hf;  // d = 4c .. 4c + 3 of the pass
-          const f32x16& o = oacc[d0 + db];
-          *reinterpret_cast<f32x4*>(vS + l32 * (C4 * 16) + ((c ^ (l32 & (C4 - 1))) << 4)) =
-              f32x4{o[4 * q4] * a, o[4 * q4 + 1] * a, o[4 * q4 + 2] * a, o[4 * q4 + 3] * a};
-        }
+    for (int w = 1; w < ROWS_WAVES; ++w) M = fmaxf(M, sm[w][r0 + l16]);
+    const float a = (m_run[mt] == -INFINITY) ? 0.0f : __builtin_amdgcn_exp2f(m_run[mt] - M);
+    const float l_tot = quad_sum(l_run[mt]) * a;
+    if (g == 0) {
+      sl[wave][r0 + l16] = l_tot;
+      if (wave == 0) smax[r0 + l16] = M;
     }
-    __syncthreads();
-    for (int i = tid; i < rows * C4; i += ROWS_THREADS) {
-      const int r = i / C4, c = i % C4;
-      f32x4 v = f32x4{};
+    if (r0 + l16 < rows) {
 #pragma unroll
-      for (int w = 0; w < ROWS_WAVES; ++w)
-        v += *reinterpret_cast<const f32x4*>(reinterpret_cast<char*>(lds) + w * WLDS + r * (C4 * 16) + ((c ^ (r & (C4 - 1))) << 4));
-      const int d = d0 * 32 + 4 * c;
-      if (whole) {
-        float mr;
-        const float inv = inverse(row_l(r, &mr));
-        gstore8(out_row(r) + d * 2, u32x2{pack2<FP16>(v[0] * inv, v[1] * inv), pack2<FP16>(v[2] * inv, v[3] * inv)});
-      } else {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), slots, (uint32_t)(slice * slot + (r * D + d) * 4), 0, SC1);
+      for (int db = 0; db < DBLK; ++db) {
+        const f32x4 o = oacc[mt][db];
+        *reinterpret_cast<f32x4*>(vS + piece_at(l16, 4 * db + g)) = f32x4{o[0] * a, o[1] * a, o[2] * a, o[3] * a};
       }
     }
     __syncthreads();
+    for (int i = tid; i < min(rows - r0, ROWS_M) * C4; i += ROWS_THREADS) {
+      const int r = i / C4, c = i % C4;
+      f32x4 v = f32x4{};
+      float l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < ROWS_WAVES; ++w) {
+        v += *reinterpret_cast<const f32x4*>(reinterpret_cast<char*>(lds) + w * WLDS + piece_at(r, c));
+        l += sl[w][r0 + r];
+      }
+      if (pieces == 1) {
+        put_out(r0 + r, c, v, l);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), slots, mine + (uint32_t)((r0 * C4 + i) * 16), 0, SC1);
+        if (c == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{smax[r0 + r], l}), slots,
+                                                mine + (uint32_t)(ml_at + (r0 + r) * 8), 0, SC1);
+      }
+    }
+    if (mt + 1 < MT) __syncthreads();
   }
-  if (whole) return;
-  if (tid < rows) {
-    float mr;
-    const float lr = row_l(tid, &mr);
-    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{mr, lr}), slots,
-                                          (uint32_t)(slice * slot + (p.prow * D + 2 * tid) * 4), 0, SC1);
-  }
+  if (pieces == 1) return;
 
-  // ---- the last slice of the item to arrive combines them.  Ordering at
+  // ---- the last piece of the item to arrive combines them.  Ordering at
   // device scope as in qik_attn_kernel.h: the stores above write through and
   // are complete (vmcnt 0, every wave, then the barrier) before the arrival;
   // the slots are read with device-scope loads issued after it.
   __builtin_amdgcn_s_waitcnt(0x0F70);
   __syncthreads();
   if (tid == 0) {
-    const bool last = g_fetch_add(p.ctl + item, 1u) == (unsigned)p.nsplit - 1u;
+    const bool last = g_fetch_add(p.ctl + item, 1u) == (unsigned)pieces - 1u;
     if (last) g_store(p.ctl + item, 0u);
     slast = last ? 1 : 0;
   }
   __syncthreads();
   if (slast == 0) return;
 
-  f32x2* const ml = reinterpret_cast<f32x2*>(lds);  // [nsplit][rows]: (m, l), then (weight, -)
-  f32x4* const sums = reinterpret_cast<f32x4*>(reinterpret_cast<char*>(lds) + ROWS_WAVES * WLDS - 16 * ROWS_THREADS);
-  for (int i = tid; i < p.nsplit * rows; i += ROWS_THREADS) {
-    const int s = i / rows, r = i - s * rows;
-    ml[i] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(slots, (uint32_t)(s * slot + (p.prow * D + 2 * r) * 4), 0, SC1));
-  }
-  __syncthreads();
-  if (tid < rows) {
-    float mm = -INFINITY, ll = 0.0f;
-    for (int s = 0; s < p.nsplit; ++s) mm = fmaxf(mm, ml[s * rows + tid][0]);
-    for (int s = 0; s < p.nsplit; ++s) {
-      const f32x2 x = ml[s * rows + tid];
-      const float w = x[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[0] - mm);
-      ll = __builtin_fmaf(x[1], w, ll);
-      ml[s * rows + tid] = f32x2{w, 0.0f};
-    }
-    sm[0][tid] = inverse(ll);
-  }
-  __syncthreads();
-  // one thread per four elements of a row; where they are fewer than the
-  // threads, groups of threads take every ng-th slice each, and their sums are
-  // added in group order
-  const int n4 = rows * (D / 4);
-  const int ng = max(ROWS_THREADS / n4, 1);
-  for (int i = tid; i < n4 * ng; i += ROWS_THREADS) {
-    const int g = i / n4, at = i - g * n4;
-    const int r = at / (D / 4), c = at % (D / 4);
-    f32x4 v = f32x4{};
-#pragma unroll 8
-    for (int s = g; s < p.nsplit; s += ng) {
-      const f32x4 x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(slots, (uint32_t)(s * slot + (r * D + 4 * c) * 4), 0, SC1));
-      const float w = ml[s * rows + r][0];
+  // A thread takes four elements of a row; where those are fewer than the
+  // threads, groups of threads take every ng-th piece each.  Every one runs the
+  // online softmax over its pieces (no pass over the m first, and the loads all
+  // at once), and the groups' states are combined in group order.
+  struct State {
+    f32x4 v;
+    float m, l;
+  };
+  static_assert(sizeof(State) * ROWS_THREADS <= sizeof(lds), "the groups' states fit");
+  auto add = [](State& s, f32x4 v, float m, float l) {
+    const float mm = fmaxf(s.m, m);
+    const float a = s.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s.m - mm);
+    const float x = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mm);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(x[e], w, v[e]);
+    for (int e = 0; e < 4; ++e) s.v[e] = __builtin_fmaf(v[e], x, s.v[e] * a);
+    s.l = __builtin_fmaf(l, x, s.l * a);
+    s.m = mm;
+  };
+  float* const states = reinterpret_cast<float*>(lds);  // [6][threads]
+  const int n4_bits = __builtin_ctz(C4) + p.row_bits;   // log2 of the item's four-element pieces
+  const int ng = max(ROWS_THREADS >> n4_bits, 1);
+  for (int i = tid; i < (ng << n4_bits); i += ROWS_THREADS) {
+    const int at = i & ((1 << n4_bits) - 1);
+    State s = {f32x4{}, -INFINITY, 0.0f};
+#pragma unroll 8
+    for (int n = i >> n4_bits; n < pieces; n += ng) {
+      const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(slots, (uint32_t)(n * slot + at * 16), 0, SC1));
+      const f32x2 ml = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(slots, (uint32_t)(n * slot + ml_at + at / C4 * 8), 0, SC1));
+      add(s, v, ml[0], ml[1]);
     }
-    if (ng > 1) {
-      sums[i] = v;
+    if (ng == 1) {
+      if (at / C4 < rows) put_out(at / C4, at % C4, s.v, s.l);
       continue;
     }
-    const float inv = sm[0][r];
-    gstore8(out_row(r) + c * 8, u32x2{pack2<FP16>(v[0] * inv, v[1] * inv), pack2<FP16>(v[2] * inv, v[3] * inv)});
+#pragma unroll
+    for (int e = 0; e < 4; ++e) states[e * ROWS_THREADS + i] = s.v[e];
+    states[4 * ROWS_THREADS + i] = s.m;
+    states[5 * ROWS_THREADS + i] = s.l;
   }
   if (ng == 1) return;
   __syncthreads();
-  for (int i = tid; i < n4; i += ROWS_THREADS) {
-    const int r = i / (D / 4), c = i % (D / 4);
-    f32x4 v = sums[i];
-    for (int g = 1; g < ng; ++g) v += sums[g * n4 + i];
-    const float inv = sm[0][r];
-    gstore8(out_row(r) + c * 8, u32x2{pack2<FP16>(v[0] * inv, v[1] * inv), pack2<FP16>(v[2] * inv, v[3] * inv)});
+  if (tid < (1 << n4_bits) && tid / C4 < rows) {
+    State s = {f32x4{}, -INFINITY, 0.0f};
+#pragma unroll 1
+    for (int n = 0; n < ng; ++n) {
+      const float* x = states + (n << n4_bits) + tid;
+      add(s, f32x4{x[0], x[ROWS_THREADS], x[2 * ROWS_THREADS], x[3 * ROWS_THREADS]}, x[4 * ROWS_THREADS], x[5 * ROWS_THREADS]);
+    }
+    put_out(tid / C4, tid % C4, s.v, s.l);
   }
 }
 
