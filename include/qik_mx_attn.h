@@ -112,10 +112,11 @@ int qik_mx_attn_workspace_size(const qik_mx_attn_args* args, int64_t* bytes);
 int qik_mx_attn_fwd(const qik_mx_attn_args* args, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Host only: which kernel a call of this shape takes on a device of `cus`
- * compute units.  few: 1 for the kernel of few rows; row_tiles: 16-row tiles of
- * each (b, KV head)'s rows there; pieces: workgroups that share its keys. */
-int qik_mx_attn_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, int32_t cus,
-                     int32_t* few, int32_t* row_tiles, int32_t* pieces);
+ * compute units, with lengths (`ragged`) or without.  few: 1 for the kernel of few
+ * rows; row_tiles: 16-row tiles of each (b, KV head)'s rows there; pieces:
+ * workgroups that share its keys. */
+int qik_mx_attn_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D,
+                     int32_t ragged, int32_t cus, int32_t* few, int32_t* row_tiles, int32_t* pieces);
 
 #ifdef __cplusplus
 }

@@ -476,7 +476,7 @@ MX_ATTN_EXPORTS = (
      (ctypes.POINTER(QikMxAttnArgs), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p)),
     ("qik_mx_attn_plan", ctypes.c_int,
      (ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
-      ctypes.c_int32, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32))),
+      ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32))),
 )
 
 # of qik_rope.h

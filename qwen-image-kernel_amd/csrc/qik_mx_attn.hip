@@ -241,50 +241,55 @@ struct RowsPlan {
   int row_bits;  // log2 of the rows a piece keeps in the workspace
 };
 
-// What a call lasts, in us, from measurements at D = 128 on 256 CUs (P 1000 to
-// 131072, 64 to 2048 rows of 1 to 24 KV heads).  Of the kernel of few rows: a
-// wave's step takes 1.4 us with two tiles and eight waves on a CU, 1.9 with one
-// and sixteen; a piece 4 beside its steps; the merge 2, and 1 more for 100 KB of
-// pieces, which one workgroup reads.  Of the other: 10 and its KV tiles, which
-// run no faster than a row block's on as many CUs as it can be split over.
-double rows_cost(const RowsPlan& r, int64_t items, int64_t T, int64_t pieces, int64_t slots, int waves, int64_t D) {
-  const double step = r.mt == 1 ? 1.9 : 1.4;
-  const double merge = pieces > 1 ? 2.0 + (double)pieces * (4 << r.row_bits) * (double)D * 1e-5 : 0.0;
-  return (double)cdiv64(items * pieces, slots) * (step * (double)cdiv64(T, pieces * waves) + 4.0) + merge;
+// What a call of two tiles lasts, in us, from measurements at D = 128 on 256 CUs
+// (P 1000 to 30000, 64 to 2048 rows of 1 to 24 KV heads): here a wave's step
+// takes 1.4 us, a piece 4 beside its steps, the merge 2 and 1 more for 100 KB
+// of pieces, which one workgroup reads.  The kernel of many rows takes 10 and its
+// KV tiles, which run no faster than a row block's on the CUs it can be split over.
+double rows_cost(int64_t items, int64_t T, int64_t pieces, int cus, int waves, int64_t D) {
+  const double merge = pieces > 1 ? 2.0 + (double)pieces * (2 * ROWS_M * 4) * (double)D * 1e-5 : 0.0;
+  return (double)cdiv64(items * pieces, cus) * (1.4 * (double)cdiv64(T, pieces * waves) + 4.0) + merge;
 }
 double many_cost(int64_t blocks, int64_t T, int cus) {
   return 10.0 + (double)T * std::max(0.455, 1.23 * (double)blocks / cus);
 }
 
-RowsPlan rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, int cus) {
+RowsPlan rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, bool ragged, int cus) {
   RowsPlan r = {false, 0, 0, 0, 0, 0};
   const int64_t G = H / HKV, R = SQ * G;
   r.mt = R <= ROWS_M ? 1 : 2;
   const int64_t nrt = cdiv64(R, r.mt * ROWS_M);
-  // limits of the kernel: its grid has the entries in z, the heads and row tiles
-  // in y, and it divides by multiplication
-  if (B > 65535 || HKV > 65535 / nrt || G > INT_MAX / R || HKV * nrt > INT_MAX / HKV) return r;
+  // limits of the kernel: its grid has the entries in y and the pieces in z, less
+  // than 2^32 threads in x, and it divides by multiplication
+  if (B > 65535 || HKV * nrt > (1 << 22) || G > INT_MAX / R || HKV * nrt > INT_MAX / HKV) return r;
   r.nrt = (int)nrt;
   cus = std::max(cus, 1);
   const int waves = rows_waves((int)D, r.mt);
-  const int64_t slots = (int64_t)cus * (r.mt == 1 && D <= 128 ? 2 : 1);  // resident workgroups
   const int64_t T = std::max<int64_t>(cdiv64(P, ROWS_N) + cdiv64(SN, ROWS_N), 1);
   const int64_t items = B * HKV * nrt;
   while ((1 << r.row_bits) < std::min<int64_t>(R, r.mt * ROWS_M)) ++r.row_bits;
-  // pieces that fill the slots once, twice ... or none; every wave of a piece has
-  // a step, and an item that is cut a word of the control words
-  const int64_t most = items > QIK_ATTN_WS_CTL_BYTES / 4 ? 1 : std::max<int64_t>(T / waves, 1);
-  int64_t best = 1;
-  double cost = rows_cost(r, items, T, 1, slots, waves, D);
-  for (int64_t k = 1; k <= 4; ++k) {
-    const int64_t n = std::min(std::max<int64_t>(k * slots / items, 1), most);
-    const double c = rows_cost(r, items, T, n, slots, waves, D);
-    if (c < cost) cost = c, best = n;
+  // every wave of a piece has a step, two where there are many pieces; an item
+  // that is cut has a word of the control words
+  const int64_t steps = std::max<int64_t>(T / waves, 1);
+  const int64_t most = items > QIK_ATTN_WS_CTL_BYTES / 4 ? 1 : std::min<int64_t>(std::max<int64_t>(steps / 2, std::min<int64_t>(steps, 8)), 65535);
+  int64_t pieces = 1;
+  if (r.mt == 1) {
+    // bound by the slab's bytes: a workgroup a CU; with lengths two, as they are
+    // P in the longest entry only (131072 keys of 8 heads: 32 pieces 31.6 us, 64
+    // 34.3, 16 44.9; 24 entries of up to 8192: 3 pieces 34.8, 2 40.3, 6 36.6)
+    pieces = std::min(std::max<int64_t>(((ragged ? 2 : 1) * (int64_t)cus + items / 2) / items, 1), most);
+    r.few = true;
+  } else {
+    double cost = rows_cost(items, T, 1, cus, waves, D);
+    for (int64_t k = 1; k <= 4; ++k) {  // pieces that fill the CUs k times
+      const int64_t n = std::min(std::max<int64_t>(k * cus / items, 1), most);
+      const double c = rows_cost(items, T, n, cus, waves, D);
+      if (c < cost) cost = c, pieces = n;
+    }
+    r.few = cost < many_cost(B * HKV * cdiv64(R, BM), cdiv64(P, BN) + cdiv64(SN, BN), cus);
   }
-  r.steps = (int)cdiv64(T, best);
+  r.steps = (int)cdiv64(T, pieces);
   r.pieces = (int)cdiv64(T, r.steps);
-  const int64_t T64 = cdiv64(P, BN) + cdiv64(SN, BN);
-  r.few = r.mt == 1 || cost < many_cost(B * HKV * cdiv64(R, BM), T64, cus);
   return r;
 }
 
@@ -308,7 +313,7 @@ int plan_mx(const qik_mx_attn_args* x, MxLaunch* l) {
   const qik_attn_args& a = x->a;
   l->ws_bytes = 0;
   const int64_t G = a.H / x->HKV;
-  l->rows = rows_plan(a.B, a.SQ, a.SN, a.P, a.H, x->HKV, a.D, device_cus());
+  l->rows = rows_plan(a.B, a.SQ, a.SN, a.P, a.H, x->HKV, a.D, x->lengths != nullptr, device_cus());
   if (l->rows.few) {
     l->ws_bytes = rows_ws_bytes(l->rows, a.B, x->HKV, a.D);
     return QIK_OK;
@@ -538,7 +543,7 @@ int qik_mx_attn_fwd(const qik_mx_attn_args* x, void* ws, int64_t ws_bytes, void*
     r.row_bits = l.rows.row_bits;
     r.qk_scale = qk_scale;
     fn = reinterpret_cast<const void*>(qik::rows_kernel_of(&a, l.rows.mt));
-    grid = dim3((unsigned)l.rows.pieces, (unsigned)(x->HKV * l.rows.nrt), (unsigned)a.B);
+    grid = dim3((unsigned)(x->HKV * l.rows.nrt), (unsigned)a.B, (unsigned)l.rows.pieces);
     threads = 64u * (unsigned)qik::rows_waves((int)a.D, l.rows.mt);
     kargs[0] = &r;
   } else {
@@ -593,12 +598,12 @@ int qik_mx_attn_fwd(const qik_mx_attn_args* x, void* ws, int64_t ws_bytes, void*
   return e == hipSuccess ? QIK_OK : QIK_ERR_LAUNCH;
 }
 
-int qik_mx_attn_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, int32_t cus,
-                     int32_t* few, int32_t* row_tiles, int32_t* pieces) {
+int qik_mx_attn_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D,
+                     int32_t ragged, int32_t cus, int32_t* few, int32_t* row_tiles, int32_t* pieces) {
   if (few == nullptr || row_tiles == nullptr || pieces == nullptr) return QIK_ERR_NULL_ARG;
   if (B < 1 || SQ < 1 || SN < 0 || P < 0 || HKV < 1 || H < HKV || H % HKV != 0 || cus < 1) return QIK_ERR_SHAPE;
   if (D != 32 && D != 64 && D != 128 && D != 256) return QIK_ERR_HEAD_DIM;
-  const qik::RowsPlan r = qik::rows_plan(B, SQ, SN, P, H, HKV, D, cus);
+  const qik::RowsPlan r = qik::rows_plan(B, SQ, SN, P, H, HKV, D, ragged != 0, cus);
   *few = r.few ? 1 : 0;
   *row_tiles = r.mt * r.nrt;
   *pieces = r.pieces;

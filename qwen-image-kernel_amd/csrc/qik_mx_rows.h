@@ -9,7 +9,8 @@
 //     share the KV head times the query positions -- and its keys in steps of
 //     32.  Items are cut into pieces of the same number of steps, one a
 //     workgroup, so that sequences of any lengths fill the device evenly (a
-//     piece behind an item's last key ends at once);
+//     piece behind an item's last key ends at once; the heads come first in the
+//     grid, then the entries, so that those pieces do not fall on the same XCDs);
 //   * a workgroup's waves take its steps in turn, each with its own softmax state
 //     and its own LDS, and never wait for each other before the end;
 //   * a call lasts some microseconds, so that its instructions' way from memory
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(64 * rows_waves(D, MT), D <= 128 && MT == 1 ? 
   char* const vS = reinterpret_cast<char*>(lds) + wave * WLDS;
 
   // ---- the item and its steps [t0, t1): the slab's, then the fresh keys'
-  const int b = (int)blockIdx.z, hr = (int)blockIdx.y;
+  const int b = (int)blockIdx.y, hr = (int)blockIdx.x;
   const int rt = quotient(hr, p.by_HKV);
   const int h = hr - rt * p.HKV;
   const int row_first = rt * ROWS;
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(64 * rows_waves(D, MT), D <= 128 && MT == 1 ? 
     Pc = min(max(*((const __attribute__((address_space(4))) int32_t*)(p.lengths + b)), 0), p.P);
   const int slab = cdiv_i(Pc, ROWS_N);
   const int T = slab + cdiv_i(p.SN, ROWS_N);
-  const int t0 = (int)blockIdx.x * p.steps;
+  const int t0 = (int)blockIdx.z * p.steps;
   if (t0 >= T && t0 > 0) return;
   const int pieces = max((T + p.steps - 1) / p.steps, 1);
   const int s1 = p.P;  // absolute index of the first fresh key
@@ -398,13 +399,13 @@ __global__ void __launch_bounds__(64 * rows_waves(D, MT), D <= 128 && MT == 1 ? 
     gstore8(p.out + (b * p.so[0] + (int64_t)tok * p.so[1] + head * p.so[2]) * 2 + c * 8,
             u32x2{pack2<FP16>(v[0] * inv, v[1] * inv), pack2<FP16>(v[2] * inv, v[3] * inv)});
   };
-  const int item = b * (int)gridDim.y + hr;
+  const int item = b * (int)gridDim.x + hr;
   const int slot = rows_slot(D, 1 << p.row_bits);  // bytes of a piece
   const int ml_at = (D * 4) << p.row_bits;         // of its (m, l)
-  // the item's pieces (gridDim.x at most, less than 2^31 bytes)
-  const auto slots = make_rsrc(reinterpret_cast<const char*>(p.part) + (int64_t)item * (int)gridDim.x * slot,
+  // the item's pieces (gridDim.z at most, less than 2^31 bytes)
+  const auto slots = make_rsrc(reinterpret_cast<const char*>(p.part) + (int64_t)item * (int)gridDim.z * slot,
                                pieces == 1 ? 0 : pieces * slot);
-  const uint32_t mine = (uint32_t)((int)blockIdx.x * slot);
+  const uint32_t mine = (uint32_t)((int)blockIdx.z * slot);
   auto piece_at = [](int r, int c) { return r * (D * 4) + ((c ^ (r & (C4 - 1) & 15)) << 4); };
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
@@ -464,21 +465,16 @@ __global__ void __launch_bounds__(64 * rows_waves(D, MT), D <= 128 && MT == 1 ? 
 
   // A thread takes four elements of a row; where those are fewer than the
   // threads, groups of threads take every ng-th piece each.  Every one runs the
-  // online softmax over its pieces (no pass over the m first, and the loads all
-  // at once), and the groups' states are combined in group order.
+  // online softmax over its pieces (no pass over the m first), and the groups' states are combined in group order.
   struct State {
     f32x4 v;
     float m, l;
   };
   static_assert(sizeof(State) * ROWS_THREADS <= sizeof(lds), "the groups' states fit");
-  auto add = [](State& s, f32x4 v, float m, float l) {
-    const float mm = fmaxf(s.m, m);
-    const float a = s.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s.m - mm);
-    const float x = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mm);
+  auto add = [](State& s, f32x4 v, float l, float x) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s.v[e] = __builtin_fmaf(v[e], x, s.v[e] * a);
-    s.l = __builtin_fmaf(l, x, s.l * a);
-    s.m = mm;
+    for (int e = 0; e < 4; ++e) s.v[e] = __builtin_fmaf(v[e], x, s.v[e]);
+    s.l = __builtin_fmaf(l, x, s.l);
   };
   float* const states = reinterpret_cast<float*>(lds);  // [6][threads]
   const int n4_bits = __builtin_ctz(C4) + p.row_bits;   // log2 of the item's four-element pieces
@@ -486,11 +482,32 @@ __global__ void __launch_bounds__(64 * rows_waves(D, MT), D <= 128 && MT == 1 ? 
   for (int i = tid; i < (ng << n4_bits); i += ROWS_THREADS) {
     const int at = i & ((1 << n4_bits) - 1);
     State s = {f32x4{}, -INFINITY, 0.0f};
-#pragma unroll 8
-    for (int n = i >> n4_bits; n < pieces; n += ng) {
-      const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(slots, (uint32_t)(n * slot + at * 16), 0, SC1));
-      const f32x2 ml = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(slots, (uint32_t)(n * slot + ml_at + at / C4 * 8), 0, SC1));
-      add(s, v, ml[0], ml[1]);
+    // AHEAD pieces at a time (past the last: zeros, which the buffer's end gives,
+    // of weight zero); one after the other they cost their latency each
+    constexpr int AHEAD = 8;
+    for (int n = i >> n4_bits; n < pieces; n += AHEAD * ng) {
+      f32x4 v[AHEAD];
+      f32x2 ml[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const uint32_t off = (uint32_t)((n + k * ng) * slot);
+        v[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(slots, off + (uint32_t)(at * 16), 0, SC1));
+        ml[k] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(slots, off + (uint32_t)(ml_at + at / C4 * 8), 0, SC1));
+      }
+      float m = s.m;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (n + k * ng >= pieces) ml[k][0] = -INFINITY;
+        m = fmaxf(m, ml[k][0]);
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+      const float a = __builtin_amdgcn_exp2f(s.m - ref);  // 0 for -inf, as below
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s.v[e] *= a;
+      s.l *= a;
+      s.m = m;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) add(s, v[k], ml[k][1], __builtin_amdgcn_exp2f(ml[k][0] - ref));
     }
     if (ng == 1) {
       if (at / C4 < rows) put_out(at / C4, at % C4, s.v, s.l);
@@ -504,11 +521,15 @@ __global__ void __launch_bounds__(64 * rows_waves(D, MT), D <= 128 && MT == 1 ? 
   if (ng == 1) return;
   __syncthreads();
   if (tid < (1 << n4_bits) && tid / C4 < rows) {
-    State s = {f32x4{}, -INFINITY, 0.0f};
-#pragma unroll 1
+    const float* const x = states + tid;
+    float m = -INFINITY;
+    for (int n = 0; n < ng; ++n) m = fmaxf(m, x[4 * ROWS_THREADS + (n << n4_bits)]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    State s = {f32x4{}, m, 0.0f};
     for (int n = 0; n < ng; ++n) {
-      const float* x = states + (n << n4_bits) + tid;
-      add(s, f32x4{x[0], x[ROWS_THREADS], x[2 * ROWS_THREADS], x[3 * ROWS_THREADS]}, x[4 * ROWS_THREADS], x[5 * ROWS_THREADS]);
+      const float* y = x + (n << n4_bits);
+      add(s, f32x4{y[0], y[ROWS_THREADS], y[2 * ROWS_THREADS], y[3 * ROWS_THREADS]}, y[5 * ROWS_THREADS],
+          __builtin_amdgcn_exp2f(y[4 * ROWS_THREADS] - ref));
     }
     put_out(tid / C4, tid % C4, s.v, s.l);
   }

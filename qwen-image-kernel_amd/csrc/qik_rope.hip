@@ -1,13 +1,17 @@
 // RMSNorm over each head and the rotation by positions on several axes, of a
 // layer's Q and K in one launch, and its gradient (include/qik_rope.h).
 //
-// A byte mover: every row is read and written once.  What it must not do is
-// take a sine per element: the D / 2 angles of a token are the same for all its
-// heads, in Q and in K.  So rows are numbered token by token, the heads of Q and
-// then those of K; a workgroup takes a run of rows, its threads first issue the
-// loads of all of them, then compute the cosines and sines of the few tokens
-// that the run touches into LDS, and then turn the rows.  D / 8 lanes hold a row,
-// a lane the pairs 4t .. 4t + 3: eight neighbouring elements, or four of each half.
+// A byte mover (every row is read and written once) that computes nearly as long
+// as it moves, so the arithmetic is kept to what a row needs:
+//   * the D / 2 angles of a token are the same for all its heads, in Q and in K: a
+//     workgroup takes some tokens, computes their cosines and sines into LDS, and
+//     turns their rows of Q and then those of K, so that what belongs to a tensor
+//     (addresses, strides, the weight) is one for the whole workgroup.  With rows
+//     of both in a run and a choice for each, 4352 tokens x 48 heads x 128 took
+//     28.0 us;
+//   * D / 8 lanes hold a row, a lane the pairs 4t .. 4t + 3: eight neighbouring
+//     elements, or four of each half.  Sums over a row go by DPP;
+//   * rows are found by multiplications with the host's reciprocals.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -26,7 +30,9 @@ using qik_mx::u32x2;
 using qik_mx::u32x4;
 
 constexpr int THREADS = 256;
-constexpr int UNITS = 4;            // rows of a lane group, their loads issued together
+constexpr int UNITS = 2;            // rows of a lane group, their loads issued together
+constexpr int ROWS_AIM = 96;        // rows of the larger tensor that a workgroup takes at once
+constexpr int TABLE_BYTES = 32768;  // of cosines and sines at most
 // backward: workgroups at most, each with a [2, D] sum of dw in the workspace
 constexpr int BWD_GRID = 512;
 
@@ -35,8 +41,9 @@ struct Tensor {
   const char* dy;
   char* out;                        // y, or dx
   const float* w;
-  int64_t sx[3], so[3], sdy[3];     // b, s, h in bytes
+  unsigned sx[3], so[3], sdy[3];    // b, s, h in 16 bytes
   int H;
+  unsigned by_H;                    // see quotient
   float eps;
 };
 
@@ -47,16 +54,22 @@ struct Params {
   const int32_t* axis;
   int64_t pos_b, pos_a;
   float* part;                      // backward: [grid][2][D]
-  int rows;                         // B * S * (H of both)
-  int S, heads;
-  int runs;                         // runs of rows: workgroups of the forward launch
+  int tokens;                       // B * S
+  int S;
+  unsigned by_S;
+  int chunk;                        // tokens a workgroup takes at once
 };
 
-template <int D>
-constexpr int run_rows() { return THREADS / (D / 8) * UNITS; }
+// n / d by ceil(2^32 / d) (0 for d = 1): exact while n * d < 2^32 (for a larger
+// product the estimate is at most one too large, which the last line takes back)
+__device__ __forceinline__ int quotient(int n, int d, unsigned by) {
+  if (by == 0u) return n;
+  const unsigned q = __umulhi((unsigned)n, by);
+  return (int)(q * (unsigned)d > (unsigned)n ? q - 1u : q);
+}
 
 // the lane's eight elements of a row: pairs 4t .. 4t + 3, in order
-template <int D, bool FP16, bool HALVES>
+template <int D, bool HALVES>
 __device__ __forceinline__ u32x4 load_pairs(const char* row, int t) {
   if constexpr (HALVES) {
     const u32x2 a = *reinterpret_cast<const u32x2*>(row + t * 8);
@@ -86,26 +99,41 @@ constexpr int first_of(int i) { return HALVES ? i : 2 * i; }
 template <bool HALVES>
 constexpr int second_of(int i) { return HALVES ? i + 4 : 2 * i + 1; }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+// the sum over a row's TPR lanes, in each of them: quad_perm {1, 0, 3, 2} and {2, 3,
+// 0, 1}, then mirrors of 8 and 16 lanes (whose halves are equal by then), then
+// the other 16
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v) {
-#pragma unroll
-  for (int k = TPR / 2; k >= 1; k >>= 1) v += __shfl_xor(v, k);
+  v = dpp_add<0xb1>(v);
+  v = dpp_add<0x4e>(v);
+  if constexpr (TPR >= 8) v = dpp_add<0x141>(v);
+  if constexpr (TPR >= 16) v = dpp_add<0x140>(v);
+  if constexpr (TPR >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
   return v;
 }
 
-// a row of the run: its tensor, and where it lies
+// a row: its token's place in the workgroup's table, and where it lies
 struct Row {
-  int which, token, b, s, h;
+  int token, b, s, h;
 };
-__device__ __forceinline__ Row row_of(const Params& p, int row) {
+__device__ __forceinline__ Row row_of(const Params& p, const Tensor& x, int first, int row) {
   Row r;
-  r.token = (int)((unsigned)row / (unsigned)p.heads);
-  const int h = row - r.token * p.heads;
-  r.which = h >= p.t[0].H ? 1 : 0;
-  r.h = r.which ? h - p.t[0].H : h;
-  r.b = (int)((unsigned)r.token / (unsigned)p.S);
-  r.s = r.token - r.b * p.S;
+  r.token = quotient(row, x.H, x.by_H);
+  r.h = row - r.token * x.H;
+  const int token = first + r.token;
+  r.b = quotient(token, p.S, p.by_S);
+  r.s = token - r.b * p.S;
   return r;
+}
+__device__ __forceinline__ int64_t bytes_of(const Row& r, const unsigned (&st)[3]) {
+  return (int64_t)(((uint64_t)(unsigned)r.b * st[0] + (uint64_t)(unsigned)r.s * st[1] + (uint64_t)(unsigned)r.h * st[2]) << 4);
 }
 
 // cosines and sines of the tokens [first, first + n) into cs [n][D / 2]
@@ -113,11 +141,26 @@ template <int D>
 __device__ __forceinline__ void turn_table(const Params& p, int first, int n, float2* cs) {
   for (int i = (int)threadIdx.x; i < n * (D / 2); i += THREADS) {
     const int pair = i % (D / 2), token = first + i / (D / 2);
-    const int b = (int)((unsigned)token / (unsigned)p.S), s = token - b * p.S;
+    const int b = quotient(token, p.S, p.by_S), s = token - b * p.S;
     const double turns = p.pos[b * p.pos_b + p.axis[pair] * p.pos_a + s] * p.freq[pair];
     float sn, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &sn, &c);
     cs[i] = make_float2(c, sn);
+  }
+}
+
+// r of a row from its sum of squares: the instruction's result is within an ulp
+template <int D>
+__device__ __forceinline__ float rsqrt_of(float ss, float eps) {
+  return __builtin_amdgcn_rsqf(__builtin_fmaf(ss, 1.0f / D, eps));
+}
+
+template <int D, bool HALVES>
+__device__ __forceinline__ void load_weight(const float* w, int t, float (&wv)[8]) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const float4 v = *reinterpret_cast<const float4*>(w + element_of<D, HALVES>(t, 4 * q));
+    wv[4 * q] = v.x, wv[4 * q + 1] = v.y, wv[4 * q + 2] = v.z, wv[4 * q + 3] = v.w;
   }
 }
 
@@ -127,48 +170,55 @@ __global__ void __launch_bounds__(THREADS) axial_rope_kernel(const Params p) {
   constexpr int TPR = D / 8, RPB = THREADS / TPR;
   extern __shared__ float2 cs[];
   const int t = (int)threadIdx.x % TPR;
-  const int row0 = (int)blockIdx.x * run_rows<D>() + (int)threadIdx.x / TPR;
-  const int first = (int)((unsigned)((int)blockIdx.x * run_rows<D>()) / (unsigned)p.heads);
-  const int last = (int)((unsigned)min((int)blockIdx.x * run_rows<D>() + run_rows<D>() - 1, p.rows - 1) / (unsigned)p.heads);
-  u32x4 raw[UNITS];
-  Row r[UNITS];
-#pragma unroll
-  for (int u = 0; u < UNITS; ++u) {
-    r[u] = row_of(p, min(row0 + u * RPB, p.rows - 1));
-    const Tensor& x = p.t[r[u].which];
-    raw[u] = load_pairs<D, FP16, HALVES>(x.x + r[u].b * x.sx[0] + r[u].s * x.sx[1] + r[u].h * x.sx[2], t);
-  }
-  turn_table<D>(p, first, last - first + 1, cs);
+  const int first = (int)blockIdx.x * p.chunk;
+  const int n = min(p.chunk, p.tokens - first);
+  turn_table<D>(p, first, n, cs);
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) {
-    float x[8];
-    qik_mx::unpack8<DT>(Raw8<DT>{{raw[u]}}, x);
-    const Tensor& tn = p.t[r[u].which];
+  for (int k = 0; k < 2; ++k) {
+    const Tensor& x = p.t[k];
+    const int rows = n * x.H;
+    [[maybe_unused]] float wv[8];
     if constexpr (NORM) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(x[e], x[e], ss);
-      const float rs = 1.0f / sqrtf(row_sum<TPR>(ss) * (1.0f / D) + tn.eps);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (x[e] * rs) * tn.w[element_of<D, HALVES>(t, e)];
+      if (rows > 0) load_weight<D, HALVES>(x.w, t, wv);
     }
-    float y[8];
+    for (int row0 = (int)threadIdx.x / TPR; row0 < rows; row0 += RPB * UNITS) {
+      u32x4 raw[UNITS];
+      Row r[UNITS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 c = cs[(r[u].token - first) * (D / 2) + 4 * t + i];
-      const float a = x[first_of<HALVES>(i)], b = x[second_of<HALVES>(i)];
-      y[first_of<HALVES>(i)] = a * c.x - b * c.y;
-      y[second_of<HALVES>(i)] = a * c.y + b * c.x;
+      for (int u = 0; u < UNITS; ++u) {
+        r[u] = row_of(p, x, first, min(row0 + u * RPB, rows - 1));
+        raw[u] = load_pairs<D, HALVES>(x.x + bytes_of(r[u], x.sx), t);
+      }
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        float v[8];
+        qik_mx::unpack8<DT>(Raw8<DT>{{raw[u]}}, v);
+        if constexpr (NORM) {
+          float ss = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(v[e], v[e], ss);
+          const float rs = rsqrt_of<D>(row_sum<TPR>(ss), x.eps);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = (v[e] * rs) * wv[e];
+        }
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 c = cs[r[u].token * (D / 2) + 4 * t + i];
+          const float a = v[first_of<HALVES>(i)], b = v[second_of<HALVES>(i)];
+          y[first_of<HALVES>(i)] = a * c.x - b * c.y;
+          y[second_of<HALVES>(i)] = a * c.y + b * c.x;
+        }
+        if (row0 + u * RPB < rows) store_pairs<D, HALVES>(x.out + bytes_of(r[u], x.so), t, qik_mx::pack8<DT>(y).w[0]);
+      }
     }
-    if (row0 + u * RPB < p.rows)
-      store_pairs<D, HALVES>(tn.out + r[u].b * tn.so[0] + r[u].s * tn.so[1] + r[u].h * tn.so[2], t, qik_mx::pack8<DT>(y).w[0]);
   }
 }
 
 // The gradient: as above with dy beside x; a workgroup takes every gridDim.x-th
-// run and keeps its rows' sums of dw in registers, which become one [2, D] sum in
-// the workspace at its end.
+// chunk of tokens and keeps its rows' sums of dw in registers, which become one
+// [2, D] sum in the workspace at its end.
 template <int D, bool FP16, bool HALVES, bool NORM>
 __global__ void __launch_bounds__(THREADS) axial_rope_bwd_kernel(const Params p) {
   constexpr int DT = FP16 ? QIK_DTYPE_FP16 : QIK_DTYPE_BF16;
@@ -176,59 +226,63 @@ __global__ void __launch_bounds__(THREADS) axial_rope_bwd_kernel(const Params p)
   extern __shared__ float2 cs[];
   const int t = (int)threadIdx.x % TPR;
   float dw[2][8] = {};
-  for (int run = (int)blockIdx.x; run < p.runs; run += (int)gridDim.x) {
-    const int base = run * run_rows<D>();
-    const int row0 = base + (int)threadIdx.x / TPR;
-    const int first = (int)((unsigned)base / (unsigned)p.heads);
-    const int last = (int)((unsigned)min(base + run_rows<D>() - 1, p.rows - 1) / (unsigned)p.heads);
-    u32x4 raw[UNITS], gr[UNITS];
-    Row r[UNITS];
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      r[u] = row_of(p, min(row0 + u * RPB, p.rows - 1));
-      const Tensor& x = p.t[r[u].which];
-      gr[u] = load_pairs<D, FP16, HALVES>(x.dy + r[u].b * x.sdy[0] + r[u].s * x.sdy[1] + r[u].h * x.sdy[2], t);
-      if constexpr (NORM) raw[u] = load_pairs<D, FP16, HALVES>(x.x + r[u].b * x.sx[0] + r[u].s * x.sx[1] + r[u].h * x.sx[2], t);
-    }
-    __syncthreads();  // the last run's table has been read
-    turn_table<D>(p, first, last - first + 1, cs);
+  for (int first = (int)blockIdx.x * p.chunk; first < p.tokens; first += (int)gridDim.x * p.chunk) {
+    const int n = min(p.chunk, p.tokens - first);
+    __syncthreads();  // the last chunk's table has been read
+    turn_table<D>(p, first, n, cs);
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const bool live = row0 + u * RPB < p.rows;
-      float g[8], dn[8];
-      qik_mx::unpack8<DT>(Raw8<DT>{{gr[u]}}, g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 c = cs[(r[u].token - first) * (D / 2) + 4 * t + i];
-        const float a = g[first_of<HALVES>(i)], b = g[second_of<HALVES>(i)];
-        dn[first_of<HALVES>(i)] = a * c.x + b * c.y;
-        dn[second_of<HALVES>(i)] = b * c.x - a * c.y;
-      }
-      const Tensor& tn = p.t[r[u].which];
+    for (int k = 0; k < 2; ++k) {
+      const Tensor& x = p.t[k];
+      const int rows = n * x.H;
+      [[maybe_unused]] float wv[8];
       if constexpr (NORM) {
-        float x[8];
-        qik_mx::unpack8<DT>(Raw8<DT>{{raw[u]}}, x);
-        float ss = 0.0f, dot = 0.0f;
-        float wd[8];
+        if (rows > 0) load_weight<D, HALVES>(x.w, t, wv);
+      }
+      for (int row0 = (int)threadIdx.x / TPR; row0 < rows; row0 += RPB * UNITS) {
+        u32x4 raw[UNITS], gr[UNITS];
+        Row r[UNITS];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          wd[e] = dn[e] * tn.w[element_of<D, HALVES>(t, e)];
-          ss = __builtin_fmaf(x[e], x[e], ss);
-          dot = __builtin_fmaf(x[e], wd[e], dot);
+        for (int u = 0; u < UNITS; ++u) {
+          r[u] = row_of(p, x, first, min(row0 + u * RPB, rows - 1));
+          gr[u] = load_pairs<D, HALVES>(x.dy + bytes_of(r[u], x.sdy), t);
+          if constexpr (NORM) raw[u] = load_pairs<D, HALVES>(x.x + bytes_of(r[u], x.sx), t);
         }
-        const float rs = 1.0f / sqrtf(row_sum<TPR>(ss) * (1.0f / D) + tn.eps);
-        const float pull = row_sum<TPR>(dot) * (1.0f / D) * rs * rs;  // mean(x w dn) r^2
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float add = live ? dn[e] * (x[e] * rs) : 0.0f;
-          dw[0][e] += r[u].which ? 0.0f : add;
-          dw[1][e] += r[u].which ? add : 0.0f;
-          dn[e] = rs * __builtin_fmaf(-x[e], pull, wd[e]);
+        for (int u = 0; u < UNITS; ++u) {
+          const bool live = row0 + u * RPB < rows;
+          float g[8], dn[8];
+          qik_mx::unpack8<DT>(Raw8<DT>{{gr[u]}}, g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 c = cs[r[u].token * (D / 2) + 4 * t + i];
+            const float a = g[first_of<HALVES>(i)], b = g[second_of<HALVES>(i)];
+            dn[first_of<HALVES>(i)] = a * c.x + b * c.y;
+            dn[second_of<HALVES>(i)] = b * c.x - a * c.y;
+          }
+          if constexpr (NORM) {
+            float v[8];
+            qik_mx::unpack8<DT>(Raw8<DT>{{raw[u]}}, v);
+            float ss = 0.0f, dot = 0.0f;
+            float wd[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              wd[e] = dn[e] * wv[e];
+              ss = __builtin_fmaf(v[e], v[e], ss);
+              dot = __builtin_fmaf(v[e], wd[e], dot);
+            }
+            const float rs = rsqrt_of<D>(row_sum<TPR>(ss), x.eps);
+            const float pull = row_sum<TPR>(dot) * (1.0f / D) * rs * rs;  // mean(x w dn) r^2
+            const float rs_dw = live ? rs : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              dw[k][e] = __builtin_fmaf(dn[e], v[e] * rs_dw, dw[k][e]);
+              dn[e] = rs * __builtin_fmaf(-v[e], pull, wd[e]);
+            }
+          }
+          if (live) store_pairs<D, HALVES>(x.out + bytes_of(r[u], x.so), t, qik_mx::pack8<DT>(dn).w[0]);
         }
       }
-      if (live)
-        store_pairs<D, HALVES>(tn.out + r[u].b * tn.so[0] + r[u].s * tn.so[1] + r[u].h * tn.so[2], t, qik_mx::pack8<DT>(dn).w[0]);
     }
   }
   if constexpr (NORM) {
@@ -250,25 +304,36 @@ __global__ void __launch_bounds__(THREADS) axial_rope_bwd_kernel(const Params p)
   }
 }
 
-// dw [2][D] from the workgroups' sums [n][2][D]: a workgroup takes 32 columns,
-// its 8 lane groups every 8th sum, added in group order at the end
+// dw [2][D] from the workgroups' sums [n][2][D]: a workgroup takes 16 columns,
+// each of its 64 lane groups every 64th sum (at most BWD_GRID / 64 loads, all at
+// once), added in a fixed order at the end.  With 8 groups and one load after
+// the other it took 19 us for 512 sums.
 struct SumParams {
   const float* part;
   float* dw[2];
   int n, D;
 };
-__global__ void __launch_bounds__(THREADS) rope_dw_kernel(const SumParams p) {
-  __shared__ float red[8][32];
-  const int c = (int)threadIdx.x % 32, g = (int)threadIdx.x / 32;
-  const int col = (int)blockIdx.x * 32 + c;  // of 2 D
-  float v = 0.0f;
-  for (int i = g; i < p.n; i += 8) v += p.part[(int64_t)i * 2 * p.D + col];
-  red[g][c] = v;
+constexpr int SUM_COLUMNS = 16;
+constexpr int SUM_THREADS = 1024;
+__global__ void __launch_bounds__(SUM_THREADS) rope_dw_kernel(const SumParams p) {
+  constexpr int GROUPS = SUM_THREADS / SUM_COLUMNS;
+  __shared__ float red[GROUPS][SUM_COLUMNS];
+  const int c = (int)threadIdx.x % SUM_COLUMNS, g = (int)threadIdx.x / SUM_COLUMNS;
+  const int col = (int)blockIdx.x * SUM_COLUMNS + c;  // of 2 D
+  float x[BWD_GRID / GROUPS];
+#pragma unroll
+  for (int i = 0; i < BWD_GRID / GROUPS; ++i) x[i] = g + i * GROUPS < p.n ? p.part[(int64_t)(g + i * GROUPS) * 2 * p.D + col] : 0.0f;
+#pragma unroll
+  for (int i = 1; i < BWD_GRID / GROUPS; ++i) x[0] += x[i];
+  red[g][c] = x[0];
   __syncthreads();
-  if (g != 0) return;
-  for (int i = 1; i < 8; ++i) v += red[i][c];
+#pragma unroll
+  for (int k = GROUPS / 2; k >= 1; k >>= 1) {
+    if (g < k) red[g][c] += red[g + k][c];
+    __syncthreads();
+  }
   const int w = col >= p.D ? 1 : 0;
-  if (p.dw[w] != nullptr) p.dw[w][col - w * p.D] = v;
+  if (g == 0 && p.dw[w] != nullptr) p.dw[w][col - w * p.D] = red[0][c];
 }
 
 typedef void (*rope_fn)(Params);
@@ -298,6 +363,13 @@ bool strides_ok(const int64_t st[3], const qik_axial_rope_args* a, int64_t H) {
   return qik::stride_ok(st, a->B, a->S, H, 8);
 }
 
+// (the kernels hold strides in units of 16 bytes and 32 bits)
+bool strides_fit(const int64_t st[3]) {
+  for (int i = 0; i < 3; ++i)
+    if (st[i] < 0 || st[i] / 8 > (int64_t)UINT_MAX) return false;
+  return true;
+}
+
 // Checks; rows = B * S * (H of both), norm whether the tensors have weights.
 int validate(const qik_axial_rope_args* a, bool bwd, int64_t* rows, bool* norm) {
   *rows = 0;
@@ -314,8 +386,8 @@ int validate(const qik_axial_rope_args* a, bool bwd, int64_t* rows, bool* norm) 
     heads += a->t[i].H;
   }
   if (a->B == 0 || a->S == 0 || heads == 0) return QIK_OK;
-  // (a run past the last row is still an int)
-  if (a->B > lim / a->S || a->B * a->S > (lim - 4096) / heads) return QIK_ERR_SHAPE;
+  // (a chunk of tokens past the last is still an int)
+  if (a->B > lim / a->S || a->B * a->S > (lim - BWD_GRID * 512) / heads) return QIK_ERR_SHAPE;
   if (a->positions == nullptr || a->freq == nullptr || a->axis == nullptr) return QIK_ERR_NULL_ARG;
   bool with = false, without = false;
   for (int i = 0; i < 2; ++i) {
@@ -330,6 +402,7 @@ int validate(const qik_axial_rope_args* a, bool bwd, int64_t* rows, bool* norm) 
       return QIK_ERR_ALIGN;
     if (!strides_ok(t.stride_x, a, t.H) || !strides_ok(t.stride_out, a, t.H) || (bwd && !strides_ok(t.stride_dy, a, t.H)))
       return QIK_ERR_ALIGN;
+    if (!strides_fit(t.stride_x) || !strides_fit(t.stride_out) || (bwd && !strides_fit(t.stride_dy))) return QIK_ERR_SHAPE;
   }
   if (with && without) return QIK_ERR_NULL_ARG;  // both have a weight, or neither
   *rows = a->B * a->S * heads;
@@ -337,7 +410,20 @@ int validate(const qik_axial_rope_args* a, bool bwd, int64_t* rows, bool* norm) 
   return QIK_OK;
 }
 
-void fill(const qik_axial_rope_args* a, bool bwd, int64_t rows, int run, Params* p) {
+unsigned reciprocal(int64_t d) { return d <= 1 ? 0u : (unsigned)((((int64_t)1 << 32) + d - 1) / d); }
+
+// Tokens of a chunk: ROWS_AIM rows of the tensor with more heads, fewer where
+// that leaves CUs without a workgroup, as many as the table holds at most.
+int chunk_of(const qik_axial_rope_args* a) {
+  const int64_t H = std::max<int64_t>(std::max(a->t[0].H, a->t[1].H), 1);
+  const int64_t tokens = a->B * a->S;
+  const int64_t most = TABLE_BYTES / (a->D / 2 * (int64_t)sizeof(float2));
+  int64_t n = std::min((ROWS_AIM + H - 1) / H, most);
+  const int64_t spread = tokens / (2 * (int64_t)std::max(qik::device_cus(), 1));
+  return (int)std::max<int64_t>(std::min(n, spread), 1);
+}
+
+void fill(const qik_axial_rope_args* a, bool bwd, int chunk, Params* p) {
   memset(p, 0, sizeof(*p));
   for (int i = 0; i < 2; ++i) {
     const qik_rope_tensor& t = a->t[i];
@@ -347,32 +433,28 @@ void fill(const qik_axial_rope_args* a, bool bwd, int64_t rows, int run, Params*
     d.out = static_cast<char*>(bwd ? t.dx : t.out);
     d.w = t.weight;
     for (int k = 0; k < 3; ++k) {
-      d.sx[k] = t.stride_x[k] * 2;
-      d.so[k] = t.stride_out[k] * 2;
-      d.sdy[k] = t.stride_dy[k] * 2;
+      d.sx[k] = (unsigned)(t.stride_x[k] / 8);
+      d.so[k] = (unsigned)(t.stride_out[k] / 8);
+      d.sdy[k] = (unsigned)(t.stride_dy[k] / 8);
     }
     d.H = (int)t.H;
+    d.by_H = reciprocal(t.H);
     d.eps = t.eps;
-    p->heads += d.H;
   }
   p->pos = a->positions;
   p->freq = a->freq;
   p->axis = a->axis;
   p->pos_b = a->stride_pos_b;
   p->pos_a = a->stride_pos_a;
-  p->rows = (int)rows;
+  p->tokens = (int)(a->B * a->S);
   p->S = (int)a->S;
-  p->runs = (int)((rows + run - 1) / run);
+  p->by_S = reciprocal(a->S);
+  p->chunk = chunk;
 }
 
-// rows of a run, and bytes of its tokens' table: a run touches at most (run -
-// 2) / heads + 2 tokens, and never more than its rows
-int run_of(int64_t D) { return THREADS / (int)(D / 8) * UNITS; }
-size_t table_bytes(int64_t D, int run, int heads) {
-  return (size_t)std::min((run - 2) / heads + 2, run) * (size_t)(D / 2) * sizeof(float2);
-}
+size_t table_bytes(int64_t D, int chunk) { return (size_t)chunk * (size_t)(D / 2) * sizeof(float2); }
 
-int bwd_grid(int runs) { return std::min(runs, BWD_GRID); }
+int bwd_grid(int64_t tokens, int chunk) { return (int)std::min<int64_t>((tokens + chunk - 1) / chunk, BWD_GRID); }
 
 }  // namespace qik_rope
 
@@ -385,12 +467,12 @@ int qik_axial_rope(const qik_axial_rope_args* a, void* stream) {
   const int st = validate(a, false, &rows, &norm);
   if (st != QIK_OK || rows == 0) return st;
   Params p;
-  const int run = run_of(a->D);
-  fill(a, false, rows, run, &p);
+  const int chunk = chunk_of(a);
+  fill(a, false, chunk, &p);
   void* kargs[] = {&p};
   const rope_fn fn = pick<false>(a->D, a->dtype == QIK_DTYPE_FP16, a->halves != 0, norm);
-  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)p.runs), dim3(THREADS), kargs,
-                                       table_bytes(a->D, run, p.heads), static_cast<hipStream_t>(stream));
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)((p.tokens - 1) / chunk + 1)), dim3(THREADS),
+                                       kargs, table_bytes(a->D, chunk), static_cast<hipStream_t>(stream));
   return e == hipSuccess ? QIK_OK : QIK_ERR_LAUNCH;
 }
 
@@ -402,8 +484,7 @@ int qik_axial_rope_bwd_workspace_size(const qik_axial_rope_args* a, int64_t* byt
   bool norm;
   const int st = validate(a, true, &rows, &norm);
   if (st != QIK_OK || rows == 0 || !norm) return st;
-  const int64_t run = run_of(a->D);
-  *bytes = (int64_t)bwd_grid((int)((rows + run - 1) / run)) * 2 * a->D * 4;
+  *bytes = (int64_t)bwd_grid(a->B * a->S, chunk_of(a)) * 2 * a->D * 4;
   return QIK_OK;
 }
 
@@ -414,21 +495,21 @@ int qik_axial_rope_bwd(const qik_axial_rope_args* a, void* ws, int64_t ws_bytes,
   int st = validate(a, true, &rows, &norm);
   if (st != QIK_OK || rows == 0) return st;
   Params p;
-  const int run = run_of(a->D);
-  fill(a, true, rows, run, &p);
-  const int grid = bwd_grid(p.runs);
+  const int chunk = chunk_of(a);
+  fill(a, true, chunk, &p);
+  const int grid = bwd_grid(p.tokens, chunk);
   if (norm && (ws == nullptr || !qik::aligned_to(ws, 16) || ws_bytes < (int64_t)grid * 2 * a->D * 4)) return QIK_ERR_WORKSPACE;
   p.part = static_cast<float*>(ws);
   void* kargs[] = {&p};
   const rope_fn fn = pick<true>(a->D, a->dtype == QIK_DTYPE_FP16, a->halves != 0, norm);
-  const size_t lds = std::max(table_bytes(a->D, run, p.heads), (size_t)(THREADS / (a->D / 8) * a->D * 4));
+  const size_t lds = std::max(table_bytes(a->D, chunk), (size_t)(THREADS / (a->D / 8) * a->D * 4));
   if (hipLaunchKernel(reinterpret_cast<const void*>(fn), dim3((unsigned)grid), dim3(THREADS), kargs, lds,
                       static_cast<hipStream_t>(stream)) != hipSuccess)
     return QIK_ERR_LAUNCH;
   if (!norm) return QIK_OK;
   SumParams s = {p.part, {a->t[0].H > 0 ? a->t[0].dw : nullptr, a->t[1].H > 0 ? a->t[1].dw : nullptr}, grid, (int)a->D};
   void* sargs[] = {&s};
-  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(rope_dw_kernel), dim3((unsigned)(2 * a->D / 32)), dim3(THREADS),
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(rope_dw_kernel), dim3((unsigned)(2 * a->D / SUM_COLUMNS)), dim3(SUM_THREADS),
                                        sargs, 0, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? QIK_OK : QIK_ERR_LAUNCH;
 }

@@ -33,7 +33,7 @@ import torch
 
 from . import _lib
 from .attention import _kernel_layout
-from .mx_slab import _DTYPES, HEAD_DIMS, MXSlab, slab_values
+from .mx_slab import _DTYPES, HEAD_DIMS, MXSlab, load_args, slab_values
 
 FP8_E4M3_MAX = 448.0
 
@@ -254,17 +254,21 @@ class _MXLayerView(_SlabLayer):
     def __init__(self, cache: "MXKVCache", layer: int):
         self._c = cache
         self._layer = layer
+        self._lengths = cache.lengths[layer]
+        self._calls: dict = {}  # store geometry -> (argument struct, operands that need a copy)
+        self._slabs: dict = {}  # rows -> (k, v MXSlab views, argument struct of get)
 
     def store(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """k, v ``[B, P, H, D]`` post-RoPE become rows 0 .. P - 1 of every batch entry, whose length is then P."""
         c = self._c
-        P = self._check(k, v)
+        P = k.shape[1] if k.dim() == 4 else 0
+        call = self._call(k, v)
         if P > c.capacity:
             raise ValueError(f"prefix of {P} tokens exceeds the slab capacity {c.capacity}")
-        if P == 0 or k.numel() == 0:
-            c.lengths[self._layer].fill_(P)
+        if P == 0 or call is None:
+            self._lengths.fill_(P)
         else:
-            self._launch(k, v, None, False)
+            self._launch(call, k, v, None, False)
         c._host_lengths[self._layer], c._exact[self._layer] = P, True
 
     def append(self, k: torch.Tensor, v: torch.Tensor, at: torch.Tensor | int | None = None) -> None:
@@ -276,16 +280,17 @@ class _MXLayerView(_SlabLayer):
         unless it is them.  Rows past the capacity are not written; where the
         host knows the lengths (they came from ``store``, or from appends with
         None or an int outside of graph capture) that is a ValueError instead."""
-        c = self._c
-        S = self._check(k, v)
-        n, exact = c._host_lengths[self._layer], c._exact[self._layer]
-        lengths = c.lengths[self._layer]
+        c, i, lengths = self._c, self._layer, self._lengths
+        S = k.shape[1] if k.dim() == 4 else 0
+        call = self._call(k, v)
+        grow = True
         if isinstance(at, torch.Tensor):
-            if tuple(at.shape) != (c.batch_size,) or at.dtype != torch.int32 or at.device != lengths.device:
+            if at.shape != lengths.shape or at.dtype != torch.int32 or at.device != lengths.device:
                 raise ValueError(f"at must be int32 [{c.batch_size}] on {lengths.device}, "
                                  f"got {at.dtype} {tuple(at.shape)} on {at.device}")
-            first, last = lengths.data_ptr(), lengths.data_ptr() + 4 * c.batch_size
-            if not at.is_contiguous() or (at.data_ptr() != first and first - 4 * c.batch_size < at.data_ptr() < last):
+            first, here = lengths.data_ptr(), at.data_ptr()
+            grow = here == first and at.is_contiguous()
+            if not grow and (not at.is_contiguous() or abs(here - first) < 4 * c.batch_size):
                 at = at.clone(memory_format=torch.contiguous_format)
             n, exact = c.capacity, False
         elif at is not None:
@@ -293,57 +298,69 @@ class _MXLayerView(_SlabLayer):
             if at < 0 or at + S > c.capacity:
                 raise ValueError(f"{S} tokens at {at} exceed the slab capacity {c.capacity}")
             lengths.fill_(at)
-            n, exact = at + S, True
-            at = lengths
+            n, exact, at = at + S, True, lengths
         else:
+            n, exact, at = c._host_lengths[i], c._exact[i], lengths
             if exact and n + S > c.capacity:
                 raise ValueError(f"{S} tokens behind {n} exceed the slab capacity {c.capacity}")
-            n, at = min(n + S, c.capacity), lengths
+            n = min(n + S, c.capacity)
             if torch.cuda.is_current_stream_capturing():
                 # a replay grows the entries further than the host sees
                 n, exact = c.capacity, False
-        if k.numel():
-            self._launch(k, v, at, at.data_ptr() == lengths.data_ptr())
-        elif at.data_ptr() != lengths.data_ptr():
+        if call is not None:
+            self._launch(call, k, v, at, grow)
+        elif not grow:
             lengths.copy_((at + S).clamp_(0, c.capacity))
         elif S:
             lengths.add_(S).clamp_(0, c.capacity)
-        c._host_lengths[self._layer], c._exact[self._layer] = n, exact
+        c._host_lengths[i], c._exact[i] = n, exact
 
-    def _check(self, k: torch.Tensor, v: torch.Tensor) -> int:
+    def _call(self, k: torch.Tensor, v: torch.Tensor):
+        """The prepared store of operands like these; None where there are no rows."""
+        key = (k.shape, k.stride(), k.dtype, k.device, k.data_ptr() & 15,
+               v.shape, v.stride(), v.dtype, v.device, v.data_ptr() & 15)
+        hit = self._calls.get(key)
+        if hit is None:
+            hit = self._prepare(k, v)
+            if len(self._calls) >= 8:
+                self._calls.clear()
+            self._calls[key] = hit
+        return hit[0]
+
+    def _prepare(self, k: torch.Tensor, v: torch.Tensor):
         c = self._c
         H, D = c.num_heads, c.head_dim
         if k.shape != v.shape or k.dim() != 4 or tuple(k.shape[2:]) != (H, D):
             raise ValueError(f"k, v must be [B, P, {H}, {D}] matching the slab, got {tuple(k.shape)}, {tuple(v.shape)}")
         if k.shape[0] != c.batch_size:
             raise ValueError(f"batch {k.shape[0]} != slab batch {c.batch_size}")
-        return k.shape[1]
+        if k.numel() == 0:
+            return (None,)
+        laid = [self._readable(t) for t in (k, v)]
+        full = self._views(c.capacity)
+        a = _lib.QikMxSlabStoreArgs(_lib.ABI_VERSION, _DTYPES[c.dtype], None, None, full[0].struct(), full[1].struct(),
+                                    None, self._lengths.data_ptr(), None, *k.shape, c.capacity,
+                                    *(_lib._i64x3(*t.stride()[:3]) for t in laid))
+        return ((a, laid[0] is not k or laid[1] is not v),)
 
-    def _launch(self, k, v, at, grow: bool) -> None:
-        c = self._c
-        i, dev = self._layer, c.lengths.device
-        k, v = (_kernel_layout(t if t.stride(-1) == 1 else t.contiguous())
-                for t in (k.to(device=dev, dtype=c.dtype), v.to(device=dev, dtype=c.dtype)))
-        gkey = (i, k.shape, k.stride(), v.stride())
-        a = c._args_cache.get(gkey)
-        if a is None:
-            B, S, H, D = k.shape
-            full = self._slabs(c.capacity)
-            a = _lib.QikMxSlabStoreArgs(_lib.ABI_VERSION, _DTYPES[c.dtype], None, None, full[0].struct(), full[1].struct(),
-                                        None, c.lengths[i].data_ptr(), None, B, S, H, D, c.capacity,
-                                        _lib._i64x3(*k.stride()[:3]), _lib._i64x3(*v.stride()[:3]))
-            if len(c._args_cache) >= 4 * max(c.num_layers, 1):
-                c._args_cache.clear()
-            c._args_cache[gkey] = a
+    def _readable(self, t: torch.Tensor) -> torch.Tensor:
+        """t in the cache's dtype, on its device, in a layout that the kernel reads in place."""
+        t = t.to(device=self._lengths.device, dtype=self._c.dtype)
+        return _kernel_layout(t if t.stride(-1) == 1 else t.contiguous())
+
+    def _launch(self, call, k, v, at, grow: bool) -> None:
+        a, copy = call
+        if copy:
+            k, v = self._readable(k), self._readable(v)
         a = _lib.QikMxSlabStoreArgs.from_buffer_copy(a)
         a.k, a.v = k.data_ptr(), v.data_ptr()
         if at is not None:
             a.at = at.data_ptr()
             if grow:
-                a.arrivals = c._arrivals.data_ptr() + 4 * i
-        idx = dev.index
+                a.arrivals = self._c._arrivals.data_ptr() + 4 * self._layer
+        idx = self._lengths.device.index
         fn = _lib.load().qik_mx_slab_store
-        if idx != torch.cuda.current_device():
+        if idx != torch._C._cuda_getDevice():
             with torch.cuda.device(idx):
                 st = fn(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(idx))
         else:
@@ -351,21 +368,22 @@ class _MXLayerView(_SlabLayer):
         if st:
             _lib.check(st, "qik_mx_slab_store")
 
-    def _slabs(self, P: int) -> tuple[MXSlab, MXSlab]:
-        c, i = self._c, self._layer
-        hit = c._views.get((i, P))
+    def _views(self, P: int):
+        hit = self._slabs.get(P)
         if hit is None:
-            hit = tuple(MXSlab(codes[i, :, :, :P].transpose(1, 2), scales[i, :, :, :P].transpose(1, 2), c.lengths[i])
-                        for codes, scales in ((c.k_codes, c.k_scales), (c.v_codes, c.v_scales)))
-            if len(c._views) >= 4 * max(c.num_layers, 1):
-                c._views.clear()
-            c._views[(i, P)] = hit
+            c, i = self._c, self._layer
+            k, v = (MXSlab(codes[i, :, :, :P].transpose(1, 2), scales[i, :, :, :P].transpose(1, 2), self._lengths)
+                    for codes, scales in ((c.k_codes, c.k_scales), (c.v_codes, c.v_scales)))
+            if len(self._slabs) >= 8:
+                self._slabs.clear()
+            hit = self._slabs[P] = (k, v, load_args(k, v, c.dtype))
         return hit
 
     def get(self):
         """(k, v): the values of the layer's rows, ``[B, P, H, D]`` in the cache's dtype, zeros behind each entry's
         length; P as in ``views()``."""
-        return slab_values(*self._slabs(self._c._host_lengths[self._layer]), self._c.dtype)
+        k, _, args = self._views(self._c._host_lengths[self._layer])
+        return slab_values(args, self._lengths, k._shape, self._c.dtype)
 
     def views(self, P: int | None = None):
         """(k, v, None) for block_causal_flash_attention: ``MXSlab`` views of the first P rows, with the entries'
@@ -376,7 +394,8 @@ class _MXLayerView(_SlabLayer):
             P = c._host_lengths[self._layer]
         elif not 0 <= P <= c.capacity:
             raise ValueError(f"{P} rows of a slab of {c.capacity}")
-        return (*self._slabs(P), None)
+        k, v, _ = self._views(P)
+        return k, v, None
 
 
 class MXKVCache:
@@ -416,8 +435,6 @@ class MXKVCache:
         self._arrivals = torch.zeros(num_layers, dtype=torch.int32, device=device)
         self._host_lengths = [0] * num_layers   # no entry of the layer is longer
         self._exact = [True] * num_layers       # ... and every one is that long, if the program changed none
-        self._args_cache: dict = {}             # store geometry -> argument struct
-        self._views: dict = {}                  # (layer, rows) -> MXSlab views
         self.layers = [_MXLayerView(self, i) for i in range(num_layers)]
 
     def get_layer(self, i: int) -> _MXLayerView:

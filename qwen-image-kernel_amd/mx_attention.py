@@ -32,20 +32,20 @@ class _Call:
 
 # Prepared calls by the operands' geometry (shapes, strides, types, devices and alignments).
 _CALLS: dict = {}
-
-
-def _geometry(t):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device, t.data_ptr() & 15)
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def mx_slab_attention(query, key, value, prefix_lengths, key_valid, cache_k, cache_v, uniform_full) -> torch.Tensor:
     if not isinstance(cache_k, MXSlab) or not isinstance(cache_v, MXSlab):
         raise ValueError("cache_k and cache_v must both be MXSlab, or neither")
-    uniform = bool(uniform_full) and key_valid is None
+    uniform = uniform_full and key_valid is None
     L = None if uniform else prefix_lengths
-    gkey = (query.shape, query.stride(), query.dtype, query.device, query.data_ptr() & 15,
-            _geometry(key), _geometry(value), _geometry(L), _geometry(key_valid), uniform,
-            cache_k._shape, cache_k._layout, cache_k.device, cache_v._shape, cache_v._layout, cache_v.device)
+    q, k, v = query.data_ptr(), key.data_ptr(), value.data_ptr()
+    gkey = (query.shape, query.stride(), query.dtype, query.device, key.shape, key.stride(), key.dtype, key.device,
+            value.shape, value.stride(), value.dtype, value.device, (q & 15, k & 15, v & 15) if (q | k | v) & 15 else 0,
+            cache_k._layout, cache_v._layout, uniform,
+            None if L is None else (L.shape, L.stride(), L.dtype, L.device),
+            None if key_valid is None else (key_valid.shape, key_valid.stride(), key_valid.dtype, key_valid.device))
     c = _CALLS.get(gkey)
     if c is None:
         c = _prepare(query, key, value, L, key_valid, cache_k, cache_v, uniform)
@@ -58,11 +58,12 @@ def mx_slab_attention(query, key, value, prefix_lengths, key_valid, cache_k, cac
     if c.copy is not None:
         query, key, value = (t.clone(memory_format=torch.contiguous_format) if f else t
                              for f, t in zip(c.copy, (query, key, value)))
+        q, k, v = query.data_ptr(), key.data_ptr(), value.data_ptr()
     if c.slab_copy:
         cache_k, cache_v = cache_k.readable(), cache_v.readable()
     x = _lib.QikMxAttnArgs.from_buffer_copy(c.args)
     a = x.a
-    a.q, a.k_new, a.v_new, a.out = query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr()
+    a.q, a.k_new, a.v_new, a.out = q, k, v, out.data_ptr()
     if L is not None:
         if c.L:
             L = L.to(torch.int32).contiguous()
@@ -70,12 +71,13 @@ def mx_slab_attention(query, key, value, prefix_lengths, key_valid, cache_k, cac
     if key_valid is not None:
         key_valid = _valid_bytes(key_valid, c.valid)
         a.key_valid = key_valid.data_ptr()
-    k, v = x.k_slab, x.v_slab
-    k.codes, k.scales = cache_k._codes.data_ptr(), cache_k._scales.data_ptr()
-    v.codes, v.scales = cache_v._codes.data_ptr(), cache_v._scales.data_ptr()
+    s = x.k_slab
+    s.codes, s.scales = cache_k._codes.data_ptr(), cache_k._scales.data_ptr()
+    s = x.v_slab
+    s.codes, s.scales = cache_v._codes.data_ptr(), cache_v._scales.data_ptr()
     if cache_k._lengths is not None:
         x.lengths = cache_k._lengths.data_ptr()
-    if c.index != torch.cuda.current_device():
+    if c.index != _current_device():
         with torch.cuda.device(c.index):
             st = _launch(c, x)
     else:
@@ -86,15 +88,14 @@ def mx_slab_attention(query, key, value, prefix_lengths, key_valid, cache_k, cac
 
 
 def _launch(c: _Call, x: _lib.QikMxAttnArgs) -> int:
-    handle = torch._C._cuda_getCurrentRawStream(c.index)
-    ws = _attn._workspace(c.device, handle, c.ws_bytes) if c.ws_bytes else None
-    return _lib.load().qik_mx_attn_fwd(ctypes.byref(x), None if ws is None else ws.data_ptr(), c.ws_bytes, handle)
+    handle = _raw_stream(c.index)
+    ws = _attn._workspace(c.device, handle, c.ws_bytes).data_ptr() if c.ws_bytes else None
+    return _lib.load().qik_mx_attn_fwd(ctypes.byref(x), ws, c.ws_bytes, handle)
 
 
 def _valid_bytes(key_valid: torch.Tensor, how: str) -> torch.Tensor:
     """key_valid as bytes, zero for a hidden key, with a dense last dimension."""
-    t = key_valid.view(torch.uint8) if how == "view" else key_valid if how == "" else (key_valid != 0).view(torch.uint8)
-    return t
+    return key_valid.view(torch.uint8) if how == "view" else key_valid if how == "" else (key_valid != 0).view(torch.uint8)
 
 
 def _prepare(query, key, value, L, key_valid, cache_k, cache_v, uniform) -> _Call:
@@ -170,6 +171,8 @@ def _prepare(query, key, value, L, key_valid, cache_k, cache_v, uniform) -> _Cal
     a.sm_scale = float(D) ** -0.5
     x.k_slab, x.v_slab = (t.struct() for t in slabs)
     x.HKV, x.stride_lengths_b = HKV, stride_L
+    if cache_k.lengths is not None:  # (the plan goes by whether there are lengths)
+        x.lengths = cache_k.lengths.data_ptr()
     lib = _lib.load()
     nbytes = ctypes.c_int64(0)
     with torch.cuda.device(dev):

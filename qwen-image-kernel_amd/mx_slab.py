@@ -51,8 +51,9 @@ class MXSlab:
                 raise ValueError("lengths must be contiguous")
         self._codes, self._scales, self._lengths = codes, scales, lengths
         self._shape = torch.Size((*codes.shape[:3], D))
-        # what a prepared call depends on beside the shape
-        self._layout = (codes.stride(), scales.stride(), codes.data_ptr() % 16, scales.data_ptr() % 8, lengths is None)
+        # what a prepared call depends on
+        self._layout = (codes.stride(), scales.stride(), codes.data_ptr() % 16, scales.data_ptr() % 8, lengths is None,
+                        self._shape, codes.device)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -77,7 +78,7 @@ class MXSlab:
     def in_place(self) -> bool:
         """Whether the kernels read this layout as it is (include/qik_mx_attn.h)."""
         B, P, H, D = self._shape
-        (cb, cp, ch, cd), (eb, ep, eh, ed), cbase, ebase, _ = self._layout
+        (cb, cp, ch, cd), (eb, ep, eh, ed), cbase, ebase = self._layout[:4]
         n = D // 32
         return (cd == 1 and (ed == 1 or n == 1) and cbase == 0 and ebase % n == 0
                 and (B == 1 or (cb % 16 == 0 and eb % n == 0)) and (H == 1 or (ch % 16 == 0 and eh % n == 0))
@@ -98,25 +99,28 @@ class MXSlab:
         return f"MXSlab({tuple(self._shape)}, lengths={self._lengths is not None}, device={str(self.device)!r})"
 
 
-def slab_values(k: MXSlab, v: MXSlab, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
-    """The values of both slabs' rows, ``[B, P, H, D]`` in dtype, zeros behind ``k.lengths``."""
+def load_args(k: MXSlab, v: MXSlab, dtype: torch.dtype) -> _lib.QikMxSlabLoadArgs:
+    """The argument struct of ``slab_values``, without the outputs' addresses."""
     if dtype not in _DTYPES:
         raise ValueError(f"dtype must be bf16 or fp16, got {dtype}")
     if not k.codes.is_cuda:
         raise ValueError("a slab is read on a HIP device")
-    k, v = k.readable(), v.readable()
-    out = [torch.empty(k.shape, dtype=dtype, device=k.device) for _ in range(2)]
-    lengths = k.lengths
-    B, P, H, D = k.shape
-    a = _lib.QikMxSlabLoadArgs(_lib.ABI_VERSION, _DTYPES[dtype], k.struct(), v.struct(),
-                               None if lengths is None else lengths.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
-                               B, P, H, D)
-    idx = k.device.index
-    if idx != torch.cuda.current_device():
+    return _lib.QikMxSlabLoadArgs(_lib.ABI_VERSION, _DTYPES[dtype], k.struct(), v.struct(),
+                                  None if k.lengths is None else k.lengths.data_ptr(), None, None, *k.shape)
+
+
+def slab_values(args: _lib.QikMxSlabLoadArgs, like: torch.Tensor, shape, dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values of both slabs' rows, ``[B, P, H, D]`` in dtype on like's device, zeros behind the lengths."""
+    a = _lib.QikMxSlabLoadArgs.from_buffer_copy(args)
+    k, v = like.new_empty(shape, dtype=dtype), like.new_empty(shape, dtype=dtype)
+    a.k, a.v = k.data_ptr(), v.data_ptr()
+    idx = like.device.index
+    fn = _lib.load().qik_mx_slab_load
+    if idx != torch._C._cuda_getDevice():
         with torch.cuda.device(idx):
-            st = _lib.load().qik_mx_slab_load(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(idx))
+            st = fn(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(idx))
     else:
-        st = _lib.load().qik_mx_slab_load(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(idx))
+        st = fn(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(idx))
     if st:
         _lib.check(st, "qik_mx_slab_load")
-    return out[0], out[1]
+    return k, v

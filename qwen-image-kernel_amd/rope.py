@@ -24,6 +24,7 @@ __all__ = ["AxialRope", "fused_qk_norm_rope"]
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 _HEAD_DIMS = (32, 64, 128, 256)
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 class AxialRope:
@@ -75,6 +76,7 @@ class AxialRope:
         self._freq = torch.tensor(freq, dtype=torch.float64, device=dev)
         self._axis = torch.tensor(axis, dtype=torch.int32, device=dev)
         self._shape = tuple(self.positions.shape)
+        self._plans: dict = {}  # prepared calls by the operands' geometry, forward and backward
 
     @property
     def device(self) -> torch.device:
@@ -88,26 +90,22 @@ class AxialRope:
 class _Plan:
     """What one geometry needs at call time; no tensor."""
 
-    __slots__ = ("args", "index", "copies", "shapes", "ws_bytes")
-
-
-# Prepared calls by geometry, forward and backward.
-_PLANS: dict = {}
-
-
-def _geometry(t):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device, t.data_ptr() & 15)
+    __slots__ = ("args", "index", "copies", "casts", "norm", "shapes", "ws_bytes")
 
 
 def _plan(rope: AxialRope, xs, ws, eps, grads=None) -> _Plan:
-    key = (tuple(_geometry(x) for x in xs), tuple(_geometry(w) for w in ws), eps, rope._shape, rope.pairs,
-           rope.positions.device, rope.head_dim, None if grads is None else tuple(_geometry(g) for g in grads))
-    p = _PLANS.get(key)
+    q, k, wq, wk = xs[0], xs[-1], ws[0], ws[-1]
+    key = (len(xs), q.shape, q.stride(), q.dtype, q.device, q.data_ptr() & 15,
+           k.shape, k.stride(), k.dtype, k.device, k.data_ptr() & 15, eps,
+           None if wq is None else (wq.shape, wq.stride(), wq.dtype, wq.device, wq.data_ptr() & 15),
+           None if wk is None else (wk.shape, wk.stride(), wk.dtype, wk.device, wk.data_ptr() & 15),
+           None if grads is None else tuple((g.stride(), g.data_ptr() & 15) for g in grads))
+    p = rope._plans.get(key)
     if p is None:
         p = _prepare(rope, xs, ws, eps, grads)
-        if len(_PLANS) >= 128:
-            _PLANS.clear()
-        _PLANS[key] = p
+        if len(rope._plans) >= 32:
+            rope._plans.clear()
+        rope._plans[key] = p
     return p
 
 
@@ -138,7 +136,10 @@ def _prepare(rope: AxialRope, xs, ws, eps, grads) -> _Plan:
     p.shapes = [tuple(x.shape) for x in xs]
     groups = (xs,) if grads is None else (xs, grads)
     laid = [[_layout(t) for t in g] for g in groups]
-    p.copies = [tuple(u is not t for u, t in zip(l, g)) for l, g in zip(laid, groups)]
+    # operands that the kernel cannot read in place go through dense copies, at each call
+    p.copies = [c if any(c) else None for c in (tuple(u is not t for u, t in zip(l, g)) for l, g in zip(laid, groups))]
+    p.norm = ws[0] is not None
+    p.casts = p.norm and any(w.dtype != torch.float32 or not w.is_contiguous() or w.data_ptr() % 16 != 0 for w in ws)
     a = _lib.QikAxialRopeArgs()
     a.abi_version, a.dtype = _lib.ABI_VERSION, _DTYPES[x0.dtype]
     a.halves, a.naxes = int(rope.pairs == "halves"), len(rope.axes_dims)
@@ -175,66 +176,71 @@ def _layout(t: torch.Tensor) -> torch.Tensor:
 
 
 def _dense(ts, copies):
+    if copies is None:
+        return ts
     return [t.clone(memory_format=torch.contiguous_format) if c else t for t, c in zip(ts, copies)]
 
 
 def _fp32(w: torch.Tensor) -> torch.Tensor:
-    if w.dtype != torch.float32 or not w.is_contiguous():
-        w = w.to(torch.float32).contiguous()
+    w = w.to(torch.float32).contiguous()
     return w if w.data_ptr() % 16 == 0 else w.clone()
 
 
-def _call(p: _Plan, name: str, *args) -> None:
-    fn = getattr(_lib.load(), name)
-    if p.index != torch.cuda.current_device():
-        with torch.cuda.device(p.index):
-            st = fn(*args, torch._C._cuda_getCurrentRawStream(p.index))
+def _call(index: int, fn, name: str, *args) -> None:
+    if index != _current_device():
+        with torch.cuda.device(index):
+            st = fn(*args, _raw_stream(index))
     else:
-        st = fn(*args, torch._C._cuda_getCurrentRawStream(p.index))
+        st = fn(*args, _raw_stream(index))
     if st:
         _lib.check(st, name)
 
 
-def _forward(rope: AxialRope, positions, xs, ws, eps):
-    p = _plan(rope, xs, ws, eps)
-    if True in p.copies[0]:
-        xs = _dense(xs, p.copies[0])
-    if ws[0] is not None:
-        ws = [_fp32(w) for w in ws]
+def _struct(p: _Plan, rope: AxialRope) -> _lib.QikAxialRopeArgs:
     a = _lib.QikAxialRopeArgs.from_buffer_copy(p.args)
-    a.positions, a.freq, a.axis = positions.data_ptr(), rope._freq.data_ptr(), rope._axis.data_ptr()
+    a.positions, a.freq, a.axis = rope.positions.data_ptr(), rope._freq.data_ptr(), rope._axis.data_ptr()
+    return a
+
+
+def _forward(rope: AxialRope, xs, ws, eps):
+    p = _plan(rope, xs, ws, eps)
+    xs = _dense(xs, p.copies[0])
+    if p.casts:
+        ws = [_fp32(w) for w in ws]
+    a = _struct(p, rope)
     outs = []
-    for i, x in enumerate(xs):
-        t = a.t[i]
-        out = x.new_empty(p.shapes[i])
+    for t, x, w, shape in zip(a.t, xs, ws, p.shapes):
+        out = x.new_empty(shape)
         t.x, t.out = x.data_ptr(), out.data_ptr()
-        if ws[0] is not None:
-            t.weight = ws[i].data_ptr()
+        if p.norm:
+            t.weight = w.data_ptr()
         outs.append(out)
-    _call(p, "qik_axial_rope", ctypes.byref(a))
+    _call(p.index, _lib.load().qik_axial_rope, "qik_axial_rope", ctypes.byref(a))
     return outs
 
 
-def _backward(rope: AxialRope, positions, xs, ws, eps, grads):
+def _backward(rope: AxialRope, xs, ws, eps, grads):
     """(dx of each, dw of each in fp32 or None)."""
     p = _plan(rope, xs, ws, eps, grads)
     xs, grads = _dense(xs, p.copies[0]), _dense(grads, p.copies[1])
-    if ws[0] is not None:
+    if p.casts:
         ws = [_fp32(w) for w in ws]
-    a = _lib.QikAxialRopeArgs.from_buffer_copy(p.args)
-    a.positions, a.freq, a.axis = positions.data_ptr(), rope._freq.data_ptr(), rope._axis.data_ptr()
+    a = _struct(p, rope)
     dx, dw = [], []
-    for i, x in enumerate(xs):
-        t = a.t[i]
-        dx.append(x.new_empty(p.shapes[i]))
-        t.x, t.dy, t.dx = x.data_ptr(), grads[i].data_ptr(), dx[i].data_ptr()
-        dw.append(None)
-        if ws[0] is not None:
+    for t, x, w, g in zip(a.t, xs, ws, grads):
+        d = x.new_empty(x.shape)
+        t.x, t.dy, t.dx = x.data_ptr(), g.data_ptr(), d.data_ptr()
+        dx.append(d)
+        if p.norm:
             # (with no rows nothing is launched: the sums are zeros)
-            dw[i] = (torch.empty_like if p.ws_bytes and x.shape[2] else torch.zeros_like)(ws[i])
-            t.weight, t.dw = ws[i].data_ptr(), dw[i].data_ptr()
-    ws_mem = xs[0].new_empty(p.ws_bytes, dtype=torch.uint8) if p.ws_bytes else None
-    _call(p, "qik_axial_rope_bwd", ctypes.byref(a), None if ws_mem is None else ws_mem.data_ptr(), p.ws_bytes)
+            d = (torch.empty_like if p.ws_bytes and x.shape[2] else torch.zeros_like)(w)
+            t.weight, t.dw = w.data_ptr(), d.data_ptr()
+            dw.append(d)
+        else:
+            dw.append(None)
+    mem = xs[0].new_empty(p.ws_bytes, dtype=torch.uint8) if p.ws_bytes else None
+    _call(p.index, _lib.load().qik_axial_rope_bwd, "qik_axial_rope_bwd", ctypes.byref(a),
+          None if mem is None else mem.data_ptr(), p.ws_bytes)
     return dx, dw
 
 
@@ -247,23 +253,22 @@ class _NormRope(torch.autograd.Function):
         ctx.rope, ctx.eps, ctx.n = rope, eps, n
         # the positions are saved with the inputs: a change before the backward pass is an error there
         ctx.save_for_backward(rope.positions, *ts)
-        return tuple(_forward(rope, rope.positions, xs, ws, eps))
+        return tuple(_forward(rope, xs, ws, eps))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
-        positions, *ts = ctx.saved_tensors
+        _, *ts = ctx.saved_tensors  # (and the positions are the saved ones)
         xs, ws = ts[:ctx.n], ts[ctx.n:]
-        dx, dw = _backward(ctx.rope, positions, xs, ws, ctx.eps, [g if g.dtype == x.dtype else g.to(x.dtype)
-                                                                  for g, x in zip(grads, xs)])
-        dw = [None if d is None else d.to(w.dtype) for d, w in zip(dw, ws)]
+        dx, dw = _backward(ctx.rope, xs, ws, ctx.eps, grads)
+        dw = [d if d is None or d.dtype == w.dtype else d.to(w.dtype) for d, w in zip(dw, ws)]
         return (None, None, None, *dx, *dw)
 
 
 def _run(rope: AxialRope, xs, ws, eps):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*xs, *ws)):
         return _NormRope.apply(rope, eps, len(xs), *xs, *ws)
-    return _forward(rope, rope.positions, xs, ws, eps)
+    return _forward(rope, xs, ws, eps)
 
 
 def norm_rope(x, weight, rope: AxialRope, eps: float) -> torch.Tensor:
