@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(NTHREADS * KSPLIT, (KSPLIT == 1 && D <= 128) ?
   // per group: K stage 0, K stage 1, V stage 0, V stage 1 (one contiguous block)
   __shared__ u32x4 stg[4 * KSPLIT][TILE_BYTES / 16];
   __shared__ uint32_t skv[KSPLIT][2][BN / 4];   // key_valid bytes of each stage's tile (4 per word)
-  __shared__ int skvall[KSPLIT][2];             // 1 when every key of the stage's tile is valid
+  __shared__ int skvall[KSPLIT][2];             // 1 when every key of the stage's tile is valid (4-bit slab: -1 when none is)
   __shared__ int sred[KSPLIT][NWAVES];
   __shared__ int snext;                         // queue position handed out to this workgroup
   __shared__ f32x2 sml[KSPLIT == 2 ? NTHREADS : 1];  // group 1's (m, l) at the merge
@@ -829,7 +829,13 @@ __global__ void __launch_bounds__(NTHREADS * KSPLIT, (KSPLIT == 1 && D <= 128) ?
         // wave 0 holds the tile's BN bytes, one per lane
         reinterpret_cast<uint8_t*>(skv[grp][stage])[tid] = (uint8_t)kvbyte;
         const int allv = __all(kvbyte != 0u);
-        if (tid == 0) skvall[grp][stage] = allv;
+        if constexpr (MX) {
+          // -1: no key of the tile is valid
+          const int anyv = __any(kvbyte != 0u);
+          if (tid == 0) skvall[grp][stage] = anyv ? allv : -1;
+        } else {
+          if (tid == 0) skvall[grp][stage] = allv;
+        }
       }
     };
 
@@ -864,6 +870,9 @@ __global__ void __launch_bounds__(NTHREADS * KSPLIT, (KSPLIT == 1 && D <= 128) ?
       const int n_in = (seg0 ? slab_keys() : p.SN) - t * BN;  // keys of this tile inside its segment
       const int kv0 = (seg0 ? 0 : s1) + t * BN;        // absolute index of the tile's first key
       if (kv0 > wave_maxL) return;                     // no row of this wave sees the tile
+      if constexpr (MX && KV) {
+        if (__builtin_amdgcn_readfirstlane(skvall[grp][stage]) < 0) return;  // nor does any row at all
+      }
 
       // S^T[n, m] = sum_d K[n, d] Q[m, d]; lane holds m = l32, n = 8(i/4) + 4hf + i%4 (+32)
       f32x16 sa = f32x16{}, sb = f32x16{};

@@ -95,7 +95,7 @@ def _launch(c: _Call, x: _lib.QikMxAttnArgs) -> int:
 
 def _valid_bytes(key_valid: torch.Tensor, how: str) -> torch.Tensor:
     """key_valid as bytes, zero for a hidden key, with a dense last dimension."""
-    return key_valid.view(torch.uint8) if how == "view" else key_valid if how == "" else (key_valid != 0).view(torch.uint8)
+    return key_valid.view(torch.uint8) if how == "view" else key_valid if how == "" else (key_valid != 0).contiguous().view(torch.uint8)
 
 
 def _prepare(query, key, value, L, key_valid, cache_k, cache_v, uniform) -> _Call:
@@ -150,8 +150,6 @@ def _prepare(query, key, value, L, key_valid, cache_k, cache_v, uniform) -> _Cal
         dense = key_valid.shape[1] <= 1 or key_valid.stride(1) == 1
         c.valid = "view" if dense and key_valid.dtype == torch.bool else "" if dense and key_valid.dtype == torch.uint8 else "test"
         kb = _valid_bytes(key_valid, c.valid)
-        if not (kb.shape[1] <= 1 or kb.stride(1) == 1):
-            raise ValueError("key_valid must be dense along the keys")
         a.key_valid = kb.data_ptr()
         a.stride_valid_b = kb.stride(0) if key_valid.shape[0] > 1 else 0
     # operands that the kernel cannot read in place go through dense copies, at each call

@@ -90,7 +90,7 @@ class AxialRope:
 class _Plan:
     """What one geometry needs at call time; no tensor."""
 
-    __slots__ = ("args", "index", "copies", "casts", "norm", "shapes", "ws_bytes")
+    __slots__ = ("args", "index", "copies", "casts", "norm", "shapes", "like", "ws_bytes")
 
 
 def _plan(rope: AxialRope, xs, ws, eps, grads=None) -> _Plan:
@@ -138,6 +138,7 @@ def _prepare(rope: AxialRope, xs, ws, eps, grads) -> _Plan:
     laid = [[_layout(t) for t in g] for g in groups]
     # operands that the kernel cannot read in place go through dense copies, at each call
     p.copies = [c if any(c) else None for c in (tuple(u is not t for u, t in zip(l, g)) for l, g in zip(laid, groups))]
+    p.like = all(x.is_contiguous() for x in xs)
     p.norm = ws[0] is not None
     p.casts = p.norm and any(w.dtype != torch.float32 or not w.is_contiguous() or w.data_ptr() % 16 != 0 for w in ws)
     a = _lib.QikAxialRopeArgs()
@@ -210,7 +211,7 @@ def _forward(rope: AxialRope, xs, ws, eps):
     a = _struct(p, rope)
     outs = []
     for t, x, w, shape in zip(a.t, xs, ws, p.shapes):
-        out = x.new_empty(shape)
+        out = torch.empty_like(x) if p.like else x.new_empty(shape)
         t.x, t.out = x.data_ptr(), out.data_ptr()
         if p.norm:
             t.weight = w.data_ptr()
@@ -228,7 +229,7 @@ def _backward(rope: AxialRope, xs, ws, eps, grads):
     a = _struct(p, rope)
     dx, dw = [], []
     for t, x, w, g in zip(a.t, xs, ws, grads):
-        d = x.new_empty(x.shape)
+        d = torch.empty_like(x) if p.like else x.new_empty(x.shape)
         t.x, t.dy, t.dx = x.data_ptr(), g.data_ptr(), d.data_ptr()
         dx.append(d)
         if p.norm:
@@ -266,7 +267,9 @@ class _NormRope(torch.autograd.Function):
 
 
 def _run(rope: AxialRope, xs, ws, eps):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*xs, *ws)):
+    if torch.is_grad_enabled() and (xs[0].requires_grad or xs[-1].requires_grad
+                                    or (ws[0] is not None and ws[0].requires_grad)
+                                    or (ws[-1] is not None and ws[-1].requires_grad)):
         return _NormRope.apply(rope, eps, len(xs), *xs, *ws)
     return _forward(rope, xs, ws, eps)
 
