@@ -1,10 +1,13 @@
 """GPU tests of the 4-bit slab and of ``block_causal_flash_attention`` over it, against the float64 oracle."""
 
+import ctypes
+
 import pytest
 import torch
 
 import qwen_image_kernel_amd as qik
 from oracle import mx_slab as om
+from qwen_image_kernel_amd import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -31,7 +34,7 @@ def _mx(codes, scales, P, lengths=None):
 
 def _check(out, parts, D, dtype):
     want, lim = parts["out"], om.bound(parts, D, dtype)
-    off = (out.cpu().double() - want).abs()
+    off = (out.to(want.device).double() - want).abs()
     assert torch.isfinite(out).all()
     worst = float((off / lim).max()) if off.numel() else 0.0
     assert worst <= 1.0, worst
@@ -50,7 +53,8 @@ def _case(B, SQ, SN, P, H, HKV, D, dtype, seed, L=None, valid=None, lengths=None
     ok = om.allowed(B, SQ, P, SN, None if uniform else L, valid, ln)
     keys, values = (torch.cat((om.decode(c[:, :, :P], s[:, :, :P]).transpose(1, 2), t.double()), 1)
                     for (c, s), t in ((kc, k), (vc, v)))
-    parts = om.attention(q.double(), keys, values, ok)
+    on = DEV if SQ * (P + SN) * H > 2_000_000 else "cpu"   # where the oracle computes
+    parts = om.attention(*(t.to(on) for t in (q.double(), keys, values, ok)))
     _check(out, parts, D, dtype)
     return out, ok
 
@@ -103,17 +107,36 @@ SHAPES = [
     (1, 1, 0, 1, 1, 1), (1, 1, 1, 31, 4, 1), (2, 1, 1, 1000, 8, 2), (1, 1, 0, 4097, 32, 8), (3, 5, 5, 129, 12, 4),
     (1, 8, 8, 300, 8, 1), (1, 1, 1, 3, 64, 1), (2, 3, 70, 32, 6, 6), (1, 2, 64, 65, 3, 3), (1, 1, 9, 20000, 2, 1),
 ]
-MANY = [(1, 65, 65, 70, 2, 2), (2, 130, 40, 333, 4, 2), (1, 300, 300, 64, 7, 1), (1, 257, 0, 1500, 3, 3)]
+# the kernel of many rows in each of its forms: a row block for a workgroup of two
+# groups, two such workgroups for a row block, the queue, the queue with items of
+# eight pieces; grouped heads
+MANY = [(1, 700, 700, 150, 24, 24), (2, 1024, 1000, 300, 8, 8), (2, 700, 690, 150, 48, 24), (1, 2816, 70, 500, 24, 24)]
+# more rows than a tile, few enough for the other
+MORE = [(1, 65, 65, 70, 2, 2), (2, 130, 40, 333, 4, 2), (1, 300, 300, 64, 7, 1), (1, 257, 0, 1500, 3, 3)]
 
 
-@pytest.mark.parametrize("shape", SHAPES + MANY)
+def _few(shape, D=128, ragged=False):
+    """Whether a call of this shape runs the kernel of few rows on this device."""
+    B, SQ, SN, P, H, HKV = shape
+    few, tiles, pieces = (ctypes.c_int32() for _ in range(3))
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    assert _lib.load().qik_mx_attn_plan(B, SQ, SN, P, H, HKV, D, int(ragged), cus, ctypes.byref(few), ctypes.byref(tiles),
+                                        ctypes.byref(pieces)) == 0
+    return bool(few.value)
+
+
+def test_both_kernels_are_covered():
+    assert all(_few(s) for s in SHAPES + MORE) and not any(_few(s) for s in MANY)
+
+
+@pytest.mark.parametrize("shape", SHAPES + MORE + MANY)
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_uniform(shape, D, dtype):
     _case(*shape, D, dtype, 7 + D, uniform=True)
 
 
-@pytest.mark.parametrize("shape", SHAPES[2:6] + MANY[:2])
+@pytest.mark.parametrize("shape", SHAPES[2:6] + MORE[:2] + MANY[:2])
 @pytest.mark.parametrize("D", [32, 256])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_other_head_dims(shape, D, dtype):
@@ -124,7 +147,7 @@ def test_other_head_dims(shape, D, dtype):
           valid=torch.rand(B, P + SN, generator=g) < 0.7)
 
 
-@pytest.mark.parametrize("shape", SHAPES + MANY)
+@pytest.mark.parametrize("shape", SHAPES + MORE + MANY)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_masks_and_lengths(shape, dtype):
     """Ragged lengths (one empty), causal limits of each entry, rows and keys that see nothing."""
