@@ -142,7 +142,8 @@ def block_causal_flash_attention(
 
     ``cache_k`` and ``cache_v`` may be ``MXSlab`` (a 4-bit slab, such as
     ``MXKVCache`` layers give): then key and value may have fewer heads than
-    query (query head h reads head h // (H / HKV)), prefix_lengths may be [B, SQ],
+    query (query head h reads head h // (H / HKV)), prefix_lengths may be [B, SQ] or
+    None (every key),
     a slab's ``lengths`` say how many of its rows each batch entry has, and keys
     that key_valid hides may hold anything (see mx_attention.py).
 

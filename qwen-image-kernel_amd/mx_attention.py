@@ -1,7 +1,7 @@
 """Attention over a 4-bit slab and fresh keys: ``block_causal_flash_attention`` with ``MXSlab`` caches.
 
-Row q of batch entry b attends key kv iff kv <= L[b, q] (every key with
-``uniform_full`` and no mask) and key_valid[b, kv] says so; the slab's rows are
+Row q of batch entry b attends key kv iff kv <= L[b, q] (every key where L is None,
+or with ``uniform_full`` and no mask) and key_valid[b, kv] says so; the slab's rows are
 keys 0 .. P - 1, of which entry b has ``lengths[b]``, and fresh key n is key P +
 n.  Rows that attend nothing are zeros.  Softmax statistics and sums are fp32,
 the probabilities are rounded to the query's type for the second product, as in
@@ -38,7 +38,7 @@ _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurre
 def mx_slab_attention(query, key, value, prefix_lengths, key_valid, cache_k, cache_v, uniform_full) -> torch.Tensor:
     if not isinstance(cache_k, MXSlab) or not isinstance(cache_v, MXSlab):
         raise ValueError("cache_k and cache_v must both be MXSlab, or neither")
-    uniform = uniform_full and key_valid is None
+    uniform = prefix_lengths is None or (uniform_full and key_valid is None)
     L = None if uniform else prefix_lengths
     q, k, v = query.data_ptr(), key.data_ptr(), value.data_ptr()
     gkey = (query.shape, query.stride(), query.dtype, query.device, key.shape, key.stride(), key.dtype, key.device,

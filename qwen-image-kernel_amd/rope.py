@@ -70,17 +70,22 @@ class AxialRope:
                 freq.append(thetas[a] ** -power / (2 * math.pi))  # turns per unit
                 axis.append(a)
         dev = positions.device
-        self.positions = positions.detach().to(torch.float64).contiguous()
+        self._positions = positions.detach().to(torch.float64).contiguous()
         self.axes_dims, self.head_dim, self.theta = axes_dims, D, thetas
         self.pairs, self.spectrum = pairs, spectrum
         self._freq = torch.tensor(freq, dtype=torch.float64, device=dev)
         self._axis = torch.tensor(axis, dtype=torch.int32, device=dev)
-        self._shape = tuple(self.positions.shape)
+        self._shape = tuple(self._positions.shape)
         self._plans: dict = {}  # prepared calls by the operands' geometry, forward and backward
 
     @property
+    def positions(self) -> torch.Tensor:
+        """fp64 ``[A, S]`` or ``[B, A, S]``; may be written to, not replaced."""
+        return self._positions
+
+    @property
     def device(self) -> torch.device:
-        return self.positions.device
+        return self._positions.device
 
     def __repr__(self) -> str:
         return (f"AxialRope(positions={self._shape}, axes_dims={self.axes_dims}, theta={self.theta}, "
@@ -199,7 +204,7 @@ def _call(index: int, fn, name: str, *args) -> None:
 
 def _struct(p: _Plan, rope: AxialRope) -> _lib.QikAxialRopeArgs:
     a = _lib.QikAxialRopeArgs.from_buffer_copy(p.args)
-    a.positions, a.freq, a.axis = rope.positions.data_ptr(), rope._freq.data_ptr(), rope._axis.data_ptr()
+    a.positions, a.freq, a.axis = rope._positions.data_ptr(), rope._freq.data_ptr(), rope._axis.data_ptr()
     return a
 
 
@@ -253,7 +258,7 @@ class _NormRope(torch.autograd.Function):
         xs, ws = list(ts[:n]), list(ts[n:])
         ctx.rope, ctx.eps, ctx.n = rope, eps, n
         # the positions are saved with the inputs: a change before the backward pass is an error there
-        ctx.save_for_backward(rope.positions, *ts)
+        ctx.save_for_backward(rope._positions, *ts)
         return tuple(_forward(rope, xs, ws, eps))
 
     @staticmethod

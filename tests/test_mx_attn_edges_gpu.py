@@ -509,3 +509,19 @@ def test_refusals_on_the_device():
     refused(q, k, v, L, None, cache_k=_mx(kc[0][:1], kc[1][:1], 20))
     refused(q, k, v, L, None, cache_k=_mx(kc[0][:, :1], kc[1][:, :1], 20))
     refused(q, k, v, L, None, cache_v=k)
+
+
+@pytest.mark.parametrize("shape", [FEW, MANY, (2, 40, 40, 64, 6, 3)])
+def test_without_lengths_every_key_counts(shape):
+    """prefix_lengths None, with and without a mask and slab lengths: as full lengths, to the bit."""
+    B, SQ, SN, P, H, HKV = shape
+    q, k, v, kc, vc = _inputs(shape, seed=23)
+    valid = torch.rand(B, P + SN, generator=torch.Generator().manual_seed(23)) > 0.3
+    full = torch.full((SQ,), P + SN - 1, dtype=torch.int32)
+    ln = torch.tensor([P // 3] * (B - 1) + [P], dtype=torch.int32, device=DEV)
+    for mask in (None, valid):
+        for lengths in (None, ln):
+            ck, cv = (_mx(*t, P, lengths) for t in (kc, vc))
+            want = _call(q, k, v, ck, cv, full, mask)
+            for uniform in (False, True):
+                assert torch.equal(_call(q, k, v, ck, cv, None, mask, uniform), want)
