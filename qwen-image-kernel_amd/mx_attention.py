@@ -115,6 +115,8 @@ def _prepare(query, key, value, L, key_valid, cache_k, cache_v, uniform) -> _Cal
     for name, t in (("cache_k", cache_k), ("cache_v", cache_v)):
         if tuple(t.shape) != (B, P, HKV, D):
             raise ValueError(f"{name} must be [{B}, P, {HKV}, {D}], got {tuple(t.shape)}")
+    if (cache_k.lengths is None) != (cache_v.lengths is None):
+        raise ValueError("cache_k and cache_v must both have lengths, or neither")
     dev = query.device
     for name, t in (("key", key), ("value", value), ("cache_k", cache_k), ("cache_v", cache_v)):
         if t.device != dev:

@@ -27,7 +27,8 @@ class MXSlab:
     the low half) and ``scales`` uint8 ``[B, P, H, D / 32]`` (E8M0), any strides
     with the last dimension dense; a layout that the kernels cannot read in
     place is copied at each call.  ``lengths`` int32 ``[B]`` on the same device:
-    rows from ``lengths[b]`` on are not part of entry b (None: all P are)."""
+    rows from ``lengths[b]`` on are not part of entry b (None: all P are); the
+    two slabs of a call have the same (K's are read)."""
 
     __slots__ = ("_codes", "_scales", "_lengths", "_shape", "_layout")
 

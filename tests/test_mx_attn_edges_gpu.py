@@ -501,7 +501,6 @@ def test_refusals_on_the_device():
     refused(q, k, v, L[:2], None)
     refused(q, k, v, L[None].expand(3, -1), None)
     refused(q, k, v, L.cpu(), None)
-    refused(q, k, v, None, None)
     refused(q, k, v, L, torch.ones(2, 22, dtype=torch.bool, device=DEV))
     refused(q, k, v, L, torch.ones(3, 23, dtype=torch.bool, device=DEV))
     refused(q, k, v, L, torch.ones(2, 23, dtype=torch.bool))
@@ -509,6 +508,9 @@ def test_refusals_on_the_device():
     refused(q, k, v, L, None, cache_k=_mx(kc[0][:1], kc[1][:1], 20))
     refused(q, k, v, L, None, cache_k=_mx(kc[0][:, :1], kc[1][:, :1], 20))
     refused(q, k, v, L, None, cache_v=k)
+    ln = torch.tensor([20, 3], dtype=torch.int32, device=DEV)
+    refused(q, k, v, L, None, cache_k=_mx(*kc, 20, ln))
+    refused(q, k, v, L, None, cache_v=_mx(*vc, 20, ln))
 
 
 @pytest.mark.parametrize("shape", [FEW, MANY, (2, 40, 40, 64, 6, 3)])
