@@ -2,7 +2,9 @@
 // include/qik_mx_attn.h.  The slab's store and load are byte movers (a thread
 // takes eight elements of a row, a quad of lanes a block of 32); the attention
 // runs the kernel of qik_mx_rows.h for few query rows and that of
-// qik_attn_kernel.h, in its 4-bit instance, for others.
+// qik_attn_kernel.h, in its 4-bit instance, for others (4096 rows against 2560 slab
+// rows and 4096 fresh keys, 24 heads of 128: 328 us, 1020 TFLOP/s, as with a slab
+// of bf16 K and fp8 V; the codes are turned while the matrix cores work).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -28,7 +30,7 @@ constexpr int UNITS = 4;  // rows of a thread, their loads issued before any of 
 // A workgroup takes rows of one (b, h): blockIdx.y, and every gridDim.y-th on;
 // blockIdx.z: K or V.  With rows of all heads in one number and a division for
 // each, the arithmetic took longer than the bytes (2560 x 24 x 128: 10.2 us
-// stored, 11.9 loaded).
+// stored, 11.9 loaded; so 9.0 and 8.3, 4.4 and 4.8 TB/s).
 template <int D>
 constexpr int rows_of_group() { return THREADS / (D / 8) * UNITS; }
 

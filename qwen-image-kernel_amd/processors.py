@@ -6,9 +6,11 @@ step of the attention layer between the projections on this package's HIP
 kernels:
 
 * Q/K: per-head RMSNorm + RoPE (``fused_rms_norm_rope``), both in one launch
-  (qik_rms_rope_pair);
-* prefix extraction: ``layer_cache.store`` (qik_slab_store on a HIP slab);
-* attention: ``block_causal_flash_attention`` (qik_attn_fwd_ws) -- prefill over the
+  (qik_rms_rope_pair; qik_axial_rope where ``rotary_emb`` is an ``AxialRope``);
+* prefix extraction: ``layer_cache.store`` (qik_slab_store on a HIP slab,
+  qik_mx_slab_store on an ``MXKVCache``'s);
+* attention: ``block_causal_flash_attention`` (qik_attn_fwd_ws, qik_mx_attn_fwd
+  over a 4-bit slab) -- prefill over the
   joint sequence with per-row causal lengths from the segment list, decode of
   the target rows against the slab views (no torch.cat), or full attention
   without a cache;
