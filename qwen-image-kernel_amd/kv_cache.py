@@ -256,7 +256,7 @@ class _MXLayerView(_SlabLayer):
         self._layer = layer
         self._lengths = cache.lengths[layer]
         self._calls: dict = {}  # store geometry -> (argument struct, operands that need a copy)
-        self._slabs: dict = {}  # rows -> (k, v MXSlab views, argument struct of get)
+        self._full = None       # (k, v MXSlab views of the whole capacity, argument struct of get)
 
     def store(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """k, v ``[B, P, H, D]`` post-RoPE become rows 0 .. P - 1 of every batch entry, whose length is then P."""
@@ -337,7 +337,7 @@ class _MXLayerView(_SlabLayer):
         if k.numel() == 0:
             return (None,)
         laid = [self._readable(t) for t in (k, v)]
-        full = self._views(c.capacity)
+        full = self._slabs()
         a = _lib.QikMxSlabStoreArgs(_lib.ABI_VERSION, _DTYPES[c.dtype], None, None, full[0].struct(), full[1].struct(),
                                     None, self._lengths.data_ptr(), None, *k.shape, c.capacity,
                                     *(_lib._i64x3(*t.stride()[:3]) for t in laid))
@@ -368,22 +368,20 @@ class _MXLayerView(_SlabLayer):
         if st:
             _lib.check(st, "qik_mx_slab_store")
 
-    def _views(self, P: int):
-        hit = self._slabs.get(P)
-        if hit is None:
+    def _slabs(self):
+        if self._full is None:
             c, i = self._c, self._layer
-            k, v = (MXSlab(codes[i, :, :, :P].transpose(1, 2), scales[i, :, :, :P].transpose(1, 2), self._lengths)
+            k, v = (MXSlab(codes[i].transpose(1, 2), scales[i].transpose(1, 2), self._lengths)
                     for codes, scales in ((c.k_codes, c.k_scales), (c.v_codes, c.v_scales)))
-            if len(self._slabs) >= 8:
-                self._slabs.clear()
-            hit = self._slabs[P] = (k, v, load_args(k, v, c.dtype))
-        return hit
+            self._full = (k, v, load_args(k, v, c.dtype))
+        return self._full
 
     def get(self):
         """(k, v): the values of the layer's rows, ``[B, P, H, D]`` in the cache's dtype, zeros behind each entry's
         length; P as in ``views()``."""
-        k, _, args = self._views(self._c._host_lengths[self._layer])
-        return slab_values(args, self._lengths, k._shape, self._c.dtype)
+        c = self._c
+        args = self._slabs()[2]
+        return slab_values(args, self._lengths, (c.batch_size, c._host_lengths[self._layer], c.num_heads, c.head_dim), c.dtype)
 
     def views(self, P: int | None = None):
         """(k, v, None) for block_causal_flash_attention: ``MXSlab`` views of the first P rows, with the entries'
@@ -394,12 +392,12 @@ class _MXLayerView(_SlabLayer):
             P = c._host_lengths[self._layer]
         elif not 0 <= P <= c.capacity:
             raise ValueError(f"{P} rows of a slab of {c.capacity}")
-        k, v, _ = self._views(P)
-        return k, v, None
+        k, v, _ = self._slabs()
+        return k.first(P), v.first(P), None
 
 
 class MXKVCache:
-    """Single-slab prefix KV cache with K and V in MXFP4: one allocation per buffer for all layers.
+    """Single-slab prefix KV cache with K and V in MXFP4: one allocation for all layers' codes and scales.
 
     Codes ``k_codes``, ``v_codes`` uint8 ``[L, B, H, P_max, D / 2]`` and block
     scales ``k_scales``, ``v_scales`` uint8 ``[L, B, H, P_max, D / 32]``, the
@@ -428,11 +426,14 @@ class MXKVCache:
         self.num_layers, self.batch_size, self.capacity = num_layers, batch, prefix_max
         self.num_heads, self.head_dim, self.dtype = num_heads, head_dim, dtype
         shape = (num_layers, batch, num_heads, prefix_max)
-        self.k_codes, self.v_codes = (torch.zeros(*shape, head_dim // 2, dtype=torch.uint8, device=device) for _ in range(2))
-        self.k_scales, self.v_scales = (torch.zeros(*shape, head_dim // 32, dtype=torch.uint8, device=device)
-                                        for _ in range(2))
-        self.lengths = torch.zeros(num_layers, batch, dtype=torch.int32, device=device)
-        self._arrivals = torch.zeros(num_layers, dtype=torch.int32, device=device)
+        rows = num_layers * batch * num_heads * prefix_max
+        widths = (head_dim // 2, head_dim // 2, head_dim // 32, head_dim // 32)
+        # (the codes first: their part is a multiple of 16 bytes long, the scales' of what their rows need)
+        parts = torch.zeros(rows * sum(widths), dtype=torch.uint8, device=device).split([rows * w for w in widths])
+        self.k_codes, self.v_codes, self.k_scales, self.v_scales = (t.view(*shape, w) for t, w in zip(parts, widths))
+        counts = torch.zeros(num_layers * (batch + 1), dtype=torch.int32, device=device)
+        self.lengths = counts[:num_layers * batch].view(num_layers, batch)
+        self._arrivals = counts[num_layers * batch:]
         self._host_lengths = [0] * num_layers   # no entry of the layer is longer
         self._exact = [True] * num_layers       # ... and every one is that long, if the program changed none
         self.layers = [_MXLayerView(self, i) for i in range(num_layers)]

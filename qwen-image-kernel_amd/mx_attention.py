@@ -29,8 +29,11 @@ class _Call:
 
     __slots__ = ("args", "ws_bytes", "index", "device", "copy", "slab_copy", "L", "valid", "shape", "like")
 
+    # args: without the number of slab rows; ws_bytes: by that number
 
-# Prepared calls by the operands' geometry (shapes, strides, types, devices and alignments).
+
+# Prepared calls by the operands' geometry (shapes, strides, types, devices and alignments), of which
+# the number of slab rows is no part: a serving step's call has a row more than the last one's.
 _CALLS: dict = {}
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
@@ -52,6 +55,10 @@ def mx_slab_attention(query, key, value, prefix_lengths, key_valid, cache_k, cac
         if len(_CALLS) >= 256:
             _CALLS.clear()
         _CALLS[gkey] = c
+    P = cache_k._shape[1]
+    ws_bytes = c.ws_bytes.get(P)
+    if ws_bytes is None or cache_v._shape[1] != P:
+        ws_bytes = _rows(c, P, query, key, key_valid, cache_v)
     out = torch.empty_like(query) if c.like else query.new_empty(c.shape)
     if c.args is None:
         return out
@@ -59,10 +66,12 @@ def mx_slab_attention(query, key, value, prefix_lengths, key_valid, cache_k, cac
         query, key, value = (t.clone(memory_format=torch.contiguous_format) if f else t
                              for f, t in zip(c.copy, (query, key, value)))
         q, k, v = query.data_ptr(), key.data_ptr(), value.data_ptr()
-    if c.slab_copy:
-        cache_k, cache_v = cache_k.readable(), cache_v.readable()
     x = _lib.QikMxAttnArgs.from_buffer_copy(c.args)
+    if c.slab_copy:  # (dense copies, whose strides go by the rows)
+        cache_k, cache_v = cache_k.readable(), cache_v.readable()
+        x.k_slab, x.v_slab = cache_k.struct(), cache_v.struct()
     a = x.a
+    a.P = P
     a.q, a.k_new, a.v_new, a.out = q, k, v, out.data_ptr()
     if L is not None:
         if c.L:
@@ -79,18 +88,38 @@ def mx_slab_attention(query, key, value, prefix_lengths, key_valid, cache_k, cac
         x.lengths = cache_k._lengths.data_ptr()
     if c.index != _current_device():
         with torch.cuda.device(c.index):
-            st = _launch(c, x)
+            st = _launch(c, x, ws_bytes)
     else:
-        st = _launch(c, x)
+        st = _launch(c, x, ws_bytes)
     if st:
         _lib.check(st, "qik_mx_attn_fwd")
     return out
 
 
-def _launch(c: _Call, x: _lib.QikMxAttnArgs) -> int:
+def _launch(c: _Call, x: _lib.QikMxAttnArgs, ws_bytes: int) -> int:
     handle = _raw_stream(c.index)
-    ws = _attn._workspace(c.device, handle, c.ws_bytes).data_ptr() if c.ws_bytes else None
-    return _lib.load().qik_mx_attn_fwd(ctypes.byref(x), ws, c.ws_bytes, handle)
+    ws = _attn._workspace(c.device, handle, ws_bytes).data_ptr() if ws_bytes else None
+    return _lib.load().qik_mx_attn_fwd(ctypes.byref(x), ws, ws_bytes, handle)
+
+
+def _rows(c: _Call, P: int, query, key, key_valid, cache_v) -> int:
+    """What depends on the number of slab rows, checked; the workspace's bytes."""
+    if cache_v.shape[1] != P:
+        raise ValueError(f"cache_k has {P} rows, cache_v {cache_v.shape[1]}")
+    if query.numel() == 0:
+        c.ws_bytes[P] = 0
+        return 0
+    if key_valid is not None:
+        assert key_valid.shape[1] >= P + key.shape[1], "key_valid must be [B, KV_TOTAL]"
+    x = _lib.QikMxAttnArgs.from_buffer_copy(c.args)
+    x.a.P = P
+    nbytes = ctypes.c_int64(0)
+    with torch.cuda.device(c.device):
+        _lib.check(_lib.load().qik_mx_attn_workspace_size(ctypes.byref(x), ctypes.byref(nbytes)), "qik_mx_attn_fwd")
+    if len(c.ws_bytes) >= 64:
+        c.ws_bytes.clear()
+    c.ws_bytes[P] = nbytes.value
+    return nbytes.value
 
 
 def _valid_bytes(key_valid: torch.Tensor, how: str) -> torch.Tensor:
@@ -111,9 +140,8 @@ def _prepare(query, key, value, L, key_valid, cache_k, cache_v, uniform) -> _Cal
         raise ValueError(f"key must be [{B}, SN, HKV, {D}], got {tuple(key.shape)}")
     if HKV == 0 and H != 0 or (HKV and H % HKV != 0):
         raise ValueError(f"{H} query heads do not share {HKV} key heads evenly")
-    P = cache_k.shape[1]
     for name, t in (("cache_k", cache_k), ("cache_v", cache_v)):
-        if tuple(t.shape) != (B, P, HKV, D):
+        if t.shape[0] != B or tuple(t.shape[2:]) != (HKV, D):
             raise ValueError(f"{name} must be [{B}, P, {HKV}, {D}], got {tuple(t.shape)}")
     if (cache_k.lengths is None) != (cache_v.lengths is None):
         raise ValueError("cache_k and cache_v must both have lengths, or neither")
@@ -125,7 +153,7 @@ def _prepare(query, key, value, L, key_valid, cache_k, cache_v, uniform) -> _Cal
     c.index, c.device = dev.index, dev
     c.shape = tuple(query.shape)
     c.like = torch.empty_like(query, device="meta").is_contiguous()
-    c.args, c.ws_bytes, c.copy, c.slab_copy, c.L, c.valid = None, 0, None, False, False, ""
+    c.args, c.ws_bytes, c.copy, c.slab_copy, c.L, c.valid = None, {}, None, False, False, ""
     if query.numel() == 0:
         return c
     x = _lib.QikMxAttnArgs()
@@ -141,11 +169,11 @@ def _prepare(query, key, value, L, key_valid, cache_k, cache_v, uniform) -> _Cal
         c.L = L.dtype != torch.int32 or not L.is_contiguous()
         a.prefix_lengths = L.data_ptr()
     flags = _lib.UNIFORM_L if uniform else 0
-    if P > 0:
+    if cache_k.shape[1] > 0:
         flags |= _lib.HAS_CACHE
     if key_valid is not None:
         _attn._check_aux("key_valid", key_valid, dev)
-        assert key_valid.dim() == 2 and key_valid.shape[1] >= P + SN, "key_valid must be [B, KV_TOTAL]"
+        assert key_valid.dim() == 2, "key_valid must be [B, KV_TOTAL]"
         if key_valid.shape[0] not in (1, B):
             raise ValueError(f"key_valid batch dim must be 1 or B={B}, got {key_valid.shape[0]}")
         flags |= _lib.HAS_KEY_VALID
@@ -163,7 +191,7 @@ def _prepare(query, key, value, L, key_valid, cache_k, cache_v, uniform) -> _Cal
     a.abi_version, a.dtype, a.flags = _lib.ABI_VERSION, _DTYPES[query.dtype], flags
     a.q, a.k_new, a.v_new = (t.data_ptr() for t in laid)
     a.out = laid[0].data_ptr()
-    a.B, a.SQ, a.SN, a.P, a.H, a.D = B, SQ, SN, P, H, D
+    a.B, a.SQ, a.SN, a.H, a.D = B, SQ, SN, H, D
     a.stride_q = _lib._i64x3(*laid[0].stride()[:3])
     a.stride_k_new = _lib._i64x3(*laid[1].stride()[:3])
     a.stride_v_new = _lib._i64x3(*laid[2].stride()[:3])
@@ -173,9 +201,5 @@ def _prepare(query, key, value, L, key_valid, cache_k, cache_v, uniform) -> _Cal
     x.HKV, x.stride_lengths_b = HKV, stride_L
     if cache_k.lengths is not None:  # (the plan goes by whether there are lengths)
         x.lengths = cache_k.lengths.data_ptr()
-    lib = _lib.load()
-    nbytes = ctypes.c_int64(0)
-    with torch.cuda.device(dev):
-        _lib.check(lib.qik_mx_attn_workspace_size(ctypes.byref(x), ctypes.byref(nbytes)), "qik_mx_attn_fwd")
-    c.args, c.ws_bytes = x, nbytes.value
+    c.args = x
     return c

@@ -52,17 +52,30 @@ class MXSlab:
                 raise ValueError("lengths must be contiguous")
         self._codes, self._scales, self._lengths = codes, scales, lengths
         self._shape = torch.Size((*codes.shape[:3], D))
-        # what a prepared call depends on
+        # what a prepared call depends on, beside the number of rows
+        B, P, H, _ = codes.shape
         self._layout = (codes.stride(), scales.stride(), codes.data_ptr() % 16, scales.data_ptr() % 8, lengths is None,
-                        self._shape, codes.device)
+                        B, H, D, codes.device, min(P, 2))
+
+    def first(self, P: int) -> "MXSlab":
+        """The slab's first P rows: the same memory and lengths, no tensor operation."""
+        s = MXSlab.__new__(MXSlab)
+        s._codes, s._scales, s._lengths = self._codes, self._scales, self._lengths
+        B, own, H, D = self._shape
+        if not 0 <= P <= own:
+            raise ValueError(f"{P} rows of a slab of {own}")
+        s._shape = torch.Size((B, P, H, D))
+        few = min(P, 2)
+        s._layout = self._layout if self._layout[-1] == few else (*self._layout[:-1], few)
+        return s
 
     @property
     def codes(self) -> torch.Tensor:
-        return self._codes
+        return self._codes[:, :self._shape[1]]
 
     @property
     def scales(self) -> torch.Tensor:
-        return self._scales
+        return self._scales[:, :self._shape[1]]
 
     @property
     def lengths(self) -> torch.Tensor | None:
@@ -89,7 +102,7 @@ class MXSlab:
         """This slab, or a dense copy of it where the kernels cannot read its layout in place."""
         if self.in_place():
             return self
-        return MXSlab(*(t.clone(memory_format=torch.contiguous_format) for t in (self._codes, self._scales)), self._lengths)
+        return MXSlab(*(t.clone(memory_format=torch.contiguous_format) for t in (self.codes, self.scales)), self._lengths)
 
     def struct(self) -> _lib.QikMxSlab:
         """The argument struct of a slab that is ``in_place``."""
@@ -101,7 +114,7 @@ class MXSlab:
 
 
 def load_args(k: MXSlab, v: MXSlab, dtype: torch.dtype) -> _lib.QikMxSlabLoadArgs:
-    """The argument struct of ``slab_values``, without the outputs' addresses."""
+    """The argument struct of ``slab_values``, without the outputs' addresses and the number of rows."""
     if dtype not in _DTYPES:
         raise ValueError(f"dtype must be bf16 or fp16, got {dtype}")
     if not k.codes.is_cuda:
@@ -113,6 +126,7 @@ def load_args(k: MXSlab, v: MXSlab, dtype: torch.dtype) -> _lib.QikMxSlabLoadArg
 def slab_values(args: _lib.QikMxSlabLoadArgs, like: torch.Tensor, shape, dtype) -> tuple[torch.Tensor, torch.Tensor]:
     """The values of both slabs' rows, ``[B, P, H, D]`` in dtype on like's device, zeros behind the lengths."""
     a = _lib.QikMxSlabLoadArgs.from_buffer_copy(args)
+    a.P = shape[1]
     k, v = like.new_empty(shape, dtype=dtype), like.new_empty(shape, dtype=dtype)
     a.k, a.v = k.data_ptr(), v.data_ptr()
     idx = like.device.index

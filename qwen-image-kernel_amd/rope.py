@@ -27,6 +27,37 @@ _HEAD_DIMS = (32, 64, 128, 256)
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
+class _Spectrum:
+    """The frequencies of a head's pairs and the axis of each on a device, and the calls prepared with them; one for
+    all AxialRopes of the same parameters, which a program makes anew at every step."""
+
+    __slots__ = ("freq", "axis", "plans")
+
+
+_SPECTRA: dict = {}  # by the axes' dimensions, theta, the kind of spectrum and the device
+
+
+def _spectrum(axes_dims, thetas, spectrum, device) -> _Spectrum:
+    key = (axes_dims, thetas, spectrum, device)
+    s = _SPECTRA.get(key)
+    if s is None:
+        D = sum(axes_dims)
+        freq, axis = [], []
+        for a, d in enumerate(axes_dims):
+            for i in range(d // 2):
+                power = 2 * len(freq) / D if spectrum == "shared" else 2 * i / d
+                freq.append(thetas[a] ** -power / (2 * math.pi))  # turns per unit
+                axis.append(a)
+        s = _Spectrum()
+        s.freq = torch.tensor(freq, dtype=torch.float64, device=device)
+        s.axis = torch.tensor(axis, dtype=torch.int32, device=device)
+        s.plans = {}  # prepared calls by the operands' geometry, forward and backward
+        if len(_SPECTRA) >= 64:
+            _SPECTRA.clear()
+        _SPECTRA[key] = s
+    return s
+
+
 class AxialRope:
     """Positions of a step's tokens on several axes, and the pairs' frequencies.
 
@@ -63,20 +94,11 @@ class AxialRope:
         thetas = tuple(float(t) for t in theta) if isinstance(theta, (tuple, list)) else (float(theta),) * len(axes_dims)
         if len(thetas) != len(axes_dims) or not all(math.isfinite(t) and t > 0 for t in thetas):
             raise ValueError(f"theta must be positive, one or {len(axes_dims)}, got {theta}")
-        freq, axis = [], []
-        for a, d in enumerate(axes_dims):
-            for i in range(d // 2):
-                power = 2 * len(freq) / D if spectrum == "shared" else 2 * i / d
-                freq.append(thetas[a] ** -power / (2 * math.pi))  # turns per unit
-                axis.append(a)
-        dev = positions.device
         self._positions = positions.detach().to(torch.float64).contiguous()
         self.axes_dims, self.head_dim, self.theta = axes_dims, D, thetas
         self.pairs, self.spectrum = pairs, spectrum
-        self._freq = torch.tensor(freq, dtype=torch.float64, device=dev)
-        self._axis = torch.tensor(axis, dtype=torch.int32, device=dev)
+        self._spectrum = _spectrum(axes_dims, thetas, spectrum, positions.device)
         self._shape = tuple(self._positions.shape)
-        self._plans: dict = {}  # prepared calls by the operands' geometry, forward and backward
 
     @property
     def positions(self) -> torch.Tensor:
@@ -100,17 +122,18 @@ class _Plan:
 
 def _plan(rope: AxialRope, xs, ws, eps, grads=None) -> _Plan:
     q, k, wq, wk = xs[0], xs[-1], ws[0], ws[-1]
-    key = (len(xs), q.shape, q.stride(), q.dtype, q.device, q.data_ptr() & 15,
+    key = (rope._shape, rope.pairs, len(xs), q.shape, q.stride(), q.dtype, q.device, q.data_ptr() & 15,
            k.shape, k.stride(), k.dtype, k.device, k.data_ptr() & 15, eps,
            None if wq is None else (wq.shape, wq.stride(), wq.dtype, wq.device, wq.data_ptr() & 15),
            None if wk is None else (wk.shape, wk.stride(), wk.dtype, wk.device, wk.data_ptr() & 15),
            None if grads is None else tuple((g.stride(), g.data_ptr() & 15) for g in grads))
-    p = rope._plans.get(key)
+    plans = rope._spectrum.plans
+    p = plans.get(key)
     if p is None:
         p = _prepare(rope, xs, ws, eps, grads)
-        if len(rope._plans) >= 32:
-            rope._plans.clear()
-        rope._plans[key] = p
+        if len(plans) >= 64:
+            plans.clear()
+        plans[key] = p
     return p
 
 
@@ -163,7 +186,7 @@ def _prepare(rope: AxialRope, xs, ws, eps, grads) -> _Plan:
     p.args, p.ws_bytes = a, 0
     if grads is not None and ws[0] is not None and x0.shape[0] * S and any(s[2] for s in p.shapes):
         # sized with any addresses that pass the checks
-        any_ptr = rope._freq.data_ptr()
+        any_ptr = rope._spectrum.freq.data_ptr()
         q = _lib.QikAxialRopeArgs.from_buffer_copy(a)
         q.positions = q.freq = q.axis = any_ptr
         for t in q.t:
@@ -204,7 +227,8 @@ def _call(index: int, fn, name: str, *args) -> None:
 
 def _struct(p: _Plan, rope: AxialRope) -> _lib.QikAxialRopeArgs:
     a = _lib.QikAxialRopeArgs.from_buffer_copy(p.args)
-    a.positions, a.freq, a.axis = rope._positions.data_ptr(), rope._freq.data_ptr(), rope._axis.data_ptr()
+    s = rope._spectrum
+    a.positions, a.freq, a.axis = rope._positions.data_ptr(), s.freq.data_ptr(), s.axis.data_ptr()
     return a
 
 

@@ -294,3 +294,21 @@ def test_refusals_on_the_device():
     for p in (torch.zeros(3, 9, dtype=torch.bool, device=DEV), torch.zeros(3, 9, dtype=torch.complex64, device=DEV)):
         with pytest.raises(ValueError):
             qik.AxialRope(p, _axes(64))
+
+
+def test_plans_made_anew_share_their_frequencies():
+    """Objects of the same parameters, of other positions, lengths, batch forms and pairings, used in turn."""
+    B, H, D = 2, 2, 64
+    g = torch.Generator().manual_seed(9)
+    cases = []
+    for S, per, pairs in ((5, False, "interleaved"), (5, False, "halves"), (5, True, "interleaved"), (8, False, "interleaved")):
+        x, w, _ = _inputs(g, B, S, H, H, D, torch.bfloat16)
+        cases.append((x, w, torch.randint(-50, 50, (B, 3, S) if per else (3, S), generator=g), pairs))
+    for _ in range(2):
+        for x, w, pos, pairs in cases:
+            rope = qik.AxialRope(pos.to(DEV), _axes(D), pairs=pairs)
+            out = qik.fused_qk_norm_rope(*(t.to(DEV) for t in (*x, *w)), rope, EPS)
+            angle = oa.angles(pos, _axes(D), 1e4, "axis")
+            for i in range(2):
+                xd, wd = x[i].double(), w[i].double()
+                _within(out[i], oa.forward(xd, wd, angle, pairs, EPS), oa.forward_bound(xd, wd, angle, pairs, EPS, torch.bfloat16))

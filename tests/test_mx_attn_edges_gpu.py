@@ -152,6 +152,35 @@ def test_layouts(shape):
             assert torch.equal(_call(qd, kd, vd, *pair, uniform=True), want)
 
 
+@pytest.mark.parametrize("pad", [0, 8])
+def test_row_counts_share_a_prepared_call(pad):
+    """One geometry with another number of rows at each call, in place and (scales at odd strides) through copies."""
+    B, SN, H, HKV, D = 2, 2, 4, 2, 64
+    q, k, v, kc, vc = _inputs((B, SN, SN, 200, H, HKV), D, pad=0)
+
+    def slab(codes, scales):
+        wide = torch.zeros(*scales.shape[:-1], 3, dtype=torch.uint8)
+        wide[..., :2] = scales
+        s = wide[..., :2].to(DEV) if not pad else wide.to(DEV)[..., :2]
+        return qik.MXSlab(codes.to(DEV).transpose(1, 2), s.transpose(1, 2))
+
+    ck, cv = slab(*kc), slab(*vc)
+    assert ck.in_place() == (pad == 0)
+    for P in (200, 199, 3, 2, 1, 0, 64, 200):
+        L = P + torch.arange(SN, dtype=torch.int32)
+        for mask in (None, torch.rand(B, P + SN, generator=torch.Generator().manual_seed(P)) > 0.2):
+            a, b = ck.first(P), cv.first(P)
+            assert a.shape == (B, P, HKV, D) and a.codes.shape == (B, P, HKV, D // 2) and a.scales.shape == (B, P, HKV, D // 32)
+            _check(_call(q, k, v, a, b, L, mask), _parts(q, k, v, kc, vc, P, om.allowed(B, SN, P, SN, L, mask)), D, torch.bfloat16)
+            if mask is not None and P:
+                with pytest.raises(AssertionError):
+                    _call(q, k, v, a, b, L, mask[:, 1:])
+    with pytest.raises(ValueError):
+        _call(q, k, v, ck.first(3), cv.first(4), torch.arange(SN, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        ck.first(201)
+
+
 def test_shared_slab():
     """One prefix for every entry of a batch: a slab expanded over the batch is read in place."""
     q, k, v, kc, vc = _inputs((3, 4, 4, 70, 4, 2))
