@@ -249,17 +249,44 @@ struct RowsPlan {
   int row_bits;  // log2 of the rows a piece keeps in the workspace
 };
 
-// What a call of two tiles lasts, in us, from measurements at D = 128 on 256 CUs
-// (P 1000 to 30000, 64 to 2048 rows of 1 to 24 KV heads): here a wave's step
-// takes 1.4 us, a piece 4 beside its steps, the merge 2 and 1 more for 100 KB
-// of pieces, which one workgroup reads.  The kernel of many rows takes 10 and its
-// KV tiles, which run no faster than a row block's on the CUs it can be split over.
-double rows_cost(int64_t items, int64_t T, int64_t pieces, int cus, int waves, int64_t D) {
-  const double merge = pieces > 1 ? 2.0 + (double)pieces * (2 * ROWS_M * 4) * (double)D * 1e-5 : 0.0;
-  return (double)cdiv64(items * pieces, cus) * (1.4 * (double)cdiv64(T, pieces * waves) + 4.0) + merge;
+// What a call of two tiles lasts, in us, fitted to 2500 measured shapes on 256 CUs
+// (17 to 28000 rows of 1 to 24 KV heads, 1 to 4 entries, 16 to 40000 slab rows, in
+// up to 12 pieces; the errors' root mean square is 7 to 14%).  Here: rounds of as
+// many pieces as the CUs hold, each `piece` and a wave's steps, at `step` at least
+// and `fill` for each piece on the CU, one of fresh keys, which are not loaded
+// ahead, `fresh` times as long; `once`; the merge, `join` and 2.1 more for 100 KB
+// of pieces, which one workgroup reads.  The kernel of many rows: `many_once`,
+// `many_round` for each two row blocks of a CU, its KV tiles at `tile` at
+// least, as a row block's can be split over few CUs, and `block` for a CU's
+// first row block and `more` for each further one.  The choice is 0.3 to 0.8%
+// slower than the best measured one on average (by one rule, from D = 128, without
+// the rounds: 1 to 3%, and up to 1.8 times at D = 256).
+struct RowsCost {
+  int held;  // pieces on a CU at once
+  double step, fill, fresh, once, piece, join;
+  double many_once, many_round, tile, block, more;
+};
+const RowsCost& cost_of(int64_t D) {
+  static constexpr RowsCost c32 = {2, 0.72, 0.635, 1.2, 3.8, 2.6, 2.0, 1.0, 7.3, 0.28, 0.7, 0.34},
+                            c64 = {2, 0.9, 0.82, 2.0, 3.1, 3.0, 2.0, 0.5, 8.4, 0.363, 1.0, 0.45},
+                            c128 = {1, 1.36, 1.36, 2.4, 1.4, 4.7, 3.0, 3.1, 7.5, 0.46, 1.34, 1.13},
+                            c256 = {1, 2.2, 2.2, 2.5, 2.0, 7.2, 6.5, 0.0, 17.5, 1.83, 4.75, 3.7};
+  return D <= 32 ? c32 : D <= 64 ? c64 : D <= 128 ? c128 : c256;
 }
-double many_cost(int64_t blocks, int64_t T, int cus) {
-  return 10.0 + (double)T * std::max(0.455, 1.23 * (double)blocks / cus);
+// slab, fresh: steps of each kind
+double rows_cost(int64_t items, int64_t slab, int64_t fresh, int64_t pieces, int cus, int waves, int64_t D) {
+  const RowsCost& c = cost_of(D);
+  const int64_t n = items * pieces, round = (int64_t)c.held * cus, T = slab + fresh;
+  const double steps = (double)cdiv64(cdiv64(T, pieces), waves) * ((double)slab + c.fresh * (double)fresh) / (double)T;
+  double us = c.once + (double)(n / round) * (c.piece + steps * std::max(c.step, c.fill * c.held));
+  if (n % round != 0) us += c.piece + steps * std::max(c.step, c.fill * (double)cdiv64(n % round, cus));
+  return us + (pieces > 1 ? c.join + (double)pieces * (2 * ROWS_M * 4) * (double)D * 2.1e-5 : 0.0);
+}
+double many_cost(int64_t blocks, int64_t T, int cus, int64_t D) {
+  const RowsCost& c = cost_of(D);
+  const double n = (double)blocks / cus;
+  return c.many_once + c.many_round * (double)cdiv64(blocks, 2 * (int64_t)cus) +
+         (double)T * std::max(c.tile, c.block * std::min(n, 1.0) + c.more * std::max(n - 1.0, 0.0));
 }
 
 RowsPlan rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, bool ragged, int cus) {
@@ -273,7 +300,7 @@ RowsPlan rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int6
   r.nrt = (int)nrt;
   cus = std::max(cus, 1);
   const int waves = rows_waves((int)D, r.mt);
-  const int64_t T = std::max<int64_t>(cdiv64(P, ROWS_N) + cdiv64(SN, ROWS_N), 1);
+  const int64_t slab = cdiv64(P, ROWS_N), T = std::max<int64_t>(slab + cdiv64(SN, ROWS_N), 1);
   const int64_t items = B * HKV * nrt;
   while ((1 << r.row_bits) < std::min<int64_t>(R, r.mt * ROWS_M)) ++r.row_bits;
   // every wave of a piece has a step, two where there are many pieces; an item
@@ -288,13 +315,13 @@ RowsPlan rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int6
     pieces = std::min(std::max<int64_t>(((ragged ? 2 : 1) * (int64_t)cus + items / 2) / items, 1), most);
     r.few = true;
   } else {
-    double cost = rows_cost(items, T, 1, cus, waves, D);
+    double cost = rows_cost(items, slab, T - slab, 1, cus, waves, D);
     for (int64_t k = 1; k <= 4; ++k) {  // pieces that fill the CUs k times
       const int64_t n = std::min(std::max<int64_t>(k * cus / items, 1), most);
-      const double c = rows_cost(items, T, n, cus, waves, D);
+      const double c = rows_cost(items, slab, T - slab, n, cus, waves, D);
       if (c < cost) cost = c, pieces = n;
     }
-    r.few = cost < many_cost(B * HKV * cdiv64(R, BM), cdiv64(P, BN) + cdiv64(SN, BN), cus);
+    r.few = cost < many_cost(B * HKV * cdiv64(R, BM), cdiv64(P, BN) + cdiv64(SN, BN), cus, D);
   }
   r.steps = (int)cdiv64(T, pieces);
   r.pieces = (int)cdiv64(T, r.steps);
