@@ -12,6 +12,7 @@
 #include <limits.h>
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "qik_mx_attn.h"
 #include "qik_mx_block.h"
@@ -249,47 +250,57 @@ struct RowsPlan {
   int row_bits;  // log2 of the rows a piece keeps in the workspace
 };
 
-// What a call of two tiles lasts, in us, fitted to 2500 measured shapes on 256 CUs
-// (17 to 28000 rows of 1 to 24 KV heads, 1 to 4 entries, 16 to 40000 slab rows, in
-// up to 12 pieces; the errors' root mean square is 7 to 14%).  Here: rounds of as
-// many pieces as the CUs hold, each `piece` and a wave's steps, at `step` at least
-// and `fill` for each piece on the CU, one of fresh keys, which are not loaded
-// ahead, `fresh` times as long; `once`; the merge, `join` and 2.1 more for 100 KB
-// of pieces, which one workgroup reads.  The kernel of many rows: `many_once`,
-// `many_round` for each two row blocks of a CU, its KV tiles at `tile` at
-// least, as a row block's can be split over few CUs, and `block` for a CU's
-// first row block and `more` for each further one.  The choice is 0.3 to 0.8%
-// slower than the best measured one on average (by one rule, from D = 128, without
-// the rounds: 1 to 3%, and up to 1.8 times at D = 256).
+// What a call of few rows lasts, in us, fitted to 2500 measured shapes of two
+// tiles (17 to 28000 rows of 1 to 24 KV heads, 1 to 4 entries, 16 to 40000 slab
+// rows, in up to 12 pieces) and 800 of one tile (1 to 40 entries, 64 to 130000 slab
+// rows) on 256 CUs; the errors' root mean square is 7 to 18%.  Rounds of as many
+// pieces as the CUs hold, each `piece` and a wave's steps, at `step` at least and
+// `fill` for each piece on the CU, one of fresh keys, which are not loaded ahead,
+// `fresh` times as long; `once`; and where there are pieces the merge, `join` and
+// `merge` for 100 KB of them, which one workgroup reads.  `share`: how many of
+// the pieces behind an item's first have keys.
 struct RowsCost {
   int held;  // pieces on a CU at once
-  double step, fill, fresh, once, piece, join;
-  double many_once, many_round, tile, block, more;
+  double step, fill, fresh, once, piece, join, merge;
 };
-const RowsCost& cost_of(int64_t D) {
-  static constexpr RowsCost c32 = {2, 0.72, 0.635, 1.2, 3.8, 2.6, 2.0, 1.0, 7.3, 0.28, 0.7, 0.34},
-                            c64 = {2, 0.9, 0.82, 2.0, 3.1, 3.0, 2.0, 0.5, 8.4, 0.363, 1.0, 0.45},
-                            c128 = {1, 1.36, 1.36, 2.4, 1.4, 4.7, 3.0, 3.1, 7.5, 0.46, 1.34, 1.13},
-                            c256 = {1, 2.2, 2.2, 2.5, 2.0, 7.2, 6.5, 0.0, 17.5, 1.83, 4.75, 3.7};
-  return D <= 32 ? c32 : D <= 64 ? c64 : D <= 128 ? c128 : c256;
+const RowsCost& rows_cost_of(int64_t D, int mt) {
+  static constexpr RowsCost one[4] = {{3, 0.57, 0.57, 1.2, 5.2, 0.75, 2.0, 2.6}, {2, 0.7, 0.7, 2.0, 4.8, 1.5, 1.75, 2.6},
+                                      {2, 0.85, 1.1, 2.4, 3.3, 2.7, 1.9, 2.6}, {1, 2.1, 0.75, 2.5, 1.4, 4.1, 2.9, 2.6}};
+  static constexpr RowsCost two[4] = {{2, 0.72, 0.635, 1.2, 3.8, 2.6, 2.0, 2.1}, {2, 0.9, 0.82, 2.0, 3.1, 3.0, 2.0, 2.1},
+                                      {1, 1.36, 1.36, 2.4, 1.4, 4.7, 3.0, 2.1}, {1, 2.2, 2.2, 2.5, 2.0, 7.2, 6.5, 2.1}};
+  return (mt > 1 ? two : one)[D <= 32 ? 0 : D <= 64 ? 1 : D <= 128 ? 2 : 3];
 }
-// slab, fresh: steps of each kind
-double rows_cost(int64_t items, int64_t slab, int64_t fresh, int64_t pieces, int cus, int waves, int64_t D) {
-  const RowsCost& c = cost_of(D);
-  const int64_t n = items * pieces, round = (int64_t)c.held * cus, T = slab + fresh;
+// slab, fresh: steps of each kind; rows: of an item, in the workspace
+double rows_cost(const RowsCost& c, int64_t items, int64_t slab, int64_t fresh, int64_t pieces, double share, int cus,
+                 int waves, int64_t rows, int64_t D) {
+  const int64_t T = slab + fresh;
   const double steps = (double)cdiv64(cdiv64(T, pieces), waves) * ((double)slab + c.fresh * (double)fresh) / (double)T;
-  double us = c.once + (double)(n / round) * (c.piece + steps * std::max(c.step, c.fill * c.held));
-  if (n % round != 0) us += c.piece + steps * std::max(c.step, c.fill * (double)cdiv64(n % round, cus));
-  return us + (pieces > 1 ? c.join + (double)pieces * (2 * ROWS_M * 4) * (double)D * 2.1e-5 : 0.0);
+  const double n = (double)items * (1.0 + (double)(pieces - 1) * share), round = (double)c.held * cus;
+  const double full = std::floor(n / round), rest = std::ceil((n - full * round) / cus);
+  double us = c.once + full * (c.piece + steps * std::max(c.step, c.fill * c.held));
+  if (rest > 0.0) us += c.piece + steps * std::max(c.step, c.fill * rest);
+  return us + (pieces > 1 ? c.join + (double)(pieces * rows * 4 * D) * c.merge * 1e-5 : 0.0);
 }
+
+// The same of the kernel of many rows: `once`, `round` for each two row blocks of
+// a CU, its KV tiles at `tile` at least, as a row block's can be split over few
+// CUs, and `block` for a CU's first row block and `more` for each further one.
+// The choice between the two is 0.3 to 0.8% slower than the best measured one on
+// average (by one rule, from D = 128, without the rounds: 1 to 3%, and up to 1.8
+// times at D = 256).
+struct ManyCost {
+  double once, round, tile, block, more;
+};
 double many_cost(int64_t blocks, int64_t T, int cus, int64_t D) {
-  const RowsCost& c = cost_of(D);
+  static constexpr ManyCost costs[4] = {
+      {1.0, 7.3, 0.28, 0.7, 0.34}, {0.5, 8.4, 0.363, 1.0, 0.45}, {3.1, 7.5, 0.46, 1.34, 1.13}, {0.0, 17.5, 1.83, 4.75, 3.7}};
+  const ManyCost& c = costs[D <= 32 ? 0 : D <= 64 ? 1 : D <= 128 ? 2 : 3];
   const double n = (double)blocks / cus;
-  return c.many_once + c.many_round * (double)cdiv64(blocks, 2 * (int64_t)cus) +
+  return c.once + c.round * (double)cdiv64(blocks, 2 * (int64_t)cus) +
          (double)T * std::max(c.tile, c.block * std::min(n, 1.0) + c.more * std::max(n - 1.0, 0.0));
 }
 
-RowsPlan rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, bool ragged, int cus) {
+RowsPlan make_rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, bool ragged, int cus) {
   RowsPlan r = {false, 0, 0, 0, 0, 0};
   const int64_t G = H / HKV, R = SQ * G;
   r.mt = R <= ROWS_M ? 1 : 2;
@@ -307,25 +318,51 @@ RowsPlan rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int6
   // that is cut has a word of the control words
   const int64_t steps = std::max<int64_t>(T / waves, 1);
   const int64_t most = items > QIK_ATTN_WS_CTL_BYTES / 4 ? 1 : std::min<int64_t>(std::max<int64_t>(steps / 2, std::min<int64_t>(steps, 8)), 65535);
+  // Pieces that fill the CUs half, once, .. four times.  With lengths P is the
+  // longest entry's only, and the host knows no other: a mean over three shares
+  // (two tiles, beside the other kernel's estimate, as if all were that long).  Against the best measured number this loses 0.4 to 1.6%, with lengths 3 to 4
+  // (a workgroup a CU, two with lengths: 4 to 7 and 5 to 10); 131072 keys of 8 heads
+  // take 31.6 us in 32 pieces, 34.3 in 64, 44.9 in 16, 24 entries of up to 8192
+  // keys 34.2 in 3, 39.7 in 2, 36.4 in 6.
+  const RowsCost& c = rows_cost_of(D, r.mt);
+  auto cost = [&](int64_t n) {
+    const int64_t rows = (int64_t)1 << r.row_bits;
+    if (!ragged || n == 1 || r.mt > 1) return rows_cost(c, items, slab, T - slab, n, 1.0, cus, waves, rows, D);
+    double us = 0.0;
+    for (int i = 5; i <= 7; ++i) us += rows_cost(c, items, slab, T - slab, n, 0.1 * i, cus, waves, rows, D);
+    return us / 3.0;
+  };
   int64_t pieces = 1;
-  if (r.mt == 1) {
-    // bound by the slab's bytes: a workgroup a CU; with lengths two, as they are
-    // P in the longest entry only (131072 keys of 8 heads: 32 pieces 31.6 us, 64
-    // 34.3, 16 44.9; 24 entries of up to 8192: 3 pieces 34.8, 2 40.3, 6 36.6)
-    pieces = std::min(std::max<int64_t>(((ragged ? 2 : 1) * (int64_t)cus + items / 2) / items, 1), most);
-    r.few = true;
-  } else {
-    double cost = rows_cost(items, slab, T - slab, 1, cus, waves, D);
-    for (int64_t k = 1; k <= 4; ++k) {  // pieces that fill the CUs k times
-      const int64_t n = std::min(std::max<int64_t>(k * cus / items, 1), most);
-      const double c = rows_cost(items, slab, T - slab, n, cus, waves, D);
-      if (c < cost) cost = c, pieces = n;
-    }
-    r.few = cost < many_cost(B * HKV * cdiv64(R, BM), cdiv64(P, BN) + cdiv64(SN, BN), cus, D);
+  double least = cost(1);
+  for (int64_t k = 1; k <= 8; ++k) {
+    const int64_t n = std::min(std::max<int64_t>((k * cus + items) / (2 * items), 1), most);
+    if (n == pieces) continue;
+    const double us = cost(n);
+    if (us < least) least = us, pieces = n;
   }
+  r.few = r.mt == 1 || least < many_cost(B * HKV * cdiv64(R, BM), cdiv64(P, BN) + cdiv64(SN, BN), cus, D);
   r.steps = (int)cdiv64(T, pieces);
   r.pieces = (int)cdiv64(T, r.steps);
   return r;
+}
+
+// The plans of the last sizes: the layers of a step ask for the same one, and the
+// estimates take 2 us of a call's host time.
+RowsPlan rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, bool ragged, int cus) {
+  struct Entry {
+    int64_t key[9];
+    RowsPlan plan;
+  };
+  static thread_local Entry kept[8] = {};  // (D = 0 is no call's)
+  const int64_t key[9] = {B, SQ, SN, P, H, HKV, D, ragged ? 1 : 0, cus};
+  uint64_t x = 0;
+  for (int i = 0; i < 9; ++i) x = (x ^ (uint64_t)key[i]) * 0x9e3779b97f4a7c15ull;
+  Entry& e = kept[x >> 61];
+  if (memcmp(e.key, key, sizeof(key)) != 0) {
+    e.plan = make_rows_plan(B, SQ, SN, P, H, HKV, D, ragged, cus);
+    memcpy(e.key, key, sizeof(key));
+  }
+  return e.plan;
 }
 
 int64_t rows_ws_bytes(const RowsPlan& r, int64_t B, int64_t HKV, int64_t D) {

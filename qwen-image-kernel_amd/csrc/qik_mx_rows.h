@@ -32,7 +32,7 @@
 // 32 query heads on 8 KV heads of 128, MI355X: a token against 131072 keys 30.6 us,
 // 4.6 TB/s of the slab (a large copy reaches 5.15); 24 tokens of sequences of up
 // to 8192 keys 33 us, 3.6 TB/s, where the longest sequences' pieces and the
-// merge end last; a token against 1501 keys 8.6 us, of which the bytes would be
+// merge end last (of one length with the same bytes 25.6 to 29 us); a token against 1501 keys 8.6 us, of which the bytes would be
 // less than one: launch, a piece's loads and steps, and the merge one after the other.
 #ifndef QIK_MX_ROWS_H
 #define QIK_MX_ROWS_H
