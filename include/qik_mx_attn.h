@@ -114,7 +114,8 @@ int qik_mx_attn_fwd(const qik_mx_attn_args* args, void* workspace, int64_t works
 /* Host only: which kernel a call of this shape takes on a device of `cus`
  * compute units, with lengths (`ragged`) or without.  few: 1 for the kernel of few
  * rows; row_tiles: 16-row tiles of each (b, KV head)'s rows there; pieces:
- * workgroups that share its keys. */
+ * workgroups that share its keys, or with lengths of several entries and one tile
+ * the workgroups that a KV head's entries together aim at. */
 int qik_mx_attn_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D,
                      int32_t ragged, int32_t cus, int32_t* few, int32_t* row_tiles, int32_t* pieces);
 

@@ -204,14 +204,15 @@ void pick_mx(bool fp16, bool kv, Kernels* k) {
   if (fp16) kv ? pick_mx<D, true, true>(k) : pick_mx<D, true, false>(k);
   else kv ? pick_mx<D, false, true>(k) : pick_mx<D, false, false>(k);
 }
-template <int D, int MT>
+template <int D, int MT, bool SPREAD>
 rows_kernel_fn pick_rows(bool fp16, bool kv) {
-  if (fp16) return kv ? mx_rows_kernel<D, true, true, MT> : mx_rows_kernel<D, true, false, MT>;
-  return kv ? mx_rows_kernel<D, false, true, MT> : mx_rows_kernel<D, false, false, MT>;
+  if (fp16) return kv ? mx_rows_kernel<D, true, true, MT, SPREAD> : mx_rows_kernel<D, true, false, MT, SPREAD>;
+  return kv ? mx_rows_kernel<D, false, true, MT, SPREAD> : mx_rows_kernel<D, false, false, MT, SPREAD>;
 }
 template <int D>
-rows_kernel_fn pick_rows(bool fp16, bool kv, int mt) {
-  return mt == 1 ? pick_rows<D, 1>(fp16, kv) : pick_rows<D, 2>(fp16, kv);
+rows_kernel_fn pick_rows(bool fp16, bool kv, int mt, bool spread) {
+  if (spread) return pick_rows<D, 1, true>(fp16, kv);
+  return mt == 1 ? pick_rows<D, 1, false>(fp16, kv) : pick_rows<D, 2, false>(fp16, kv);
 }
 
 std::atomic<int> g_mx_slots[16][MAX_DEVICES];
@@ -231,14 +232,14 @@ Kernels mx_kernels_of(const qik_attn_args* a) {
   return k;
 }
 
-rows_kernel_fn rows_kernel_of(const qik_attn_args* a, int mt) {
+rows_kernel_fn rows_kernel_of(const qik_attn_args* a, int mt, bool spread) {
   const bool fp16 = a->dtype == QIK_DTYPE_FP16;
   const bool kv = (a->flags & QIK_HAS_KEY_VALID) != 0;
   switch (a->D) {
-    case 32: return pick_rows<32>(fp16, kv, mt);
-    case 64: return pick_rows<64>(fp16, kv, mt);
-    case 128: return pick_rows<128>(fp16, kv, mt);
-    default: return pick_rows<256>(fp16, kv, mt);
+    case 32: return pick_rows<32>(fp16, kv, mt, spread);
+    case 64: return pick_rows<64>(fp16, kv, mt, spread);
+    case 128: return pick_rows<128>(fp16, kv, mt, spread);
+    default: return pick_rows<256>(fp16, kv, mt, spread);
   }
 }
 
@@ -248,6 +249,7 @@ struct RowsPlan {
   bool few;
   int mt, nrt, steps, pieces;
   int row_bits;  // log2 of the rows a piece keeps in the workspace
+  int spread;    // pieces that the entries aim at together, 0: `pieces` each
 };
 
 // What a call of few rows lasts, in us, fitted to 2500 measured shapes of two
@@ -270,15 +272,14 @@ const RowsCost& rows_cost_of(int64_t D, int mt) {
                                       {1, 1.36, 1.36, 2.4, 1.4, 4.7, 3.0, 2.1}, {1, 2.2, 2.2, 2.5, 2.0, 7.2, 6.5, 2.1}};
   return (mt > 1 ? two : one)[D <= 32 ? 0 : D <= 64 ? 1 : D <= 128 ? 2 : 3];
 }
-// slab, fresh: steps of each kind; rows: of an item, in the workspace
-double rows_cost(const RowsCost& c, int64_t items, int64_t slab, int64_t fresh, int64_t pieces, double share, int cus,
-                 int waves, int64_t rows, int64_t D) {
-  const int64_t T = slab + fresh;
-  const double steps = (double)cdiv64(cdiv64(T, pieces), waves) * ((double)slab + c.fresh * (double)fresh) / (double)T;
-  const double n = (double)items * (1.0 + (double)(pieces - 1) * share), round = (double)c.held * cus;
+// n: all pieces (workgroups with keys), steps: of one, pieces: of the longest item,
+// mixed: how long a step lasts beside one of the slab; rows: of an item, in the workspace
+double rows_cost(const RowsCost& c, double n, double steps, double mixed, int64_t pieces, int cus, int waves, int64_t rows,
+                 int64_t D) {
+  const double wave = std::ceil(steps / waves) * mixed, round = (double)c.held * cus;
   const double full = std::floor(n / round), rest = std::ceil((n - full * round) / cus);
-  double us = c.once + full * (c.piece + steps * std::max(c.step, c.fill * c.held));
-  if (rest > 0.0) us += c.piece + steps * std::max(c.step, c.fill * rest);
+  double us = c.once + full * (c.piece + wave * std::max(c.step, c.fill * c.held));
+  if (rest > 0.0) us += c.piece + wave * std::max(c.step, c.fill * rest);
   return us + (pieces > 1 ? c.join + (double)(pieces * rows * 4 * D) * c.merge * 1e-5 : 0.0);
 }
 
@@ -300,8 +301,11 @@ double many_cost(int64_t blocks, int64_t T, int cus, int64_t D) {
          (double)T * std::max(c.tile, c.block * std::min(n, 1.0) + c.more * std::max(n - 1.0, 0.0));
 }
 
+// what a workgroup takes for the lengths of all entries and its place among them, us
+constexpr double SPREAD_US = 1.0;
+
 RowsPlan make_rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int64_t HKV, int64_t D, bool ragged, int cus) {
-  RowsPlan r = {false, 0, 0, 0, 0, 0};
+  RowsPlan r = {false, 0, 0, 0, 0, 0, 0};
   const int64_t G = H / HKV, R = SQ * G;
   r.mt = R <= ROWS_M ? 1 : 2;
   const int64_t nrt = cdiv64(R, r.mt * ROWS_M);
@@ -318,19 +322,24 @@ RowsPlan make_rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H,
   // that is cut has a word of the control words
   const int64_t steps = std::max<int64_t>(T / waves, 1);
   const int64_t most = items > QIK_ATTN_WS_CTL_BYTES / 4 ? 1 : std::min<int64_t>(std::max<int64_t>(steps / 2, std::min<int64_t>(steps, 8)), 65535);
-  // Pieces that fill the CUs half, once, .. four times.  With lengths P is the
-  // longest entry's only, and the host knows no other: a mean over three shares
-  // (two tiles, beside the other kernel's estimate, as if all were that long).  Against the best measured number this loses 0.4 to 1.6%, with lengths 3 to 4
-  // (a workgroup a CU, two with lengths: 4 to 7 and 5 to 10); 131072 keys of 8 heads
-  // take 31.6 us in 32 pieces, 34.3 in 64, 44.9 in 16, 24 entries of up to 8192
-  // keys 34.2 in 3, 39.7 in 2, 36.4 in 6.
   const RowsCost& c = rows_cost_of(D, r.mt);
+  const int64_t rows = (int64_t)1 << r.row_bits;
+  const double mixed = ((double)slab + c.fresh * (double)(T - slab)) / (double)T;
+  // Pieces that fill the CUs half, once, .. four times.  Against the best measured
+  // number this loses 0.4 to 1.6% on average (a workgroup a CU always: 4 to 7);
+  // 131072 keys of 8 heads take 31.6 us in 32 pieces, 34.3 in 64, 44.9 in 16.
+  // With lengths of several entries P is the longest's only, and a share of the
+  // pieces has no keys: a mean over three.  (Two tiles, beside the other kernel's
+  // estimate: as if all were that long.)
+  const bool several = ragged && r.mt == 1 && B > 1;
   auto cost = [&](int64_t n) {
-    const int64_t rows = (int64_t)1 << r.row_bits;
-    if (!ragged || n == 1 || r.mt > 1) return rows_cost(c, items, slab, T - slab, n, 1.0, cus, waves, rows, D);
     double us = 0.0;
-    for (int i = 5; i <= 7; ++i) us += rows_cost(c, items, slab, T - slab, n, 0.1 * i, cus, waves, rows, D);
-    return us / 3.0;
+    const int shares = several && n > 1 ? 3 : 1;
+    for (int i = 0; i < shares; ++i) {
+      const double share = shares > 1 ? 0.5 + 0.1 * i : 1.0;
+      us += rows_cost(c, (double)items * (1.0 + (double)(n - 1) * share), (double)cdiv64(T, n), mixed, n, cus, waves, rows, D);
+    }
+    return us / shares;
   };
   int64_t pieces = 1;
   double least = cost(1);
@@ -343,6 +352,24 @@ RowsPlan make_rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H,
   r.few = r.mt == 1 || least < many_cost(B * HKV * cdiv64(R, BM), cdiv64(P, BN) + cdiv64(SN, BN), cus, D);
   r.steps = (int)cdiv64(T, pieces);
   r.pieces = (int)cdiv64(T, r.steps);
+  // Or the kernel cuts what it finds into the pieces that the host aims at, which
+  // with the last ones of the entries fill the CUs half, once, .. four times (the
+  // estimate takes 0.6 P for the mean length, and SPREAD_US for finding them).
+  if (several && most > 1 && B * T < (1 << 30)) {
+    for (int64_t k = 1; k <= 8; ++k) {
+      const int64_t z = (k * cus / HKV - B) / 2 - (int64_t)(0.3 * std::sqrt((double)B));
+      if (z < 1 || z + B > 65535) continue;
+      const double of_piece = std::max(std::ceil(0.6 * (double)(B * T) / (double)z), (double)waves);
+      if (of_piece >= (double)T) continue;
+      const double n = (double)items * std::max(0.6 * (double)T / of_piece + 0.5, 1.0);
+      const double us = SPREAD_US + rows_cost(c, n, of_piece, mixed, (int64_t)std::ceil((double)T / of_piece), cus, waves, rows, D);
+      if (us < least) least = us, r.spread = (int)z;
+    }
+    if (r.spread > 0) {
+      r.steps = waves;
+      r.pieces = r.spread + (int)B;
+    }
+  }
   return r;
 }
 
@@ -367,7 +394,7 @@ RowsPlan rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, int6
 
 int64_t rows_ws_bytes(const RowsPlan& r, int64_t B, int64_t HKV, int64_t D) {
   if (r.pieces <= 1) return 0;
-  return QIK_ATTN_WS_CTL_BYTES + B * HKV * r.nrt * r.pieces * rows_slot((int)D, 1 << r.row_bits);
+  return QIK_ATTN_WS_CTL_BYTES + (r.spread > 0 ? 1 : B) * HKV * r.nrt * r.pieces * rows_slot((int)D, 1 << r.row_bits);
 }
 
 // ceil(2^32 / d) for the kernel's quotient, 0 for 1
@@ -603,12 +630,14 @@ int qik_mx_attn_fwd(const qik_mx_attn_args* x, void* ws, int64_t ws_bytes, void*
     r.KV = (int)(a.P + a.SN);
     r.uniform = (a.flags & QIK_UNIFORM_L) ? 1 : 0;
     r.steps = l.rows.steps;
+    r.B = (int)a.B;
+    r.spread = l.rows.spread;
     r.by_G = qik::reciprocal(G);
     r.by_HKV = qik::reciprocal(x->HKV);
     r.row_bits = l.rows.row_bits;
     r.qk_scale = qk_scale;
-    fn = reinterpret_cast<const void*>(qik::rows_kernel_of(&a, l.rows.mt));
-    grid = dim3((unsigned)(x->HKV * l.rows.nrt), (unsigned)a.B, (unsigned)l.rows.pieces);
+    fn = reinterpret_cast<const void*>(qik::rows_kernel_of(&a, l.rows.mt, l.rows.spread > 0));
+    grid = dim3((unsigned)(x->HKV * l.rows.nrt), l.rows.spread > 0 ? 1u : (unsigned)a.B, (unsigned)l.rows.pieces);
     threads = 64u * (unsigned)qik::rows_waves((int)a.D, l.rows.mt);
     kargs[0] = &r;
   } else {
@@ -671,7 +700,7 @@ int qik_mx_attn_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H, in
   const qik::RowsPlan r = qik::rows_plan(B, SQ, SN, P, H, HKV, D, ragged != 0, cus);
   *few = r.few ? 1 : 0;
   *row_tiles = r.mt * r.nrt;
-  *pieces = r.pieces;
+  *pieces = r.spread > 0 ? r.spread : r.pieces;
   return QIK_OK;
 }
 

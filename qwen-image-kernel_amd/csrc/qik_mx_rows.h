@@ -8,9 +8,13 @@
 //   * an item is 16 or 32 query rows of one (b, KV head) -- the query heads that
 //     share the KV head times the query positions -- and its keys in steps of
 //     32.  Items are cut into pieces of the same number of steps, one a
-//     workgroup, so that sequences of any lengths fill the device evenly (a
-//     piece behind an item's last key ends at once; the heads come first in the
-//     grid, then the entries, so that those pieces do not fall on the same XCDs);
+//     workgroup, so that sequences of any lengths fill the device evenly.  With
+//     lengths of several entries (SPREAD) every workgroup reads them all, takes
+//     the number of steps that cuts their sum into as many pieces as the host
+//     aims at, and finds its own among them (24 entries of up to 8192 keys, ten
+//     draws: 33.0 us with the number that the longest gave for all, 30.5 so; the
+//     same bytes in entries of one length 25.6 to 29).  The heads come first in the grid, so
+//     that pieces without keys do not fall on the same XCDs;
 //   * a workgroup's waves take its steps in turn, each with its own softmax state
 //     and its own LDS, and never wait for each other before the end;
 //   * a call lasts some microseconds, so that its instructions' way from memory
@@ -31,8 +35,8 @@
 //     does not depend on which one that is.
 // 32 query heads on 8 KV heads of 128, MI355X: a token against 131072 keys 30.6 us,
 // 4.6 TB/s of the slab (a large copy reaches 5.15); 24 tokens of sequences of up
-// to 8192 keys 33 us, 3.6 TB/s, where the longest sequences' pieces and the
-// merge end last (of one length with the same bytes 25.6 to 29 us); a token against 1501 keys 8.6 us, of which the bytes would be
+// to 8192 keys 30.5 us, 3.9 TB/s, where the pieces are two a CU and not quite
+// even, and the merge ends last; a token against 1501 keys 8.6 us, of which the bytes would be
 // less than one: launch, a piece's loads and steps, and the merge one after the other.
 #ifndef QIK_MX_ROWS_H
 #define QIK_MX_ROWS_H
@@ -67,7 +71,8 @@ struct RowsParams {
   int R;                     // query rows of a KV head: SQ * G, row r is head r % G of position r / G
   int SN, P, HKV, G, KV;
   int uniform;
-  int steps;                 // of a piece
+  int steps;                 // of a piece (SPREAD: at least)
+  int B, spread;             // SPREAD: entries; pieces that all of them aim at
   unsigned by_G, by_HKV;     // ceil(2^32 / G), ceil(2^32 / HKV): see quotient
   int row_bits;              // log2 of the rows a piece keeps in the workspace, a power of two
   float qk_scale;
@@ -100,11 +105,24 @@ __device__ __forceinline__ float quad_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// the sum over lanes 0 .. l in each lane l
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 to the next row, 31 to the upper half
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+
 // n / d by ceil(2^32 / d) (0 for d = 1): exact while n * d < 2^32
 __device__ __forceinline__ int quotient(int n, unsigned by) { return by == 0u ? n : (int)__umulhi((unsigned)n, by); }
 
-// MT: 16-row tiles of an item.
-template <int D, bool FP16, bool KV, int MT>
+// MT: 16-row tiles of an item.  SPREAD: the grid's z are the pieces of all entries
+// of a head, one entry after the other; else its y are the entries and z the
+// pieces of each.
+template <int D, bool FP16, bool KV, int MT, bool SPREAD>
 __global__ void __launch_bounds__(64 * rows_waves(D, MT), D <= 128 && MT == 1 ? 4 : 1) mx_rows_kernel(const RowsParams p) {
   constexpr int ROWS_WAVES = rows_waves(D, MT);
   constexpr int ROWS_THREADS = 64 * ROWS_WAVES;
@@ -128,19 +146,46 @@ __global__ void __launch_bounds__(64 * rows_waves(D, MT), D <= 128 && MT == 1 ? 
   char* const vS = reinterpret_cast<char*>(lds) + wave * WLDS;
 
   // ---- the item and its steps [t0, t1): the slab's, then the fresh keys'
-  const int b = (int)blockIdx.y, hr = (int)blockIdx.x;
+  const int hr = (int)blockIdx.x;
   const int rt = quotient(hr, p.by_HKV);
   const int h = hr - rt * p.HKV;
   const int row_first = rt * ROWS;
   const int rows = min(p.R - row_first, ROWS);
-  int Pc = p.P;
-  if (p.lengths != nullptr)
+  int b = (int)blockIdx.y, piece = (int)blockIdx.z, steps = p.steps, Pc = p.P;
+  const int fresh = cdiv_i(p.SN, ROWS_N);
+  if constexpr (SPREAD) {
+    // lanes hold the entries first + lane
+    auto length = [&](int first) { return first + lane < p.B ? min(max(gload_i32(p.lengths + first + lane), 0), p.P) : 0; };
+    auto steps_of = [&](int first, int len) { return first + lane < p.B ? cdiv_i(len, ROWS_N) + fresh : 0; };
+    const int own = length(0);
+    int sum = steps_of(0, own);  // (the host: less than 2^30 in all)
+    for (int first = 64; first < p.B; first += 64) sum += steps_of(first, length(first));
+    sum = __builtin_amdgcn_readlane(wave_scan(sum), 63);
+    // (so the pieces are spread + B at most, the grid's z)
+    steps = max(__builtin_amdgcn_readfirstlane((int)((unsigned)(sum + p.spread - 1) / (unsigned)p.spread)), steps);
+    int before = 0;
+    b = -1;
+    for (int first = 0; first < p.B && b < 0; first += 64) {
+      const int len = first == 0 ? own : length(first);
+      const int n = first + lane < p.B ? max((int)((unsigned)(steps_of(first, len) + steps - 1) / (unsigned)steps), 1) : 0;
+      const int upto = wave_scan(n), all = __builtin_amdgcn_readlane(upto, 63);
+      if (piece - before < all) {
+        const int l = __builtin_ctzll(__ballot(upto > piece - before));
+        b = first + l;
+        piece -= before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
+        Pc = __builtin_amdgcn_readlane(len, l);
+      }
+      before += all;
+    }
+    if (b < 0) return;
+  } else if (p.lengths != nullptr) {
     Pc = min(max(*((const __attribute__((address_space(4))) int32_t*)(p.lengths + b)), 0), p.P);
+  }
   const int slab = cdiv_i(Pc, ROWS_N);
-  const int T = slab + cdiv_i(p.SN, ROWS_N);
-  const int t0 = (int)blockIdx.z * p.steps;
+  const int T = slab + fresh;
+  const int t0 = piece * steps;
   if (t0 >= T && t0 > 0) return;
-  const int pieces = max((T + p.steps - 1) / p.steps, 1);
+  const int pieces = max((T + steps - 1) / steps, 1);
   const int s1 = p.P;  // absolute index of the first fresh key
 
   // Q as the B operand: lane holds Q[m, g * D/4 + 8j .. + 8], the order in which
@@ -168,7 +213,7 @@ __global__ void __launch_bounds__(64 * rows_waves(D, MT), D <= 128 && MT == 1 ? 
     }
   }
   // the steps that a row sees
-  int t1 = min(T, t0 + p.steps);
+  int t1 = min(T, t0 + steps);
   if (!p.uniform) {
     Lmax = wave_reduce_i32<true>(Lmax);
     Lmin = wave_reduce_i32<false>(Lmin);
@@ -408,9 +453,9 @@ __global__ void __launch_bounds__(64 * rows_waves(D, MT), D <= 128 && MT == 1 ? 
   const int slot = rows_slot(D, 1 << p.row_bits);  // bytes of a piece
   const int ml_at = (D * 4) << p.row_bits;         // of its (m, l)
   // the item's pieces (gridDim.z at most, less than 2^31 bytes)
-  const auto slots = make_rsrc(reinterpret_cast<const char*>(p.part) + (int64_t)item * (int)gridDim.z * slot,
-                               pieces == 1 ? 0 : pieces * slot);
-  const uint32_t mine = (uint32_t)((int)blockIdx.z * slot);
+  const int64_t first_slot = SPREAD ? (int64_t)hr * (int)gridDim.z + ((int)blockIdx.z - piece) : (int64_t)item * (int)gridDim.z;
+  const auto slots = make_rsrc(reinterpret_cast<const char*>(p.part) + first_slot * slot, pieces == 1 ? 0 : pieces * slot);
+  const uint32_t mine = (uint32_t)(piece * slot);
   auto piece_at = [](int r, int c) { return r * (D * 4) + ((c ^ (r & (C4 - 1) & 15)) << 4); };
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {

@@ -556,3 +556,31 @@ def test_without_lengths_every_key_counts(shape):
             want = _call(q, k, v, ck, cv, full, mask)
             for uniform in (False, True):
                 assert torch.equal(_call(q, k, v, ck, cv, None, mask, uniform), want)
+
+
+@pytest.mark.parametrize("B,S,P,H,HKV,D,dtype", [(2, 1, 2000, 8, 2, 128, torch.bfloat16), (7, 3, 900, 4, 4, 64, torch.float16),
+                                                 (64, 1, 300, 4, 1, 128, torch.bfloat16), (65, 2, 257, 2, 1, 32, torch.bfloat16),
+                                                 (130, 1, 700, 1, 1, 64, torch.bfloat16), (3, 1, 1500, 4, 4, 256, torch.float16),
+                                                 (300, 1, 100, 2, 2, 64, torch.bfloat16)])
+@pytest.mark.parametrize("how", ["spread", "one long", "none", "negative and past the end", "all"])
+def test_entries_of_many_lengths(B, S, P, H, HKV, D, dtype, how):
+    """The pieces of all entries together: none lost, none read twice, whatever the lengths sum up to."""
+    q, k, v, kc, vc = _inputs((B, S, S, P, H, HKV), D, dtype, pad=0)
+    g = torch.Generator().manual_seed(B)
+    ln = torch.randint(0, P + 1, (B,), generator=g, dtype=torch.int32)
+    if how == "one long":
+        ln = ln.clamp_max(3)
+        ln[B - 1] = P
+    elif how == "none":
+        ln.zero_()
+    elif how == "all":
+        ln.fill_(P)
+    elif how != "spread":
+        ln = torch.where(torch.rand(B, generator=g) < 0.5, ln - P, ln + P // 2)
+    slabs = [_mx(*t, P, ln.to(DEV)) for t in (kc, vc)]
+    ok = om.allowed(B, S, P, S, None, None, ln)
+    _check(_call(q, k, v, *slabs), _parts(q, k, v, kc, vc, P, ok), D, dtype)
+    out = _call(q, k[:, :0], v[:, :0], *slabs)   # the slab alone
+    _check(out, _parts(q, k[:, :0], v[:, :0], kc, vc, P, ok[..., :P]), D, dtype)
+    assert (out[(ln <= 0).to(DEV)] == 0).all()
+    assert torch.equal(out, _call(q, k[:, :0], v[:, :0], *slabs))
