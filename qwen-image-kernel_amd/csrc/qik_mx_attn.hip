@@ -355,7 +355,7 @@ RowsPlan make_rows_plan(int64_t B, int64_t SQ, int64_t SN, int64_t P, int64_t H,
   // Or the kernel cuts what it finds into the pieces that the host aims at, which
   // with the last ones of the entries fill the CUs half, once, .. four times (the
   // estimate takes 0.6 P for the mean length, and SPREAD_US for finding them).
-  if (several && most > 1 && B * T < (1 << 30)) {
+  if (several && P > 0 && most > 1 && B * T < (1 << 30)) {
     for (int64_t k = 1; k <= 8; ++k) {
       const int64_t z = (k * cus / HKV - B) / 2 - (int64_t)(0.3 * std::sqrt((double)B));
       if (z < 1 || z + B > 65535) continue;
@@ -412,7 +412,8 @@ int plan_mx(const qik_mx_attn_args* x, MxLaunch* l) {
   const qik_attn_args& a = x->a;
   l->ws_bytes = 0;
   const int64_t G = a.H / x->HKV;
-  l->rows = rows_plan(a.B, a.SQ, a.SN, a.P, a.H, x->HKV, a.D, x->lengths != nullptr, device_cus());
+  // (without slab rows the lengths are not read)
+  l->rows = rows_plan(a.B, a.SQ, a.SN, a.P, a.H, x->HKV, a.D, a.P > 0 && x->lengths != nullptr, device_cus());
   if (l->rows.few) {
     l->ws_bytes = rows_ws_bytes(l->rows, a.B, x->HKV, a.D);
     return QIK_OK;

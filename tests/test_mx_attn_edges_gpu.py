@@ -584,3 +584,13 @@ def test_entries_of_many_lengths(B, S, P, H, HKV, D, dtype, how):
     _check(out, _parts(q, k[:, :0], v[:, :0], kc, vc, P, ok[..., :P]), D, dtype)
     assert (out[(ln <= 0).to(DEV)] == 0).all()
     assert torch.equal(out, _call(q, k[:, :0], v[:, :0], *slabs))
+
+
+@pytest.mark.parametrize("S", [1, 3])
+def test_lengths_of_a_slab_without_rows(S):
+    """Entries with lengths over no slab row: the fresh keys alone, also where they are cut into pieces."""
+    B, SN, H, HKV, D = 3, 2000, 4, 2, 128
+    q, k, v, kc, vc = _inputs((B, S, SN, 0, H, HKV), D, pad=4)
+    ln = torch.tensor([0, 7, -2], dtype=torch.int32, device=DEV)
+    slabs = [_mx(*t, 0, ln) for t in (kc, vc)]
+    _check(_call(q, k, v, *slabs), _parts(q, k, v, kc, vc, 0, om.allowed(B, S, 0, SN)), D, torch.bfloat16)
