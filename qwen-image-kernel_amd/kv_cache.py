@@ -257,6 +257,7 @@ class _MXLayerView(_SlabLayer):
         self._lengths = cache.lengths[layer]
         self._calls: dict = {}  # store geometry -> (argument struct, operands that need a copy)
         self._full = None       # (k, v MXSlab views of the whole capacity, argument struct of get)
+        self._rows, self._views = -1, None  # what views() gave last, and for how many rows
 
     def store(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """k, v ``[B, P, H, D]`` post-RoPE become rows 0 .. P - 1 of every batch entry, whose length is then P."""
@@ -392,8 +393,10 @@ class _MXLayerView(_SlabLayer):
             P = c._host_lengths[self._layer]
         elif not 0 <= P <= c.capacity:
             raise ValueError(f"{P} rows of a slab of {c.capacity}")
-        k, v, _ = self._slabs()
-        return k.first(P), v.first(P), None
+        if P != self._rows:
+            k, v, _ = self._slabs()
+            self._rows, self._views = P, (k.first(P), v.first(P), None)
+        return self._views
 
 
 class MXKVCache:
