@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import weakref
 
 import torch
 
@@ -274,6 +275,27 @@ def _backward(rope: AxialRope, xs, ws, eps, grads):
     return dx, dw
 
 
+# A leaf's node of the backward pass belongs to the stream on which the first graph
+# that is still alive was recorded, and the backward pass waits on that stream.  A
+# capture on another one would not survive that, so it is refused while it can be:
+# by leaf, that stream and the recorded calls.
+_LEAVES: dict = {}
+
+
+def _record(call, leaves, stream: int, capturing: bool) -> None:
+    """Note that `call` (its ctx) is recorded on `stream`; RuntimeError if a capture could not run its backward pass."""
+    for t in leaves:
+        here = _LEAVES.get(id(t))
+        alive = [] if here is None else [r for r in here[1] if r() is not None]
+        if alive and capturing and here[0] != stream:
+            raise RuntimeError("a graph of the same leaves, recorded on another stream, is alive: its outputs have to be "
+                               "dropped before a call with gradients is captured")
+        if not alive and len(_LEAVES) >= 4096:
+            for k in [k for k, (_, refs) in _LEAVES.items() if all(r() is None for r in refs)]:
+                del _LEAVES[k]
+        _LEAVES[id(t)] = (here[0] if alive else stream, [*alive, weakref.ref(call)])
+
+
 class _NormRope(torch.autograd.Function):
     """One or two tensors: (rope, eps, n, x.., w..) -> y.."""
 
@@ -281,6 +303,9 @@ class _NormRope(torch.autograd.Function):
     def forward(ctx, rope, eps, n, *ts):
         xs, ws = list(ts[:n]), list(ts[n:])
         ctx.rope, ctx.eps, ctx.n = rope, eps, n
+        leaves = [t for t in ts if t is not None and t.requires_grad and t.is_leaf]
+        if leaves and xs[0].is_cuda:
+            _record(ctx, leaves, _raw_stream(xs[0].device.index), torch.cuda.is_current_stream_capturing())
         # the positions are saved with the inputs: a change before the backward pass is an error there
         ctx.save_for_backward(rope._positions, *ts)
         return tuple(_forward(rope, xs, ws, eps))

@@ -312,3 +312,28 @@ def test_plans_made_anew_share_their_frequencies():
             for i in range(2):
                 xd, wd = x[i].double(), w[i].double()
                 _within(out[i], oa.forward(xd, wd, angle, pairs, EPS), oa.forward_bound(xd, wd, angle, pairs, EPS, torch.bfloat16))
+
+
+def test_a_capture_beside_a_live_graph_is_refused():
+    x, w, d, _, rope = _one()
+    leaves = [t.requires_grad_() for t in (*x, *w)]
+    alive = qik.fused_qk_norm_rope(*leaves, rope, EPS)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(RuntimeError, match="alive"):
+            qik.fused_qk_norm_rope(*leaves, rope, EPS)
+        with torch.no_grad():
+            free = qik.fused_qk_norm_rope(*leaves, rope, EPS)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(alive, free))
+    want = [t.clone() for t in torch.autograd.grad(alive, leaves, d)]
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = torch.autograd.grad(qik.fused_qk_norm_rope(*leaves, rope, EPS), leaves, d)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))

@@ -308,3 +308,27 @@ def test_rope_oracle_gradient_against_differences(pairs):
     w = torch.randn(32, generator=g, dtype=torch.float64).requires_grad_()
     angle = oa.angles(torch.randn(3, 3, generator=g) * 30, (4, 14, 14), 1e4, "axis")
     assert torch.autograd.gradcheck(lambda a, b: oa.forward(a, b, angle, pairs, 1e-3), (x, w))
+
+
+def test_leaves_of_a_live_graph():
+    """A capture is refused while a graph of the same leaves from another stream is alive, and only then."""
+    from qwen_image_kernel_amd import rope as R
+
+    class Call:
+        pass
+
+    a, b = torch.ones(2, requires_grad=True), torch.ones(2, requires_grad=True)
+    eager = Call()
+    R._record(eager, [a], 1, False)
+    R._record(Call(), [a, b], 2, False)          # dropped at once; a's first graph is still stream 1's
+    with pytest.raises(RuntimeError):
+        R._record(Call(), [b, a], 2, True)
+    R._record(Call(), [b], 2, True)
+    R._record(Call(), [a], 1, True)              # the same stream
+    later = Call()
+    R._record(later, [a], 2, False)
+    del eager
+    with pytest.raises(RuntimeError):            # `later` keeps the node of stream 1
+        R._record(Call(), [a], 2, True)
+    del later
+    R._record(Call(), [a], 2, True)
