@@ -748,7 +748,7 @@ __global__ void __launch_bounds__(NTHREADS * KSPLIT, (KSPLIT == 1 && D <= 128) ?
       }
     } else {
       if (early) issue_seg(has_slab(), 0, 0);
-      Lrow = live ? Lraw : -1;
+      Lrow = live ? max(Lraw, -1) : -1;  // (any negative length: Lrow - kv0 stays in range)
       const int lmax = wave_reduce_i32<true>(live ? Lrow : -1);
       wave_minL = wave_reduce_i32<false>(live ? Lrow : INT_MAX);
       wave_maxL = lmax;

@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(64 * rows_waves(D, MT), D <= 128 && MT == 1 ? 
     for (int j = 0; j < KSTEPS; ++j) qreg[mt][j] = gload16(qr + 16 * j);
     Lrow[mt] = p.KV - 1;
     if (!p.uniform) {
-      const int Lraw = gload_i32(p.L + b * p.sL_b + tok);
+      const int Lraw = max(gload_i32(p.L + b * p.sL_b + tok), -1);  // (any negative length: Lrow - kv0 stays in range)
       Lrow[mt] = live ? Lraw : -1;
       Lmax = max(Lmax, Lrow[mt]);
       Lmin = min(Lmin, live ? Lraw : INT_MAX);

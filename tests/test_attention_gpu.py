@@ -677,3 +677,21 @@ def test_random_configurations_vs_oracle(cfg):
     if heads is not None:
         o, ref = o[:, :, heads], ref[:, :, heads]
     _check(o, ref, what=f"random {cfg['seed']}")
+
+
+@pytest.mark.parametrize("SQ,SN,P", [(40, 40, 400), (1100, 1100, 0), (2816, 70, 500)])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+def test_lengths_far_below_zero(SQ, SN, P, D):
+    """Rows of length -2^31 and the like, next to rows that see keys, see nothing."""
+    g = torch.Generator().manual_seed(SQ + D)
+    q = _rand((1, SQ, 6, D), g).to(DEV)
+    k, v, ck, cv = (_rand((1, n, 6, D), g).to(DEV) for n in (SN, SN, P, P))
+    L = torch.randint(0, P + SN, (SQ,), generator=g, dtype=torch.int32).to(DEV)
+    none = (torch.rand(SQ, generator=g) < 0.4).to(DEV)
+    none[0], L[0] = False, P + SN - 1
+    cache = dict(cache_k=ck, cache_v=cv) if P else {}
+    for valid in (None, (torch.rand(1, P + SN, generator=g) < 0.8).to(DEV)):
+        want = qik.block_causal_flash_attention(q, k, v, torch.where(none, -1, L), valid, **cache)
+        assert (want[:, none] == 0).all()
+        for low in (-2 ** 31, -2 ** 31 + 3, -2):
+            assert torch.equal(qik.block_causal_flash_attention(q, k, v, torch.where(none, low, L), valid, **cache), want), low

@@ -594,3 +594,24 @@ def test_lengths_of_a_slab_without_rows(S):
     ln = torch.tensor([0, 7, -2], dtype=torch.int32, device=DEV)
     slabs = [_mx(*t, 0, ln) for t in (kc, vc)]
     _check(_call(q, k, v, *slabs), _parts(q, k, v, kc, vc, 0, om.allowed(B, S, 0, SN)), D, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("shape", [FEW, (1, 40, 40, 400, 2, 2), MANY])
+def test_causal_lengths_far_below_zero(shape, D, dtype):
+    """Rows of length -2^31 and the like, next to rows that see keys, see nothing."""
+    B, SQ, SN, P, H, HKV = shape
+    q, k, v, kc, vc = _inputs(shape, D, dtype, seed=31)
+    ck, cv = _mx(*kc, P), _mx(*vc, P)
+    g = torch.Generator().manual_seed(31)
+    L = torch.randint(0, P + SN, (B, SQ), generator=g, dtype=torch.int32)
+    none = torch.rand(B, SQ, generator=g) < 0.4
+    none[:, 1] = True
+    none[:, 0], L[:, 0] = False, P + SN - 1
+    valid = torch.rand(B, P + SN, generator=g) < 0.8
+    for mask in (None, valid):
+        want = _call(q, k, v, ck, cv, torch.where(none, -1, L), mask)
+        assert (want.cpu()[none] == 0).all()
+        for low in (-2 ** 31, -2 ** 31 + 3, -2):
+            assert torch.equal(_call(q, k, v, ck, cv, torch.where(none, low, L), mask), want), low
