@@ -220,7 +220,7 @@ def block_causal_flash_attention(
         _check_aux("prefix_lengths", prefix_lengths, dev)
         L = prefix_lengths
         if L.dtype != torch.int32 or not L.is_contiguous():
-            L = L.to(torch.int32).contiguous()
+            L = _int32(L)
         assert L.numel() >= SQ, "prefix_lengths must be [SQ]"
 
     if debug_tiles is not None:
@@ -267,6 +267,13 @@ def _check_aux(name: str, t: torch.Tensor, dev: torch.device) -> None:
         raise ValueError(f"{name} must be a tensor on {dev}")
     if t.device != dev:
         raise ValueError(f"{name} is on {t.device}; it must be on the query's device {dev}")
+
+
+def _int32(L: torch.Tensor) -> torch.Tensor:
+    """Causal lengths as dense int32; 64-bit ones past its range become the nearest: no key, or every one."""
+    if L.dtype == torch.int64:
+        L = L.clamp(-1, 2 ** 31 - 1)
+    return L.to(torch.int32).contiguous()
 
 
 # Argument structs by call geometry: everything of qik_attn_args except the

@@ -75,7 +75,7 @@ def mx_slab_attention(query, key, value, prefix_lengths, key_valid, cache_k, cac
     a.q, a.k_new, a.v_new, a.out = q, k, v, out.data_ptr()
     if L is not None:
         if c.L:
-            L = L.to(torch.int32).contiguous()
+            L = _attn._int32(L)
         a.prefix_lengths = L.data_ptr()
     if key_valid is not None:
         key_valid = _valid_bytes(key_valid, c.valid)

@@ -695,3 +695,17 @@ def test_lengths_far_below_zero(SQ, SN, P, D):
         assert (want[:, none] == 0).all()
         for low in (-2 ** 31, -2 ** 31 + 3, -2):
             assert torch.equal(qik.block_causal_flash_attention(q, k, v, torch.where(none, low, L), valid, **cache), want), low
+
+
+def test_lengths_in_64_bits():
+    """Past 32 bits a length is as its nearest one: no key, or every one."""
+    g = torch.Generator().manual_seed(41)
+    S = 300
+    q, k, v = (_rand((1, S, 2, 128), g).to(DEV) for _ in range(3))
+    L = torch.randint(-1, S, (S,), generator=g)
+    far = torch.tensor([-2 ** 63, -2 ** 40, -2 ** 32, 2 ** 31, 2 ** 32, 2 ** 40, 2 ** 63 - 1])
+    pick = far[torch.randint(0, far.numel(), (S,), generator=g)]
+    where = torch.rand(S, generator=g) < 0.5
+    near = torch.where(pick < 0, -1, S - 1)
+    want = qik.block_causal_flash_attention(q, k, v, torch.where(where, near, L).to(torch.int32).to(DEV), None)
+    assert torch.equal(qik.block_causal_flash_attention(q, k, v, torch.where(where, pick, L).to(DEV), None), want)

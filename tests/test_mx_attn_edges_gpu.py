@@ -615,3 +615,21 @@ def test_causal_lengths_far_below_zero(shape, D, dtype):
         assert (want.cpu()[none] == 0).all()
         for low in (-2 ** 31, -2 ** 31 + 3, -2):
             assert torch.equal(_call(q, k, v, ck, cv, torch.where(none, low, L), mask), want), low
+
+
+@pytest.mark.parametrize("shape", [FEW, MANY])
+def test_causal_lengths_in_64_bits(shape):
+    """Past 32 bits a length is as its nearest one: no key, or every one."""
+    B, SQ, SN, P, H, HKV = shape
+    q, k, v, kc, vc = _inputs(shape, seed=37)
+    ck, cv = _mx(*kc, P), _mx(*vc, P)
+    g = torch.Generator().manual_seed(37)
+    L = torch.randint(-1, P + SN, (SQ,), generator=g)
+    far = torch.tensor([-2 ** 63, -2 ** 40, -2 ** 32, 2 ** 31, 2 ** 32, 2 ** 40, 2 ** 63 - 1])
+    where = torch.rand(SQ, generator=g) < 0.5
+    where[0] = True
+    pick = far[torch.randint(0, far.numel(), (SQ,), generator=g)]
+    near = torch.where(pick < 0, -1, P + SN - 1)
+    want = _call(q, k, v, ck, cv, torch.where(where, near, L).to(torch.int32))
+    assert torch.equal(_call(q, k, v, ck, cv, torch.where(where, pick, L)), want)
+    assert torch.equal(_call(q, k, v, ck, cv, torch.where(where, pick, L)[None].expand(B, -1)), want)
