@@ -1,11 +1,14 @@
 """GPU tests of the 4-bit slab where it can go wrong: hidden values, layouts, lengths, places, streams, graphs, the
 processor's path."""
 
+import ctypes
+
 import pytest
 import torch
 
 import qwen_image_kernel_amd as qik
 from oracle import mx_slab as om
+from qwen_image_kernel_amd import _lib
 from test_mx_attn_gpu import DEV, _check, _few, _mx, _randn, _slab
 
 pytestmark = pytest.mark.gpu
@@ -633,3 +636,50 @@ def test_causal_lengths_in_64_bits(shape):
     want = _call(q, k, v, ck, cv, torch.where(where, near, L).to(torch.int32))
     assert torch.equal(_call(q, k, v, ck, cv, torch.where(where, pick, L)), want)
     assert torch.equal(_call(q, k, v, ck, cv, torch.where(where, pick, L)[None].expand(B, -1)), want)
+
+
+def _spreads(B, SQ, SN, P, H, HKV, D) -> bool:
+    """Whether the kernel deals out the keys of all entries together: the plan then aims at more pieces than an entry alone
+    is ever cut into (a piece has a step of 32 keys for each of 8 waves, two from 8 pieces on)."""
+    few, tiles, pieces = (ctypes.c_int32() for _ in range(3))
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    assert _lib.load().qik_mx_attn_plan(B, SQ, SN, P, H, HKV, D, 1, cus, ctypes.byref(few), ctypes.byref(tiles),
+                                        ctypes.byref(pieces)) == 0
+    steps = max((-(-P // 32) + -(-SN // 32)) // 8, 1)
+    return few.value == 1 and tiles.value == 1 and pieces.value > max(steps // 2, min(steps, 8))
+
+
+# B, SQ, SN, P, H, HKV, D, dtype: entries below, at and past a wave's 64, past two and four times that
+TOGETHER = [(24, 1, 1, 4000, 16, 4, 128, torch.bfloat16), (64, 1, 2, 1100, 4, 1, 128, torch.bfloat16),
+            (65, 1, 0, 1100, 4, 1, 128, torch.float16), (65, 2, 2, 4500, 4, 2, 32, torch.bfloat16),
+            (128, 1, 1, 1100, 4, 1, 128, torch.bfloat16), (130, 1, 0, 1100, 8, 2, 64, torch.float16),
+            (129, 3, 3, 1100, 4, 1, 256, torch.bfloat16), (200, 1, 2, 1600, 4, 1, 128, torch.bfloat16),
+            (300, 1, 0, 620, 2, 2, 256, torch.bfloat16), (300, 1, 2, 1558, 4, 1, 32, torch.float16)]
+
+
+@pytest.mark.parametrize("case", TOGETHER)
+def test_entries_dealt_out_together(case):
+    """Pieces over all entries, in chunks of a wave's lanes: no key lost, none read twice, with and without masks."""
+    B, SQ, SN, P, H, HKV, D, dtype = case
+    assert _spreads(*case[:-1])
+    g = torch.Generator().manual_seed(B + D)
+    q, k, v = (_randn(g, B, n, h, D).to(dtype) for n, h in ((SQ, H), (SN, HKV), (SN, HKV)))
+    kc, vc = ((torch.randint(0, 256, (B, HKV, P, D // 2), generator=g, dtype=torch.uint8),
+               torch.randint(123, 127, (B, HKV, P, D // 32), generator=g, dtype=torch.uint8)) for _ in range(2))
+    every = torch.randint(0, P + 1, (B,), generator=g, dtype=torch.int32)
+    one = every.clamp_max(3)
+    one[B * 2 // 3] = P
+    few = torch.where(torch.arange(B) < B - 3, 0, every)
+    ends = torch.where(torch.rand(B, generator=g) < 0.5, every - P, every + P // 2)
+    L = torch.randint(-1, P + SN, (B, SQ), generator=g, dtype=torch.int32)
+    valid = torch.rand(B, P + SN, generator=g) < 0.8
+    keys, values = (torch.cat((om.decode(c, s).transpose(1, 2).to(DEV), t.to(DEV).double()), 1) for (c, s), t in ((kc, k), (vc, v)))
+    for ln, lengths, mask in ((every, None, None), (every, L, None), (every, None, valid), (every, L, valid), (one, None, None),
+                              (one, L, valid), (few, None, None), (few, None, valid), (torch.full_like(every, P), None, None),
+                              (torch.zeros_like(every), None, None), (ends, None, None), (ends, L, valid)):
+        slabs = [_mx(*t, P, ln.to(DEV)) for t in (kc, vc)]
+        out = _call(q, k, v, *slabs, lengths, mask)
+        ok = om.allowed(B, SQ, P, SN, lengths, mask, ln).to(DEV)
+        _check(out, om.attention(q.to(DEV).double(), keys, values, ok), D, dtype)
+        assert (out[~ok.any(-1)] == 0).all()
+        assert torch.equal(out, _call(q, k, v, *slabs, lengths, mask))
