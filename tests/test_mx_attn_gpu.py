@@ -164,3 +164,24 @@ def test_masks_and_lengths(shape, dtype):
     _case(*shape, 128, dtype, 5, L=L[0], valid=valid)
     out, ok = _case(*shape, 128, dtype, 6, L=L, valid=valid, lengths=lengths)
     assert (out.cpu()[~ok.any(-1)] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("e", [0, 255])
+def test_every_code_at_the_ends_of_the_scale(dtype, e):
+    """Scale byte 0 is 2^-127, also for elements that are not zero; 255 makes its block NaN."""
+    cache = qik.MXKVCache(1, 1, 4, 2, 32, device=DEV, dtype=dtype)
+    codes = torch.arange(16, dtype=torch.uint8)
+    cache.k_codes[0] = (codes | (codes.flip(0) << 4)).to(DEV)
+    cache.v_codes[0] = (codes.flip(0) | (codes << 4)).to(DEV)
+    cache.k_scales.fill_(e)
+    cache.v_scales.fill_(e)
+    cache.lengths.fill_(4)
+    cache._host_lengths[0] = 4
+    for t, c in zip(cache.get_layer(0).get(), (cache.k_codes, cache.v_codes)):
+        want = om.decode(c[0].transpose(1, 2), torch.full((1, 4, 2, 1), e, dtype=torch.uint8)).to(dtype)
+        if e == 255:
+            assert t.isnan().all() and want.isnan().all()
+        else:
+            assert torch.equal(t.cpu().double(), want.double())
+            assert dtype == torch.float16 or (t != 0).sum() == t.numel() * 14 // 16
