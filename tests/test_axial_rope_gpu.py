@@ -337,3 +337,24 @@ def test_a_capture_beside_a_live_graph_is_refused():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_offsets_past_32_bits():
+    """Entries, then tokens, behind 4 GB of each other, in the inputs and in the gradients that come in."""
+    B, S, Hq, Hk, D = 2, 5, 3, 2, 64
+    x, w, d, _, rope = _one(B, S, Hq, Hk, D)
+    buf = torch.zeros(2_400_000_000, dtype=torch.bfloat16, device=DEV)
+
+    def both(xs, ds):
+        leaves = [t.detach().requires_grad_() for t in (*xs, *w)]
+        out = qik.fused_qk_norm_rope(*leaves, rope, EPS)
+        return [*out, *torch.autograd.grad(out, leaves, ds)]
+
+    want = both(x, d)
+    for strides in ((2_300_000_000, 512, 64, 1), (512, 550_000_000, 64, 1)):
+        def put(t, i):   # in turn within the 512 elements of a row of tokens
+            return buf[4096 * i:].as_strided(t.shape, strides).copy_(t)
+
+        for which in ((0,), (1,), (2, 3)):
+            ts = [put(t, i) if i in which else t for i, t in enumerate((*x, *d))]
+            assert all(torch.equal(a, b) for a, b in zip(both(ts[:2], ts[2:]), want)), (strides, which)

@@ -683,3 +683,23 @@ def test_entries_dealt_out_together(case):
         _check(out, om.attention(q.to(DEV).double(), keys, values, ok), D, dtype)
         assert (out[~ok.any(-1)] == 0).all()
         assert torch.equal(out, _call(q, k, v, *slabs, lengths, mask))
+
+
+def test_store_and_read_past_32_bits():
+    """Rows of a slab and of the states behind 4 GB; an entry's last rows, which alone are not zeros."""
+    B, H, D, cap, S = 2, 16, 256, 1_200_000, 3
+    assert H * B * cap * D // 2 > 2 ** 32
+    cache = qik.MXKVCache(1, B, cap, H, D, device=DEV)
+    buf = torch.zeros(2_300_000_000 + 2 * S * H * D, dtype=torch.bfloat16, device=DEV)
+    x = _states(3, B, S, H, D)
+    far = [buf[i * S * H * D:].as_strided((B, S, H, D), (2_300_000_000 // 8 * 8, H * D, D, 1)).copy_(t) for i, t in enumerate(x)]
+    layer = cache.get_layer(0)
+    layer.append(*far, cap - S)
+    assert cache.lengths[0].tolist() == [cap] * B
+    got = layer.get()
+    for t, g, codes, scales in zip(x, got, (cache.k_codes, cache.v_codes), (cache.k_scales, cache.v_scales)):
+        wc, we = _bytes_of(t)
+        assert torch.equal(codes[0, :, :, -S:].cpu(), wc) and torch.equal(scales[0, :, :, -S:].cpu(), we)
+        assert not codes[0, -1, -1, :-S].any() and not codes[0, 0, 0, :-S].any()
+        assert torch.equal(g[:, -S:].cpu().double(), om.decode(wc, we).transpose(1, 2))
+        assert not g[-1, -1000:-S].any()
