@@ -270,7 +270,7 @@ class _MXLayerView(_SlabLayer):
             self._lengths.fill_(P)
         else:
             self._launch(call, k, v, None, False)
-        c._host_lengths[self._layer], c._exact[self._layer] = P, True
+        self._note(P, True, P)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, at: torch.Tensor | int | None = None) -> None:
         """k, v ``[B, S, H, D]`` become rows ``at[b]`` .. ``at[b] + S - 1`` of batch entry b, whose length is then
@@ -280,7 +280,8 @@ class _MXLayerView(_SlabLayer):
         ``[B]`` device tensor, which must not overlap the layer's ``lengths``
         unless it is them.  Rows past the capacity are not written; where the
         host knows the lengths (they came from ``store``, or from appends with
-        None or an int outside of graph capture) that is a ValueError instead."""
+        None or an int, and no store or append of the layer was ever captured
+        into a graph) that is a ValueError instead."""
         c, i, lengths = self._c, self._layer, self._lengths
         S = k.shape[1] if k.dim() == 4 else 0
         call = self._call(k, v)
@@ -293,28 +294,43 @@ class _MXLayerView(_SlabLayer):
             grow = here == first and at.is_contiguous()
             if not grow and (not at.is_contiguous() or abs(here - first) < 4 * c.batch_size):
                 at = at.clone(memory_format=torch.contiguous_format)
-            n, exact = c.capacity, False
+            n, exact, most = c.capacity, False, c.capacity
         elif at is not None:
             at = int(at)
             if at < 0 or at + S > c.capacity:
                 raise ValueError(f"{S} tokens at {at} exceed the slab capacity {c.capacity}")
             lengths.fill_(at)
-            n, exact, at = at + S, True, lengths
+            n, exact, most, at = at + S, True, at + S, lengths
         else:
-            n, exact, at = c._host_lengths[i], c._exact[i], lengths
+            n, exact, most, at = c._host_lengths[i], c._exact[i], c.capacity, lengths
             if exact and n + S > c.capacity:
                 raise ValueError(f"{S} tokens behind {n} exceed the slab capacity {c.capacity}")
             n = min(n + S, c.capacity)
-            if torch.cuda.is_current_stream_capturing():
-                # a replay grows the entries further than the host sees
-                n, exact = c.capacity, False
         if call is not None:
             self._launch(call, k, v, at, grow)
         elif not grow:
             lengths.copy_((at + S).clamp_(0, c.capacity))
         elif S:
             lengths.add_(S).clamp_(0, c.capacity)
+        self._note(n, exact, most)
+
+    def _note(self, n: int, exact: bool, most: int) -> None:
+        """Keep what the host knows after a call: no entry is longer than n, and with `exact` each is that long; `most`: how
+        long replays of the call may leave one."""
+        c, i = self._c, self._layer
+        if self._capturing():
+            # nothing has run yet, and a replay comes when the program likes, unseen by the host
+            n, c._captured[i] = c._host_lengths[i], max(most, c._captured[i] or 0)
+        if c._captured[i] is not None:
+            n, exact = max(n, c._captured[i]), False
         c._host_lengths[i], c._exact[i] = n, exact
+
+    def _capturing(self) -> bool:
+        idx = self._lengths.device.index
+        if idx == torch._C._cuda_getDevice():
+            return torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(idx):
+            return torch.cuda.is_current_stream_capturing()
 
     def _call(self, k: torch.Tensor, v: torch.Tensor):
         """The prepared store of operands like these; None where there are no rows."""
@@ -387,7 +403,8 @@ class _MXLayerView(_SlabLayer):
     def views(self, P: int | None = None):
         """(k, v, None) for block_causal_flash_attention: ``MXSlab`` views of the first P rows, with the entries'
         lengths.  P by default is the longest length as far as the host knows it (the capacity after an append whose
-        places only the device knows); fewer rows plan a call for fewer keys, and leave out what lies behind them."""
+        places only the device knows, and from the first captured append on, whose replays the host does not see); fewer
+        rows plan a call for fewer keys, and leave out what lies behind them."""
         c = self._c
         if P is None:
             P = c._host_lengths[self._layer]
@@ -439,6 +456,7 @@ class MXKVCache:
         self._arrivals = counts[num_layers * batch:]
         self._host_lengths = [0] * num_layers   # no entry of the layer is longer
         self._exact = [True] * num_layers       # ... and every one is that long, if the program changed none
+        self._captured: list = [None] * num_layers  # the longest that replays of captured calls may leave, None without such
         self.layers = [_MXLayerView(self, i) for i in range(num_layers)]
 
     def get_layer(self, i: int) -> _MXLayerView:

@@ -703,3 +703,42 @@ def test_store_and_read_past_32_bits():
         assert not codes[0, -1, -1, :-S].any() and not codes[0, 0, 0, :-S].any()
         assert torch.equal(g[:, -S:].cpu().double(), om.decode(wc, we).transpose(1, 2))
         assert not g[-1, -1000:-S].any()
+
+
+@pytest.mark.parametrize("fill", ["store", "append at an int", "append"])
+def test_a_cache_filled_anew_after_its_step_was_captured(fill):
+    """get() and the default views hold what replays appended behind an eager store or append, as an eager cache's do."""
+    B, H, HKV, D, cap = 2, 4, 2, 64, 300
+    caches = [qik.MXKVCache(1, B, cap, HKV, D, device=DEV) for _ in range(2)]
+    for c in caches:
+        c.get_layer(0).store(*_states(1, B, 80, HKV, D))
+    k, v = (torch.empty(B, 1, HKV, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        caches[0].get_layer(0).append(k, v)
+    for c in caches:
+        layer = c.get_layer(0)
+        if fill == "store":
+            layer.store(*_states(2, B, 50, HKV, D))
+        elif fill == "append":
+            layer.append(*_states(2, B, 50, HKV, D))
+        else:
+            layer.append(*_states(2, B, 10, HKV, D), 40)
+    for i in range(10):
+        k.copy_(_states(10 + i, B, 1, HKV, D)[0])
+        v.copy_(_states(30 + i, B, 1, HKV, D)[1])
+        graph.replay()
+        caches[1].get_layer(0).append(k, v)
+    torch.cuda.synchronize()
+    n = int(caches[1].lengths[0, 0])
+    assert torch.equal(caches[0].lengths, caches[1].lengths) and n == (140 if fill == "append" else 60)
+    q = _randn(torch.Generator().manual_seed(3), B, 1, H, D).to(torch.bfloat16).to(DEV)
+    for c in caches:
+        ck, cv, _ = c.get_layer(0).views()
+        keys = [om.decode(x[0, :, :, :n], e[0, :, :, :n]).transpose(1, 2) for x, e in ((c.k_codes, c.k_scales), (c.v_codes, c.v_scales))]
+        _check(_call(q, k[:, :0], v[:, :0], ck, cv), om.attention(q.cpu().double(), *keys, om.allowed(B, 1, n, 0)), D, torch.bfloat16)
+        for got, want in zip(c.get_layer(0).get(), keys):
+            assert torch.equal(got[:, :n].cpu().double(), want) and not got[:, n:].any()
+    for t in ("k_codes", "k_scales", "v_codes", "v_scales"):
+        assert torch.equal(*(getattr(c, t)[:, :, :, :n] for c in caches))

@@ -332,3 +332,94 @@ def test_leaves_of_a_live_graph():
         R._record(Call(), [a], 2, True)
     del later
     R._record(Call(), [a], 2, True)
+
+
+# ---- what the host knows of a cache's lengths ------------------------------
+
+@pytest.fixture
+def cache_on_the_host(monkeypatch):
+    """MXKVCache with its buffers in host memory and the store's effect on the lengths in the launch's place; a call made
+    while `capturing[0]` changes nothing and is appended to `recorded`, which a replay runs."""
+    from qwen_image_kernel_amd import kv_cache as K
+
+    zeros, capturing, recorded = torch.zeros, [False], []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: None, raising=False)
+
+    def launch(layer, call, k, v, at, grow):
+        def run():
+            lengths = layer._lengths.data     # as a kernel does: no version moves
+            first = torch.zeros_like(lengths) if at is None else at
+            lengths.copy_((first + k.shape[1]).clamp(0, layer._c.capacity))
+        recorded.append(run) if capturing[0] else run()
+
+    monkeypatch.setattr(K._MXLayerView, "_launch", launch)
+    monkeypatch.setattr(K, "load_args", lambda *a: None)
+
+    def make(layers=1, batch=2, capacity=100):
+        with monkeypatch.context() as m:
+            m.setattr(torch, "zeros", lambda *a, device=None, **kw: zeros(*a, **kw))
+            return qik.MXKVCache(layers, batch, capacity, 1, 32)
+
+    return make, capturing, recorded
+
+
+def _states(n, batch=2):
+    return [torch.zeros(batch, n, 1, 32, dtype=torch.bfloat16) for _ in range(2)]
+
+
+def test_replays_of_captured_steps_are_reckoned_with(cache_on_the_host):
+    """However a layer is filled after its step was captured, its default views hold what replays appended."""
+    make, capturing, recorded = cache_on_the_host
+    for fill in (lambda layer: layer.store(*_states(50)), lambda layer: layer.append(*_states(5), 45),
+                 lambda layer: layer.store(*_states(0))):
+        cache = make()
+        layer = cache.get_layer(0)
+        layer.store(*_states(80))
+        del recorded[:]
+        capturing[0] = True
+        layer.append(*_states(1))
+        capturing[0] = False
+        assert cache.lengths[0].tolist() == [80, 80] and layer.views()[0].shape[1] == 100
+        fill(layer)
+        start = int(cache.lengths[0, 0])
+        for i in range(10):
+            recorded[0]()
+            assert int(cache.lengths[0, 0]) == start + i + 1 <= layer.views()[0].shape[1]
+        layer.append(*_states(3))
+        assert int(cache.lengths[0, 0]) == start + 13 <= layer.views()[0].shape[1]
+        layer.append(*_states(60))               # (no ValueError by a count that is not theirs)
+        layer.append(*_states(60))
+        assert cache.lengths[0].tolist() == [100, 100]
+
+
+def test_captured_stores_and_places_are_no_present_lengths(cache_on_the_host):
+    """A captured call moves no length before it is replayed, and any time after."""
+    make, capturing, recorded = cache_on_the_host
+    cache = make(2)
+    layer, other = cache.get_layer(0), cache.get_layer(1)
+    layer.store(*_states(60))
+    other.store(*_states(7))
+    del recorded[:]
+    capturing[0] = True
+    layer.store(*_states(20))
+    capturing[0] = False
+    assert layer.views()[0].shape[1] == 60
+    recorded[0]()
+    layer.append(*_states(90))                   # behind 20, not 60: some rows do not fit, and none is refused
+    layer.store(*_states(3))
+    assert layer.views()[0].shape[1] == 20       # what a replay may leave
+    recorded[0]()
+    assert cache.lengths[0].tolist() == [20, 20]
+    capturing[0] = True
+    layer.append(*_states(2), 70)
+    capturing[0] = False
+    assert layer.views()[0].shape[1] == 72
+    cache.lengths[0].fill_(20)
+    recorded[1]()
+    assert layer.views()[0].shape[1] >= 72
+    # the other layer's lengths are still known
+    assert other.views()[0].shape[1] == 7
+    other.append(*_states(93))
+    with pytest.raises(ValueError):
+        other.append(*_states(1))
