@@ -27,6 +27,7 @@ fp8-V one 768, with a length for each batch entry and tokens appended behind it
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -267,7 +268,8 @@ class _MXLayerView(_SlabLayer):
         if P > c.capacity:
             raise ValueError(f"prefix of {P} tokens exceeds the slab capacity {c.capacity}")
         if P == 0 or call is None:
-            self._lengths.fill_(P)
+            with c._writing_lengths():
+                self._lengths.fill_(P)
         else:
             self._launch(call, k, v, None, False)
         self._note(P, True, P)
@@ -280,8 +282,9 @@ class _MXLayerView(_SlabLayer):
         ``[B]`` device tensor, which must not overlap the layer's ``lengths``
         unless it is them.  Rows past the capacity are not written; where the
         host knows the lengths (they came from ``store``, or from appends with
-        None or an int, and no store or append of the layer was ever captured
-        into a graph) that is a ValueError instead."""
+        None or an int, no store or append of the layer was ever captured into a
+        graph, and the program never wrote into ``lengths`` itself) that is a
+        ValueError instead."""
         c, i, lengths = self._c, self._layer, self._lengths
         S = k.shape[1] if k.dim() == 4 else 0
         call = self._call(k, v)
@@ -299,19 +302,19 @@ class _MXLayerView(_SlabLayer):
             at = int(at)
             if at < 0 or at + S > c.capacity:
                 raise ValueError(f"{S} tokens at {at} exceed the slab capacity {c.capacity}")
-            lengths.fill_(at)
+            with c._writing_lengths():
+                lengths.fill_(at)
             n, exact, most, at = at + S, True, at + S, lengths
         else:
-            n, exact, most, at = c._host_lengths[i], c._exact[i], c.capacity, lengths
+            n, exact, most, at = c._host_lengths[i], c._exact[i] and not c._lengths_written(), c.capacity, lengths
             if exact and n + S > c.capacity:
                 raise ValueError(f"{S} tokens behind {n} exceed the slab capacity {c.capacity}")
             n = min(n + S, c.capacity)
         if call is not None:
             self._launch(call, k, v, at, grow)
-        elif not grow:
-            lengths.copy_((at + S).clamp_(0, c.capacity))
-        elif S:
-            lengths.add_(S).clamp_(0, c.capacity)
+        elif S or not grow:
+            with c._writing_lengths():
+                lengths.copy_((at + S).clamp_(0, c.capacity))
         self._note(n, exact, most)
 
     def _note(self, n: int, exact: bool, most: int) -> None:
@@ -423,9 +426,10 @@ class MXKVCache:
     scales ``k_scales``, ``v_scales`` uint8 ``[L, B, H, P_max, D / 32]``, the
     format of ``quantize_mx`` (an infinity or NaN makes its block NaN);
     ``lengths`` int32 ``[L, B]``, kept on the device by ``store`` and ``append``.  A
-    program may lower lengths itself (an entry that ends and starts anew);
-    they grow through ``append`` alone.  ``num_heads`` counts the keys' heads,
-    which may be fewer than the queries'.  HIP devices only."""
+    program may lower lengths itself (an entry that ends and starts anew), by
+    torch's in-place operations; they grow through ``append`` alone.  ``append``
+    then no longer says when an entry is full.  ``num_heads`` counts the keys'
+    heads, which may be fewer than the queries'.  HIP devices only."""
 
     def __init__(
         self,
@@ -451,13 +455,29 @@ class MXKVCache:
         # (the codes first: their part is a multiple of 16 bytes long, the scales' of what their rows need)
         parts = torch.zeros(rows * sum(widths), dtype=torch.uint8, device=device).split([rows * w for w in widths])
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = (t.view(*shape, w) for t, w in zip(parts, widths))
-        counts = torch.zeros(num_layers * (batch + 1), dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # (an inference tensor does not say whether it was written to)
+            counts = torch.zeros(num_layers * (batch + 1), dtype=torch.int32, device=device)
         self.lengths = counts[:num_layers * batch].view(num_layers, batch)
         self._arrivals = counts[num_layers * batch:]
         self._host_lengths = [0] * num_layers   # no entry of the layer is longer
         self._exact = [True] * num_layers       # ... and every one is that long, if the program changed none
         self._captured: list = [None] * num_layers  # the longest that replays of captured calls may leave, None without such
+        # `lengths` counts torch's writes into it, whatever view they go through; the kernels' are no such
+        self._version, self._program_writes = self.lengths._version, False
         self.layers = [_MXLayerView(self, i) for i in range(num_layers)]
+
+    def _lengths_written(self) -> bool:
+        """Whether the program ever wrote into ``lengths`` itself."""
+        if self.lengths._version != self._version:
+            self._program_writes = True
+        return self._program_writes
+
+    @contextlib.contextmanager
+    def _writing_lengths(self):
+        """Around the cache's own writes by torch."""
+        self._lengths_written()
+        yield
+        self._version = self.lengths._version
 
     def get_layer(self, i: int) -> _MXLayerView:
         return self.layers[i]

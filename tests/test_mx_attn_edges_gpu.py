@@ -742,3 +742,25 @@ def test_a_cache_filled_anew_after_its_step_was_captured(fill):
             assert torch.equal(got[:, :n].cpu().double(), want) and not got[:, n:].any()
     for t in ("k_codes", "k_scales", "v_codes", "v_scales"):
         assert torch.equal(*(getattr(c, t)[:, :, :, :n] for c in caches))
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_an_entry_that_starts_anew(inference):
+    """Entries set back by the program take tokens again, in every entry up to the slab's last row and no further."""
+    B, H, D, cap = 3, 2, 64, 9
+    with torch.inference_mode(inference):
+        cache = qik.MXKVCache(1, B, cap, H, D, device=DEV)
+        layer = cache.get_layer(0)
+        layer.store(*_states(1, B, 8, H, D))
+        cache.lengths[0, 1:] = torch.tensor([0, 3], dtype=torch.int32, device=DEV)
+        k, v = _states(2, B, 4, H, D)
+        layer.append(k, v)
+        assert cache.lengths[0].tolist() == [9, 4, 7] and int(cache._arrivals[0]) == 0
+        for t, codes, scales in ((k, cache.k_codes, cache.k_scales), (v, cache.v_codes, cache.v_scales)):
+            wc, we = _bytes_of(t)
+            for b, at in enumerate((8, 0, 3)):
+                n = min(4, cap - at)
+                assert torch.equal(codes[0, b, :, at:at + n].cpu(), wc[b, :, :n])
+                assert torch.equal(scales[0, b, :, at:at + n].cpu(), we[b, :, :n])
+        layer.append(*_states(3, B, 9, H, D))
+        assert cache.lengths[0].tolist() == [9] * B

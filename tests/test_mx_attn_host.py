@@ -415,7 +415,7 @@ def test_captured_stores_and_places_are_no_present_lengths(cache_on_the_host):
     layer.append(*_states(2), 70)
     capturing[0] = False
     assert layer.views()[0].shape[1] == 72
-    cache.lengths[0].fill_(20)
+    cache.lengths.data[0] = 20                   # (the capture wrote none)
     recorded[1]()
     assert layer.views()[0].shape[1] >= 72
     # the other layer's lengths are still known
@@ -423,3 +423,37 @@ def test_captured_stores_and_places_are_no_present_lengths(cache_on_the_host):
     other.append(*_states(93))
     with pytest.raises(ValueError):
         other.append(*_states(1))
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_entries_that_start_anew_are_not_refused(cache_on_the_host, inference):
+    """append(None) goes by the entries' lengths where the program lowered them, whichever way it wrote."""
+    make = cache_on_the_host[0]
+    with torch.inference_mode(inference):
+        for lower in (lambda c: c.lengths[0].zero_(), lambda c: c.lengths.fill_(1), lambda c: c.lengths[0, :].sub_(8),
+                      lambda c: c.get_layer(0).views()[0].lengths.zero_(), lambda c: c.lengths.view(-1)[:2].copy_(torch.zeros(2))):
+            cache = make(capacity=9)
+            layer = cache.get_layer(0)
+            layer.store(*_states(8))
+            lower(cache)
+            for _ in range(20):
+                before = cache.lengths[0].clone()
+                layer.append(*_states(2))
+                assert torch.equal(cache.lengths[0], (before + 2).clamp(max=9)) and layer.views()[0].shape[1] == 9
+                cache.lengths[0, 0] = 0
+        # an entry of the other layer, and what the cache writes itself
+        cache = make(2, capacity=9)
+        layer, other = cache.get_layer(0), cache.get_layer(1)
+        layer.store(*_states(3))
+        layer.append(*_states(1), 4)
+        other.store(*_states(0))
+        other.append(*_states(0))
+        with pytest.raises(ValueError):
+            layer.append(*_states(5))
+        with pytest.raises(ValueError):
+            other.append(*_states(10))
+        cache.lengths[1].zero_()
+        other.store(*_states(9))
+        layer.append(*_states(5))
+        other.append(*_states(1))
+        assert cache.lengths.tolist() == [[9, 9], [9, 9]]
