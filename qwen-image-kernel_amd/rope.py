@@ -7,7 +7,8 @@ and K together.  The angles are computed on the device as they are needed, D / 2
 a token for all heads of Q and K (include/qik_rope.h): position times frequency
 and its fraction of a turn in fp64, sine and cosine in fp32.  The norm and the
 rotation are fp32 and the result is rounded once, where the call with a table
-rounds between them as well.  These calls record gradients.
+rounds between them as well.  These calls record gradients (backward; a
+forward-mode derivative is refused).
 """
 
 from __future__ import annotations
@@ -17,6 +18,7 @@ import math
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .attention import _kernel_layout
@@ -321,9 +323,10 @@ class _NormRope(torch.autograd.Function):
 
 
 def _run(rope: AxialRope, xs, ws, eps):
-    if torch.is_grad_enabled() and (xs[0].requires_grad or xs[-1].requires_grad
-                                    or (ws[0] is not None and ws[0].requires_grad)
-                                    or (ws[-1] is not None and ws[-1].requires_grad)):
+    # (a dual tensor need not require gradients: inside a forward-mode level the Function refuses it by itself)
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (xs[0].requires_grad or xs[-1].requires_grad
+                                                                      or (ws[0] is not None and ws[0].requires_grad)
+                                                                      or (ws[-1] is not None and ws[-1].requires_grad)):
         return _NormRope.apply(rope, eps, len(xs), *xs, *ws)
     return _forward(rope, xs, ws, eps)
 

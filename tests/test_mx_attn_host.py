@@ -457,3 +457,24 @@ def test_entries_that_start_anew_are_not_refused(cache_on_the_host, inference):
         layer.append(*_states(5))
         other.append(*_states(1))
         assert cache.lengths.tolist() == [[9, 9], [9, 9]]
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """A dual tensor is refused whether or not it requires gradients, and is not taken for a plain one."""
+    from torch.autograd import forward_ad
+
+    from qwen_image_kernel_amd import rope as R
+
+    class Rope:
+        _positions = torch.zeros(1)
+
+    monkeypatch.setattr(R, "_forward", lambda rope, xs, ws, eps: [torch.zeros_like(x) for x in xs])
+    x, w = torch.ones(1, 1, 1, 32), torch.ones(32)
+    with forward_ad.dual_level():
+        dual, dual_w = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, w))
+        for xs, ws in (((dual,), (w,)), ((x, dual), (w, w)), ((x,), (dual_w,)), ((dual, x), (None, None)),
+                       ((forward_ad.make_dual(x.clone().requires_grad_(), x),), (w,))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    R._run(Rope, xs, ws, (1e-6, 1e-6))
+        assert R._run(Rope, (x,), (w,), (1e-6,))[0].shape == x.shape
