@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 import weakref
 
 import torch
@@ -282,20 +283,22 @@ def _backward(rope: AxialRope, xs, ws, eps, grads):
 # capture on another one would not survive that, so it is refused while it can be:
 # by leaf, that stream and the recorded calls.
 _LEAVES: dict = {}
+_LEAVES_LOCK = threading.RLock()  # threads may share leaves; a finalizer may run a call while this one is noted
 
 
 def _record(call, leaves, stream: int, capturing: bool) -> None:
     """Note that `call` (its ctx) is recorded on `stream`; RuntimeError if a capture could not run its backward pass."""
-    for t in leaves:
-        here = _LEAVES.get(id(t))
-        alive = [] if here is None else [r for r in here[1] if r() is not None]
-        if alive and capturing and here[0] != stream:
-            raise RuntimeError("a graph of the same leaves, recorded on another stream, is alive: its outputs have to be "
-                               "dropped before a call with gradients is captured")
-        if not alive and len(_LEAVES) >= 4096:
-            for k in [k for k, (_, refs) in _LEAVES.items() if all(r() is None for r in refs)]:
-                del _LEAVES[k]
-        _LEAVES[id(t)] = (here[0] if alive else stream, [*alive, weakref.ref(call)])
+    with _LEAVES_LOCK:
+        for t in leaves:
+            here = _LEAVES.get(id(t))
+            alive = [] if here is None else [r for r in here[1] if r() is not None]
+            if alive and capturing and here[0] != stream:
+                raise RuntimeError("a graph of the same leaves, recorded on another stream, is alive: its outputs have to be "
+                                   "dropped before a call with gradients is captured")
+            if not alive and len(_LEAVES) >= 4096:
+                for k in [k for k, (_, refs) in _LEAVES.items() if all(r() is None for r in refs)]:
+                    del _LEAVES[k]
+            _LEAVES[id(t)] = (here[0] if alive else stream, [*alive, weakref.ref(call)])
 
 
 class _NormRope(torch.autograd.Function):

@@ -478,3 +478,33 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
                 with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
                     R._run(Rope, xs, ws, (1e-6, 1e-6))
         assert R._run(Rope, (x,), (w,), (1e-6,))[0].shape == x.shape
+
+
+def test_two_threads_record_calls_of_one_leaf(monkeypatch):
+    """A call noted while another thread notes one of the same leaf is not lost, and a capture is refused for it."""
+    import threading
+
+    from qwen_image_kernel_amd import rope as R
+
+    class Call:
+        pass
+
+    calls, leaf = [Call(), Call()], torch.ones(2, requires_grad=True)
+    other = threading.Thread(target=lambda: R._record(calls[1], [leaf], 1, False))
+
+    class Leaves(dict):
+        def get(self, key):
+            here = super().get(key)
+            if threading.current_thread() is not other:   # the other thread's turn, between this one's look and its note
+                if not other.ident:
+                    other.start()
+                other.join(0.5)
+            return here
+
+    monkeypatch.setattr(R, "_LEAVES", Leaves())
+    R._record(calls[0], [leaf], 1, False)
+    other.join()
+    assert len(R._LEAVES[id(leaf)][1]) == 2
+    del calls[0]
+    with pytest.raises(RuntimeError):
+        R._record(Call(), [leaf], 2, True)
