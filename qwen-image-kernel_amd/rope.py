@@ -279,22 +279,25 @@ def _backward(rope: AxialRope, xs, ws, eps, grads):
 
 
 # A leaf's node of the backward pass belongs to the stream on which the first graph
-# that is still alive was recorded, and the backward pass waits on that stream.  A
-# capture on another one would not survive that, so it is refused while it can be:
-# by leaf, that stream and the recorded calls.
+# that is still alive was recorded, also when that graph's own backward pass is over,
+# and the backward pass ties that stream to its own by waits.  So a captured pass
+# takes another stream (a warm-up's) into the capture.  The default stream cannot be
+# captured: the process would end, so the capture is refused while it can be.  By
+# leaf: the kind of that stream, and the recorded calls.
 _LEAVES: dict = {}
 _LEAVES_LOCK = threading.RLock()  # threads may share leaves; a finalizer may run a call while this one is noted
 
 
 def _record(call, leaves, stream: int, capturing: bool) -> None:
-    """Note that `call` (its ctx) is recorded on `stream`; RuntimeError if a capture could not run its backward pass."""
+    """Note that `call` (its ctx) is recorded on `stream` (any value that tells apart what a capture cannot join);
+    RuntimeError if a capture could not run its backward pass."""
     with _LEAVES_LOCK:
         for t in leaves:
             here = _LEAVES.get(id(t))
             alive = [] if here is None else [r for r in here[1] if r() is not None]
             if alive and capturing and here[0] != stream:
-                raise RuntimeError("a graph of the same leaves, recorded on another stream, is alive: its outputs have to be "
-                                   "dropped before a call with gradients is captured")
+                raise RuntimeError("a graph of the same leaves, recorded on the default stream, is alive: its outputs have to "
+                                   "be dropped before a call with gradients is captured")
             if not alive and len(_LEAVES) >= 4096:
                 for k in [k for k, (_, refs) in _LEAVES.items() if all(r() is None for r in refs)]:
                     del _LEAVES[k]
@@ -310,7 +313,9 @@ class _NormRope(torch.autograd.Function):
         ctx.rope, ctx.eps, ctx.n = rope, eps, n
         leaves = [t for t in ts if t is not None and t.requires_grad and t.is_leaf]
         if leaves and xs[0].is_cuda:
-            _record(ctx, leaves, _raw_stream(xs[0].device.index), torch.cuda.is_current_stream_capturing())
+            # (the default stream's handle is 0; a capture is never on it)
+            side = int(_raw_stream(xs[0].device.index) != 0)
+            _record(ctx, leaves, side, torch.cuda.is_current_stream_capturing())
         # the positions are saved with the inputs: a change before the backward pass is an error there
         ctx.save_for_backward(rope._positions, *ts)
         return tuple(_forward(rope, xs, ws, eps))

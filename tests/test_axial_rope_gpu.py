@@ -358,3 +358,38 @@ def test_offsets_past_32_bits():
         for which in ((0,), (1,), (2, 3)):
             ts = [put(t, i) if i in which else t for i, t in enumerate((*x, *d))]
             assert all(torch.equal(a, b) for a, b in zip(both(ts[:2], ts[2:]), want)), (strides, which)
+
+
+def test_a_capture_beside_a_warm_up_that_lives_on():
+    """Warm up on a side stream, keep its outputs and loss, capture on the graph's own stream: as torch's own recipe goes."""
+    x, w, d, _, rope = _one(B=2, S=40)
+    leaves = [t.requires_grad_() for t in (*x, *w)]
+
+    def loss_of(outs):
+        return sum((o.float() * g.float()).sum() for o, g in zip(outs, d))
+
+    side, stream = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        kept = qik.fused_qk_norm_rope(*leaves, rope, EPS)
+        kept_loss = loss_of(kept)
+        kept_loss.backward()
+        never_run = qik.fused_qk_norm_rope(*leaves, rope, EPS)
+    torch.cuda.synchronize()
+    want = [*(t.detach().clone() for t in kept), *(t.grad.clone() for t in leaves)]
+    for t in leaves:
+        t.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        outs = qik.fused_qk_norm_rope(*leaves, rope, EPS)
+        loss_of(outs).backward()
+    got = [*outs, *(t.grad for t in leaves)]
+    for _ in range(4):
+        for t in got:
+            t.detach().zero_()
+        graph.replay()
+        again = torch.autograd.grad(never_run, leaves, d, retain_graph=True)   # the other stream's graph, between the replays
+        torch.cuda.synchronize()
+        assert all(torch.equal(a.detach(), b) for a, b in zip(got, want))
+        assert all(torch.equal(a, b) for a, b in zip(again, want[2:]))
+    del kept, kept_loss, never_run
