@@ -27,7 +27,6 @@ fp8-V one 768, with a length for each batch entry and tokens appended behind it
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
@@ -256,6 +255,7 @@ class _MXLayerView(_SlabLayer):
         self._c = cache
         self._layer = layer
         self._lengths = cache.lengths[layer]
+        self._index = self._lengths.device.index
         self._calls: dict = {}  # store geometry -> (argument struct, operands that need a copy)
         self._full = None       # (k, v MXSlab views of the whole capacity, argument struct of get)
         self._rows, self._views = -1, None  # what views() gave last, and for how many rows
@@ -268,8 +268,7 @@ class _MXLayerView(_SlabLayer):
         if P > c.capacity:
             raise ValueError(f"prefix of {P} tokens exceeds the slab capacity {c.capacity}")
         if P == 0 or call is None:
-            with c._writing_lengths():
-                self._lengths.fill_(P)
+            c._write_lengths(self._lengths.fill_, P)
         else:
             self._launch(call, k, v, None, False)
         self._note(P, True, P)
@@ -302,8 +301,7 @@ class _MXLayerView(_SlabLayer):
             at = int(at)
             if at < 0 or at + S > c.capacity:
                 raise ValueError(f"{S} tokens at {at} exceed the slab capacity {c.capacity}")
-            with c._writing_lengths():
-                lengths.fill_(at)
+            c._write_lengths(lengths.fill_, at)
             n, exact, most, at = at + S, True, at + S, lengths
         else:
             n, exact, most, at = c._host_lengths[i], c._exact[i] and not c._lengths_written(), c.capacity, lengths
@@ -313,8 +311,7 @@ class _MXLayerView(_SlabLayer):
         if call is not None:
             self._launch(call, k, v, at, grow)
         elif S or not grow:
-            with c._writing_lengths():
-                lengths.copy_((at + S).clamp_(0, c.capacity))
+            c._write_lengths(lengths.copy_, (at + S).clamp_(0, c.capacity))
         self._note(n, exact, most)
 
     def _note(self, n: int, exact: bool, most: int) -> None:
@@ -329,10 +326,9 @@ class _MXLayerView(_SlabLayer):
         c._host_lengths[i], c._exact[i] = n, exact
 
     def _capturing(self) -> bool:
-        idx = self._lengths.device.index
-        if idx == torch._C._cuda_getDevice():
+        if self._index == torch._C._cuda_getDevice():
             return torch.cuda.is_current_stream_capturing()
-        with torch.cuda.device(idx):
+        with torch.cuda.device(self._index):
             return torch.cuda.is_current_stream_capturing()
 
     def _call(self, k: torch.Tensor, v: torch.Tensor):
@@ -378,7 +374,7 @@ class _MXLayerView(_SlabLayer):
             a.at = at.data_ptr()
             if grow:
                 a.arrivals = self._c._arrivals.data_ptr() + 4 * self._layer
-        idx = self._lengths.device.index
+        idx = self._index
         fn = _lib.load().qik_mx_slab_store
         if idx != torch._C._cuda_getDevice():
             with torch.cuda.device(idx):
@@ -472,11 +468,10 @@ class MXKVCache:
             self._program_writes = True
         return self._program_writes
 
-    @contextlib.contextmanager
-    def _writing_lengths(self):
-        """Around the cache's own writes by torch."""
+    def _write_lengths(self, write, value) -> None:
+        """A write of the cache's own by torch."""
         self._lengths_written()
-        yield
+        write(value)
         self._version = self.lengths._version
 
     def get_layer(self, i: int) -> _MXLayerView:
