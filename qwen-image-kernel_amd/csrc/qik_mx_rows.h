@@ -35,9 +35,10 @@
 //     does not depend on which one that is.
 // 32 query heads on 8 KV heads of 128, MI355X: a token against 131072 keys 30.6 us,
 // 4.6 TB/s of the slab (a large copy reaches 5.15); 24 tokens of sequences of up
-// to 8192 keys 30.5 us, 3.9 TB/s, where the pieces are two a CU and not quite
-// even, and the merge ends last; a token against 1501 keys 8.6 us, of which the bytes would be
-// less than one: launch, a piece's loads and steps, and the merge one after the other.
+// to 8192 keys 30 to 33 us, 3.7 to 4.0 TB/s, where the pieces are two a CU and not
+// quite even, and the merge ends last; a token against 1501 keys 8.6 us, of which
+// the bytes would be less than one: launch, a piece's loads and steps, and the merge
+// one after the other.
 #ifndef QIK_MX_ROWS_H
 #define QIK_MX_ROWS_H
 
